@@ -342,6 +342,122 @@ B2A_API int b2a_decode_attention_block(b2a_context* ctx, int act_dtype, int cach
                                        void* y, int B, int hidden, int Hq, int Hkv, int D, int max_seq, float scale,
                                        double rope_theta, int window, void* stream);
 
+/* ------------------------------------------------------------ paged 4-bit KV cache */
+
+/* A layer's KV cache held in 4 bits, in pages.  No counterpart exists in the reference.
+ *   pages      : DEVICE bytes [num_pages][num_kv_heads][page_size * head_dim * 5 / 4]
+ *                (b2a_kv4_page_bytes per page), 16-byte aligned.
+ *   page_table : DEVICE int32 [B][max_pages]; entry i of a row names the page that holds the
+ *                sequence's positions [i * page_size, (i + 1) * page_size), -1: none.  Entries the
+ *                call needs outside [0, num_pages) raise the device status; those outputs are NaN.
+ *   page_size  : a multiple of 16, at most 1024.   head_dim: 64, 96, 128 or 256.
+ * A row of head_dim values is held in groups of 32 as 4-bit codes with an fp16 scale and minimum:
+ *     s = f16((max - min) * f32(1/15)),  z = f16(min),  c = clamp(rint((x - z) * (1 / s)), 0, 15)
+ * in 32-bit arithmetic, each operation rounded (c = 0 where s = 0), and stands for s * c + z: 0.625
+ * bytes a value.  A group with a value that is not finite, or whose s or z leaves the fp16 range,
+ * holds NaN and raises the device status.
+ * A (page, head) slab is a row of blocks of 16 positions, 20 * head_dim bytes each: K codes
+ * (8 * head_dim bytes), K params (2 * head_dim), V codes, V params.  With d = 32 y + 16 x + r the
+ * code of (key 0..15, d) is in byte ((y * 8 + g) * 4 + t) * 8 + x * 4 + 2 e + h, in the low nibble
+ * when bit 3 of d is clear, else in the high one, where
+ *     K: g = key % 8, h = key / 8, t = (d % 8) / 2, e = d % 2
+ *     V: g = d % 8,   h = key / 8, t = (key % 8) / 2, e = key % 2
+ * and the params are fp16 pairs (s, z), number ((key % 8) * 2 + key / 8) * (head_dim / 32) + y.
+ * The struct is read during the call. */
+typedef struct b2a_kv4_cache {
+    void* pages;
+    const int32_t* page_table;
+    int num_pages;
+    int page_size;
+    int max_pages;
+    int num_kv_heads;
+    int head_dim;
+} b2a_kv4_cache;
+
+/* Bytes of one page of one layer; 0 for sizes the cache does not take. */
+B2A_API size_t b2a_kv4_page_bytes(int num_kv_heads, int head_dim, int page_size);
+
+/* Append T new K/V rows per sequence: optional zero-centred RMS norm of the keys (k_norm_w [D],
+ * as b2a_decode), RoPE at position ctx_lens[b] + t, quantisation, store.
+ *   k_new, v_new : [B][T] token rows of [Hkv][D] in act_dtype (FLOAT16 / BFLOAT16), consecutive
+ *       tokens kv_token_stride elements apart (0: Hkv * D; a fused [Q|K|V] row passes its width),
+ *       a multiple of 8; 16-byte aligned.
+ *   ctx_lens : DEVICE int32 [B], tokens cached before the call.  new_lens : DEVICE int32 [B] with
+ *       the tokens that exist, 0..T, or NULL (T each).  The pages of positions [ctx_lens[b],
+ *       ctx_lens[b] + new_lens[b]) must be in the table and belong to no other row
+ *       (b2a_pages_reserve sees to both).  Lengths that do not fit the table raise the device
+ *       status, store nothing and give NaN.
+ *   k_held, v_held : optional [B,T,Hkv,D] act_dtype, the rows as the cache holds them (zeros where
+ *       t >= new_lens[b]): the values every later step sees, for a prompt's own attention.
+ * Sequences of one call must not share the pages they write. */
+B2A_API int b2a_kv4_append(b2a_context* ctx, const b2a_kv4_cache* cache, int act_dtype, const void* k_new,
+                           const void* v_new, int64_t kv_token_stride, const int32_t* ctx_lens,
+                           const int32_t* new_lens, int B, int T, int rope_mode, double rope_theta,
+                           const float* k_norm_w, float norm_eps, void* k_held, void* v_held, void* stream);
+
+/* Attention of T tokens per sequence over the cache: query t sits at position p = ctx_lens[b] + t
+ * and sees the cached keys [max(0, p - window + 1), p] (window 0: [0, p]); its own position and
+ * those before it must have been appended.
+ *   q : [B][T] token rows of [Hq][D], q_token_stride elements apart (0: Hq * D); optional norm
+ *       (q_norm_w) and RoPE at p, as b2a_decode.   o : [B,T,Hq,D], act_dtype.
+ * Rows t >= new_lens[b] give zeros.  Softmax and sums are held in fp32; q and the probabilities
+ * are rounded once to 11 significant bits for the tensor cores. */
+B2A_API int b2a_kv4_attention(b2a_context* ctx, const b2a_kv4_cache* cache, int act_dtype, const void* q,
+                              int64_t q_token_stride, const int32_t* ctx_lens, const int32_t* new_lens, int B, int T,
+                              int Hq, float scale, int rope_mode, double rope_theta, int window,
+                              const float* q_norm_w, float norm_eps, void* o, void* stream);
+
+/* b2a_kv4_append of the new rows, then b2a_kv4_attention of their queries, which see the new rows
+ * as the cache holds them: a decode step (T = 1), the verification of a draft (T of a few), or a
+ * chunk of a prompt on a cached prefix.  q_norm_w and k_norm_w: both or neither. */
+B2A_API int b2a_kv4_decode(b2a_context* ctx, const b2a_kv4_cache* cache, int act_dtype, const void* q,
+                           int64_t q_token_stride, const void* k_new, const void* v_new, int64_t kv_token_stride,
+                           const int32_t* ctx_lens, const int32_t* new_lens, int B, int T, int Hq, float scale,
+                           int rope_mode, double rope_theta, int window, const float* q_norm_w, const float* k_norm_w,
+                           float norm_eps, void* k_held, void* v_held, void* o, void* stream);
+
+/* The pages of a cache as a whole: one page table and one count per page serve all layers.
+ *   page_table : DEVICE int32 [n_seq][max_pages], -1: none.
+ *   ref_counts : DEVICE int32 [num_pages], the table entries that name each page; 0: free.
+ *   pages      : n_layers arrays [num_pages][page_bytes], layer_stride bytes apart (whatever they
+ *                hold; page_bytes a multiple of 16).  Only reserve and compact touch them.
+ * Results depend on the state at the call's start alone: free pages are given out lowest first, in
+ * the order of rows and slots.  Table entries >= num_pages raise the device status and are left. */
+typedef struct b2a_page_pool {
+    int32_t* page_table;
+    int32_t* ref_counts;
+    void* pages;
+    int64_t layer_stride;
+    int64_t page_bytes;
+    int n_seq;
+    int max_pages;
+    int num_pages;
+    int n_layers;
+} b2a_page_pool;
+
+/* Row i of the table becomes what row parents[i] (DEVICE int32 [n_seq]) was; -1 empties it.  A beam
+ * step, n samples of one prompt, moving rows and retiring sequences are all this.  Pages are shared,
+ * not copied; counts follow. */
+B2A_API int b2a_pages_fork(b2a_context* ctx, const b2a_page_pool* pool, const int32_t* parents, void* stream);
+
+/* Slots that hold no position of [keep_from[row], keep_to[row]) give their page back (DEVICE int32
+ * [n_seq]; keep_from NULL: 0): trims a rejected draft, drops what left a sliding window, frees a row
+ * (keep_to 0). */
+B2A_API int b2a_pages_free(b2a_context* ctx, const b2a_page_pool* pool, const int32_t* keep_from,
+                           const int32_t* keep_to, int page_size, void* stream);
+
+/* Every slot that positions [ctx_lens[row], ctx_lens[row] + new_lens[row]) fall into gets a page of
+ * its own: an empty slot a free page, a slot whose page has a count above 1 at the call's start a
+ * copy (all layers), whose original loses one count.  All or nothing: where too few pages are free
+ * nothing changes.  counts: DEVICE int32 [2] = pages given out, pages missing. */
+B2A_API int b2a_pages_reserve(b2a_context* ctx, const b2a_page_pool* pool, const int32_t* ctx_lens,
+                              const int32_t* new_lens, int page_size, int32_t* counts, void* stream);
+
+/* With n pages in use, those at n or above move into the free places below n, both in ascending
+ * order (contents of all layers, counts, table entries), so that pages [n, num_pages) are free.
+ * counts: DEVICE int32 [2] = n, pages moved. */
+B2A_API int b2a_pages_compact(b2a_context* ctx, const b2a_page_pool* pool, int32_t* counts, void* stream);
+
 /* ------------------------------------------------------------ multi-GPU */
 
 /* One process driving several GPUs of a node: the multi-device counterpart of

@@ -20,6 +20,9 @@ Operator mirrors
   ``WB/runtime/kernels/DirectMlAttentionKernel.java:99-210,370-420``).
 * :func:`prefill_causal` -- the causal GQA prefill of the decoder runtimes.
 * :func:`decode` -- the fused decode step (QK-norm, RoPE, KV append, attention).
+* :func:`kv4_append`, :func:`kv4_decode`, :func:`kv4_attention` -- a KV cache held in 4 bits, in pages;
+  :func:`pages_reserve`, :func:`pages_fork`, :func:`pages_free`, :func:`pages_compact` -- its pages
+  (no counterpart in the reference).
 * :class:`QwenAttentionShaders` -- ``rope_and_append`` / ``gqa_attention_decode``
   (``WB/windows/QwenAttentionShaders.java:82-263``).
 * :class:`Gemma3FusedAttentionContext` -- ``Gemma3WarpFusedAttentionContextKernel.context``
@@ -66,9 +69,24 @@ def build(verbose: bool = False) -> str:
 
 
 _vp = ctypes.c_void_p
+_i64 = ctypes.c_int64
 _i = ctypes.c_int
 _f = ctypes.c_float
 _d = ctypes.c_double
+
+
+class _Kv4Cache(ctypes.Structure):
+    """b2a_kv4_cache."""
+
+    _fields_ = [("pages", _vp), ("page_table", _vp), ("num_pages", _i), ("page_size", _i), ("max_pages", _i),
+                ("num_kv_heads", _i), ("head_dim", _i)]
+
+
+class _PagePool(ctypes.Structure):
+    """b2a_page_pool."""
+
+    _fields_ = [("page_table", _vp), ("ref_counts", _vp), ("pages", _vp), ("layer_stride", _i64),
+                ("page_bytes", _i64), ("n_seq", _i), ("max_pages", _i), ("num_pages", _i), ("n_layers", _i)]
 
 
 def lib() -> ctypes.CDLL:
@@ -112,6 +130,18 @@ def lib() -> ctypes.CDLL:
         L.b2a_linear.argtypes = [_vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]
         L.b2a_decode_attention_block.argtypes = [_vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i,
                                                  _i, _i, _i, _i, _f, _d, _i, _vp]
+        cache, pool = ctypes.POINTER(_Kv4Cache), ctypes.POINTER(_PagePool)
+        L.b2a_kv4_page_bytes.argtypes = [_i, _i, _i]
+        L.b2a_kv4_page_bytes.restype = ctypes.c_size_t
+        L.b2a_kv4_append.argtypes = [_vp, cache, _i, _vp, _vp, _i64, _vp, _vp, _i, _i, _i, _d, _vp, _f, _vp, _vp, _vp]
+        L.b2a_kv4_attention.argtypes = [_vp, cache, _i, _vp, _i64, _vp, _vp, _i, _i, _i, _f, _i, _d, _i, _vp, _f, _vp,
+                                        _vp]
+        L.b2a_kv4_decode.argtypes = [_vp, cache, _i, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i, _i, _i, _f, _i, _d, _i,
+                                     _vp, _vp, _f, _vp, _vp, _vp, _vp]
+        L.b2a_pages_fork.argtypes = [_vp, pool, _vp, _vp]
+        L.b2a_pages_free.argtypes = [_vp, pool, _vp, _vp, _i, _vp]
+        L.b2a_pages_reserve.argtypes = [_vp, pool, _vp, _vp, _i, _vp, _vp]
+        L.b2a_pages_compact.argtypes = [_vp, pool, _vp, _vp]
         L.b2a_group_create.argtypes = [_i, _vp, ctypes.POINTER(_vp)]
         L.b2a_group_destroy.argtypes = [_vp]
         L.b2a_group_last_error.argtypes = [_vp, ctypes.c_char_p, ctypes.c_size_t]
@@ -126,6 +156,8 @@ def lib() -> ctypes.CDLL:
                      "b2a_reserve_decode", "b2a_check_device_status", "b2a_mha", "b2a_prefill_causal", "b2a_decode",
                      "b2a_qwen_rope_and_append", "b2a_qwen_gqa_attention_decode", "b2a_qwen_decode_step", "b2a_prefill_gemma",
                      "b2a_gemma_fused_attention_context", "b2a_partition_units", "b2a_test_inject_wait_timeout",
+                     "b2a_kv4_append", "b2a_kv4_attention", "b2a_kv4_decode", "b2a_pages_fork", "b2a_pages_free",
+                     "b2a_pages_reserve", "b2a_pages_compact",
                      "b2a_linear", "b2a_decode_attention_block", "b2a_group_create", "b2a_group_destroy", "b2a_group_last_error", "b2a_group_size",
                      "b2a_group_context", "b2a_group_check_device_status", "b2a_sharded_decode", "b2a_sharded_mha"):
             getattr(L, name).restype = _i
@@ -354,6 +386,185 @@ def decode_attention_block(ctx: Context, x, w_qkv, b_qkv, k_cache, v_cache, ctx_
         _ptr(v_cache), kv_layout, _ptr(ctx_lens), _ptr(w_o), _ptr(residual), _ptr(y), B, hidden, num_q_heads,
         num_kv_heads, D, max_seq, scale, rope_theta, window, _stream(stream)))
     return y
+
+
+# ------------------------------------------------- paged 4-bit KV cache
+def kv4_page_bytes(num_kv_heads: int, head_dim: int, page_size: int) -> int:
+    """Bytes of one page of one layer: allocate pages as uint8 [num_pages, num_kv_heads,
+    page_size * head_dim * 5 // 4] (or [layers, ...], a layer's slice being one cache)."""
+    n = lib().b2a_kv4_page_bytes(num_kv_heads, head_dim, page_size)
+    if n == 0:
+        raise ValueError("page_size must be a multiple of 16 up to 1024, head_dim 64, 96, 128 or 256")
+    return n
+
+
+def _int32(t, name, shape, optional=False):
+    """A device int32 tensor of that shape, as a pointer."""
+    if t is None:
+        if optional:
+            return None
+        raise ValueError(f"{name} must not be None")
+    if str(t.dtype) != "torch.int32" or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+    return _ptr(t)
+
+
+def _token_rows(t, name, shape):
+    """Pointer and token stride of [B,T,H,D] rows: heads side by side, one distance from each token to
+    the next (a slice of a fused [Q|K|V] projection is one)."""
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if not t.is_cuda:
+        raise ValueError("tensors must live on the CUDA device (GpuBuffer); got a host tensor")
+    B, T, H, D = shape
+    sb, st, sh, sd = t.stride()
+    step = st if T > 1 else sb if B > 1 else H * D
+    if sd != 1 or (H > 1 and sh != D) or (T > 1 and B > 1 and sb != T * st):
+        raise ValueError(f"{name} must hold its tokens at one distance and its heads side by side, "
+                         f"got strides {t.stride()}")
+    return ctypes.c_void_p(t.data_ptr()), step
+
+
+def _kv4_cache(pages, page_table, B, D, num_kv_heads=None):
+    import torch
+    if pages.dtype != torch.uint8 or pages.dim() != 3:
+        raise ValueError("pages must be uint8 [num_pages, num_kv_heads, page_size * head_dim * 5 // 4]")
+    if num_kv_heads is not None and pages.shape[1] != num_kv_heads:
+        raise ValueError(f"pages hold {pages.shape[1]} kv heads, the new rows {num_kv_heads}")
+    page_size, rest = divmod(pages.shape[2] * 4, D * 5)
+    if rest or page_size == 0:
+        raise ValueError(f"a page of {pages.shape[2]} bytes per kv head holds no whole rows of head_dim {D}")
+    if page_table.dim() != 2:
+        raise ValueError("page_table must be int32 [B, max_pages]")
+    table = _int32(page_table, "page_table", (B, page_table.shape[1]))
+    return _Kv4Cache(_ptr(pages), table, pages.shape[0], page_size, page_table.shape[1], pages.shape[1], D)
+
+
+def _same_dtype(first, **others):
+    for name, t in others.items():
+        if t is not None and t.dtype != first.dtype:
+            raise ValueError(f"{name} must have element type {first.dtype}, got {t.dtype}")
+
+
+def _norm_w(t, name, D):
+    if t is not None and (str(t.dtype) != "torch.float32" or t.numel() != D):
+        raise ValueError(f"{name} must be float32 [{D}]")
+    return _ptr(t)
+
+
+def _dense(t, name, shape, optional=False):
+    if t is None and optional:
+        return None
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    return _ptr(t)
+
+
+def kv4_append(ctx: Context, k_new, v_new, pages, page_table, ctx_lens, *, new_lens=None, rope_mode: int = ROPE_NEOX,
+               rope_theta: float = 10000.0, k_norm_w=None, norm_eps: float = 1e-6, k_held=None, v_held=None,
+               stream=None):
+    """Append new K/V rows [B,T,Hkv,D] (fp16 / bf16; slices of fused rows may be passed) to a paged 4-bit
+    cache: key norm, RoPE at ctx_lens[b] + t, quantisation, store.  pages: uint8 [num_pages, Hkv,
+    page_size * D * 5 // 4]; page_table int32 [B, max_pages]; ctx_lens, new_lens int32 [B] (new_lens: how many
+    of the T tokens exist).  k_held / v_held [B,T,Hkv,D] receive the rows as the cache holds them."""
+    B, T, Hkv, D = k_new.shape
+    cache = _kv4_cache(pages, page_table, B, D, Hkv)
+    k, step = _token_rows(k_new, "k_new", k_new.shape)
+    v, v_step = _token_rows(v_new, "v_new", k_new.shape)
+    if v_step != step:
+        raise ValueError("k_new and v_new must have one token stride")
+    _same_dtype(k_new, v_new=v_new, k_held=k_held, v_held=v_held)
+    ctx.check(lib().b2a_kv4_append(
+        ctx.handle, ctypes.byref(cache), _dtype_code(k_new), k, v, step, _int32(ctx_lens, "ctx_lens", (B,)),
+        _int32(new_lens, "new_lens", (B,), True), B, T, rope_mode, rope_theta, _norm_w(k_norm_w, "k_norm_w", D),
+        norm_eps, _dense(k_held, "k_held", k_new.shape, True), _dense(v_held, "v_held", k_new.shape, True),
+        _stream(stream)))
+
+
+def kv4_attention(ctx: Context, q, pages, page_table, ctx_lens, o, scale: float, *, new_lens=None,
+                  rope_mode: int = ROPE_NEOX, rope_theta: float = 10000.0, window: int = 0, q_norm_w=None,
+                  norm_eps: float = 1e-6, stream=None):
+    """Attention of tokens q [B,T,Hq,D] at positions ctx_lens[b] + t over the paged 4-bit cache, which must
+    hold those positions already; o [B,T,Hq,D]; rows t >= new_lens[b] give zeros."""
+    B, T, Hq, D = q.shape
+    cache = _kv4_cache(pages, page_table, B, D)
+    qp, q_step = _token_rows(q, "q", q.shape)
+    _same_dtype(q, o=o)
+    ctx.check(lib().b2a_kv4_attention(
+        ctx.handle, ctypes.byref(cache), _dtype_code(q), qp, q_step, _int32(ctx_lens, "ctx_lens", (B,)),
+        _int32(new_lens, "new_lens", (B,), True), B, T, Hq, scale, rope_mode, rope_theta, window,
+        _norm_w(q_norm_w, "q_norm_w", D), norm_eps, _dense(o, "o", q.shape), _stream(stream)))
+    return o
+
+
+def kv4_decode(ctx: Context, q, k_new, v_new, pages, page_table, ctx_lens, o, scale: float, *, new_lens=None,
+               rope_mode: int = ROPE_NEOX, rope_theta: float = 10000.0, window: int = 0, q_norm_w=None, k_norm_w=None,
+               norm_eps: float = 1e-6, k_held=None, v_held=None, stream=None):
+    """kv4_append of k_new / v_new [B,T,Hkv,D], then kv4_attention of q [B,T,Hq,D]: a decode step (T = 1), the
+    verification of a draft, or a chunk of a prompt on a cached prefix."""
+    B, T, Hq, D = q.shape
+    Hkv = k_new.shape[2] if k_new.dim() == 4 else 0
+    cache = _kv4_cache(pages, page_table, B, D, Hkv)
+    qp, q_step = _token_rows(q, "q", q.shape)
+    k, step = _token_rows(k_new, "k_new", (B, T, Hkv, D))
+    v, v_step = _token_rows(v_new, "v_new", (B, T, Hkv, D))
+    if v_step != step:
+        raise ValueError("k_new and v_new must have one token stride")
+    _same_dtype(q, k_new=k_new, v_new=v_new, o=o, k_held=k_held, v_held=v_held)
+    ctx.check(lib().b2a_kv4_decode(
+        ctx.handle, ctypes.byref(cache), _dtype_code(q), qp, q_step, k, v, step, _int32(ctx_lens, "ctx_lens", (B,)),
+        _int32(new_lens, "new_lens", (B,), True), B, T, Hq, scale, rope_mode, rope_theta, window,
+        _norm_w(q_norm_w, "q_norm_w", D), _norm_w(k_norm_w, "k_norm_w", D), norm_eps,
+        _dense(k_held, "k_held", k_new.shape, True), _dense(v_held, "v_held", k_new.shape, True),
+        _dense(o, "o", q.shape), _stream(stream)))
+    return o
+
+
+def _page_pool(page_table, ref_counts, pages=None):
+    if page_table.dim() != 2 or ref_counts.dim() != 1:
+        raise ValueError("page_table must be int32 [n_seq, max_pages], ref_counts int32 [num_pages]")
+    n_seq, max_pages = page_table.shape
+    pool = _PagePool(_int32(page_table, "page_table", page_table.shape),
+                     _int32(ref_counts, "ref_counts", ref_counts.shape), None, 0, 0, n_seq, max_pages,
+                     ref_counts.shape[0], 0)
+    if pages is not None:
+        if pages.dim() < 2 or pages.shape[1] != ref_counts.shape[0]:
+            raise ValueError(f"pages must be [n_layers, {ref_counts.shape[0]}, ...], got {list(pages.shape)}")
+        pool.pages, pool.n_layers = _ptr(pages), pages.shape[0]
+        pool.page_bytes = pages[0, 0].numel() * pages.element_size()
+        pool.layer_stride = pool.page_bytes * pages.shape[1]
+    return pool
+
+
+def pages_fork(ctx: Context, page_table, ref_counts, parents, stream=None):
+    """Row i of page_table becomes what row parents[i] was (-1: empty); pages are shared, counts follow."""
+    pool = _page_pool(page_table, ref_counts)
+    ctx.check(lib().b2a_pages_fork(ctx.handle, ctypes.byref(pool), _int32(parents, "parents", (pool.n_seq,)),
+                                   _stream(stream)))
+
+
+def pages_free(ctx: Context, page_table, ref_counts, keep_from, keep_to, page_size: int, stream=None):
+    """Give back the pages of slots that hold no position of [keep_from[row], keep_to[row]) (keep_from None: 0)."""
+    pool = _page_pool(page_table, ref_counts)
+    ctx.check(lib().b2a_pages_free(ctx.handle, ctypes.byref(pool), _int32(keep_from, "keep_from", (pool.n_seq,), True),
+                                   _int32(keep_to, "keep_to", (pool.n_seq,)), page_size, _stream(stream)))
+
+
+def pages_reserve(ctx: Context, page_table, ref_counts, ctx_lens, new_lens, pages, page_size: int, counts, stream=None):
+    """Give every slot that positions [ctx_lens, ctx_lens + new_lens) fall into a page of its own: a free page, or
+    a copy of a page that other rows hold too.  pages: [n_layers, num_pages, ...]; counts int32 [2] receives the
+    pages given out and the pages missing (then nothing changed)."""
+    pool = _page_pool(page_table, ref_counts, pages)
+    ctx.check(lib().b2a_pages_reserve(
+        ctx.handle, ctypes.byref(pool), _int32(ctx_lens, "ctx_lens", (pool.n_seq,)),
+        _int32(new_lens, "new_lens", (pool.n_seq,)), page_size, _int32(counts, "counts", (2,)), _stream(stream)))
+
+
+def pages_compact(ctx: Context, page_table, ref_counts, pages, counts, stream=None):
+    """Move the n pages in use to the front of the pool; counts int32 [2] receives n and the pages moved."""
+    pool = _page_pool(page_table, ref_counts, pages)
+    ctx.check(lib().b2a_pages_compact(ctx.handle, ctypes.byref(pool), _int32(counts, "counts", (2,)),
+                                      _stream(stream)))
 
 
 def _ptr_array(tensors):

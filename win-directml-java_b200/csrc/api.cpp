@@ -57,6 +57,9 @@ struct b2a_context {
     // test hook (b2a_test_inject_wait_timeout): the next tcgen05 attention launch
     // leaves one K/V copy unissued
     bool inject_wait_timeout = false;
+    // paged cache: the page operations' lists
+    void* pg_ws = nullptr;
+    size_t pg_ws_bytes = 0;
     // b2a_set_decode_early_start: tensor-core decodes launched with programmatic serialisation
     bool decode_early_start = false;
     // test hook (b2a_test_last_attention_kernel): the kernel the last whole-sequence
@@ -105,7 +108,7 @@ int ensure_buffer(b2a_context* ctx, void** buf, size_t* have, size_t need, const
     if (*have >= need) return B2A_OK;
     const size_t other =
         ctx->dec_ws_bytes + ctx->pf_ws_bytes + ctx->split_ws_bytes + ctx->blk_ws_bytes + ctx->rope_tab_bytes +
-        ctx->lin_ws_bytes - *have;
+        ctx->lin_ws_bytes + ctx->pg_ws_bytes - *have;
     if (ctx->ws_limit != 0 && need + other > ctx->ws_limit)
         return fail(ctx, B2A_EOOM, "%s workspace of %zu bytes exceeds the context limit of %zu bytes", what,
                     need + other, ctx->ws_limit);
@@ -356,6 +359,7 @@ B2A_API int b2a_destroy(b2a_context* ctx) {
         if (ctx->blk_ws) cudaFree(ctx->blk_ws);
         if (ctx->rope_tab) cudaFree(ctx->rope_tab);
         if (ctx->lin_ws) cudaFree(ctx->lin_ws);
+        if (ctx->pg_ws) cudaFree(ctx->pg_ws);
     }
     delete ctx;
     return B2A_OK;
@@ -386,7 +390,7 @@ B2A_API int b2a_set_decode_early_start(b2a_context* ctx, int enable) {
 B2A_API int b2a_workspace_bytes(const b2a_context* ctx, size_t* bytes) {
     if (!ctx || !bytes) return B2A_EINVAL;
     *bytes = ctx->dec_ws_bytes + ctx->pf_ws_bytes + ctx->split_ws_bytes + ctx->blk_ws_bytes + ctx->rope_tab_bytes +
-             ctx->lin_ws_bytes;
+             ctx->lin_ws_bytes + ctx->pg_ws_bytes;
     return B2A_OK;
 }
 
@@ -438,6 +442,9 @@ B2A_API int b2a_check_device_status(b2a_context* ctx, void* stream) {
     if (flags & 1) msg += "a ctx_lens entry was outside [0, max_seq); its outputs are NaN. ";
     if (flags & 2) msg += "decode work items exceeded the workspace capacity. ";
     if (flags & 4) msg += "a bf16 input exceeded the fp16 operand range (|x| > 65504). ";
+    if (flags & 16) msg += "a page_table entry that was needed named no page of the pool. ";
+    if (flags & 32) msg += "a k or v value was not finite or beyond the 4-bit cache's range; its group holds NaN. ";
+    if (flags & 64) msg += "a parents entry was outside [-1, n_seq); its row is unchanged. ";
     // a timed-out pipeline is reported as such; the other flags are failed device-side argument checks
     return fail(ctx, (flags & 8) ? B2A_ETIMEOUT : B2A_EDEVICE, "%s", msg.c_str());
 }
@@ -1106,6 +1113,255 @@ B2A_API int b2a_decode_attention_block(b2a_context* ctx, int act_dtype, int cach
     // 3. y = attn W_o^T + residual
     return run_linear(ctx, act_dtype, act_dtype, attn, w_o, nullptr, residual, y, B, hidden, Hq * D, stream,
                       ctx->decode_early_start);
+}
+
+// ----------------------------------------------------------------- paged 4-bit cache
+namespace {
+
+bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
+
+// Fills the cache part of p from the caller's description.
+int check_kv4_cache(b2a_context* ctx, const b2a_kv4_cache* cache, Kv4Params& p) {
+    if (!cache || !cache->pages || !cache->page_table)
+        return fail(ctx, B2A_EINVAL, "the cache, its pages and its page_table must not be null");
+    const int D = cache->head_dim, ps = cache->page_size;
+    if (cache->num_kv_heads <= 0) return fail(ctx, B2A_EINVAL, "numKeyValueHeads must be positive");
+    if (D != 64 && D != 96 && D != 128 && D != 256)
+        return fail(ctx, B2A_ENOTSUP, "the 4-bit cache holds headDim 64, 96, 128 or 256, got %d", D);
+    if (ps <= 0 || ps % 16 != 0 || ps > kMaxPageSize)
+        return fail(ctx, B2A_EINVAL, "page_size %d is not a multiple of 16 in [16, %d]", ps, kMaxPageSize);
+    if (cache->num_pages <= 0 || cache->max_pages <= 0)
+        return fail(ctx, B2A_EINVAL, "num_pages and max_pages must be > 0");
+    if ((int64_t)cache->max_pages * ps > INT32_MAX)
+        return fail(ctx, B2A_EINVAL, "max_pages * page_size exceeds the position range");
+    if (!aligned16(cache->pages)) return fail(ctx, B2A_EINVAL, "the pages must be 16-byte aligned");
+    p.pages = static_cast<uint8_t*>(cache->pages);
+    p.page_table = cache->page_table;
+    p.num_pages = cache->num_pages;
+    p.page_size = ps;
+    p.max_pages = cache->max_pages;
+    p.Hkv = cache->num_kv_heads;
+    p.D = D;
+    p.status = ctx->status;
+    return B2A_OK;
+}
+
+int check_kv4_tokens(b2a_context* ctx, int act_dtype, const int32_t* ctx_lens, const int32_t* new_lens, int B, int T,
+                     int rope_mode, double rope_theta, float norm_eps, Kv4Params& p) {
+    if (act_dtype != B2A_FLOAT16 && act_dtype != B2A_BFLOAT16)
+        return fail(ctx, B2A_ENOTSUP, "the 4-bit cache takes FLOAT16 or BFLOAT16 rows, got %d", act_dtype);
+    if (!ctx_lens) return fail(ctx, B2A_EINVAL, "ctx_lens must not be null");
+    if (B <= 0 || T <= 0) return fail(ctx, B2A_EINVAL, "batch and new tokens must be > 0");
+    if ((int64_t)B * T > (1 << 24)) return fail(ctx, B2A_EINVAL, "batch * new tokens exceeds 2^24");
+    if (rope_mode != B2A_ROPE_NONE && rope_mode != B2A_ROPE_NEOX && rope_mode != B2A_ROPE_GEMMA)
+        return fail(ctx, B2A_EINVAL, "unknown rope mode %d", rope_mode);
+    if (rope_mode != B2A_ROPE_NONE && !(rope_theta > 0.0)) return fail(ctx, B2A_EINVAL, "rope theta must be > 0");
+    if (!(norm_eps >= 0.f)) return fail(ctx, B2A_EINVAL, "norm_eps must not be negative");
+    p.act_dtype = act_dtype;
+    p.ctx_lens = ctx_lens;
+    p.new_lens = new_lens;
+    p.B = B;
+    p.T = T;
+    p.rope_mode = rope_mode;
+    p.norm_eps = norm_eps;
+    if (rope_mode != B2A_ROPE_NONE) inv_freq_table(rope_theta, p.D, p.inv_freq);
+    return B2A_OK;
+}
+
+int check_kv4_new(b2a_context* ctx, const void* k_new, const void* v_new, int64_t kv_stride, void* k_held,
+                  void* v_held, const float* k_norm_w, Kv4Params& p) {
+    if (!k_new || !v_new) return fail(ctx, B2A_EINVAL, "k_new and v_new must not be null");
+    if (!aligned16(k_new) || !aligned16(v_new) || !aligned16(k_held) || !aligned16(v_held))
+        return fail(ctx, B2A_EINVAL, "k_new, v_new, k_held and v_held must be 16-byte aligned");
+    const int64_t row = (int64_t)p.Hkv * p.D;
+    if (kv_stride == 0) kv_stride = row;
+    if (kv_stride < row || kv_stride % 8 != 0)
+        return fail(ctx, B2A_EINVAL, "kv_token_stride must be at least Hkv * D and a multiple of 8");
+    p.k_new = k_new;
+    p.v_new = v_new;
+    p.kv_stride = kv_stride;
+    p.k_held = k_held;
+    p.v_held = v_held;
+    p.k_norm_w = k_norm_w;
+    return B2A_OK;
+}
+
+int check_kv4_query(b2a_context* ctx, const void* q, int64_t q_stride, int Hq, float scale, int window,
+                    const float* q_norm_w, void* o, Kv4Params& p) {
+    if (!q || !o) return fail(ctx, B2A_EINVAL, "q and o must not be null");
+    const int rc = check_heads(ctx, Hq, p.Hkv);
+    if (rc) return rc;
+    if (!aligned16(q) || !aligned16(o)) return fail(ctx, B2A_EINVAL, "q and o must be 16-byte aligned");
+    if (q_stride == 0) q_stride = (int64_t)Hq * p.D;
+    if (q_stride < (int64_t)Hq * p.D || q_stride % 8 != 0)
+        return fail(ctx, B2A_EINVAL, "q_token_stride must be at least Hq * D and a multiple of 8");
+    if ((int64_t)p.B * p.T * Hq > INT32_MAX) return fail(ctx, B2A_EINVAL, "batch * new tokens * heads exceeds 2^31");
+    if (window < 0) return fail(ctx, B2A_EINVAL, "window must not be negative");
+    if (!(scale == scale) || scale <= 0.f) return fail(ctx, B2A_EINVAL, "scale must be a positive number");
+    p.q = q;
+    p.q_stride = q_stride;
+    p.Hq = Hq;
+    p.G = Hq / p.Hkv;
+    p.scale = scale;
+    p.window = window;
+    p.q_norm_w = q_norm_w;
+    p.o = o;
+    return B2A_OK;
+}
+
+int check_pool(b2a_context* ctx, const b2a_page_pool* pool, bool with_pages, PagePoolParams& p) {
+    if (!pool || !pool->page_table || !pool->ref_counts)
+        return fail(ctx, B2A_EINVAL, "the pool, its page_table and its ref_counts must not be null");
+    if (pool->n_seq <= 0 || pool->max_pages <= 0 || pool->num_pages <= 0)
+        return fail(ctx, B2A_EINVAL, "n_seq, max_pages and num_pages must be > 0");
+    if ((int64_t)pool->n_seq * pool->max_pages > INT32_MAX)
+        return fail(ctx, B2A_EINVAL, "the page table exceeds 2^31 entries");
+    if (with_pages) {
+        if (!pool->pages) return fail(ctx, B2A_EINVAL, "the pool's pages must not be null");
+        if (pool->n_layers <= 0 || pool->page_bytes <= 0 || pool->page_bytes % 16 != 0 || !aligned16(pool->pages))
+            return fail(ctx, B2A_EINVAL, "pages need n_layers > 0, 16-byte alignment and a multiple of 16 bytes");
+        if (pool->n_layers > 1 && (pool->layer_stride % 16 != 0 ||
+                                   pool->layer_stride < (int64_t)pool->num_pages * pool->page_bytes))
+            return fail(ctx, B2A_EINVAL, "layer_stride must be a multiple of 16 and at least num_pages * page_bytes");
+    }
+    p.page_table = pool->page_table;
+    p.n_seq = pool->n_seq;
+    p.max_pages = pool->max_pages;
+    p.ref_counts = pool->ref_counts;
+    p.num_pages = pool->num_pages;
+    p.pages = static_cast<uint8_t*>(pool->pages);
+    p.n_layers = pool->n_layers;
+    p.layer_stride = pool->layer_stride;
+    p.page_bytes = pool->page_bytes;
+    p.status = ctx->status;
+    return B2A_OK;
+}
+
+int pages_workspace(b2a_context* ctx, int num_pages, int** out) {
+    const int rc = ensure_buffer(ctx, &ctx->pg_ws, &ctx->pg_ws_bytes, pages_workspace_ints(num_pages) * sizeof(int),
+                                 "page operations");
+    *out = static_cast<int*>(ctx->pg_ws);
+    return rc;
+}
+
+}  // namespace
+
+B2A_API size_t b2a_kv4_page_bytes(int num_kv_heads, int head_dim, int page_size) {
+    if (num_kv_heads <= 0 || page_size <= 0 || page_size % 16 != 0 || page_size > kMaxPageSize) return 0;
+    if (head_dim != 64 && head_dim != 96 && head_dim != 128 && head_dim != 256) return 0;
+    return (size_t)num_kv_heads * page_size / 4 * 5 * head_dim;
+}
+
+B2A_API int b2a_kv4_append(b2a_context* ctx, const b2a_kv4_cache* cache, int act_dtype, const void* k_new,
+                           const void* v_new, int64_t kv_token_stride, const int32_t* ctx_lens,
+                           const int32_t* new_lens, int B, int T, int rope_mode, double rope_theta,
+                           const float* k_norm_w, float norm_eps, void* k_held, void* v_held, void* stream) {
+    if (!ctx) return B2A_EINVAL;
+    Kv4Params p{};
+    int rc = check_kv4_cache(ctx, cache, p);
+    if (!rc) rc = check_kv4_tokens(ctx, act_dtype, ctx_lens, new_lens, B, T, rope_mode, rope_theta, norm_eps, p);
+    if (!rc) rc = check_kv4_new(ctx, k_new, v_new, kv_token_stride, k_held, v_held, k_norm_w, p);
+    if (rc) return rc;
+    DeviceGuard guard(ctx->device);
+    const cudaError_t e = launch_kv4_append(p, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "cache append launch");
+    return B2A_OK;
+}
+
+B2A_API int b2a_kv4_attention(b2a_context* ctx, const b2a_kv4_cache* cache, int act_dtype, const void* q,
+                              int64_t q_token_stride, const int32_t* ctx_lens, const int32_t* new_lens, int B, int T,
+                              int Hq, float scale, int rope_mode, double rope_theta, int window,
+                              const float* q_norm_w, float norm_eps, void* o, void* stream) {
+    if (!ctx) return B2A_EINVAL;
+    Kv4Params p{};
+    int rc = check_kv4_cache(ctx, cache, p);
+    if (!rc) rc = check_kv4_tokens(ctx, act_dtype, ctx_lens, new_lens, B, T, rope_mode, rope_theta, norm_eps, p);
+    if (!rc) rc = check_kv4_query(ctx, q, q_token_stride, Hq, scale, window, q_norm_w, o, p);
+    if (rc) return rc;
+    DeviceGuard guard(ctx->device);
+    const cudaError_t e = launch_kv4_attn(p, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "cache attention launch");
+    return B2A_OK;
+}
+
+B2A_API int b2a_kv4_decode(b2a_context* ctx, const b2a_kv4_cache* cache, int act_dtype, const void* q,
+                           int64_t q_token_stride, const void* k_new, const void* v_new, int64_t kv_token_stride,
+                           const int32_t* ctx_lens, const int32_t* new_lens, int B, int T, int Hq, float scale,
+                           int rope_mode, double rope_theta, int window, const float* q_norm_w, const float* k_norm_w,
+                           float norm_eps, void* k_held, void* v_held, void* o, void* stream) {
+    if (!ctx) return B2A_EINVAL;
+    Kv4Params p{};
+    int rc = check_kv4_cache(ctx, cache, p);
+    if (!rc) rc = check_kv4_tokens(ctx, act_dtype, ctx_lens, new_lens, B, T, rope_mode, rope_theta, norm_eps, p);
+    if (!rc) rc = check_kv4_new(ctx, k_new, v_new, kv_token_stride, k_held, v_held, k_norm_w, p);
+    if (!rc) rc = check_kv4_query(ctx, q, q_token_stride, Hq, scale, window, q_norm_w, o, p);
+    if (rc) return rc;
+    if ((q_norm_w == nullptr) != (k_norm_w == nullptr))
+        return fail(ctx, B2A_EINVAL, "q_norm_w and k_norm_w must be given together");
+    DeviceGuard guard(ctx->device);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    cudaError_t e = launch_kv4_append(p, s);
+    if (e == cudaSuccess) e = launch_kv4_attn(p, s);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "cache decode launch");
+    return B2A_OK;
+}
+
+B2A_API int b2a_pages_fork(b2a_context* ctx, const b2a_page_pool* pool, const int32_t* parents, void* stream) {
+    if (!ctx) return B2A_EINVAL;
+    PagePoolParams p{};
+    const int rc = check_pool(ctx, pool, false, p);
+    if (rc) return rc;
+    if (!parents) return fail(ctx, B2A_EINVAL, "parents must not be null");
+    if (p.n_seq > kMaxForkRows) return fail(ctx, B2A_ENOTSUP, "fork takes at most %d rows", kMaxForkRows);
+    DeviceGuard guard(ctx->device);
+    const cudaError_t e = launch_pages_fork(p, parents, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "page fork launch");
+    return B2A_OK;
+}
+
+B2A_API int b2a_pages_free(b2a_context* ctx, const b2a_page_pool* pool, const int32_t* keep_from,
+                           const int32_t* keep_to, int page_size, void* stream) {
+    if (!ctx) return B2A_EINVAL;
+    PagePoolParams p{};
+    const int rc = check_pool(ctx, pool, false, p);
+    if (rc) return rc;
+    if (!keep_to) return fail(ctx, B2A_EINVAL, "keep_to must not be null");
+    if (page_size <= 0) return fail(ctx, B2A_EINVAL, "page_size must be > 0");
+    DeviceGuard guard(ctx->device);
+    const cudaError_t e = launch_pages_free(p, keep_from, keep_to, page_size, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "page free launch");
+    return B2A_OK;
+}
+
+B2A_API int b2a_pages_reserve(b2a_context* ctx, const b2a_page_pool* pool, const int32_t* ctx_lens,
+                              const int32_t* new_lens, int page_size, int32_t* counts, void* stream) {
+    if (!ctx) return B2A_EINVAL;
+    PagePoolParams p{};
+    int rc = check_pool(ctx, pool, true, p);
+    if (rc) return rc;
+    if (!ctx_lens || !new_lens || !counts) return fail(ctx, B2A_EINVAL, "ctx_lens, new_lens and counts must not be null");
+    if (page_size <= 0) return fail(ctx, B2A_EINVAL, "page_size must be > 0");
+    DeviceGuard guard(ctx->device);
+    int* ws = nullptr;
+    if ((rc = pages_workspace(ctx, p.num_pages, &ws))) return rc;
+    const cudaError_t e = launch_pages_reserve(p, ctx_lens, new_lens, page_size, counts, ws, ctx->sm_count,
+                                               static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "page reserve launch");
+    return B2A_OK;
+}
+
+B2A_API int b2a_pages_compact(b2a_context* ctx, const b2a_page_pool* pool, int32_t* counts, void* stream) {
+    if (!ctx) return B2A_EINVAL;
+    PagePoolParams p{};
+    int rc = check_pool(ctx, pool, true, p);
+    if (rc) return rc;
+    if (!counts) return fail(ctx, B2A_EINVAL, "counts must not be null");
+    DeviceGuard guard(ctx->device);
+    int* ws = nullptr;
+    if ((rc = pages_workspace(ctx, p.num_pages, &ws))) return rc;
+    const cudaError_t e = launch_pages_compact(p, counts, ws, ctx->sm_count, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "page compact launch");
+    return B2A_OK;
 }
 
 // ----------------------------------------------------------------- sharding

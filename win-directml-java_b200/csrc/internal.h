@@ -212,6 +212,55 @@ bool linear_tc_supported(int in_dtype, int K, int64_t ldx, int64_t ldw, const vo
 int linear_split_plan(int M, int N, int K, int sm_count, size_t* acc_bytes, size_t* counter_ints);
 cudaError_t launch_linear_tc(const LinearArgs& a, int* status, cudaStream_t stream);
 
+// Attention over, and appending to, the paged 4-bit KV cache (layout: kv4.cuh).
+struct Kv4Params {
+    const void* q;       // [B][T] token rows of Hq * D elements, q_stride elements apart
+    const void* k_new;   // [B][T] token rows of Hkv * D elements, kv_stride elements apart
+    const void* v_new;
+    int act_dtype;       // element type of q, k_new, v_new, o and the held rows (FLOAT16 / BFLOAT16)
+    int64_t q_stride, kv_stride;
+    uint8_t* pages;      // [num_pages][Hkv][page_size / 16][20 D] bytes
+    const int* page_table;  // device [B][max_pages], -1: none
+    int num_pages, page_size, max_pages;
+    const int* ctx_lens;    // device [B]: tokens cached before the new ones
+    const int* new_lens;    // device [B] or NULL (T for every sequence)
+    int B, T, Hq, Hkv, G, D;
+    int window;
+    int rope_mode;
+    float scale;
+    const float* q_norm_w;
+    const float* k_norm_w;
+    float norm_eps;
+    void* o;             // [B][T][Hq][D]
+    void* k_held;        // [B][T][Hkv][D] or NULL
+    void* v_held;
+    int* status;         // bits 0 (lengths), 4 (page table entry), 5 (value outside the cache's range)
+    double inv_freq[kMaxHeadDim / 2];
+};
+constexpr int kMaxPageSize = 1024;
+cudaError_t launch_kv4_append(const Kv4Params& p, cudaStream_t stream);
+cudaError_t launch_kv4_attn(const Kv4Params& p, cudaStream_t stream);
+
+// The page table, reference counts and pages of a paged cache (pages.cu).
+struct PagePoolParams {
+    int* page_table;  // device [n_seq][max_pages]
+    int n_seq, max_pages;
+    int* ref_counts;  // device [num_pages]
+    int num_pages;
+    uint8_t* pages;   // [n_layers] x layer_stride bytes, each [num_pages][page_bytes]
+    int n_layers;
+    int64_t layer_stride, page_bytes;  // multiples of 16
+    int* status;      // bits 0 (lengths), 4 (page table entry), 6 (parents entry)
+};
+constexpr int kMaxForkRows = 56 * 1024;  // rows of one table column in shared memory
+size_t pages_workspace_ints(int num_pages);
+cudaError_t launch_pages_free(const PagePoolParams& p, const int* keep_from, const int* keep_to, int page_size,
+                              cudaStream_t stream);
+cudaError_t launch_pages_fork(const PagePoolParams& p, const int* parents, cudaStream_t stream);
+cudaError_t launch_pages_reserve(const PagePoolParams& p, const int* ctx_lens, const int* new_lens, int page_size,
+                                 int* counts, int* ws, int sm_count, cudaStream_t stream);
+cudaError_t launch_pages_compact(const PagePoolParams& p, int* counts, int* ws, int sm_count, cudaStream_t stream);
+
 // Sets the message b2a_last_error(NULL, ...) returns on this thread.
 void set_thread_error(const char* msg);
 
