@@ -57,6 +57,10 @@ struct b2a_context {
     // test hook (b2a_test_inject_wait_timeout): the next tcgen05 attention launch
     // leaves one K/V copy unissued
     bool inject_wait_timeout = false;
+    // paged 4-bit cache: [merge counters][partial slots][q operands][q sums]
+    void* kv4_ws = nullptr;
+    size_t kv4_ws_bytes = 0;
+    size_t kv4_counter_bytes = 0;
     // paged cache: the page operations' lists
     void* pg_ws = nullptr;
     size_t pg_ws_bytes = 0;
@@ -108,7 +112,7 @@ int ensure_buffer(b2a_context* ctx, void** buf, size_t* have, size_t need, const
     if (*have >= need) return B2A_OK;
     const size_t other =
         ctx->dec_ws_bytes + ctx->pf_ws_bytes + ctx->split_ws_bytes + ctx->blk_ws_bytes + ctx->rope_tab_bytes +
-        ctx->lin_ws_bytes + ctx->pg_ws_bytes - *have;
+        ctx->lin_ws_bytes + ctx->pg_ws_bytes + ctx->kv4_ws_bytes - *have;
     if (ctx->ws_limit != 0 && need + other > ctx->ws_limit)
         return fail(ctx, B2A_EOOM, "%s workspace of %zu bytes exceeds the context limit of %zu bytes", what,
                     need + other, ctx->ws_limit);
@@ -360,6 +364,7 @@ B2A_API int b2a_destroy(b2a_context* ctx) {
         if (ctx->rope_tab) cudaFree(ctx->rope_tab);
         if (ctx->lin_ws) cudaFree(ctx->lin_ws);
         if (ctx->pg_ws) cudaFree(ctx->pg_ws);
+        if (ctx->kv4_ws) cudaFree(ctx->kv4_ws);
     }
     delete ctx;
     return B2A_OK;
@@ -390,7 +395,7 @@ B2A_API int b2a_set_decode_early_start(b2a_context* ctx, int enable) {
 B2A_API int b2a_workspace_bytes(const b2a_context* ctx, size_t* bytes) {
     if (!ctx || !bytes) return B2A_EINVAL;
     *bytes = ctx->dec_ws_bytes + ctx->pf_ws_bytes + ctx->split_ws_bytes + ctx->blk_ws_bytes + ctx->rope_tab_bytes +
-             ctx->lin_ws_bytes + ctx->pg_ws_bytes;
+             ctx->lin_ws_bytes + ctx->pg_ws_bytes + ctx->kv4_ws_bytes;
     return B2A_OK;
 }
 
@@ -1209,6 +1214,43 @@ int check_kv4_query(b2a_context* ctx, const void* q, int64_t q_stride, int Hq, f
     return B2A_OK;
 }
 
+// The preparation (q's operands, and the append where p has new rows), then the attention, at most
+// kKv4MaxBatch sequences and 2^31 blocks of the split's stream at a time.
+int run_kv4_attention(b2a_context* ctx, Kv4Params& p, cudaStream_t stream) {
+    DeviceGuard guard(ctx->device);
+    auto r256 = [](size_t x) { return (x + 255) / 256 * 256; };
+    const int64_t seq_blocks = (int64_t)p.max_pages * p.page_size / 16 + 1 + kKv4GapBlocksMax;
+    const int per_launch = (int)std::max<int64_t>(1, std::min<int64_t>(kKv4MaxBatch, INT32_MAX / seq_blocks));
+    size_t partial_bytes = 0, units_per_seq = 0, counter_bytes = 0;
+    kv4_attn_workspace(p, ctx->device, &partial_bytes, &units_per_seq);
+    if (partial_bytes == 0) return fail(ctx, B2A_ECUDA, "no attention kernel for this device");
+    const size_t counters = (size_t)std::min(p.B, per_launch) * units_per_seq;
+    const size_t part = r256(partial_bytes), frag = r256(kv4_frag_bytes(p) * p.B), sums = r256(kv4_sums_bytes(p) * p.B);
+    const int rc = ensure_counted_buffer(ctx, &ctx->kv4_ws, &ctx->kv4_ws_bytes, &ctx->kv4_counter_bytes, counters,
+                                         part + frag + sums, "4-bit cache attention", stream, false, &counter_bytes);
+    if (rc) return rc;
+    char* base = static_cast<char*>(ctx->kv4_ws);
+    p.counters = reinterpret_cast<int*>(base);
+    p.partials = reinterpret_cast<float*>(base + counter_bytes);
+    p.q_frag = reinterpret_cast<uint4*>(base + counter_bytes + part);
+    p.q_sums = reinterpret_cast<float*>(base + counter_bytes + part + frag);
+    cudaError_t e = launch_kv4_prepare(p, stream);
+    const int B = p.B;
+    for (int b0 = 0; e == cudaSuccess && b0 < B; b0 += per_launch) {
+        Kv4Params s = p;
+        s.B = std::min(per_launch, B - b0);
+        s.page_table += (int64_t)b0 * p.max_pages;
+        s.ctx_lens += b0;
+        if (s.new_lens) s.new_lens += b0;
+        s.o = static_cast<char*>(p.o) + (int64_t)b0 * p.T * p.Hq * p.D * 2;
+        s.q_frag = reinterpret_cast<uint4*>(reinterpret_cast<char*>(p.q_frag) + kv4_frag_bytes(p) * b0);
+        s.q_sums = reinterpret_cast<float*>(reinterpret_cast<char*>(p.q_sums) + kv4_sums_bytes(p) * b0);
+        e = launch_kv4_attn(s, ctx->device, stream);
+    }
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "4-bit cache attention launch");
+    return B2A_OK;
+}
+
 int check_pool(b2a_context* ctx, const b2a_page_pool* pool, bool with_pages, PagePoolParams& p) {
     if (!pool || !pool->page_table || !pool->ref_counts)
         return fail(ctx, B2A_EINVAL, "the pool, its page_table and its ref_counts must not be null");
@@ -1263,7 +1305,7 @@ B2A_API int b2a_kv4_append(b2a_context* ctx, const b2a_kv4_cache* cache, int act
     if (!rc) rc = check_kv4_new(ctx, k_new, v_new, kv_token_stride, k_held, v_held, k_norm_w, p);
     if (rc) return rc;
     DeviceGuard guard(ctx->device);
-    const cudaError_t e = launch_kv4_append(p, static_cast<cudaStream_t>(stream));
+    const cudaError_t e = launch_kv4_prepare(p, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_fail(ctx, e, "cache append launch");
     return B2A_OK;
 }
@@ -1278,10 +1320,7 @@ B2A_API int b2a_kv4_attention(b2a_context* ctx, const b2a_kv4_cache* cache, int 
     if (!rc) rc = check_kv4_tokens(ctx, act_dtype, ctx_lens, new_lens, B, T, rope_mode, rope_theta, norm_eps, p);
     if (!rc) rc = check_kv4_query(ctx, q, q_token_stride, Hq, scale, window, q_norm_w, o, p);
     if (rc) return rc;
-    DeviceGuard guard(ctx->device);
-    const cudaError_t e = launch_kv4_attn(p, static_cast<cudaStream_t>(stream));
-    if (e != cudaSuccess) return cuda_fail(ctx, e, "cache attention launch");
-    return B2A_OK;
+    return run_kv4_attention(ctx, p, static_cast<cudaStream_t>(stream));
 }
 
 B2A_API int b2a_kv4_decode(b2a_context* ctx, const b2a_kv4_cache* cache, int act_dtype, const void* q,
@@ -1298,12 +1337,7 @@ B2A_API int b2a_kv4_decode(b2a_context* ctx, const b2a_kv4_cache* cache, int act
     if (rc) return rc;
     if ((q_norm_w == nullptr) != (k_norm_w == nullptr))
         return fail(ctx, B2A_EINVAL, "q_norm_w and k_norm_w must be given together");
-    DeviceGuard guard(ctx->device);
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    cudaError_t e = launch_kv4_append(p, s);
-    if (e == cudaSuccess) e = launch_kv4_attn(p, s);
-    if (e != cudaSuccess) return cuda_fail(ctx, e, "cache decode launch");
-    return B2A_OK;
+    return run_kv4_attention(ctx, p, static_cast<cudaStream_t>(stream));
 }
 
 B2A_API int b2a_pages_fork(b2a_context* ctx, const b2a_page_pool* pool, const int32_t* parents, void* stream) {

@@ -234,12 +234,25 @@ struct Kv4Params {
     void* o;             // [B][T][Hq][D]
     void* k_held;        // [B][T][Hkv][D] or NULL
     void* v_held;
-    int* status;         // bits 0 (lengths), 4 (page table entry), 5 (value outside the cache's range)
+    int* status;         // bits 0 (lengths), 3 (wait), 4 (page table entry), 5 (value outside the cache's range)
+    // workspace: the queries as MMA operands with their sums (kv4_append.cu), the merge counters
+    // (zero between launches) and partial slots of the attention kernel
+    uint4* q_frag;
+    float* q_sums;
+    int* counters;
+    float* partials;
     double inv_freq[kMaxHeadDim / 2];
 };
 constexpr int kMaxPageSize = 1024;
-cudaError_t launch_kv4_append(const Kv4Params& p, cudaStream_t stream);
-cudaError_t launch_kv4_attn(const Kv4Params& p, cudaStream_t stream);
+constexpr int kKv4MaxBatch = 2048;      // sequences of one attention launch
+constexpr int kKv4GapBlocksMax = 16;    // largest per-unit allowance of the attention's split, in blocks
+// Appends k_new / v_new where given and lays out q where given.
+cudaError_t launch_kv4_prepare(const Kv4Params& p, cudaStream_t stream);
+size_t kv4_frag_bytes(const Kv4Params& p);  // per sequence
+size_t kv4_sums_bytes(const Kv4Params& p);  // per sequence
+void kv4_attn_workspace(const Kv4Params& p, int device, size_t* partial_bytes, size_t* units_per_seq);
+// Directly behind launch_kv4_prepare on the stream: it starts before that kernel has ended.
+cudaError_t launch_kv4_attn(const Kv4Params& p, int device, cudaStream_t stream);
 
 // The page table, reference counts and pages of a paged cache (pages.cu).
 struct PagePoolParams {
