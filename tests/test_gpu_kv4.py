@@ -363,3 +363,38 @@ def test_refusals(ctx):
         b200attn.kv4_append(ctx, z, z, torch.zeros(4, 2, 16 * 40, dtype=torch.uint8, device="cuda"), t["table"], t["ctx"])
     assert ei.value.status == b200attn.B2A_ENOTSUP
     ctx.check_device_status()
+
+
+@pytest.mark.parametrize("D,Hq,dtype", [(64, 4, oracle.F16), (64, 7, oracle.F16), (96, 5, oracle.BF16), (128, 12, oracle.BF16),
+                                        (256, 4, oracle.F16), (256, 6, oracle.F16), (256, 3, oracle.BF16)])
+def test_a_key_held_as_nan_reaches_only_the_rows_that_see_it(ctx, D, Hq, dtype):
+    """A value group or a key group that is held as NaN: the rows before it are untouched; the rows that see it
+    are NaN, in that group alone (value) or whole (key); with a window it leaves sight again."""
+    import torch
+    import b200attn
+    for which, window in (("v", 0), ("k", 0), ("v", 20), ("k", 20)):
+        c = Case(ctx=[45, 8], T=30, Hq=Hq, Hkv=1, D=D, rope=None, dtype=dtype, window=window, seed=D + Hq)
+        x = c.k if which == "k" else c.v
+        x[0, 4, 0, 33] = np.nan
+        t = c.device()
+        b200attn.kv4_decode(ctx, t["q"], t["k"], t["v"], t["pages"], t["table"], t["ctx"], t["o"], c.scale,
+                            window=window, **c.more())
+        with pytest.raises(b200attn.B200RuntimeException):
+            ctx.check_device_status()
+        x[0, 4, 0, 32:64] = 0.0  # the model without it, for the rows that do not see it
+        x[0, 4, 0, 33] = 0.0
+        o, tol, _, _ = c.expect()
+        got = to_np(t["o"])
+        sees = np.zeros((2, 30), bool)
+        sees[0, 4:(24 if window else 30)] = True
+        bad = np.zeros(got.shape, bool)
+        bad[sees] = True
+        if which == "v":
+            bad[..., :32] = False
+            bad[..., 64:] = False
+        np.testing.assert_array_equal(np.isnan(got), bad, err_msg=f"{which} window {window}")
+        if which == "v":  # other groups of the rows that see it are as if it were a number
+            ok = ~bad
+        else:
+            ok = np.broadcast_to(~sees[..., None, None], got.shape)
+        assert np.all(np.abs(got - o)[ok] <= tol[ok])

@@ -398,66 +398,114 @@ def kv4_page_bytes(num_kv_heads: int, head_dim: int, page_size: int) -> int:
     return n
 
 
-def _int32(t, name, shape, optional=False):
-    """A device int32 tensor of that shape, as a pointer."""
-    if t is None:
-        if optional:
-            return None
-        raise ValueError(f"{name} must not be None")
-    if str(t.dtype) != "torch.int32" or tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} must be int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
-    return _ptr(t)
+# These calls are short on the device, so the checks are written for few Python operations.
+_rt = None  # (torch.int32, torch.uint8, torch.float32, {dtype: code}, current device, raw current stream)
+
+
+def _runtime():
+    global _rt
+    if _rt is None:
+        import torch
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+            (lambda device: torch.cuda.current_stream(device).cuda_stream)
+        _rt = (torch.int32, torch.uint8, torch.float32,
+               {torch.float32: FLOAT32, torch.float16: FLOAT16, torch.bfloat16: BFLOAT16},
+               torch.cuda.current_device, raw)
+    return _rt
+
+
+def _raw_stream(stream):
+    if stream is not None:
+        return stream.cuda_stream
+    rt = _rt or _runtime()
+    return rt[5](rt[4]())
+
+
+def _address(t, name):
+    if not t.is_cuda:
+        raise ValueError("tensors must live on the CUDA device (GpuBuffer); got a host tensor")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous (row-major TensorLayout)")
+    return t.data_ptr()
+
+
+def _int32(t, name, shape):
+    """Address of a device int32 tensor of that shape."""
+    if t is None or t.dtype is not (_rt or _runtime())[0] or t.shape != shape:
+        raise ValueError(f"{name} must be int32 {list(shape)}, got "
+                         f"{None if t is None else f'{t.dtype} {list(t.shape)}'}")
+    return _address(t, name)
 
 
 def _token_rows(t, name, shape):
-    """Pointer and token stride of [B,T,H,D] rows: heads side by side, one distance from each token to
+    """Address and token stride of [B,T,H,D] rows: heads side by side, one distance from each token to
     the next (a slice of a fused [Q|K|V] projection is one)."""
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} expected shape {tuple(shape)}, got {tuple(t.shape)}")
     if not t.is_cuda:
         raise ValueError("tensors must live on the CUDA device (GpuBuffer); got a host tensor")
     B, T, H, D = shape
+    if t.is_contiguous():
+        return t.data_ptr(), H * D
     sb, st, sh, sd = t.stride()
     step = st if T > 1 else sb if B > 1 else H * D
     if sd != 1 or (H > 1 and sh != D) or (T > 1 and B > 1 and sb != T * st):
         raise ValueError(f"{name} must hold its tokens at one distance and its heads side by side, "
                          f"got strides {t.stride()}")
-    return ctypes.c_void_p(t.data_ptr()), step
+    return t.data_ptr(), step
 
 
 def _kv4_cache(pages, page_table, B, D, num_kv_heads=None):
-    import torch
-    if pages.dtype != torch.uint8 or pages.dim() != 3:
+    if pages.dtype is not (_rt or _runtime())[1] or pages.dim() != 3:
         raise ValueError("pages must be uint8 [num_pages, num_kv_heads, page_size * head_dim * 5 // 4]")
-    if num_kv_heads is not None and pages.shape[1] != num_kv_heads:
-        raise ValueError(f"pages hold {pages.shape[1]} kv heads, the new rows {num_kv_heads}")
-    page_size, rest = divmod(pages.shape[2] * 4, D * 5)
+    num_pages, heads, row = pages.shape
+    if num_kv_heads is not None and heads != num_kv_heads:
+        raise ValueError(f"pages hold {heads} kv heads, the new rows {num_kv_heads}")
+    page_size, rest = divmod(row * 4, D * 5)
     if rest or page_size == 0:
-        raise ValueError(f"a page of {pages.shape[2]} bytes per kv head holds no whole rows of head_dim {D}")
+        raise ValueError(f"a page of {row} bytes per kv head holds no whole rows of head_dim {D}")
     if page_table.dim() != 2:
         raise ValueError("page_table must be int32 [B, max_pages]")
-    table = _int32(page_table, "page_table", (B, page_table.shape[1]))
-    return _Kv4Cache(_ptr(pages), table, pages.shape[0], page_size, page_table.shape[1], pages.shape[1], D)
+    max_pages = page_table.shape[1]
+    return _Kv4Cache(_address(pages, "pages"), _int32(page_table, "page_table", (B, max_pages)), num_pages, page_size,
+                     max_pages, heads, D)
 
 
-def _same_dtype(first, **others):
-    for name, t in others.items():
-        if t is not None and t.dtype != first.dtype:
-            raise ValueError(f"{name} must have element type {first.dtype}, got {t.dtype}")
+def _kv4_dtype(t):
+    code = (_rt or _runtime())[3].get(t.dtype)
+    if code is None:
+        raise ValueError(f"unsupported element type {t.dtype}")
+    return code
+
+
+def _row_like(t, name, first, shape):
+    """Address of a contiguous output or input of first's element type, or None."""
+    if t is None:
+        return None
+    if t.dtype is not first.dtype:
+        raise ValueError(f"{name} must have element type {first.dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name} expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    return _address(t, name)
 
 
 def _norm_w(t, name, D):
-    if t is not None and (str(t.dtype) != "torch.float32" or t.numel() != D):
-        raise ValueError(f"{name} must be float32 [{D}]")
-    return _ptr(t)
-
-
-def _dense(t, name, shape, optional=False):
-    if t is None and optional:
+    if t is None:
         return None
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} expected shape {tuple(shape)}, got {tuple(t.shape)}")
-    return _ptr(t)
+    if t.dtype is not (_rt or _runtime())[2] or t.numel() != D:
+        raise ValueError(f"{name} must be float32 [{D}]")
+    return _address(t, name)
+
+
+def _kv_rows(k_new, v_new, first, shape):
+    """Addresses of the new k and v rows and their token stride."""
+    k, step = _token_rows(k_new, "k_new", shape)
+    v, v_step = _token_rows(v_new, "v_new", shape)
+    if v_step != step:
+        raise ValueError("k_new and v_new must have one token stride")
+    if k_new.dtype is not first.dtype or v_new.dtype is not first.dtype:
+        raise ValueError(f"k_new and v_new must have element type {first.dtype}, got {k_new.dtype}, {v_new.dtype}")
+    return k, v, step
 
 
 def kv4_append(ctx: Context, k_new, v_new, pages, page_table, ctx_lens, *, new_lens=None, rope_mode: int = ROPE_NEOX,
@@ -467,18 +515,17 @@ def kv4_append(ctx: Context, k_new, v_new, pages, page_table, ctx_lens, *, new_l
     cache: key norm, RoPE at ctx_lens[b] + t, quantisation, store.  pages: uint8 [num_pages, Hkv,
     page_size * D * 5 // 4]; page_table int32 [B, max_pages]; ctx_lens, new_lens int32 [B] (new_lens: how many
     of the T tokens exist).  k_held / v_held [B,T,Hkv,D] receive the rows as the cache holds them."""
-    B, T, Hkv, D = k_new.shape
+    shape = k_new.shape
+    B, T, Hkv, D = shape
     cache = _kv4_cache(pages, page_table, B, D, Hkv)
-    k, step = _token_rows(k_new, "k_new", k_new.shape)
-    v, v_step = _token_rows(v_new, "v_new", k_new.shape)
-    if v_step != step:
-        raise ValueError("k_new and v_new must have one token stride")
-    _same_dtype(k_new, v_new=v_new, k_held=k_held, v_held=v_held)
-    ctx.check(lib().b2a_kv4_append(
-        ctx.handle, ctypes.byref(cache), _dtype_code(k_new), k, v, step, _int32(ctx_lens, "ctx_lens", (B,)),
-        _int32(new_lens, "new_lens", (B,), True), B, T, rope_mode, rope_theta, _norm_w(k_norm_w, "k_norm_w", D),
-        norm_eps, _dense(k_held, "k_held", k_new.shape, True), _dense(v_held, "v_held", k_new.shape, True),
-        _stream(stream)))
+    k, v, step = _kv_rows(k_new, v_new, k_new, shape)
+    rc = (_lib or lib()).b2a_kv4_append(
+        ctx._h, cache, _kv4_dtype(k_new), k, v, step, _int32(ctx_lens, "ctx_lens", (B,)),
+        None if new_lens is None else _int32(new_lens, "new_lens", (B,)), B, T, rope_mode, rope_theta,
+        _norm_w(k_norm_w, "k_norm_w", D), norm_eps, _row_like(k_held, "k_held", k_new, shape),
+        _row_like(v_held, "v_held", k_new, shape), _raw_stream(stream))
+    if rc:
+        ctx.check(rc)
 
 
 def kv4_attention(ctx: Context, q, pages, page_table, ctx_lens, o, scale: float, *, new_lens=None,
@@ -486,14 +533,16 @@ def kv4_attention(ctx: Context, q, pages, page_table, ctx_lens, o, scale: float,
                   norm_eps: float = 1e-6, stream=None):
     """Attention of tokens q [B,T,Hq,D] at positions ctx_lens[b] + t over the paged 4-bit cache, which must
     hold those positions already; o [B,T,Hq,D]; rows t >= new_lens[b] give zeros."""
-    B, T, Hq, D = q.shape
+    shape = q.shape
+    B, T, Hq, D = shape
     cache = _kv4_cache(pages, page_table, B, D)
-    qp, q_step = _token_rows(q, "q", q.shape)
-    _same_dtype(q, o=o)
-    ctx.check(lib().b2a_kv4_attention(
-        ctx.handle, ctypes.byref(cache), _dtype_code(q), qp, q_step, _int32(ctx_lens, "ctx_lens", (B,)),
-        _int32(new_lens, "new_lens", (B,), True), B, T, Hq, scale, rope_mode, rope_theta, window,
-        _norm_w(q_norm_w, "q_norm_w", D), norm_eps, _dense(o, "o", q.shape), _stream(stream)))
+    qp, q_step = _token_rows(q, "q", shape)
+    rc = (_lib or lib()).b2a_kv4_attention(
+        ctx._h, cache, _kv4_dtype(q), qp, q_step, _int32(ctx_lens, "ctx_lens", (B,)),
+        None if new_lens is None else _int32(new_lens, "new_lens", (B,)), B, T, Hq, scale, rope_mode, rope_theta,
+        window, _norm_w(q_norm_w, "q_norm_w", D), norm_eps, _row_like(o, "o", q, shape), _raw_stream(stream))
+    if rc:
+        ctx.check(rc)
     return o
 
 
@@ -502,21 +551,21 @@ def kv4_decode(ctx: Context, q, k_new, v_new, pages, page_table, ctx_lens, o, sc
                norm_eps: float = 1e-6, k_held=None, v_held=None, stream=None):
     """kv4_append of k_new / v_new [B,T,Hkv,D], then kv4_attention of q [B,T,Hq,D]: a decode step (T = 1), the
     verification of a draft, or a chunk of a prompt on a cached prefix."""
-    B, T, Hq, D = q.shape
+    shape = q.shape
+    B, T, Hq, D = shape
     Hkv = k_new.shape[2] if k_new.dim() == 4 else 0
+    kv_shape = (B, T, Hkv, D)
     cache = _kv4_cache(pages, page_table, B, D, Hkv)
-    qp, q_step = _token_rows(q, "q", q.shape)
-    k, step = _token_rows(k_new, "k_new", (B, T, Hkv, D))
-    v, v_step = _token_rows(v_new, "v_new", (B, T, Hkv, D))
-    if v_step != step:
-        raise ValueError("k_new and v_new must have one token stride")
-    _same_dtype(q, k_new=k_new, v_new=v_new, o=o, k_held=k_held, v_held=v_held)
-    ctx.check(lib().b2a_kv4_decode(
-        ctx.handle, ctypes.byref(cache), _dtype_code(q), qp, q_step, k, v, step, _int32(ctx_lens, "ctx_lens", (B,)),
-        _int32(new_lens, "new_lens", (B,), True), B, T, Hq, scale, rope_mode, rope_theta, window,
-        _norm_w(q_norm_w, "q_norm_w", D), _norm_w(k_norm_w, "k_norm_w", D), norm_eps,
-        _dense(k_held, "k_held", k_new.shape, True), _dense(v_held, "v_held", k_new.shape, True),
-        _dense(o, "o", q.shape), _stream(stream)))
+    qp, q_step = _token_rows(q, "q", shape)
+    k, v, step = _kv_rows(k_new, v_new, q, kv_shape)
+    rc = (_lib or lib()).b2a_kv4_decode(
+        ctx._h, cache, _kv4_dtype(q), qp, q_step, k, v, step, _int32(ctx_lens, "ctx_lens", (B,)),
+        None if new_lens is None else _int32(new_lens, "new_lens", (B,)), B, T, Hq, scale, rope_mode, rope_theta,
+        window, _norm_w(q_norm_w, "q_norm_w", D), _norm_w(k_norm_w, "k_norm_w", D), norm_eps,
+        _row_like(k_held, "k_held", q, kv_shape), _row_like(v_held, "v_held", q, kv_shape),
+        _row_like(o, "o", q, shape), _raw_stream(stream))
+    if rc:
+        ctx.check(rc)
     return o
 
 
@@ -524,30 +573,35 @@ def _page_pool(page_table, ref_counts, pages=None):
     if page_table.dim() != 2 or ref_counts.dim() != 1:
         raise ValueError("page_table must be int32 [n_seq, max_pages], ref_counts int32 [num_pages]")
     n_seq, max_pages = page_table.shape
-    pool = _PagePool(_int32(page_table, "page_table", page_table.shape),
-                     _int32(ref_counts, "ref_counts", ref_counts.shape), None, 0, 0, n_seq, max_pages,
-                     ref_counts.shape[0], 0)
-    if pages is not None:
-        if pages.dim() < 2 or pages.shape[1] != ref_counts.shape[0]:
-            raise ValueError(f"pages must be [n_layers, {ref_counts.shape[0]}, ...], got {list(pages.shape)}")
-        pool.pages, pool.n_layers = _ptr(pages), pages.shape[0]
-        pool.page_bytes = pages[0, 0].numel() * pages.element_size()
-        pool.layer_stride = pool.page_bytes * pages.shape[1]
-    return pool
+    num_pages = ref_counts.shape[0]
+    table = _int32(page_table, "page_table", (n_seq, max_pages))
+    refs = _int32(ref_counts, "ref_counts", (num_pages,))
+    if pages is None:
+        return _PagePool(table, refs, None, 0, 0, n_seq, max_pages, num_pages, 0)
+    if pages.dim() < 2 or pages.shape[1] != num_pages:
+        raise ValueError(f"pages must be [n_layers, {num_pages}, ...], got {list(pages.shape)}")
+    n_layers = pages.shape[0]
+    layer = pages.numel() // n_layers * pages.element_size()
+    return _PagePool(table, refs, _address(pages, "pages"), layer, layer // num_pages, n_seq, max_pages, num_pages,
+                     n_layers)
 
 
 def pages_fork(ctx: Context, page_table, ref_counts, parents, stream=None):
     """Row i of page_table becomes what row parents[i] was (-1: empty); pages are shared, counts follow."""
     pool = _page_pool(page_table, ref_counts)
-    ctx.check(lib().b2a_pages_fork(ctx.handle, ctypes.byref(pool), _int32(parents, "parents", (pool.n_seq,)),
-                                   _stream(stream)))
+    rc = (_lib or lib()).b2a_pages_fork(ctx._h, pool, _int32(parents, "parents", (pool.n_seq,)), _raw_stream(stream))
+    if rc:
+        ctx.check(rc)
 
 
 def pages_free(ctx: Context, page_table, ref_counts, keep_from, keep_to, page_size: int, stream=None):
     """Give back the pages of slots that hold no position of [keep_from[row], keep_to[row]) (keep_from None: 0)."""
     pool = _page_pool(page_table, ref_counts)
-    ctx.check(lib().b2a_pages_free(ctx.handle, ctypes.byref(pool), _int32(keep_from, "keep_from", (pool.n_seq,), True),
-                                   _int32(keep_to, "keep_to", (pool.n_seq,)), page_size, _stream(stream)))
+    rows = (pool.n_seq,)
+    rc = (_lib or lib()).b2a_pages_free(ctx._h, pool, None if keep_from is None else _int32(keep_from, "keep_from", rows),
+                                        _int32(keep_to, "keep_to", rows), page_size, _raw_stream(stream))
+    if rc:
+        ctx.check(rc)
 
 
 def pages_reserve(ctx: Context, page_table, ref_counts, ctx_lens, new_lens, pages, page_size: int, counts, stream=None):
@@ -555,16 +609,20 @@ def pages_reserve(ctx: Context, page_table, ref_counts, ctx_lens, new_lens, page
     a copy of a page that other rows hold too.  pages: [n_layers, num_pages, ...]; counts int32 [2] receives the
     pages given out and the pages missing (then nothing changed)."""
     pool = _page_pool(page_table, ref_counts, pages)
-    ctx.check(lib().b2a_pages_reserve(
-        ctx.handle, ctypes.byref(pool), _int32(ctx_lens, "ctx_lens", (pool.n_seq,)),
-        _int32(new_lens, "new_lens", (pool.n_seq,)), page_size, _int32(counts, "counts", (2,)), _stream(stream)))
+    rows = (pool.n_seq,)
+    rc = (_lib or lib()).b2a_pages_reserve(ctx._h, pool, _int32(ctx_lens, "ctx_lens", rows),
+                                           _int32(new_lens, "new_lens", rows), page_size,
+                                           _int32(counts, "counts", (2,)), _raw_stream(stream))
+    if rc:
+        ctx.check(rc)
 
 
 def pages_compact(ctx: Context, page_table, ref_counts, pages, counts, stream=None):
     """Move the n pages in use to the front of the pool; counts int32 [2] receives n and the pages moved."""
     pool = _page_pool(page_table, ref_counts, pages)
-    ctx.check(lib().b2a_pages_compact(ctx.handle, ctypes.byref(pool), _int32(counts, "counts", (2,)),
-                                      _stream(stream)))
+    rc = (_lib or lib()).b2a_pages_compact(ctx._h, pool, _int32(counts, "counts", (2,)), _raw_stream(stream))
+    if rc:
+        ctx.check(rc)
 
 
 def _ptr_array(tensors):

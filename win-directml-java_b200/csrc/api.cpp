@@ -57,6 +57,10 @@ struct b2a_context {
     // test hook (b2a_test_inject_wait_timeout): the next tcgen05 attention launch
     // leaves one K/V copy unissued
     bool inject_wait_timeout = false;
+    // the inverse frequencies of the last (theta, head dim) a cache call rotated with
+    double kv4_inv_freq[kMaxHeadDim / 2] = {};
+    double kv4_theta = 0.0;
+    int kv4_inv_dim = 0;
     // paged 4-bit cache: [merge counters][partial slots][q operands][q sums]
     void* kv4_ws = nullptr;
     size_t kv4_ws_bytes = 0;
@@ -1169,7 +1173,14 @@ int check_kv4_tokens(b2a_context* ctx, int act_dtype, const int32_t* ctx_lens, c
     p.T = T;
     p.rope_mode = rope_mode;
     p.norm_eps = norm_eps;
-    if (rope_mode != B2A_ROPE_NONE) inv_freq_table(rope_theta, p.D, p.inv_freq);
+    if (rope_mode != B2A_ROPE_NONE) {
+        if (ctx->kv4_theta != rope_theta || ctx->kv4_inv_dim != p.D) {
+            inv_freq_table(rope_theta, p.D, ctx->kv4_inv_freq);
+            ctx->kv4_theta = rope_theta;
+            ctx->kv4_inv_dim = p.D;
+        }
+        memcpy(p.inv_freq, ctx->kv4_inv_freq, sizeof(double) * (p.D / 2));
+    }
     return B2A_OK;
 }
 
@@ -1234,7 +1245,7 @@ int run_kv4_attention(b2a_context* ctx, Kv4Params& p, cudaStream_t stream) {
     p.partials = reinterpret_cast<float*>(base + counter_bytes);
     p.q_frag = reinterpret_cast<uint4*>(base + counter_bytes + part);
     p.q_sums = reinterpret_cast<float*>(base + counter_bytes + part + frag);
-    cudaError_t e = launch_kv4_prepare(p, stream);
+    cudaError_t e = launch_kv4_prepare(p, ctx->sm_count, stream);
     const int B = p.B;
     for (int b0 = 0; e == cudaSuccess && b0 < B; b0 += per_launch) {
         Kv4Params s = p;
@@ -1305,7 +1316,7 @@ B2A_API int b2a_kv4_append(b2a_context* ctx, const b2a_kv4_cache* cache, int act
     if (!rc) rc = check_kv4_new(ctx, k_new, v_new, kv_token_stride, k_held, v_held, k_norm_w, p);
     if (rc) return rc;
     DeviceGuard guard(ctx->device);
-    const cudaError_t e = launch_kv4_prepare(p, static_cast<cudaStream_t>(stream));
+    const cudaError_t e = launch_kv4_prepare(p, ctx->sm_count, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_fail(ctx, e, "cache append launch");
     return B2A_OK;
 }

@@ -247,7 +247,7 @@ constexpr int kMaxPageSize = 1024;
 constexpr int kKv4MaxBatch = 2048;      // sequences of one attention launch
 constexpr int kKv4GapBlocksMax = 16;    // largest per-unit allowance of the attention's split, in blocks
 // Appends k_new / v_new where given and lays out q where given.
-cudaError_t launch_kv4_prepare(const Kv4Params& p, cudaStream_t stream);
+cudaError_t launch_kv4_prepare(const Kv4Params& p, int sm_count, cudaStream_t stream);
 size_t kv4_frag_bytes(const Kv4Params& p);  // per sequence
 size_t kv4_sums_bytes(const Kv4Params& p);  // per sequence
 void kv4_attn_workspace(const Kv4Params& p, int device, size_t* partial_bytes, size_t* units_per_seq);

@@ -79,13 +79,13 @@ __device__ __forceinline__ double kv4_warp_sum(double v) {
     return v;
 }
 
-// Optional zero-centred RMS norm and RoPE at position pos of a row whose element lane + 32 j is
-// x[j]; the whole warp, vec[0..D) is its scratch.  The arithmetic is that of b2a_decode's prologue
-// (double sum of squares and angles; NeoX rotates in float, Gemma in double), each operation
-// rounded by itself, so that the codes decided on the result are reproducible.
+// Optional zero-centred RMS norm, and RoPE with the position's (cos, sin) cs[0 .. D/2), of a row whose
+// element lane + 32 j is x[j]; the whole warp, vec[0..D) is its scratch.  The arithmetic is that of
+// b2a_decode's prologue (double sum of squares and angles; NeoX rotates in float, Gemma in double),
+// each operation rounded by itself, so that the codes decided on the result are reproducible.
 template <int D>
 __device__ __forceinline__ void kv4_norm_rope(float (&x)[D / 32], const float* norm_w, float eps, int rope_mode,
-                                              const double* inv_freq, int pos, float* vec, int lane) {
+                                              const double2* cs, float* vec, int lane) {
     if (norm_w != nullptr) {
         double ss = 0.0;
 #pragma unroll
@@ -102,8 +102,7 @@ __device__ __forceinline__ void kv4_norm_rope(float (&x)[D / 32], const float* n
     __syncwarp();
     for (int i = lane; i < D / 2; i += 32) {
         const float a = vec[i], b = vec[i + D / 2];
-        double s, c;
-        sincos((double)pos * inv_freq[i], &s, &c);
+        const double c = cs[i].x, s = cs[i].y;
         if (rope_mode == 2) {
             vec[i] = (float)__dsub_rn(__dmul_rn((double)a, c), __dmul_rn((double)b, s));
             vec[i + D / 2] = (float)__dadd_rn(__dmul_rn((double)b, c), __dmul_rn((double)a, s));

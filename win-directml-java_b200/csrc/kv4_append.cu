@@ -3,14 +3,19 @@
 // holds them for callers that want the prompt's own attention to see the same values, and the
 // queries' norm, RoPE and layout as the warp MMA's B operand (kv4_attn.cu).
 //
-// One warp per query row and per (token, kv head, K or V).  The launch lets the attention kernel
+// kv4_prepare_kernel: a CTA takes rows of one token (query heads, key heads, value heads), a warp one
+// row at a time; the token's sines and cosines are computed once per CTA. It lets the attention kernel
 // behind it start at once: that kernel plans and requests its first old blocks meanwhile.
+// kv4_store_kernel: prompts. A CTA takes one block of 16 positions and walks kv heads; a thread holds
+// 8 channels of a row (16-byte loads), the block is assembled in shared memory and stored whole.
+#include <algorithm>
+
 #include "kv4.cuh"
 
 namespace b2a {
 namespace {
 
-constexpr int kPrepWarps = 4;
+constexpr int kPrepWarps = 8;
 
 // Query row r = token * G + head of the group, of (sequence b, kv head).  Its element 16 x + 8 j +
 // 2 t + e of group y goes to half e of operand word (y, lane 4 (r % 8) + t, 2 x + j) of 8-row tile
@@ -18,28 +23,25 @@ constexpr int kPrepWarps = 4;
 // 16 times larger); fp16 activations keep a second word with what the first rounding lost.
 // q_sums: sum of the group's operand values 2^-24 per group, then scale log2(e) 2^(E + 24).
 template <int D>
-__device__ __forceinline__ void prepare_query(const Kv4Params& p, int b, int kvh, int r, float* vec, int lane) {
+__device__ __forceinline__ void prepare_query(const Kv4Params& p, int64_t tok, int h, int L, int t, int n, bool ok,
+                                              const double2* cs, float* vec, int lane) {
     constexpr int kGroups = D / 32;
     const int tiles = (p.T * p.G + 7) / 8;
-    const int64_t tile = ((int64_t)b * p.Hkv + kvh) * tiles + (r >> 3);
+    const int kvh = h / p.G, r = t * p.G + h - kvh * p.G;
+    const int64_t tile = (tok / p.T * p.Hkv + kvh) * tiles + (r >> 3);
     __half* frag = reinterpret_cast<__half*>(p.q_frag + tile * (kGroups * 32 * 2));
     float* sums = p.q_sums + tile * (kGroups + 1) * 8 + (r & 7);
-    const int t = r / p.G, hg = r - t * p.G;
-    int L = 0, n = 0;
-    const bool ok = kv4_lens(p, b, L, n);
-    if (!ok && lane == 0) atomicOr(p.status, 1);
-    const int64_t tok = (int64_t)b * p.T + t;
-    const int h = kvh * p.G + hg;
-    const bool there = t < n;
-    if (!there && t < p.T)
+    if (t >= n) {  // no such row: the attention reads no operands of it
         for (int d = lane; d < D; d += 32)
             store_from_float(p.o, (tok * p.Hq + h) * D + d, ok ? 0.f : __int_as_float(0x7fc00000), p.act_dtype);
+        return;
+    }
     float x[kGroups], top = 0.f;
 #pragma unroll
     for (int y = 0; y < kGroups; ++y)
-        x[y] = there ? load_as_float(p.q, tok * p.q_stride + (int64_t)h * D + lane + 32 * y, p.act_dtype) : 0.f;
+        x[y] = load_as_float(p.q, tok * p.q_stride + (int64_t)h * D + lane + 32 * y, p.act_dtype);
     bool fine = true;
-    if (there) kv4_norm_rope<D>(x, p.q_norm_w, p.norm_eps, p.rope_mode, p.inv_freq, L + t, vec, lane);
+    kv4_norm_rope<D>(x, p.q_norm_w, p.norm_eps, p.rope_mode, cs, vec, lane);
 #pragma unroll
     for (int y = 0; y < kGroups; ++y) {
         top = fmaxf(top, fabsf(x[y]));
@@ -69,17 +71,12 @@ __device__ __forceinline__ void prepare_query(const Kv4Params& p, int b, int kvh
 }
 
 template <int D>
-__device__ __forceinline__ void append_row(const Kv4Params& p, int64_t row, float* vec, int lane) {
-    const int is_v = (int)(row & 1);
-    const int64_t tok = (row >> 1) / p.Hkv;
-    const int kvh = (int)((row >> 1) - tok * p.Hkv);
-    const int b = (int)(tok / p.T), t = (int)(tok - (int64_t)b * p.T);
-    int L, n;
-    const bool ok = kv4_lens(p, b, L, n);
+__device__ __forceinline__ void append_row(const Kv4Params& p, int64_t tok, int kvh, bool is_v, int L, int t, int n,
+                                           bool ok, const double2* cs, float* vec, int lane) {
+    const int b = (int)(tok / p.T);
     void* held = is_v ? p.v_held : p.k_held;
     const int64_t held_at = (tok * p.Hkv + kvh) * D;
-    if (!ok || t >= n) {
-        if (!ok && lane == 0) atomicOr(p.status, 1);
+    if (t >= n) {
         if (held)
             for (int d = lane; d < D; d += 32)
                 store_from_float(held, held_at + d, ok ? 0.f : __int_as_float(0x7fc00000), p.act_dtype);
@@ -91,7 +88,7 @@ __device__ __forceinline__ void append_row(const Kv4Params& p, int64_t row, floa
 #pragma unroll
     for (int j = 0; j < D / 32; ++j)
         x[j] = load_as_float(src, tok * p.kv_stride + (int64_t)kvh * D + lane + 32 * j, p.act_dtype);
-    if (!is_v) kv4_norm_rope<D>(x, p.k_norm_w, p.norm_eps, p.rope_mode, p.inv_freq, pos, vec, lane);
+    if (!is_v) kv4_norm_rope<D>(x, p.k_norm_w, p.norm_eps, p.rope_mode, cs, vec, lane);
     int code[D / 32];
     __half2 sz[D / 32];
     if (!kv4_quantise(x, code, sz) && lane == 0) atomicOr(p.status, 32);
@@ -109,38 +106,279 @@ __device__ __forceinline__ void append_row(const Kv4Params& p, int64_t row, floa
     }
 }
 
+// Rows of a token: Hq queries (where p.q), Hkv keys and Hkv values (where `append`); block (token,
+// chunk) takes rows [chunk * per, (chunk + 1) * per).
 template <int D>
-__global__ void __launch_bounds__(kPrepWarps * 32) kv4_prepare_kernel(const __grid_constant__ Kv4Params p,
-                                                                      int64_t q_rows, int64_t kv_rows) {
+__global__ void __launch_bounds__(kPrepWarps * 32) kv4_prepare_kernel(const __grid_constant__ Kv4Params p, int append,
+                                                                      int chunks, int per) {
     __shared__ float vec_all[kPrepWarps * D];
+    __shared__ double2 cs[D / 2];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t row = (int64_t)blockIdx.x * kPrepWarps + warp;
-    if (row < q_rows) {
-        const int per = (p.T * p.G + 7) / 8 * 8;  // rows of (sequence, kv head), whole tiles
-        const int64_t bk = row / per;
-        const int b = (int)(bk / p.Hkv);
-        prepare_query<D>(p, b, (int)(bk - (int64_t)b * p.Hkv), (int)(row - bk * per), vec_all + warp * D, lane);
-    } else if (row - q_rows < kv_rows) {
-        append_row<D>(p, row - q_rows, vec_all + warp * D, lane);
+    const int64_t tok = blockIdx.x / chunks;
+    const int chunk = (int)(blockIdx.x - tok * chunks);
+    const int b = (int)(tok / p.T), t = (int)(tok - (int64_t)b * p.T);
+    int L, n;
+    const bool ok = kv4_lens(p, b, L, n);
+    if (!ok && threadIdx.x == 0) atomicOr(p.status, 1);
+    if (p.rope_mode != 0 && threadIdx.x < D / 2) {
+        double sn, c;
+        sincos((double)(L + t) * p.inv_freq[threadIdx.x], &sn, &c);
+        cs[threadIdx.x] = make_double2(c, sn);
     }
+    __syncthreads();
+    const int nq = p.q ? p.Hq : 0, rows = nq + (append ? 2 * p.Hkv : 0);
+    const int end = min(rows, (chunk + 1) * per);
+    for (int r = chunk * per + warp; r < end; r += kPrepWarps) {
+        if (r < nq) prepare_query<D>(p, tok, r, L, t, n, ok, cs, vec_all + warp * D, lane);
+        else
+            append_row<D>(p, tok, (r - nq) >> 1, (r - nq) & 1, L, t, n, ok, cs, vec_all + warp * D, lane);
+    }
+}
+
+// ------------------------------------------------------------------ prompts
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
+    const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = Elem<T>::to_float(e[i]);
+}
+
+// One block of 16 positions of a sequence, all kv heads of a chunk.  Thread: key row tid / (D / 8),
+// channels 8 (tid % (D / 8)) .. + 7; the four threads of a group share its minimum and maximum.  A key
+// chunk is rotated with its partner chunk D / 2 away, which the thread loads too (it comes from L1).
+template <int D, typename T>
+__global__ void __launch_bounds__(2 * D) kv4_store_kernel(const __grid_constant__ Kv4Params p, int blocks, int chunks,
+                                                          int per) {
+    constexpr int kChunks = D / 8, kGroups = D / 32, kThreads = 2 * D;
+    extern __shared__ __align__(16) unsigned char smem[];
+    uint8_t* const stage = smem;                                          // two blocks
+    double* const part = reinterpret_cast<double*>(smem + 2 * 20 * D);    // [16][kChunks] sums of squares
+    void* const cs = smem + 2 * 20 * D + 16 * kChunks * 8;                // [16][D / 2] (cos, sin)
+    const int tid = threadIdx.x;
+    const int row = tid / kChunks, k = tid - row * kChunks;
+    const int chunk = blockIdx.x % chunks;
+    const int64_t bb = blockIdx.x / chunks;
+    const int b = (int)(bb / blocks);
+    int L, n;
+    const bool ok = kv4_lens(p, b, L, n);
+    if (!ok && tid == 0) atomicOr(p.status, 1);
+    const int blk = L / kKv4Block + (int)(bb - (int64_t)b * blocks);
+    const int t = blk * kKv4Block + row - L;  // this row's token
+    const int t_first = blk * kKv4Block - L;
+    if (t_first >= p.T) return;
+    const bool there = t >= 0 && t < n;
+    const int h0 = chunk * per, h1 = min(p.Hkv, h0 + per);
+    const int64_t tok = (int64_t)b * p.T + t;
+    if (t >= n && t < p.T) {  // rows that do not exist
+        const uint32_t v = ok ? 0u : 0x7fff7fffu;
+        for (int h = h0; h < h1; ++h) {
+            const int64_t at = (tok * p.Hkv + h) * D + 8 * k;
+            if (p.k_held) *reinterpret_cast<uint4*>(static_cast<T*>(p.k_held) + at) = make_uint4(v, v, v, v);
+            if (p.v_held) *reinterpret_cast<uint4*>(static_cast<T*>(p.v_held) + at) = make_uint4(v, v, v, v);
+        }
+    }
+    if (t_first >= n) return;  // nothing to store (the whole CTA)
+    if (p.rope_mode != 0) {
+        for (int i = tid; i < 16 * (D / 2); i += kThreads) {
+            const int pos = blk * kKv4Block + i / (D / 2);
+            double sn, c;
+            sincos((double)pos * p.inv_freq[i % (D / 2)], &sn, &c);
+            if (p.rope_mode == 2) static_cast<double2*>(cs)[i] = make_double2(c, sn);
+            else static_cast<float2*>(cs)[i] = make_float2((float)c, (float)sn);
+        }
+    }
+    const bool full = t_first >= 0 && t_first + kKv4Block <= n;
+    const int half = k < kChunks / 2 ? 0 : 1, k2 = half ? k - kChunks / 2 : k + kChunks / 2;
+    float wn[8], wn2[8];  // key norm weights of both chunks
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        wn[i] = p.k_norm_w ? p.k_norm_w[8 * k + i] : 0.f;
+        wn2[i] = p.k_norm_w ? p.k_norm_w[8 * k2 + i] : 0.f;
+    }
+    uint4 nk = make_uint4(0, 0, 0, 0), nk2 = nk, nv = nk;  // the next head's loads
+    auto fetch = [&](int h) {
+        if (!there || h >= h1) return;
+        const T* kr = static_cast<const T*>(p.k_new) + tok * p.kv_stride + (int64_t)h * D;
+        nk = *reinterpret_cast<const uint4*>(kr + 8 * k);
+        nk2 = *reinterpret_cast<const uint4*>(kr + 8 * k2);
+        nv = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.v_new) + tok * p.kv_stride + (int64_t)h * D + 8 * k);
+    };
+    // one row chunk into the block at `dst`; its bytes of the codes and the group's params
+    auto quantise = [&](const float (&x)[8], bool is_v, uint8_t* dst, void* held, int h) {
+        float lo = x[0], hi = x[0], odd = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            lo = fminf(lo, x[i]);
+            hi = fmaxf(hi, x[i]);
+            odd = fmaf(x[i], 0.f, odd);  // NaN where some value is not finite
+        }
+#pragma unroll
+        for (int o = 1; o <= 2; o <<= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            odd += __shfl_xor_sync(0xffffffffu, odd, o);
+        }
+        __half s = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f)), z = __float2half_rn(lo);
+        const float sf = __half2float(s), zf = __half2float(z);
+        const bool fine = odd == 0.f && isfinite(sf) && isfinite(zf);
+        const float inv = sf > 0.f && fine ? __fdiv_rn(1.0f, sf) : 0.f;
+        uint32_t codes = 0;
+        uint4 out;
+        uint32_t* ow = &out.x;
+        float v[8];
+        const float ns = fine ? sf : __int_as_float(0x7fc00000), nz = fine ? zf : ns;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            // 0 .. 15 first, then to the nearest whole number (ties to even) by 1.5 * 2^23
+            float c = fminf(fmaxf(__fmul_rn(__fsub_rn(x[i], zf), inv), 0.f), 15.f);
+            c = __fadd_rn(c, 12582912.f);
+            codes |= (__float_as_uint(c) & 15u) << (4 * i);
+            v[i] = fmaf(__fsub_rn(c, 12582912.f), ns, nz);
+        }
+        if (!fine) {
+            codes = 0;
+            s = z = __ushort_as_half(0x7fff);
+            if (there) atomicOr(p.status, 32);
+        }
+        if (held && there) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ow[i] = Elem<T>::pack(v[2 * i], v[2 * i + 1]);
+            *reinterpret_cast<uint4*>(static_cast<T*>(held) + (tok * p.Hkv + h) * D + 8 * k) = out;
+        }
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, codes, 1);
+        const int j = k & 1, x16 = (k >> 1) & 1, y = k >> 2, g = row & 7, r = row >> 3;
+        const uint32_t low = j ? other : codes, high = j ? codes : other;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int i = 4 * j + e;  // channels 8 .. + i and 8 further
+            const uint8_t byte = (uint8_t)((low >> (4 * i) & 15u) | (high >> (4 * i) & 15u) << 4);
+            const int at = is_v ? ((y * 8 + i) * 4 + (g >> 1)) * 8 + x16 * 4 + 2 * (g & 1) + r
+                                : ((y * 8 + g) * 4 + (i >> 1)) * 8 + x16 * 4 + 2 * (i & 1) + r;
+            dst[at] = byte;
+        }
+        if ((k & 3) == 0)
+            reinterpret_cast<__half2*>(dst + kv4_off_kparam(D))[kv4_param(row, y, kGroups)] = __halves2half2(s, z);
+    };
+    fetch(h0);
+    __syncthreads();
+    for (int h = h0; h < h1; ++h) {
+        uint8_t* dst = stage + ((h - h0) & 1) * 20 * D;
+        float x[8], y[8], v[8];
+        unpack8<T>(nk, x);
+        unpack8<T>(nk2, y);
+        unpack8<T>(nv, v);
+        fetch(h + 1);
+        if (p.k_norm_w) {
+            double ss = 0.0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss += (double)x[i] * (double)x[i];
+            part[tid] = ss;
+            __syncthreads();
+            ss = 0.0;
+            for (int i = 0; i < kChunks; ++i) ss += part[row * kChunks + i];
+            __syncthreads();
+            const float rms = (float)(1.0 / sqrt(__dadd_rn(ss / (double)D, (double)p.norm_eps)));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = (float)__dmul_rn((double)__fmul_rn(x[i], rms), __dadd_rn(1.0, (double)wn[i]));
+                y[i] = (float)__dmul_rn((double)__fmul_rn(y[i], rms), __dadd_rn(1.0, (double)wn2[i]));
+            }
+        }
+        if (p.rope_mode == 2) {
+            const double2* c = static_cast<const double2*>(cs) + row * (D / 2) + 8 * (half ? k2 : k);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                x[i] = half ? (float)__dadd_rn(__dmul_rn((double)x[i], c[i].x), __dmul_rn((double)y[i], c[i].y))
+                            : (float)__dsub_rn(__dmul_rn((double)x[i], c[i].x), __dmul_rn((double)y[i], c[i].y));
+        } else if (p.rope_mode == 1) {
+            const float2* c = static_cast<const float2*>(cs) + row * (D / 2) + 8 * (half ? k2 : k);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float u = __fmul_rn(x[i], c[i].x), w = __fmul_rn(y[i], c[i].y);
+                x[i] = half ? __fadd_rn(w, u) : __fsub_rn(u, w);
+            }
+        }
+        quantise(x, false, dst, p.k_held, h);
+        quantise(v, true, dst + kv4_off_v(D), p.v_held, h);
+        __syncthreads();
+        uint8_t* block = kv4_block_ptr(p, b, h, blk * kKv4Block);
+        if (block == nullptr) {
+            if (tid == 0) atomicOr(p.status, 16);
+        } else if (full) {
+            for (int i = tid; i < 20 * D / 16; i += kThreads)
+                reinterpret_cast<uint4*>(block)[i] = reinterpret_cast<const uint4*>(dst)[i];
+        } else {
+            // the rows that exist: their bytes of the codes, their params
+            auto mine = [&](int key) {
+                const int tk = t_first + key;
+                return tk >= 0 && tk < n;
+            };
+            for (int i = tid; i < 16 * D; i += kThreads) {
+                const bool is_v = i >= 8 * D;
+                const int a = is_v ? i - 8 * D : i;
+                const int r = a & 1, e = (a >> 1) & 1, q = (a >> 3) & 3, g = (a >> 5) & 7;
+                const int at = is_v ? kv4_off_v(D) + a : a;
+                if (mine(is_v ? 2 * q + e + 8 * r : g + 8 * r)) block[at] = dst[at];
+            }
+            for (int i = tid; i < 2 * 16 * kGroups; i += kThreads) {
+                const int w = i % (16 * kGroups), key = (w / kGroups >> 1) + 8 * (w / kGroups & 1);
+                const int at = (i < 16 * kGroups ? kv4_off_kparam(D) : kv4_off_vparam(D)) + 4 * w;
+                if (mine(key)) *reinterpret_cast<uint32_t*>(block + at) = *reinterpret_cast<const uint32_t*>(dst + at);
+            }
+        }
+    }
+}
+
+// Tokens per sequence from which whole blocks are stored: below it a block would be mostly absent rows.
+constexpr int kStoreMinTokens = 16;
+
+template <int D, typename T>
+cudaError_t launch_store(const Kv4Params& p, int sm_count, cudaStream_t stream) {
+    const int blocks = (p.T + 2 * kKv4Block - 2) / kKv4Block;  // blocks that T tokens can touch
+    const int64_t ctas = (int64_t)p.B * blocks;
+    // a CTA computes its block's sines once for all its heads: heads are cut only where CTAs are few
+    const int want = (int)std::min<int64_t>(p.Hkv, std::max<int64_t>(1, 4 * sm_count / ctas));
+    const int per = (p.Hkv + want - 1) / want, chunks = (p.Hkv + per - 1) / per;
+    const size_t smem = 2 * 20 * D + 16 * (D / 8) * 8 + 16 * (D / 2) * (p.rope_mode == 2 ? sizeof(double2) : sizeof(float2));
+    auto kern = kv4_store_kernel<D, T>;
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+    }
+    kern<<<(unsigned)(ctas * chunks), 2 * D, smem, stream>>>(p, blocks, chunks, per);
+    return cudaGetLastError();
+}
+
+template <int D>
+cudaError_t launch_prepare(const Kv4Params& p, int sm_count, cudaStream_t stream) {
+    int append = p.k_new ? 1 : 0;
+    if (append && p.T >= kStoreMinTokens) {
+        const cudaError_t e = p.act_dtype == kF16 ? launch_store<D, __half>(p, sm_count, stream)
+                                                  : launch_store<D, __nv_bfloat16>(p, sm_count, stream);
+        if (e != cudaSuccess || !p.q) return e;
+        append = 0;
+    }
+    // a row per warp while that leaves the GPU room, else longer runs of rows that share their sines
+    const int64_t tokens = (int64_t)p.B * p.T;
+    const int rows = (p.q ? p.Hq : 0) + (append ? 2 * p.Hkv : 0);
+    const int most = (rows + kPrepWarps - 1) / kPrepWarps;
+    const int want = (int)std::max<int64_t>(1, std::min<int64_t>(most, 8 * sm_count / tokens));
+    const int per = (rows + want - 1) / want, chunks = (rows + per - 1) / per;
+    kv4_prepare_kernel<D><<<(unsigned)(tokens * chunks), kPrepWarps * 32, 0, stream>>>(p, append, chunks, per);
+    return cudaGetLastError();
 }
 
 }  // namespace
 
-cudaError_t launch_kv4_prepare(const Kv4Params& p, cudaStream_t stream) {
-    const int64_t q_rows = p.q ? (int64_t)p.B * p.Hkv * ((p.T * p.G + 7) / 8 * 8) : 0;
-    const int64_t kv_rows = p.k_new ? (int64_t)p.B * p.T * p.Hkv * 2 : 0;
-    const unsigned grid = (unsigned)((q_rows + kv_rows + kPrepWarps - 1) / kPrepWarps);
-    constexpr int kT = kPrepWarps * 32;
+cudaError_t launch_kv4_prepare(const Kv4Params& p, int sm_count, cudaStream_t stream) {
     switch (p.D) {
-        case 64: kv4_prepare_kernel<64><<<grid, kT, 0, stream>>>(p, q_rows, kv_rows); break;
-        case 96: kv4_prepare_kernel<96><<<grid, kT, 0, stream>>>(p, q_rows, kv_rows); break;
-        case 128: kv4_prepare_kernel<128><<<grid, kT, 0, stream>>>(p, q_rows, kv_rows); break;
-        case 256: kv4_prepare_kernel<256><<<grid, kT, 0, stream>>>(p, q_rows, kv_rows); break;
+        case 64: return launch_prepare<64>(p, sm_count, stream);
+        case 96: return launch_prepare<96>(p, sm_count, stream);
+        case 128: return launch_prepare<128>(p, sm_count, stream);
+        case 256: return launch_prepare<256>(p, sm_count, stream);
         default: return cudaErrorInvalidValue;
     }
-    return cudaGetLastError();
 }
 
 }  // namespace b2a

@@ -4,27 +4,38 @@
 //     S_j = scale * sum_y ( s_yj * sum_{i in y} q_i c_ij  +  z_yj * sum_{i in y} q_i )
 //     o_i = ( sum_j (P_j s_yj) c_ij  +  sum_j P_j z_yj ) / sum_j P_j,   P_j = exp(S_j - max)
 // so both products run on the codes themselves: the scale of a key's group multiplies the group's
-// score (32 bits) or the probability before it is rounded for the second product, and the minima
-// enter through sums.  No value is ever dequantised.
+// score (32 bits) or the probability (the second product's B operand), and the minima enter through
+// one more MMA each: z (keys x groups) times the sums of q, and z^T (groups x keys, with rows of
+// ones below it, which give sum_j P_j) times P.  No value is ever dequantised.
 //
 // Bound.  A key costs 1.25 D bytes per kv head for G query heads, about 3.2 G flop per byte: HBM,
-// provided the instructions per key stay few.  Per 16 keys and 32 channels a warp spends ten integer
-// instructions on 2 x 512 codes (two masks and a shift per word; the block layout is the MMA's own
-// operand order) and four MMAs of 16 keys (K) or 16 channels (V^T) x 8 query rows.
+// provided the instructions per key stay few.  Per 16 keys and 32 channels a warp spends twenty
+// integer instructions on 2 x 512 codes (two masks and a shift per word pair; the block layout is
+// the MMA's own operand order) and four MMAs of 16 keys (K) or 16 channels (V^T) x 8 columns.
 //
-// Work split.  A unit is (sequence, kv head, tile of 8 * kTiles query rows); a query row is (token,
-// head of the group), so one cache byte serves every head of its group and every token of a draft.
-// The blocks of 16 keys of all units form one stream and every CTA takes an equal range of it
-// (stream-K); the pieces of a cut unit meet through partial slots (m, l, O) that the last one to
-// finish joins.  Inside a piece each warp walks its own blocks with its own ring of bulk copies: one
-// copy of 20 D bytes is a block, its address comes from page-table entries fetched 32 blocks at a
-// time, and the warps meet only at the end of the piece.
+// Precision.  q and P are f16 operands.  One rounding of each is far below a bf16 result's own; for
+// fp16 results each is carried as two words (hi + lo): with at most four query rows the lo words take
+// the columns 4..7 of the same MMAs (kSplit 1, nothing extra to multiply), else a second column tile
+// (kSplit 2).  The rounding of P s is corrected exactly: lo = fma(P, s, -hi) + P_lo s.
 //
-// Softmax.  The running maximum moves only when a score exceeds it by more than 2^8 (in base 2: by
-// 8), so a block normally costs no reduction across lanes: probabilities are at most 2^8 and sums
-// are exact enough in fp32 whatever the reference point.  The same slow path moves the power of two
-// 2^vexp that keeps P s within fp16: s 2^-vexp is at most 2^7, which leaves 2^21 of range below the
-// largest weight before fp16 subnormals begin.
+// The tensor cores add to their fp32 accumulators by truncation, a loss towards zero that grows with
+// the number of blocks, and the codes are all positive.  Every second block therefore enters as
+// s c + z = -s (15 - c) + z + 15 s: its codes complemented (free, in the masks), its P s negated, so
+// that the accumulators stay near the difference of two like sums; 15 sum P s is one more MMA.  The
+// sums over minima, scales and P are added to their totals in fp32 outside the MMA.
+//
+// Work split.  A unit is (sequence, kv head, tile of query rows); a query row is (token, head of the
+// group), so one cache byte serves every head of its group and every token of a draft.  The blocks
+// of 16 keys of all units form one stream and every CTA takes an equal range of it (stream-K); the
+// pieces of a cut unit meet through partial slots (m, l, O) that the last one to finish joins.
+// Inside a piece each warp walks its own blocks with its own ring of bulk copies: one copy of 20 D
+// bytes is a block, its address comes from page-table entries fetched 32 blocks at a time, and the
+// warps meet only at the end of the piece.
+//
+// Softmax.  P is computed against a reference that moves only when a probability would exceed 2^15 /
+// s_max (s_max: the largest value scale seen, at least 1), to where the largest is 2^7 / s_max: a
+// block normally costs no reduction across lanes, P and P s stay inside fp16 with at least 2^21 of
+// range below the largest weight before subnormals begin, and sums are in fp32 throughout.
 #include <mutex>
 #include <type_traits>
 
@@ -36,33 +47,43 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr float kLowest = -1e37f;   // a running maximum before any key: finite, so differences are
-constexpr float kSlack = 8.f;       // how far a score may exceed the running maximum (log2)
+constexpr float kLowest = -1e37f;  // largest score before any key: finite, so differences are numbers
 
-template <int D, int kTiles, bool kSplitQ>
-struct AttnGeo {
+template <int D_, int kTiles_, int kSplit_>
+struct Cfg {
+    static constexpr int D = D_;
+    static constexpr int kTiles = kTiles_;  // column tiles of 8 in the second product
+    static constexpr int kSplit = kSplit_;  // 0: one word, 1: lo words in columns 4..7, 2: in tile 1
+    static constexpr int kRows = kSplit == 1 ? 4 : (kSplit == 2 ? 8 : 8 * kTiles);
+    static constexpr int kSTiles = kSplit == 2 ? 1 : kTiles;  // column tiles of scores
+    static constexpr int kCols = 8 * kSTiles;                 // columns of a warp's merged output
     static constexpr int kGroups = D / kKv4Group;
     static constexpr int kBlockBytes = kv4_block_bytes(D);
-    static constexpr int kStages = D <= 128 ? 4 : 3;
-    static constexpr int kRows = 8 * kTiles;
-    static constexpr int kCtas = D * kTiles <= 64 ? 4 : (D * kTiles <= 128 ? 3 : 2);  // per SM: the registers' bound
+    static constexpr int kSub = D <= 96 ? 2 : 1;  // blocks per ring stage
+    static constexpr int kStages = D <= 96 ? 3 : (D <= 128 ? 4 : 3);
+    static constexpr int kStageBytes = kSub * kBlockBytes;
+    // CTAs per SM, the registers' bound
+    static constexpr int kCtas = D <= 64 ? (kTiles == 1 ? 4 : 3) : (D <= 128 ? (kTiles == 1 ? 3 : 2) : (kTiles == 1 ? 3 : 2));
     // fixed cost of a piece in blocks of streaming time, charged to every unit by the split
     static constexpr int kGapBlocks = D <= 64 ? 16 : (D <= 128 ? 8 : 4);
-    static constexpr int kMinBlocks = 8;  // smallest range of a CTA: two blocks per warp
-    static constexpr size_t kRingBytes = size_t(kWarps) * kStages * kBlockBytes;
-    static constexpr size_t kMergeBytes = size_t(kWarps) * kRows * D * 4;
+    static constexpr int kMinBlocks = 8;  // smallest range of a CTA
+    // q's operand words in shared memory where the accumulators leave no registers for them
+    static constexpr bool kQShared = D * kTiles >= 256;
+    // head dim 256: the value params are regrouped in shared memory (their rows lie 128 bytes
+    // apart, so that reading pairs of keys directly would meet in the same banks)
+    static constexpr bool kRegroup = D >= 256;
     static constexpr size_t a128(size_t x) { return (x + 127) / 128 * 128; }
+    static constexpr size_t kRingBytes = size_t(kWarps) * kStages * kStageBytes;
+    static constexpr size_t kMergeBytes = size_t(kWarps) * kCols * D * 4;
     static constexpr size_t oBars = a128(kRingBytes > kMergeBytes ? kRingBytes : kMergeBytes);
     static constexpr size_t oMl = oBars + kWarps * kStages * 8;
-    static constexpr size_t oMisc = a128(oMl + size_t(kWarps) * kRows * 2 * 4);
-    // q operand words in shared memory: the second (fp16) words always, the first ones where the
-    // accumulators leave no registers for them
-    static constexpr bool kQShared = D * kTiles >= 256;
+    static constexpr size_t oMisc = a128(oMl + size_t(kWarps) * kCols * 2 * 4);
     static constexpr size_t kQWords = size_t(kTiles) * kGroups * 32 * 16;
     static constexpr size_t oQ = oMisc + 128;
-    static constexpr size_t oQlo = oQ + (kQShared ? kQWords : 0);
-    static constexpr size_t oPrefix = oQlo + (kSplitQ ? kQWords : 0);
+    static constexpr size_t oPairs = oQ + (kQShared ? kQWords : 0);
+    static constexpr size_t oPrefix = oPairs + (kRegroup ? kWarps * 512 : 0);
     static size_t total(int B) { return oPrefix + size_t(3 * B + 1) * 4; }
+    static_assert(kGapBlocks <= kKv4GapBlocksMax, "host launch split assumes this bound");
 };
 
 // The blocks of 16 positions that some new token of a sequence sees: how many, and the first.
@@ -95,31 +116,64 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
     asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x.x), "=r"(x.y) : "r"(a));
     return x;
 }
-// The A operand of one 16 x 16 tile of codes.
-__device__ __forceinline__ void code_frag(uint32_t (&a)[4], uint32_t w) {
+// The A operand of one 16 x 16 tile of codes, or of 15 - codes (flip all ones).
+__device__ __forceinline__ void code_frag(uint32_t (&a)[4], uint32_t w, uint32_t flip = 0) {
     const uint32_t h = w >> 8;
-    a[0] = w & 0x000F000Fu;
-    a[1] = h & 0x000F000Fu;
-    a[2] = w & 0x00F000F0u;
-    a[3] = h & 0x00F000F0u;
+    a[0] = (w ^ flip) & 0x000F000Fu;
+    a[1] = (h ^ flip) & 0x000F000Fu;
+    a[2] = (w ^ flip) & 0x00F000F0u;
+    a[3] = (h ^ flip) & 0x00F000F0u;
 }
-__device__ __forceinline__ float2 half2_f(uint32_t x) { return __half22float2(*reinterpret_cast<__half2*>(&x)); }
+__device__ __forceinline__ void lds128(uint32_t a, uint32_t* x) {
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(a));
+}
+__device__ __forceinline__ void sts32(uint32_t a, uint32_t x) {
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(x) : "memory");
+}
+// n consecutive params (4 bytes each), 8- or 16-byte aligned as the layout gives them
+template <int N>
+__device__ __forceinline__ void lds_params(uint32_t a, uint32_t (&x)[N]) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) lds128(a + i * 4, x + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const uint2 w = lds64(a + i * 4);
+            x[i] = w.x;
+            x[i + 1] = w.y;
+        }
+    }
+}
+__device__ __forceinline__ __half2 h2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
+__device__ __forceinline__ uint32_t u32(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
+__device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
+__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
+__device__ __forceinline__ float nan_f() { return __int_as_float(0x7fc00000); }
+// NaN halves become zero
+__device__ __forceinline__ uint32_t no_nan(uint32_t x) {
+    if ((x & 0x7fffu) > 0x7c00u) x &= 0xffff0000u;
+    if ((x >> 16 & 0x7fffu) > 0x7c00u) x &= 0x0000ffffu;
+    return x;
+}
 
-template <int D, int kTiles, bool kSplitQ>
-__global__ void __launch_bounds__(kThreads, AttnGeo<D, kTiles, kSplitQ>::kCtas) kv4_attn_kernel(const __grid_constant__ Kv4Params p) {
-    using Gm = AttnGeo<D, kTiles, kSplitQ>;
-    constexpr int kGroups = Gm::kGroups, kStages = Gm::kStages, kRows = Gm::kRows;
+template <typename C>
+__global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __grid_constant__ Kv4Params p) {
+    constexpr int D = C::D, kTiles = C::kTiles, kSTiles = C::kSTiles, kSplit = C::kSplit;
+    constexpr int kGroups = C::kGroups, kStages = C::kStages, kRows = C::kRows, kSub = C::kSub, kCols = C::kCols;
+    constexpr uint32_t kOnes = 0x3C003C00u;  // f16x2 (1, 1)
     extern __shared__ __align__(128) unsigned char smem[];
     float* merge_s = reinterpret_cast<float*>(smem);
-    float* ml_s = reinterpret_cast<float*>(smem + Gm::oMl);
-    int* misc = reinterpret_cast<int*>(smem + Gm::oMisc);
-    int* prefix = reinterpret_cast<int*>(smem + Gm::oPrefix);
+    float* ml_s = reinterpret_cast<float*>(smem + C::oMl);
+    int* misc = reinterpret_cast<int*>(smem + C::oMisc);
+    int* prefix = reinterpret_cast<int*>(smem + C::oPrefix);
     int* ctx_s = prefix + p.B + 1;  // cached and new tokens per sequence, 0 and 0 where they do not fit
     int* new_s = ctx_s + p.B;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, t4 = lane & 3;
-    const uint32_t ring = smem_u32(smem) + warp * kStages * Gm::kBlockBytes;
-    const uint32_t bars = smem_u32(smem + Gm::oBars) + warp * kStages * 8;
+    const uint32_t ring = smem_u32(smem) + warp * kStages * C::kStageBytes;
+    const uint32_t bars = smem_u32(smem + C::oBars) + warp * kStages * 8;
+    const uint32_t pairs = smem_u32(smem + C::oPairs) + warp * 512;
 
     if (lane == 0) {
 #pragma unroll
@@ -139,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, AttnGeo<D, kTiles, kSplitQ>::kCtas) 
             ctx_s[b] = L;
             new_s[b] = n;
             const int nb = seq_blocks(p, L, n, lo);
-            run += nb ? nb + Gm::kGapBlocks : 0;
+            run += nb ? nb + C::kGapBlocks : 0;
         }
         int incl = run;
 #pragma unroll
@@ -155,18 +209,19 @@ __global__ void __launch_bounds__(kThreads, AttnGeo<D, kTiles, kSplitQ>::kCtas) 
             prefix[b] = acc;
             int lo;
             const int nb = seq_blocks(p, ctx_s[b], new_s[b], lo);
-            acc += nb ? nb + Gm::kGapBlocks : 0;
+            acc += nb ? nb + C::kGapBlocks : 0;
         }
         if (tid == kThreads - 1) prefix[p.B] = acc;
         __syncthreads();
     }
-    const int row_tiles = (p.T * p.G + kRows - 1) / kRows;
+    const int all_rows = p.T * p.G;
+    const int row_tiles = (all_rows + kRows - 1) / kRows;
     const int per_seq = p.Hkv * row_tiles;
     const long long total = (long long)prefix[p.B] * per_seq;
-    const long long R = max((long long)Gm::kMinBlocks, (total + gridDim.x - 1) / gridDim.x);
-    const int q_tiles = (p.T * p.G + 7) / 8;  // tiles of 8 rows that the preparation laid out
-    bool dep_done = false, dead = false;  // dead: a copy of this warp did not arrive in time
-    uint32_t it = 0;  // blocks this warp has consumed since the launch began: ring slot and parity
+    const long long R = max((long long)C::kMinBlocks, (total + gridDim.x - 1) / gridDim.x);
+    const int q_tiles = (all_rows + 7) / 8;  // tiles of 8 rows that the preparation laid out
+    bool dep_done = false, dead = false;     // dead: a copy of this warp did not arrive in time
+    uint32_t it = 0;  // stages this warp has consumed since the launch began: ring slot and parity
 
     for (long long pos = (long long)blockIdx.x * R, end = min(total, pos + R); pos < end;) {
         int lo_b = 0, hi_b = p.B - 1;
@@ -179,7 +234,7 @@ __global__ void __launch_bounds__(kThreads, AttnGeo<D, kTiles, kSplitQ>::kCtas) 
         const int L = ctx_s[b], n = new_s[b];
         int first_blk;
         const int n_blk = seq_blocks(p, L, n, first_blk);
-        const int n_v = n_blk + Gm::kGapBlocks;
+        const int n_v = n_blk + C::kGapBlocks;
         const long long seq_base = (long long)prefix[b] * per_seq;
         const int r = (int)((pos - seq_base) / n_v);
         const long long u_start = seq_base + (long long)r * n_v, u_end = u_start + n_blk;
@@ -191,53 +246,66 @@ __global__ void __launch_bounds__(kThreads, AttnGeo<D, kTiles, kSplitQ>::kCtas) 
         const int kvh = r / row_tiles, rt = r - kvh * row_tiles;
         // tokens of this tile's rows, and the blocks of the piece that they see
         const int t_lo = rt * kRows / p.G, t_hi = min(n - 1, (rt * kRows + kRows - 1) / p.G);
-        const int key_lo = p.window > 0 ? max(0, L + t_lo - p.window + 1) : 0, key_hi = L + t_hi;
+        const int key_lo = p.window > 0 ? max(0, L + t_lo - p.window + 1) : 0;
         const int blk0 = max(first_blk + (int)(pos - u_start), key_lo / kKv4Block);
-        const int blk1 = t_lo <= t_hi ? min(first_blk + (int)(piece_end - u_start), key_hi / kKv4Block + 1) : blk0;
+        const int blk1 =
+            t_lo <= t_hi ? min(first_blk + (int)(piece_end - u_start), (L + t_hi) / kKv4Block + 1) : blk0;
+        const int key_hi = min(L + t_hi, blk1 * kKv4Block - 1);  // last key that some row takes from this piece
         const long long c0 = u_start / R, c1 = (u_end - 1) / R;
         const int n_split = (int)(c1 - c0) + 1;
         const int my_slot = 2 * blockIdx.x + (pos == (long long)blockIdx.x * R ? 0 : 1);
         const int unit = b * per_seq + r;
         pos = piece_end;
 
-        // ------------------------------------------------------------ this warp's blocks
+        // ------------------------------------------------------------ this warp's stages
+        // stage i holds blocks blk0 + (warp + 4 i) kSub + 0 .. kSub - 1 (those below blk1)
         const int bpp = p.page_size / kKv4Block;
-        const int my_n = max(0, (blk1 - blk0 - warp + kWarps - 1) / kWarps);
+        const int my_n = max(0, ((blk1 - blk0 + kSub - 1) / kSub - warp + kWarps - 1) / kWarps);
         bool bad = false;
-        auto entry = [&](int i) -> int64_t {  // byte offset of the warp's i-th block, per lane
-            if (i >= my_n) return 0;
-            const int blk = blk0 + warp + kWarps * i;
+        auto entry = [&](int x) -> int64_t {  // byte offset of the warp's x-th block, per lane; -1: none
+            const int blk = blk0 + (warp + kWarps * (x / kSub)) * kSub + x % kSub;
+            if (x / kSub >= my_n || blk >= blk1) return -1;
             const int slot = blk / bpp, in = blk - slot * bpp;
             const int page = p.page_table[(int64_t)b * p.max_pages + slot];
             if (page < 0 || page >= p.num_pages) {
                 bad = true;
                 return 0;
             }
-            return (((int64_t)page * p.Hkv + kvh) * bpp + in) * Gm::kBlockBytes;
+            return (((int64_t)page * p.Hkv + kvh) * bpp + in) * C::kBlockBytes;
         };
         int64_t cur = entry(lane), nxt = entry(32 + lane);
-        auto issue = [&](int i) {  // request the warp's i-th block
-            if (i > 0 && (i & 31) == 0) {
+        auto issue = [&](int i) {  // request the warp's i-th stage
+            const int x = i * kSub;
+            if (x > 0 && (x & 31) == 0) {
                 cur = nxt;
-                nxt = entry(i + 32 + lane);
+                nxt = entry(x + 32 + lane);
             }
-            const int64_t off = __shfl_sync(0xffffffffu, cur, i & 31);
+            int64_t off[kSub];
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) off[u] = __shfl_sync(0xffffffffu, cur, (x & 31) + u);
             if (lane == 0) {
                 const uint32_t s = (it + i) % kStages;
-                mbar_expect_tx(bars + s * 8, Gm::kBlockBytes);
-                bulk_load(ring + s * Gm::kBlockBytes, p.pages + off, Gm::kBlockBytes, bars + s * 8);
+                uint32_t bytes = 0;
+#pragma unroll
+                for (int u = 0; u < kSub; ++u) bytes += off[u] >= 0 ? C::kBlockBytes : 0;
+                mbar_expect_tx(bars + s * 8, bytes);
+#pragma unroll
+                for (int u = 0; u < kSub; ++u)
+                    if (off[u] >= 0)
+                        bulk_load(ring + s * C::kStageBytes + u * C::kBlockBytes, p.pages + off[u], C::kBlockBytes,
+                                  bars + s * 8);
             }
         };
-        // Blocks before the first new token's are as the kernel before the preparation left them, so
-        // the first ones are requested while the preparation kernel still runs.
         int issued = 0;
         auto fill = [&](int upto) {
             while (!dead && issued < min(upto, my_n)) issue(issued++);
         };
         if (!dep_done) {
-            const int old_blk = L / kKv4Block;  // blocks below hold no new token
+            // Blocks below the first new token's are as the kernel before the preparation left them,
+            // so the first ones are requested while the preparation kernel still runs.
+            const int old_blk = L / kKv4Block;
             int ready = 0;
-            while (ready < min(kStages, my_n) && blk0 + warp + kWarps * ready < old_blk) ++ready;
+            while (ready < min(kStages, my_n) && blk0 + (warp + kWarps * ready + 1) * kSub <= old_blk) ++ready;
             fill(ready);
             asm volatile("griddepcontrol.wait;" ::: "memory");
             dep_done = true;
@@ -245,57 +313,70 @@ __global__ void __launch_bounds__(kThreads, AttnGeo<D, kTiles, kSplitQ>::kCtas) 
         fill(kStages);
 
         // ------------------------------------------------------------ q operands
-        // B operand words of 8-row tile i: per group four words a lane (two 16-channel steps)
-        uint32_t qf[kTiles][kGroups][4];
-        uint4* const q_s = reinterpret_cast<uint4*>(smem + Gm::oQ) + lane;
-        uint4* const qlo_s = reinterpret_cast<uint4*>(smem + Gm::oQlo) + lane;
-        float qs[kTiles][kGroups][2], f0[kTiles], f1[kTiles];
-        int lim0[kTiles], lim1[kTiles];  // last visible key of rows 2t and 2t + 1
+        // B operand words per column tile and group: four a lane (two 16-channel steps), column g
+        uint32_t qf[kTiles][kGroups][4], qz[kSTiles][2];
+        float f[kSTiles][2];   // log2 units per score unit, columns 2t and 2t + 1
+        int lim[kSTiles][2];   // last key that the columns' rows see in this piece
+        uint4* const q_s = reinterpret_cast<uint4*>(smem + C::oQ) + lane;
+        auto row_of = [&](int tile, int col) { return rt * kRows + (kSplit == 1 ? (col & 3) : tile * 8 + col); };
+        const int64_t head = (int64_t)b * p.Hkv + kvh;
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
-            const int tile8 = rt * kTiles + i;
-            const int64_t at = ((int64_t)b * p.Hkv + kvh) * q_tiles + min(tile8, q_tiles - 1);
-            const uint4* src = p.q_frag + at * (kGroups * 32 * 2);
-            const float* sums = p.q_sums + at * (kGroups + 1) * 8;
+        for (int j = 0; j < kTiles; ++j) {
+            const int row = row_of(kSplit == 2 ? 0 : j, g);
+            const bool there = row < all_rows && row / p.G < n;
+            const int64_t at = head * q_tiles + (there ? row >> 3 : 0);
+            const bool lo_word = kSplit == 1 ? g >= 4 : (kSplit == 2 && j == 1);
+            const uint4* src = p.q_frag + (at * 2 + (lo_word ? 1 : 0)) * (kGroups * 32) + (row & 7) * 4 + t4;
 #pragma unroll
             for (int y = 0; y < kGroups; ++y) {
-                const int word = (i * kGroups + y) * 32;
-                if constexpr (!Gm::kQShared) {
-                    const uint4 w = src[y * 32 + lane];
-                    qf[i][y][0] = w.x, qf[i][y][1] = w.y, qf[i][y][2] = w.z, qf[i][y][3] = w.w;
-                } else if (warp == y % kWarps) {
-                    q_s[word] = src[y * 32 + lane];
-                }
-                if (kSplitQ && warp == y % kWarps) qlo_s[word] = src[(kGroups + y) * 32 + lane];
-                const float2 s = *reinterpret_cast<const float2*>(sums + y * 8 + 2 * t4);
-                qs[i][y][0] = s.x, qs[i][y][1] = s.y;
+                if (C::kQShared && warp != y % kWarps) continue;
+                uint4 w = make_uint4(0, 0, 0, 0);
+                if (there) w = src[y * 32];
+                if constexpr (C::kQShared) q_s[(j * kGroups + y) * 32] = w;
+                else qf[j][y][0] = w.x, qf[j][y][1] = w.y, qf[j][y][2] = w.z, qf[j][y][3] = w.w;
             }
-            const float2 f = *reinterpret_cast<const float2*>(sums + kGroups * 8 + 2 * t4);
-            f0[i] = f.x, f1[i] = f.y;
-            const int r0 = tile8 * 8 + 2 * t4, tok0 = r0 / p.G, tok1 = (r0 + 1) / p.G;
-            lim0[i] = tok0 < n ? L + tok0 : -1;
-            lim1[i] = tok1 < n ? L + tok1 : -1;
+            if (j < kSTiles) {
+                // the groups' sums of q, two halves each (k = group and k = 8 + group)
+                float s0 = 0.f, s1 = 0.f;
+                const float* sums = p.q_sums + at * (kGroups + 1) * 8;
+                if (there && !lo_word && 2 * t4 < kGroups) s0 = sums[2 * t4 * 8 + (row & 7)];
+                if (there && !lo_word && 2 * t4 + 1 < kGroups) s1 = sums[(2 * t4 + 1) * 8 + (row & 7)];
+                const __half2 hi = __floats2half2_rn(s0, s1);
+                qz[j][0] = u32(hi);
+                qz[j][1] = pack_half2(s0 - __low2float(hi), s1 - __high2float(hi));
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int rc = row_of(j, 2 * t4 + c), tok = rc / p.G;
+                    const bool in = rc < all_rows && tok < n;
+                    f[j][c] = in ? p.q_sums[(head * q_tiles + (rc >> 3)) * (kGroups + 1) * 8 + kGroups * 8 + (rc & 7)] : 0.f;
+                    lim[j][c] = in ? min(L + tok, key_hi) : -1;
+                }
+            }
         }
-        if (kSplitQ || Gm::kQShared) __syncthreads();
-        // keys [all_lo, all_hi] are visible to every present row of the tile (what an absent row
+        if (C::kQShared) __syncthreads();
+        // keys [all_lo, all_hi] are seen by every present row of the tile (what an absent row
         // computes is not used, and its q operand is zero)
-        const int all_hi = L + t_lo;
+        const int all_hi = min(L + t_lo, key_hi);
         const int all_lo = p.window > 0 ? L + t_hi - p.window + 1 : 0;
 
         // ------------------------------------------------------------ main loop
-        float acc[kTiles][D / 16][4], oz[kTiles][kGroups][2];
-        float m0[kTiles], m1[kTiles], l0[kTiles], l1[kTiles];
+        float acc[kTiles][D / 16][4], zl[kTiles][4];  // zl: sum P z of group g (2), sum P (2)
+        float ps[kTiles][2];                          // sum P s of group g over the complemented blocks
+        float ref[kSTiles][2], top[kSTiles][2];       // reference point of P, largest score
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
+        for (int j = 0; j < kTiles; ++j) {
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) acc[i][k][0] = acc[i][k][1] = acc[i][k][2] = acc[i][k][3] = 0.f;
-#pragma unroll
-            for (int y = 0; y < kGroups; ++y) oz[i][y][0] = oz[i][y][1] = 0.f;
-            m0[i] = m1[i] = kLowest;
-            l0[i] = l1[i] = 0.f;
+            for (int k = 0; k < D / 16; ++k) acc[j][k][0] = acc[j][k][1] = acc[j][k][2] = acc[j][k][3] = 0.f;
+            zl[j][0] = zl[j][1] = zl[j][2] = zl[j][3] = ps[j][0] = ps[j][1] = 0.f;
         }
-        int vexp = -40;          // P s is multiplied by 2^-vexp
-        float vinv = 0x1p40f;    // 2^-vexp
+#pragma unroll
+        for (int j = 0; j < kSTiles; ++j) {
+            ref[j][0] = ref[j][1] = 0.f;
+            top[j][0] = top[j][1] = kLowest;
+        }
+        bool fresh = true;  // some present row has seen no key yet: its reference is still to be set
+        float s_log = 0.f;                                 // log2 of the bound on the value scales
+        __half2 s_bound = __float2half2_rn(1.f);
 
         for (int i = 0; i < my_n && !dead; ++i) {
             const uint32_t slot = (it + i) % kStages;
@@ -307,154 +388,361 @@ __global__ void __launch_bounds__(kThreads, AttnGeo<D, kTiles, kSplitQ>::kCtas) 
                     if (!wait_bounded(bars + (it + k) % kStages * 8, ((it + k) / kStages) & 1)) break;
                 break;
             }
-            const uint32_t base = ring + slot * Gm::kBlockBytes;
-            const int key = (blk0 + warp + kWarps * i) * kKv4Block;
-            // scores, log2 units, relative to the running maximum
-            float s[kTiles][4];
+            const uint32_t stage = ring + slot * C::kStageBytes;
+            const int key0 = (blk0 + (warp + kWarps * i) * kSub) * kKv4Block;
+            const bool whole = key0 + kSub * kKv4Block - 1 <= all_hi && key0 >= all_lo;
+
+            // ---------------------------------------------------- scores against the reference
+            float x[kSub][kSTiles][4];
 #pragma unroll
-            for (int j = 0; j < kTiles; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-            const uint32_t kp = base + kv4_off_kparam(D) + g * (2 * kGroups * 4);
+            for (int u = 0; u < kSub; ++u) {
+                const uint32_t base = stage + u * C::kBlockBytes;
+                const uint32_t kp = base + kv4_off_kparam(D) + g * (2 * kGroups * 4);
+                uint32_t kw[2 * kGroups];  // params of keys g and g + 8
+                lds_params(kp, kw);
+                // minima of the groups whose sums this lane's k columns hold
+                constexpr int kPairs = (kGroups + 1) / 2;
+                const int y0 = 2 * (t4 % kPairs), y1 = min(y0 + 1, kGroups - 1);
+                const uint32_t za = high_halves(lds32(kp + y0 * 4), lds32(kp + y1 * 4));
+                const uint32_t zb = high_halves(lds32(kp + (kGroups + y0) * 4), lds32(kp + (kGroups + y1) * 4));
+                const uint32_t zf[4] = {za, zb, za, zb};
 #pragma unroll
-            for (int y = 0; y < kGroups; ++y) {
-                const uint2 w = lds64(base + y * 256 + lane * 8);
-                const float2 pa = half2_f(lds32(kp + y * 4)), pb = half2_f(lds32(kp + (kGroups + y) * 4));
-                uint32_t a[4], c[4];
-                code_frag(a, w.x);
-                code_frag(c, w.y);
-#pragma unroll
-                for (int j = 0; j < kTiles; ++j) {
-                    float d[4] = {0.f, 0.f, 0.f, 0.f};
-                    if constexpr (Gm::kQShared) {
-                        const uint4 q = q_s[(j * kGroups + y) * 32];
-                        Mma<__half>::run(d, a, q.x, q.y);
-                        Mma<__half>::run(d, c, q.z, q.w);
-                    } else {
-                        Mma<__half>::run(d, a, qf[j][y][0], qf[j][y][1]);
-                        Mma<__half>::run(d, c, qf[j][y][2], qf[j][y][3]);
-                    }
-                    if constexpr (kSplitQ) {
-                        const uint4 q = qlo_s[(j * kGroups + y) * 32];
-                        Mma<__half>::run(d, a, q.x, q.y);
-                        Mma<__half>::run(d, c, q.z, q.w);
-                    }
-                    s[j][0] += pa.x * d[0] + pa.y * qs[j][y][0];
-                    s[j][1] += pa.x * d[1] + pa.y * qs[j][y][1];
-                    s[j][2] += pb.x * d[2] + pb.y * qs[j][y][0];
-                    s[j][3] += pb.x * d[3] + pb.y * qs[j][y][1];
+                for (int j = 0; j < kSTiles; ++j) {
+                    x[u][j][0] = x[u][j][1] = x[u][j][2] = x[u][j][3] = 0.f;
+                    Mma<__half>::run(x[u][j], zf, qz[j][0], qz[j][1]);
                 }
-            }
-            const bool whole = key + kKv4Block - 1 <= all_hi && key >= all_lo;
-            const int ka = key + g, kb = ka + 8;
-            bool seen_a = true, seen_b = true;  // by some row: the block's stale rows hold anything
-            float over = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < kTiles; ++j) {
-                s[j][0] *= f0[j];
-                s[j][1] *= f1[j];
-                s[j][2] *= f0[j];
-                s[j][3] *= f1[j];
-                if (!whole) {
-                    const int w0 = p.window > 0 ? lim0[j] - p.window : -1, w1 = p.window > 0 ? lim1[j] - p.window : -1;
-                    if (ka > lim0[j] || ka <= w0) s[j][0] = -INFINITY;
-                    if (ka > lim1[j] || ka <= w1) s[j][1] = -INFINITY;
-                    if (kb > lim0[j] || kb <= w0) s[j][2] = -INFINITY;
-                    if (kb > lim1[j] || kb <= w1) s[j][3] = -INFINITY;
-                }
-                over = fmaxf(over, fmaxf(fmaxf(s[j][0], s[j][2]) - m0[j], fmaxf(s[j][1], s[j][3]) - m1[j]));
-            }
-            if (!whole) {
-                seen_a = ka <= key_hi && ka >= key_lo;
-                seen_b = kb <= key_hi && kb >= key_lo;
-            }
-            // this lane's keys' value params: scales 2^-vexp and minima
-            float va[kGroups], vb[kGroups], za[kGroups], zb[kGroups], top = 0.f;
-            const uint32_t vp = base + kv4_off_vparam(D) + g * (2 * kGroups * 4);
-#pragma unroll
-            for (int y = 0; y < kGroups; ++y) {
-                const float2 pa = half2_f(lds32(vp + y * 4)), pb = half2_f(lds32(vp + (kGroups + y) * 4));
-                va[y] = seen_a ? pa.x : 0.f;
-                vb[y] = seen_b ? pb.x : 0.f;
-                za[y] = seen_a ? pa.y : 0.f;
-                zb[y] = seen_b ? pb.y : 0.f;
-                top = fmaxf(top, fmaxf(va[y], vb[y]));
-            }
-            if (__any_sync(0xffffffffu, over > kSlack || top * vinv > 128.f)) {
-                // move the reference points: the maxima of the rows and the power of two of P s
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                float vscale = 1.f;
-                if (top * vinv > 128.f) {
-                    const int e = ilogbf(top) - 6;  // top 2^-e in [2^6, 2^7)
-                    vscale = exp2f((float)(vexp - e));
-                    vexp = e;
-                    vinv = exp2f((float)-e);
-                }
-#pragma unroll
-                for (int j = 0; j < kTiles; ++j) {
-                    float a0 = fmaxf(s[j][0], s[j][2]), a1 = fmaxf(s[j][1], s[j][3]);
-#pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) {
-                        a0 = fmaxf(a0, __shfl_xor_sync(0xffffffffu, a0, o));
-                        a1 = fmaxf(a1, __shfl_xor_sync(0xffffffffu, a1, o));
-                    }
-                    a0 = fmaxf(a0, m0[j]);
-                    a1 = fmaxf(a1, m1[j]);
-                    const float k0 = fast_exp2(m0[j] - a0), k1 = fast_exp2(m1[j] - a1);
-                    m0[j] = a0;
-                    m1[j] = a1;
-                    l0[j] *= k0;
-                    l1[j] *= k1;
-#pragma unroll
-                    for (int y = 0; y < kGroups; ++y) {
-                        oz[j][y][0] *= k0;
-                        oz[j][y][1] *= k1;
-                    }
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        acc[j][k][0] *= k0 * vscale;
-                        acc[j][k][1] *= k1 * vscale;
-                        acc[j][k][2] *= k0 * vscale;
-                        acc[j][k][3] *= k1 * vscale;
-                    }
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < kTiles; ++j) {
-                s[j][0] = fast_exp2(s[j][0] - m0[j]);
-                s[j][1] = fast_exp2(s[j][1] - m1[j]);
-                s[j][2] = fast_exp2(s[j][2] - m0[j]);
-                s[j][3] = fast_exp2(s[j][3] - m1[j]);
-                l0[j] += s[j][0] + s[j][2];
-                l1[j] += s[j][1] + s[j][3];
-            }
-            // kSel: some rows of the tile do not see some of the block's keys, whose params may be NaN:
-            // a probability of zero then counts as nothing, not as 0 * NaN
-            auto values = [&](auto sel) {
-                auto times = [](float pr, float x) { return decltype(sel)::value && pr == 0.f ? 0.f : pr * x; };
 #pragma unroll
                 for (int y = 0; y < kGroups; ++y) {
-                    const uint2 w = lds64(base + kv4_off_v(D) + y * 256 + lane * 8);
+                    const uint2 w = lds64(base + y * 256 + lane * 8);
                     uint32_t a[4], c[4];
                     code_frag(a, w.x);
                     code_frag(c, w.y);
+                    const float sa = __low2float(h2(kw[y])), sb = __low2float(h2(kw[kGroups + y]));
+                    float d[kSTiles][4];
+#pragma unroll
+                    for (int j = 0; j < kTiles; ++j) {
+                        float* dj = d[kSplit == 2 ? 0 : j];
+                        if (kSplit != 2 || j == 0) dj[0] = dj[1] = dj[2] = dj[3] = 0.f;
+                        if constexpr (C::kQShared) {
+                            const uint4 q = q_s[(j * kGroups + y) * 32];
+                            Mma<__half>::run(dj, a, q.x, q.y);
+                            Mma<__half>::run(dj, c, q.z, q.w);
+                        } else {
+                            Mma<__half>::run(dj, a, qf[j][y][0], qf[j][y][1]);
+                            Mma<__half>::run(dj, c, qf[j][y][2], qf[j][y][3]);
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < kSTiles; ++j) {
+                        x[u][j][0] += sa * d[j][0];
+                        x[u][j][1] += sa * d[j][1];
+                        x[u][j][2] += sb * d[j][2];
+                        x[u][j][3] += sb * d[j][3];
+                    }
+                }
+            }
+            float over = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) {
+                const int ka = key0 + u * kKv4Block + g, kb = ka + 8;
+#pragma unroll
+                for (int j = 0; j < kSTiles; ++j) {
+                    if constexpr (kSplit == 1) {  // hi and lo columns: lanes t and t ^ 2
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[u][j][e] += __shfl_xor_sync(0xffffffffu, x[u][j][e], 2);
+                    }
+                    x[u][j][0] = fmaf(x[u][j][0], f[j][0], -ref[j][0]);
+                    x[u][j][1] = fmaf(x[u][j][1], f[j][1], -ref[j][1]);
+                    x[u][j][2] = fmaf(x[u][j][2], f[j][0], -ref[j][0]);
+                    x[u][j][3] = fmaf(x[u][j][3], f[j][1], -ref[j][1]);
+                    if (!whole) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int key = e < 2 ? ka : kb, hi = lim[j][e & 1];
+                            // lim is cut at the piece's end: the window counts from the row's own position
+                            const int own = L + row_of(j, 2 * t4 + (e & 1)) / p.G;
+                            if (key > hi || (p.window > 0 && key <= own - p.window)) x[u][j][e] = -INFINITY;
+                        }
+                    }
+                    over = fmaxf(over, fmaxf(fmaxf(x[u][j][0], x[u][j][2]), fmaxf(x[u][j][1], x[u][j][3])));
+                }
+            }
+
+            // ---------------------------------------------------- value params
+            // sv[u][h][y]: scales of keys 2t + 8h and 2t + 8h + 1, group y
+            // zv, gv: minima and scales of these keys in group g, the A operands of their sums
+            uint32_t sv[kSub][2][C::kRegroup ? 1 : kGroups], zv[kSub][2], gv[kSub][2];
+            __half2 s_top = __float2half2_rn(0.f);
+            auto regroup = [&](int u, bool clean) {  // head dim 256: pairs of keys side by side, in shared memory
+                uint32_t w[4];  // key (lane >> 2) + 8 ((lane >> 1) & 1), groups 4 (lane & 1) + 0 .. 3
+                lds128(stage + u * C::kBlockBytes + kv4_off_vparam(D) + lane * 16, w);
+                if (!whole) {
+                    const int key = key0 + u * kKv4Block + g + 8 * ((lane >> 1) & 1);
+                    if (key < key_lo || key > key_hi) w[0] = w[1] = w[2] = w[3] = 0;
+                }
+                if (clean) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = no_nan(w[e]);
+                }
+                const bool odd = g & 1;
+                const uint32_t r0 = __shfl_xor_sync(0xffffffffu, odd ? w[0] : w[2], 4);
+                const uint32_t r1 = __shfl_xor_sync(0xffffffffu, odd ? w[1] : w[3], 4);
+                // the even key's lane makes groups 4 (lane & 1) + 0, 1, the odd one's + 2, 3
+                const uint32_t e0 = odd ? r0 : w[0], e1 = odd ? r1 : w[1], o0 = odd ? w[2] : r0, o1 = odd ? w[3] : r1;
+                const uint32_t s0 = low_halves(e0, o0), s1 = low_halves(e1, o1);
+                s_top = __hmax2_nan(s_top, __hmax2_nan(h2(s0), h2(s1)));
+                __syncwarp();  // every lane has read what was there
+                const uint32_t at = pairs + ((4 * (lane & 1) + 2 * odd) * 8 + (g >> 1) * 2 + ((lane >> 1) & 1)) * 4;
+                sts32(at, s0);
+                sts32(at + 32, s1);
+                sts32(at + 256, high_halves(e0, o0));
+                sts32(at + 288, high_halves(e1, o1));
+                __syncwarp();
+                const uint2 z = lds64(pairs + 256 + (g * 4 + t4) * 8);
+                zv[u][0] = z.x;
+                zv[u][1] = z.y;
+                const uint2 sg = lds64(pairs + (g * 4 + t4) * 8);
+                gv[u][0] = sg.x;
+                gv[u][1] = sg.y;
+            };
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) {
+                if constexpr (C::kRegroup) {
+                    regroup(u, false);
+                } else {
+                    const uint32_t vp = stage + u * C::kBlockBytes + kv4_off_vparam(D);
+                    uint32_t wa[2 * kGroups], wb[2 * kGroups];  // keys 2t, 2t + 1 (and + 8)
+                    lds_params(vp + 2 * t4 * (2 * kGroups * 4), wa);
+                    lds_params(vp + (2 * t4 + 1) * (2 * kGroups * 4), wb);
+                    const uint32_t gz = vp + (2 * t4 * 2 * kGroups + min(g, kGroups - 1)) * 4;
+                    const uint32_t w0 = lds32(gz), w1 = lds32(gz + 2 * kGroups * 4);
+                    const uint32_t w2 = lds32(gz + kGroups * 4), w3 = lds32(gz + 3 * kGroups * 4);
+                    uint32_t z0 = high_halves(w0, w1), z1 = high_halves(w2, w3);
+                    uint32_t g0 = low_halves(w0, w1), g1 = low_halves(w2, w3);
+                    uint32_t m0 = 0xffffffffu, m1 = 0xffffffffu;
+                    if (!whole) {
+                        const int key = key0 + u * kKv4Block + 2 * t4;
+                        auto in = [&](int k) { return k >= key_lo && k <= key_hi; };
+                        m0 = (in(key) ? 0xffffu : 0u) | (in(key + 1) ? 0xffff0000u : 0u);
+                        m1 = (in(key + 8) ? 0xffffu : 0u) | (in(key + 9) ? 0xffff0000u : 0u);
+                        z0 &= m0;
+                        z1 &= m1;
+                        g0 &= m0;
+                        g1 &= m1;
+                    }
+#pragma unroll
+                    for (int y = 0; y < kGroups; ++y) {
+                        sv[u][0][y] = low_halves(wa[y], wb[y]);
+                        sv[u][1][y] = low_halves(wa[kGroups + y], wb[kGroups + y]);
+                        if (!whole) {
+                            sv[u][0][y] &= m0;
+                            sv[u][1][y] &= m1;
+                        }
+                        s_top = __hmax2_nan(s_top, __hmax2_nan(h2(sv[u][0][y]), h2(sv[u][1][y])));
+                    }
+                    zv[u][0] = z0;
+                    zv[u][1] = z1;
+                    gv[u][0] = g0;
+                    gv[u][1] = g1;
+                }
+            }
+
+            // ---------------------------------------------------- rarely: move the reference point
+            if (fresh || __any_sync(0xffffffffu, over > 15.f - s_log || !__hble2(s_top, s_bound))) {
+                float sm = fmaxf(__low2float(s_top), __high2float(s_top));
+                sm = warp_max(__hisnan(__low2half(s_top)) || __hisnan(__high2half(s_top)) ? INFINITY : sm);
+                if (isinf(sm)) {
+                    // A seen key holds NaN in some group of its value: the group is NaN for the rows
+                    // that see the key, and counts as zero in the products, whose columns share it.
+#pragma unroll
+                    for (int u = 0; u < kSub; ++u) {
+                        const uint32_t vp = stage + u * C::kBlockBytes + kv4_off_vparam(D) + g * (2 * kGroups * 4);
+#pragma unroll
+                        for (int y = 0; y < kGroups; ++y) {
+                            const bool na = (lds32(vp + y * 4) & 0x7fffu) > 0x7c00u;
+                            const bool nb = (lds32(vp + (kGroups + y) * 4) & 0x7fffu) > 0x7c00u;
+#pragma unroll
+                            for (int j = 0; j < kSTiles; ++j) {
+                                unsigned hit = 0;  // bit per column
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    if ((e < 2 ? na : nb) && x[u][j][e] != -INFINITY) hit |= 1u << (2 * t4 + (e & 1));
+                                hit = __reduce_or_sync(0xffffffffu, hit);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    if (hit >> (2 * t4 + (e & 1)) & 1) acc[j][2 * y][e] = acc[j][2 * y + 1][e] = nan_f();
+                            }
+                        }
+                        if constexpr (C::kRegroup) {
+                            s_top = __float2half2_rn(0.f);
+                            regroup(u, true);
+                        } else {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                zv[u][h] = no_nan(zv[u][h]);
+                                gv[u][h] = no_nan(gv[u][h]);
+#pragma unroll
+                                for (int y = 0; y < kGroups; ++y) sv[u][h][y] = no_nan(sv[u][h][y]);
+                            }
+                        }
+                    }
+                    if constexpr (!C::kRegroup) {
+                        s_top = __float2half2_rn(0.f);
+#pragma unroll
+                        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+                            for (int y = 0; y < kGroups; ++y)
+                                s_top = __hmax2(s_top, __hmax2(h2(sv[u][0][y]), h2(sv[u][1][y])));
+                    }
+                    sm = warp_max(fmaxf(__low2float(s_top), __high2float(s_top)));
+                }
+                if (sm > __low2float(s_bound)) {  // the next power of two, at most 2^12 (2^16 / 15)
+                    s_log = (float)(ilogbf(sm) + 1);
+                    s_bound = __float2half2_rn(exp2f(s_log));
+                }
+                bool unset = false;
+#pragma unroll
+                for (int j = 0; j < kSTiles; ++j) {
+                    float keep[2];
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float m = -INFINITY;
+#pragma unroll
+                        for (int u = 0; u < kSub; ++u) m = fmaxf(m, fmaxf(x[u][j][c], x[u][j][c + 2]));
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                        const float was = top[j][c];
+                        top[j][c] = fmaxf(was, m + ref[j][c]);
+                        const float to = top[j][c] == kLowest ? 0.f : top[j][c] - 7.f + s_log, shift = ref[j][c] - to;
+                        keep[c] = was == kLowest ? 0.f : fast_exp2(shift);
+                        ref[j][c] = to;
+                        unset |= top[j][c] == kLowest && lim[j][c] >= 0;
+#pragma unroll
+                        for (int u = 0; u < kSub; ++u) {
+                            x[u][j][c] += shift;
+                            x[u][j][c + 2] += shift;
+                        }
+                    }
+                    constexpr int kBoth = kSplit == 2 ? 2 : 1;  // tile 1 holds the same columns' lo words
+#pragma unroll
+                    for (int e = 0; e < kBoth; ++e) {
+                        const int jt = kSplit == 2 ? e : j;
+#pragma unroll
+                        for (int k = 0; k < D / 16; ++k) {
+                            acc[jt][k][0] *= keep[0];
+                            acc[jt][k][1] *= keep[1];
+                            acc[jt][k][2] *= keep[0];
+                            acc[jt][k][3] *= keep[1];
+                        }
+                        zl[jt][0] *= keep[0];
+                        zl[jt][1] *= keep[1];
+                        zl[jt][2] *= keep[0];
+                        zl[jt][3] *= keep[1];
+                        ps[jt][0] *= keep[0];
+                        ps[jt][1] *= keep[1];
+                    }
+                }
+                fresh = __any_sync(0xffffffffu, unset);
+            }
+
+            // ---------------------------------------------------- P, and the second product
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) {
+                // B operands: P of keys 0..7 and 8..15 of the block (hi words; lo words where kept)
+                uint32_t ph[kSTiles][2], pl[kSplit ? kSTiles : 1][2];
+#pragma unroll
+                for (int j = 0; j < kSTiles; ++j) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float p0 = fast_exp2(x[u][j][2 * h]), p1 = fast_exp2(x[u][j][2 * h + 1]);
+                        const __half2 hi = __floats2half2_rn(p0, p1);
+                        ph[j][h] = movmatrix_trans(u32(hi));
+                        if constexpr (kSplit != 0)
+                            pl[j][h] = movmatrix_trans(pack_half2(p0 - __low2float(hi), p1 - __high2float(hi)));
+                    }
+                }
+                const bool flip = kSub == 2 ? u == 1 : (i & 1) != 0;
+                // zl += [z^T; 1] P, and for a complemented block ps += s^T P
+                uint32_t pz[kTiles][2];
+#pragma unroll
+                for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if constexpr (kSplit == 0) pz[j][h] = ph[j][h];
+                        else if constexpr (kSplit == 1) pz[j][h] = g >= 4 ? pl[0][h] : ph[0][h];
+                        else pz[j][h] = j ? pl[0][h] : ph[0][h];
+                    }
+#pragma unroll
+                for (int j = 0; j < kTiles; ++j) {
+                    const uint32_t zf[4] = {zv[u][0], kOnes, zv[u][1], kOnes};
+                    float d[4] = {0.f, 0.f, 0.f, 0.f};
+                    Mma<__half>::run(d, zf, pz[j][0], pz[j][1]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) zl[j][e] += d[e];
+                    if (flip) {
+                        const uint32_t gf[4] = {gv[u][0], 0u, gv[u][1], 0u};
+                        float c[4] = {0.f, 0.f, 0.f, 0.f};
+                        Mma<__half>::run(c, gf, pz[j][0], pz[j][1]);
+                        ps[j][0] += c[0];
+                        ps[j][1] += c[1];
+                    }
+                }
+                const uint32_t flip_codes = flip ? 0xffffffffu : 0u, flip_sign = flip ? 0x80008000u : 0u;
+                uint32_t pa[2], pb[2];  // kSplit 1: the words of the lo columns, zero in the others
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int j = 0; j < kSTiles; ++j) {
+                        ph[j][h] ^= flip_sign;
+                        if constexpr (kSplit != 0) pl[j][h] ^= flip_sign;
+                    }
+                    if constexpr (kSplit == 1) {
+                        pa[h] = g >= 4 ? ph[0][h] : 0u;
+                        pb[h] = g >= 4 ? pl[0][h] : 0u;
+                    }
+                }
+#pragma unroll
+                for (int y = 0; y < kGroups; ++y) {
+                    const uint2 w = lds64(stage + u * C::kBlockBytes + kv4_off_v(D) + y * 256 + lane * 8);
+                    uint32_t a[4], c[4];
+                    code_frag(a, w.x, flip_codes);
+                    code_frag(c, w.y, flip_codes);
                     // V^T's tile has the channel as its row: registers in the order (channel g, keys 2t),
                     // (g + 8, 2t), (g, 2t + 8), (g + 8, 2t + 8)
                     const uint32_t av[4] = {a[0], a[2], a[1], a[3]}, cv[4] = {c[0], c[2], c[1], c[3]};
-                    const float fa = va[y] * vinv, fb = vb[y] * vinv;
+                    uint32_t s[2];
+                    if constexpr (C::kRegroup) {
+                        const uint2 sp = lds64(pairs + (y * 4 + t4) * 8);
+                        s[0] = sp.x;
+                        s[1] = sp.y;
+                    } else {
+                        s[0] = sv[u][0][y];
+                        s[1] = sv[u][1][y];
+                    }
+                    uint32_t bf[kTiles][2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const __half2 sc = h2(s[h]);
+                        if constexpr (kSplit == 0) {
+#pragma unroll
+                            for (int j = 0; j < kTiles; ++j) bf[j][h] = u32(__hmul2(h2(ph[j][h]), sc));
+                        } else if constexpr (kSplit == 1) {
+                            const __half2 hi = __hmul2(h2(pa[h]), sc);  // lo columns: what the hi column holds
+                            bf[0][h] = u32(__hfma2(h2(pb[h]), sc, __hfma2(h2(ph[0][h]), sc, __hneg2(hi))));
+                        } else {
+                            const __half2 hi = __hmul2(h2(ph[0][h]), sc);
+                            bf[0][h] = u32(hi);
+                            bf[1][h] = u32(__hfma2(h2(pl[0][h]), sc, __hfma2(h2(ph[0][h]), sc, __hneg2(hi))));
+                        }
+                    }
 #pragma unroll
                     for (int j = 0; j < kTiles; ++j) {
-                        oz[j][y][0] += times(s[j][0], za[y]) + times(s[j][2], zb[y]);
-                        oz[j][y][1] += times(s[j][1], za[y]) + times(s[j][3], zb[y]);
-                        const uint32_t p0 = movmatrix_trans(pack_half2(times(s[j][0], fa), times(s[j][1], fa)));
-                        const uint32_t p1 = movmatrix_trans(pack_half2(times(s[j][2], fb), times(s[j][3], fb)));
-                        Mma<__half>::run(acc[j][2 * y], av, p0, p1);
-                        Mma<__half>::run(acc[j][2 * y + 1], cv, p0, p1);
+                        Mma<__half>::run(acc[j][2 * y], av, bf[j][0], bf[j][1]);
+                        Mma<__half>::run(acc[j][2 * y + 1], cv, bf[j][0], bf[j][1]);
                     }
                 }
-            };
-            if (!whole && p.T > 1) values(std::true_type{});
-            else values(std::false_type{});
-            __syncwarp();  // every lane has read the slot
+            }
+            __syncwarp();  // every lane has read the stage
             fill(issued + 1);
         }
         it += my_n;
@@ -464,39 +752,42 @@ __global__ void __launch_bounds__(kThreads, AttnGeo<D, kTiles, kSplitQ>::kCtas) 
 
         // ------------------------------------------------------------ epilogue
 #pragma unroll
-        for (int j = 0; j < kTiles; ++j) {
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) {
-                l0[j] += __shfl_xor_sync(0xffffffffu, l0[j], o);
-                l1[j] += __shfl_xor_sync(0xffffffffu, l1[j], o);
-#pragma unroll
-                for (int y = 0; y < kGroups; ++y) {
-                    oz[j][y][0] += __shfl_xor_sync(0xffffffffu, oz[j][y][0], o);
-                    oz[j][y][1] += __shfl_xor_sync(0xffffffffu, oz[j][y][1], o);
-                }
-            }
-            // unnormalised O in [d][row] pairs, the row index XOR-swizzled by (d >> 2) & 7 as in
+        for (int j = 0; j < kSTiles; ++j) {
+            // unnormalised O in [d][column] pairs, the column index XOR-swizzled by (d >> 2) & 7 as in
             // decode_tc.cu: pair stores and reads along d are free of bank conflicts
-            float* mw = merge_s + (warp * kTiles + j) * 8 * D;
-            const float lo = exp2f((float)(vexp + 24)), hi = exp2f((float)(vexp + 20));
+            float* mw = merge_s + (warp * kSTiles + j) * 8 * D;
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
+                float z0 = fmaf(15.f, ps[j][0], zl[j][0]), z1 = fmaf(15.f, ps[j][1], zl[j][1]);
+                if constexpr (kSplit == 2) {
+                    z0 += fmaf(15.f, ps[1][0], zl[1][0]);
+                    z1 += fmaf(15.f, ps[1][1], zl[1][1]);
+                }
+                z0 = __shfl_sync(0xffffffffu, z0, (k / 2) * 4 + t4);
+                z1 = __shfl_sync(0xffffffffu, z1, (k / 2) * 4 + t4);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int d = 16 * k + g + 8 * h, x = (d >> 2) & 7;
-                    const float u = acc[j][k][2 * h] * (h ? hi : lo) + oz[j][k / 2][0];
-                    const float v = acc[j][k][2 * h + 1] * (h ? hi : lo) + oz[j][k / 2][1];
-                    *reinterpret_cast<float2*>(mw + d * 8 + ((2 * t4) ^ (x & 6))) =
-                        (x & 1) ? make_float2(v, u) : make_float2(u, v);
+                    const int d = 16 * k + g + 8 * h, sw = (d >> 2) & 7;
+                    float u = acc[j][k][2 * h], v = acc[j][k][2 * h + 1];
+                    if constexpr (kSplit == 2) {
+                        u += acc[1][k][2 * h];
+                        v += acc[1][k][2 * h + 1];
+                    }
+                    u = fmaf(u, h ? 0x1p20f : 0x1p24f, z0);
+                    v = fmaf(v, h ? 0x1p20f : 0x1p24f, z1);
+                    *reinterpret_cast<float2*>(mw + d * 8 + ((2 * t4) ^ (sw & 6))) =
+                        (sw & 1) ? make_float2(v, u) : make_float2(u, v);
                 }
             }
             if (g == 0) {
-                const bool nan = bad || dead;
-                float* ml = ml_s + ((warp * kTiles + j) * 8 + 2 * t4) * 2;
-                ml[0] = m0[j];
-                ml[1] = nan ? __int_as_float(0x7fc00000) : l0[j];
-                ml[2] = m1[j];
-                ml[3] = nan ? __int_as_float(0x7fc00000) : l1[j];
+                float* ml = ml_s + ((warp * kSTiles + j) * 8 + 2 * t4) * 2;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float l = zl[j][2 + c];
+                    if constexpr (kSplit == 2) l += zl[1][2 + c];
+                    ml[2 * c] = top[j][c] == kLowest ? kLowest : ref[j][c];
+                    ml[2 * c + 1] = bad || dead ? nan_f() : l;
+                }
             }
         }
         __syncthreads();
@@ -504,13 +795,13 @@ __global__ void __launch_bounds__(kThreads, AttnGeo<D, kTiles, kSplitQ>::kCtas) 
         if (tid < kRows) {
             float M = kLowest, l = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ml_s[(w * kRows + tid) * 2]);
+            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ml_s[(w * kCols + tid) * 2]);
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                float* ml = ml_s + (w * kRows + tid) * 2;
-                const float x = fast_exp2(ml[0] - M);
-                l += x * ml[1];
-                ml[0] = x;
+                float* ml = ml_s + (w * kCols + tid) * 2;
+                const float k = fast_exp2(ml[0] - M);
+                l += k * (kSplit == 1 ? ml[1] + ml[9] : ml[1]);  // columns 4 further on hold the lo words
+                ml[0] = k;
             }
             ml_s[tid * 2 + 1] = l;
             if (n_split > 1) {
@@ -522,16 +813,20 @@ __global__ void __launch_bounds__(kThreads, AttnGeo<D, kTiles, kSplitQ>::kCtas) 
         const int row0 = rt * kRows;
         auto put = [&](int row, int d, float v) {
             const int q_row = row0 + row, tok = q_row / p.G;
-            if (tok < n)
+            if (q_row < all_rows && tok < n)
                 store_from_float(p.o, (((int64_t)b * p.T + tok) * p.Hq + kvh * p.G + q_row - tok * p.G) * D + d, v,
                                  p.act_dtype);
         };
         for (int e = tid; e < kRows * D; e += kThreads) {
-            const int row = e / D, d = e - row * D;
-            const float* mw = merge_s + (row >> 3) * 8 * D + d * 8 + ((row & 7) ^ ((d >> 2) & 7));
+            const int row = e / D, d = e - row * D, sw = (d >> 2) & 7;
+            const float* mw = merge_s + (row >> 3) * 8 * D + d * 8;
             float o = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) o += ml_s[(w * kRows + row) * 2] * mw[w * kRows * D];
+            for (int w = 0; w < kWarps; ++w) {
+                float v = mw[w * kCols * D + ((row & 7) ^ sw)];
+                if constexpr (kSplit == 1) v += mw[w * kCols * D + ((row + 4) ^ sw)];
+                o += ml_s[(w * kCols + row) * 2] * v;
+            }
             if (n_split == 1) put(row, d, o / ml_s[row * 2 + 1]);
             else slot[row * D + d] = o;
         }
@@ -594,50 +889,52 @@ __global__ void __launch_bounds__(kThreads, AttnGeo<D, kTiles, kSplitQ>::kCtas) 
 
 struct LaunchInfo {
     int grid = 0;
-    int occ = 0;
 };
 
 // Kernel attributes, set up once for each device (the caller has made `device` current).
-template <int D, int kTiles, bool kSplitQ>
+template <typename C>
 LaunchInfo launch_info(int device) {
     constexpr int kMaxDevices = 64;
     static std::once_flag once[kMaxDevices];
     static LaunchInfo info[kMaxDevices];
     if (device < 0 || device >= kMaxDevices) return LaunchInfo{};
     std::call_once(once[device], [device] {
-        auto kern = kv4_attn_kernel<D, kTiles, kSplitQ>;
-        const size_t smem = AttnGeo<D, kTiles, kSplitQ>::total(kKv4MaxBatch);
+        auto kern = kv4_attn_kernel<C>;
         int occ = 0, sms = 0;
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return;
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, kThreads, AttnGeo<D, kTiles, kSplitQ>::total(256)) !=
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::total(kKv4MaxBatch)) !=
             cudaSuccess)
             return;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, kThreads, C::total(256)) != cudaSuccess) return;
         if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return;
-        info[device].occ = occ;
         info[device].grid = occ * sms;
     });
     return info[device];
 }
 
-// Calls f with the instantiation for (D, rows per sequence and kv head, fp16).
+// Calls f with the instantiation for (D, query rows per sequence and kv head, element type): fp16
+// results carry q and P as two words; bf16 ones take 16 columns where there are as many rows (a
+// cache byte then serves twice as many), except at head dim 256, whose accumulators fill the
+// registers with 8.
 template <typename F>
-cudaError_t dispatch(int D, int rows, int act_dtype, F&& f) {
-    auto by_type = [&](auto d, auto tiles) {
-        return act_dtype == kF16 ? f(d, tiles, std::true_type{}) : f(d, tiles, std::false_type{});
-    };
+cudaError_t dispatch(const Kv4Params& p, F&& f) {
+    const int rows = p.T * p.G;
     auto by_rows = [&](auto d) {
-        return rows <= 8 ? by_type(d, std::integral_constant<int, 1>{}) : by_type(d, std::integral_constant<int, 2>{});
+        constexpr int D = decltype(d)::value;
+        if (p.act_dtype == kF16) return rows <= 4 ? f(Cfg<D, 1, 1>{}) : f(Cfg<D, 2, 2>{});
+        if constexpr (D < 256)
+            if (rows > 8) return f(Cfg<D, 2, 0>{});
+        return f(Cfg<D, 1, 0>{});
     };
-    switch (D) {
+    switch (p.D) {
         case 64: return by_rows(std::integral_constant<int, 64>{});
         case 96: return by_rows(std::integral_constant<int, 96>{});
         case 128: return by_rows(std::integral_constant<int, 128>{});
-        case 256: return by_type(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{});
+        case 256: return by_rows(std::integral_constant<int, 256>{});
         default: return cudaErrorInvalidValue;
     }
 }
 
-// 8-row tiles of q per (sequence, kv head), and the bytes of one tile's operand words.
+// 8-row tiles of q per (sequence, kv head).
 int q_tiles_of(const Kv4Params& p) { return (p.T * p.G + 7) / 8; }
 
 }  // namespace
@@ -648,35 +945,32 @@ size_t kv4_frag_bytes(const Kv4Params& p) {
 size_t kv4_sums_bytes(const Kv4Params& p) { return (size_t)q_tiles_of(p) * p.Hkv * (p.D / 32 + 1) * 8 * 4; }
 
 void kv4_attn_workspace(const Kv4Params& p, int device, size_t* partial_bytes, size_t* units_per_seq) {
-    const int rows = p.T * p.G;
     *partial_bytes = 0;
-    dispatch(p.D, rows, p.act_dtype, [&](auto d, auto tiles, auto split) {
-        constexpr int kD = decltype(d)::value, kT = decltype(tiles)::value;
-        const LaunchInfo li = launch_info<kD, kT, decltype(split)::value>(device);
-        *partial_bytes = (size_t)2 * li.grid * 8 * kT * (kD + 2) * sizeof(float);
-        *units_per_seq = (size_t)p.Hkv * ((rows + 8 * kT - 1) / (8 * kT));
+    dispatch(p, [&](auto cfg) {
+        using C = decltype(cfg);
+        *partial_bytes = (size_t)2 * launch_info<C>(device).grid * C::kRows * (C::D + 2) * sizeof(float);
+        *units_per_seq = (size_t)p.Hkv * ((p.T * p.G + C::kRows - 1) / C::kRows);
         return cudaSuccess;
     });
 }
 
 cudaError_t launch_kv4_attn(const Kv4Params& p, int device, cudaStream_t stream) {
-    return dispatch(p.D, p.T * p.G, p.act_dtype, [&](auto d, auto tiles, auto split) {
-        constexpr int kD = decltype(d)::value, kT = decltype(tiles)::value;
-        auto kern = kv4_attn_kernel<kD, kT, decltype(split)::value>;
-        const LaunchInfo li = launch_info<kD, kT, decltype(split)::value>(device);
+    return dispatch(p, [&](auto cfg) {
+        using C = decltype(cfg);
+        const LaunchInfo li = launch_info<C>(device);
         if (li.grid <= 0) return cudaErrorInvalidConfiguration;
         // launched with programmatic serialisation behind the preparation kernel
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)li.grid);
-        cfg.blockDim = dim3(kThreads);
-        cfg.dynamicSmemBytes = AttnGeo<kD, kT, decltype(split)::value>::total(p.B);
-        cfg.stream = stream;
+        cudaLaunchConfig_t launch = {};
+        launch.gridDim = dim3((unsigned)li.grid);
+        launch.blockDim = dim3(kThreads);
+        launch.dynamicSmemBytes = C::total(p.B);
+        launch.stream = stream;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        return cudaLaunchKernelEx(&cfg, kern, p);
+        launch.attrs = attr;
+        launch.numAttrs = 1;
+        return cudaLaunchKernelEx(&launch, kv4_attn_kernel<C>, p);
     });
 }
 
