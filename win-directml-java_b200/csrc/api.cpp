@@ -61,7 +61,7 @@ struct b2a_context {
     double kv4_inv_freq[kMaxHeadDim / 2] = {};
     double kv4_theta = 0.0;
     int kv4_inv_dim = 0;
-    // paged 4-bit cache: [merge counters][partial slots][q operands][q sums]
+    // paged 4-bit cache: [merge counters][partial slots][plan][q operands][q sums]
     void* kv4_ws = nullptr;
     size_t kv4_ws_bytes = 0;
     size_t kv4_counter_bytes = 0;
@@ -1143,6 +1143,8 @@ int check_kv4_cache(b2a_context* ctx, const b2a_kv4_cache* cache, Kv4Params& p) 
         return fail(ctx, B2A_EINVAL, "num_pages and max_pages must be > 0");
     if ((int64_t)cache->max_pages * ps > INT32_MAX)
         return fail(ctx, B2A_EINVAL, "max_pages * page_size exceeds the position range");
+    if ((int64_t)cache->num_pages * cache->num_kv_heads * (ps / 16) > INT32_MAX)
+        return fail(ctx, B2A_EINVAL, "the pool exceeds 2^31 blocks of 16 positions");
     if (!aligned16(cache->pages)) return fail(ctx, B2A_EINVAL, "the pages must be 16-byte aligned");
     p.pages = static_cast<uint8_t*>(cache->pages);
     p.page_table = cache->page_table;
@@ -1225,38 +1227,56 @@ int check_kv4_query(b2a_context* ctx, const void* q, int64_t q_stride, int Hq, f
     return B2A_OK;
 }
 
-// The preparation (q's operands, and the append where p has new rows), then the attention, at most
-// kKv4MaxBatch sequences and 2^31 blocks of the split's stream at a time.
+// The preparation (q's operands, the plan, and the append where p has new rows), then the attention,
+// at most kKv4MaxBatch sequences and 2^31 blocks of the split's stream at a time.
 int run_kv4_attention(b2a_context* ctx, Kv4Params& p, cudaStream_t stream) {
     DeviceGuard guard(ctx->device);
     auto r256 = [](size_t x) { return (x + 255) / 256 * 256; };
     const int64_t seq_blocks = (int64_t)p.max_pages * p.page_size / 16 + 1 + kKv4GapBlocksMax;
     const int per_launch = (int)std::max<int64_t>(1, std::min<int64_t>(kKv4MaxBatch, INT32_MAX / seq_blocks));
-    size_t partial_bytes = 0, units_per_seq = 0, counter_bytes = 0;
-    kv4_attn_workspace(p, ctx->device, &partial_bytes, &units_per_seq);
-    if (partial_bytes == 0) return fail(ctx, B2A_ECUDA, "no attention kernel for this device");
-    const size_t counters = (size_t)std::min(p.B, per_launch) * units_per_seq;
-    const size_t part = r256(partial_bytes), frag = r256(kv4_frag_bytes(p) * p.B), sums = r256(kv4_sums_bytes(p) * p.B);
-    const int rc = ensure_counted_buffer(ctx, &ctx->kv4_ws, &ctx->kv4_ws_bytes, &ctx->kv4_counter_bytes, counters,
-                                         part + frag + sums, "4-bit cache attention", stream, false, &counter_bytes);
+    p.split = kv4_attn_split(p, ctx->device);
+    if (p.split.n_cta <= 0) return fail(ctx, B2A_ECUDA, "no attention kernel for this device");
+    const int B = p.B, most = std::min(B, per_launch);
+    const size_t units = (size_t)most * p.split.per_seq;
+    const size_t part = r256(p.split.partial_bytes), head = r256(p.split.n_cta * sizeof(int2)),
+                 plan = r256((p.split.n_cta + units) * sizeof(Kv4Piece)), frag = r256(kv4_frag_bytes(p) * most),
+                 sums = r256(kv4_sums_bytes(p) * most);
+    size_t counter_bytes = 0;
+    const int rc = ensure_counted_buffer(ctx, &ctx->kv4_ws, &ctx->kv4_ws_bytes, &ctx->kv4_counter_bytes, units,
+                                         part + head + plan + frag + sums, "4-bit cache attention", stream, false,
+                                         &counter_bytes);
     if (rc) return rc;
-    char* base = static_cast<char*>(ctx->kv4_ws);
-    p.counters = reinterpret_cast<int*>(base);
-    p.partials = reinterpret_cast<float*>(base + counter_bytes);
-    p.q_frag = reinterpret_cast<uint4*>(base + counter_bytes + part);
-    p.q_sums = reinterpret_cast<float*>(base + counter_bytes + part + frag);
-    cudaError_t e = launch_kv4_prepare(p, ctx->sm_count, stream);
-    const int B = p.B;
+    char* at = static_cast<char*>(ctx->kv4_ws);
+    auto take = [&](size_t bytes) {
+        char* here = at;
+        at += bytes;
+        return here;
+    };
+    p.counters = reinterpret_cast<int*>(take(counter_bytes));
+    p.partials = reinterpret_cast<float*>(take(part));
+    p.plan_head = reinterpret_cast<int2*>(take(head));
+    p.plan = reinterpret_cast<Kv4Piece*>(take(plan));
+    p.q_frag = reinterpret_cast<uint4*>(take(frag));
+    p.q_sums = reinterpret_cast<float*>(take(sums));
+    cudaError_t e = cudaSuccess;
     for (int b0 = 0; e == cudaSuccess && b0 < B; b0 += per_launch) {
         Kv4Params s = p;
+        const int64_t rows = (int64_t)b0 * p.T;
+        auto advance = [&](const void* x, int64_t elems) {
+            return x ? static_cast<char*>(const_cast<void*>(x)) + elems * 2 : nullptr;
+        };
         s.B = std::min(per_launch, B - b0);
         s.page_table += (int64_t)b0 * p.max_pages;
         s.ctx_lens += b0;
         if (s.new_lens) s.new_lens += b0;
-        s.o = static_cast<char*>(p.o) + (int64_t)b0 * p.T * p.Hq * p.D * 2;
-        s.q_frag = reinterpret_cast<uint4*>(reinterpret_cast<char*>(p.q_frag) + kv4_frag_bytes(p) * b0);
-        s.q_sums = reinterpret_cast<float*>(reinterpret_cast<char*>(p.q_sums) + kv4_sums_bytes(p) * b0);
-        e = launch_kv4_attn(s, ctx->device, stream);
+        s.q = advance(p.q, rows * p.q_stride);
+        s.k_new = advance(p.k_new, rows * p.kv_stride);
+        s.v_new = advance(p.v_new, rows * p.kv_stride);
+        s.k_held = advance(p.k_held, rows * p.Hkv * p.D);
+        s.v_held = advance(p.v_held, rows * p.Hkv * p.D);
+        s.o = advance(p.o, rows * p.Hq * p.D);
+        e = launch_kv4_prepare(s, ctx->sm_count, stream);
+        if (e == cudaSuccess) e = launch_kv4_attn(s, ctx->device, stream);
     }
     if (e != cudaSuccess) return cuda_fail(ctx, e, "4-bit cache attention launch");
     return B2A_OK;

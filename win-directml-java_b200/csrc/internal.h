@@ -212,6 +212,24 @@ bool linear_tc_supported(int in_dtype, int K, int64_t ldx, int64_t ldw, const vo
 int linear_split_plan(int M, int N, int K, int sm_count, size_t* acc_bytes, size_t* counter_ints);
 cudaError_t launch_linear_tc(const LinearArgs& a, int* status, cudaStream_t stream);
 
+// A piece of the 4-bit cache attention's work: blocks [blk0, blk1) of 16 positions for unit r = (kv
+// head, query row tile) of a sequence; n_split pieces make up the unit, whose partial slots are
+// part0 and, for the k-th piece after the first, (part0 with its lowest bit cleared where part_step
+// is 2) + k part_step; my_part is this piece's.
+struct Kv4Piece {
+    int b, r, L, n;
+    int blk0, blk1, n_split, my_part;
+    int part0, part_step, pad0, pad1;
+};
+// How the attention kernel wants its work spread (kv4_attn.cu).
+struct Kv4Split {
+    int n_cta;       // CTAs of its launch
+    int per_seq;     // units per sequence
+    int gap;         // fixed cost of a piece, in blocks
+    int min_blocks;  // smallest piece
+    size_t partial_bytes;
+};
+
 // Attention over, and appending to, the paged 4-bit KV cache (layout: kv4.cuh).
 struct Kv4Params {
     const void* q;       // [B][T] token rows of Hq * D elements, q_stride elements apart
@@ -241,16 +259,19 @@ struct Kv4Params {
     float* q_sums;
     int* counters;
     float* partials;
+    int2* plan_head;  // [n_cta]: first piece and number of pieces of each attention CTA
+    Kv4Piece* plan;   // [n_cta + units]
+    Kv4Split split;
     double inv_freq[kMaxHeadDim / 2];
 };
 constexpr int kMaxPageSize = 1024;
-constexpr int kKv4MaxBatch = 2048;      // sequences of one attention launch
-constexpr int kKv4GapBlocksMax = 16;    // largest per-unit allowance of the attention's split, in blocks
-// Appends k_new / v_new where given and lays out q where given.
+constexpr int kKv4MaxBatch = 2048;      // sequences of one plan and attention launch
+constexpr int kKv4GapBlocksMax = 26;    // largest per-unit allowance of the attention's split, in blocks
+// Appends k_new / v_new where given; lays out q and plans the attention where q is given.
 cudaError_t launch_kv4_prepare(const Kv4Params& p, int sm_count, cudaStream_t stream);
 size_t kv4_frag_bytes(const Kv4Params& p);  // per sequence
 size_t kv4_sums_bytes(const Kv4Params& p);  // per sequence
-void kv4_attn_workspace(const Kv4Params& p, int device, size_t* partial_bytes, size_t* units_per_seq);
+Kv4Split kv4_attn_split(const Kv4Params& p, int device);
 // Directly behind launch_kv4_prepare on the stream: it starts before that kernel has ended.
 cudaError_t launch_kv4_attn(const Kv4Params& p, int device, cudaStream_t stream);
 

@@ -84,9 +84,9 @@ __device__ __forceinline__ double kv4_warp_sum(double v) {
 // b2a_decode's prologue (double sum of squares and angles; NeoX rotates in float, Gemma in double),
 // each operation rounded by itself, so that the codes decided on the result are reproducible.
 template <int D>
-__device__ __forceinline__ void kv4_norm_rope(float (&x)[D / 32], const float* norm_w, float eps, int rope_mode,
-                                              const double2* cs, float* vec, int lane) {
-    if (norm_w != nullptr) {
+__device__ __forceinline__ void kv4_norm_rope(float (&x)[D / 32], bool norm, const float (&norm_w)[D / 32], float eps,
+                                              int rope_mode, const double2* cs, float* vec, int lane) {
+    if (norm) {
         double ss = 0.0;
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) ss += (double)x[j] * (double)x[j];
@@ -94,7 +94,7 @@ __device__ __forceinline__ void kv4_norm_rope(float (&x)[D / 32], const float* n
         const float rms = (float)(1.0 / sqrt(__dadd_rn(ss / (double)D, (double)eps)));
 #pragma unroll
         for (int j = 0; j < D / 32; ++j)
-            x[j] = (float)__dmul_rn((double)__fmul_rn(x[j], rms), __dadd_rn(1.0, (double)norm_w[lane + 32 * j]));
+            x[j] = (float)__dmul_rn((double)__fmul_rn(x[j], rms), __dadd_rn(1.0, (double)norm_w[j]));
     }
     if (rope_mode == 0) return;
 #pragma unroll
@@ -123,14 +123,19 @@ __device__ __forceinline__ void kv4_norm_rope(float (&x)[D / 32], const float* n
 template <int N>
 __device__ __forceinline__ bool kv4_quantise(const float (&x)[N], int (&code)[N], __half2 (&sz)[N]) {
     bool fine = true;
+    float low[N], high[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) low[j] = high[j] = x[j];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            low[j] = fminf(low[j], __shfl_xor_sync(0xffffffffu, low[j], o));
+            high[j] = fmaxf(high[j], __shfl_xor_sync(0xffffffffu, high[j], o));
+        }
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-        float lo = x[j], hi = x[j];
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        }
+        const float lo = low[j], hi = high[j];
         __half s = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f)), z = __float2half_rn(lo);
         const float sf = __half2float(s), zf = __half2float(z);
         const bool ok = !__any_sync(0xffffffffu, !isfinite(x[j])) && isfinite(sf) && isfinite(zf);

@@ -3,9 +3,11 @@
 // holds them for callers that want the prompt's own attention to see the same values, and the
 // queries' norm, RoPE and layout as the warp MMA's B operand (kv4_attn.cu).
 //
-// kv4_prepare_kernel: a CTA takes rows of one token (query heads, key heads, value heads), a warp one
-// row at a time; the token's sines and cosines are computed once per CTA. It lets the attention kernel
-// behind it start at once: that kernel plans and requests its first old blocks meanwhile.
+// kv4_prepare_kernel: the first CTAs plan the attention's work; each other one takes rows of one token
+// (query heads, key heads, value heads), a warp one row at a time, and computes the token's sines and
+// cosines once. It is all latency -- lengths, rows, page table, then a chain of double-precision
+// steps -- so every read is requested before the first one is waited for, and the attention kernel
+// is launched behind it early, to be resident when it ends.
 // kv4_store_kernel: prompts. A CTA takes one block of 16 positions and walks kv heads; a thread holds
 // 8 channels of a row (16-byte loads), the block is assembled in shared memory and stored whole.
 #include <algorithm>
@@ -23,25 +25,17 @@ constexpr int kPrepWarps = 8;
 // 16 times larger); fp16 activations keep a second word with what the first rounding lost.
 // q_sums: sum of the group's operand values 2^-24 per group, then scale log2(e) 2^(E + 24).
 template <int D>
-__device__ __forceinline__ void prepare_query(const Kv4Params& p, int64_t tok, int h, int L, int t, int n, bool ok,
-                                              const double2* cs, float* vec, int lane) {
+__device__ __forceinline__ void prepare_query(const Kv4Params& p, float (&x)[D / 32], const float (&wn)[D / 32],
+                                              int64_t tok, int h, int t, const double2* cs, float* vec, int lane) {
     constexpr int kGroups = D / 32;
     const int tiles = (p.T * p.G + 7) / 8;
     const int kvh = h / p.G, r = t * p.G + h - kvh * p.G;
     const int64_t tile = (tok / p.T * p.Hkv + kvh) * tiles + (r >> 3);
     __half* frag = reinterpret_cast<__half*>(p.q_frag + tile * (kGroups * 32 * 2));
     float* sums = p.q_sums + tile * (kGroups + 1) * 8 + (r & 7);
-    if (t >= n) {  // no such row: the attention reads no operands of it
-        for (int d = lane; d < D; d += 32)
-            store_from_float(p.o, (tok * p.Hq + h) * D + d, ok ? 0.f : __int_as_float(0x7fc00000), p.act_dtype);
-        return;
-    }
-    float x[kGroups], top = 0.f;
-#pragma unroll
-    for (int y = 0; y < kGroups; ++y)
-        x[y] = load_as_float(p.q, tok * p.q_stride + (int64_t)h * D + lane + 32 * y, p.act_dtype);
+    kv4_norm_rope<D>(x, p.q_norm_w != nullptr, wn, p.norm_eps, p.rope_mode, cs, vec, lane);
+    float top = 0.f;
     bool fine = true;
-    kv4_norm_rope<D>(x, p.q_norm_w, p.norm_eps, p.rope_mode, cs, vec, lane);
 #pragma unroll
     for (int y = 0; y < kGroups; ++y) {
         top = fmaxf(top, fabsf(x[y]));
@@ -52,47 +46,45 @@ __device__ __forceinline__ void prepare_query(const Kv4Params& p, int64_t tok, i
     const int E = fine && top > 0.f ? ilogbf(top) - 13 : 0;
     const int j = (lane >> 3) & 1;
     const int word = ((r & 7) * 4 + ((lane & 7) >> 1)) * 4 + 2 * (lane >> 4) + j;
+    const float up = scalbnf(j ? 0.0625f : 1.f, -E);
+    float used[kGroups];
 #pragma unroll
     for (int y = 0; y < kGroups; ++y) {
-        const float v = fine ? scalbnf(x[y], -E) * (j ? 0.0625f : 1.f) : 0.f;
+        // -E is at most 149 + 13: in two steps, so that the factor stays finite
+        const float v = !fine ? 0.f : (E < -100 ? scalbnf(x[y], -E) * (j ? 0.0625f : 1.f) : x[y] * up);
         const __half hi = __float2half_rn(v);
         const int at = (y * 32 * 4 + word) * 2 + (lane & 1);
         frag[at] = hi;
-        float used = __half2float(hi);
+        used[y] = __half2float(hi);
         if (p.act_dtype == kF16) {
-            const __half lo = __float2half_rn(v - used);
+            const __half lo = __float2half_rn(v - used[y]);
             frag[kGroups * 32 * 4 * 2 + at] = lo;
-            used += __half2float(lo);
+            used[y] += __half2float(lo);
         }
-        const float s = warp_sum(used * (j ? 0x1p-20f : 0x1p-24f));
-        if (lane == 0) sums[y * 8] = s;
+        used[y] *= j ? 0x1p-20f : 0x1p-24f;
     }
-    if (lane == 0) sums[kGroups * 8] = fine ? scalbnf(p.scale * kLog2e, E + 24) : __int_as_float(0x7fc00000);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int y = 0; y < kGroups; ++y) used[y] += __shfl_xor_sync(0xffffffffu, used[y], o);
+    if (lane == 0) {
+#pragma unroll
+        for (int y = 0; y < kGroups; ++y) sums[y * 8] = used[y];
+        sums[kGroups * 8] = fine ? scalbnf(p.scale * kLog2e, E + 24) : __int_as_float(0x7fc00000);
+    }
 }
 
 template <int D>
-__device__ __forceinline__ void append_row(const Kv4Params& p, int64_t tok, int kvh, bool is_v, int L, int t, int n,
-                                           bool ok, const double2* cs, float* vec, int lane) {
-    const int b = (int)(tok / p.T);
+__device__ __forceinline__ void append_row(const Kv4Params& p, float (&x)[D / 32], const float (&wn)[D / 32],
+                                           int64_t tok, int kvh, bool is_v, int pos, uint8_t* block, const double2* cs,
+                                           float* vec, int lane) {
     void* held = is_v ? p.v_held : p.k_held;
     const int64_t held_at = (tok * p.Hkv + kvh) * D;
-    if (t >= n) {
-        if (held)
-            for (int d = lane; d < D; d += 32)
-                store_from_float(held, held_at + d, ok ? 0.f : __int_as_float(0x7fc00000), p.act_dtype);
-        return;
-    }
-    const int pos = L + t, key = pos % kKv4Block;
-    const void* src = is_v ? p.v_new : p.k_new;
-    float x[D / 32];
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j)
-        x[j] = load_as_float(src, tok * p.kv_stride + (int64_t)kvh * D + lane + 32 * j, p.act_dtype);
-    if (!is_v) kv4_norm_rope<D>(x, p.k_norm_w, p.norm_eps, p.rope_mode, cs, vec, lane);
+    const int key = pos % kKv4Block;
+    if (!is_v) kv4_norm_rope<D>(x, p.k_norm_w != nullptr, wn, p.norm_eps, p.rope_mode, cs, vec, lane);
     int code[D / 32];
     __half2 sz[D / 32];
     if (!kv4_quantise(x, code, sz) && lane == 0) atomicOr(p.status, 32);
-    uint8_t* block = kv4_block_ptr(p, b, kvh, pos);
     if (block == nullptr && lane == 0) atomicOr(p.status, 16);
     if (block != nullptr && is_v) block += kv4_off_v(D);
 #pragma unroll
@@ -106,33 +98,235 @@ __device__ __forceinline__ void append_row(const Kv4Params& p, int64_t tok, int 
     }
 }
 
-// Rows of a token: Hq queries (where p.q), Hkv keys and Hkv values (where `append`); block (token,
-// chunk) takes rows [chunk * per, (chunk + 1) * per).
+// Spreads the attention's work over its CTAs, in one of two ways:
+//  * pieces: every unit is cut into k near-equal pieces of at most P blocks, one piece per CTA.  P is
+//    the smallest of eight sizes, from the guaranteed one, blocks / (CTAs - units), down, that needs
+//    no more pieces than there are CTAs.
+//  * ranges: the blocks of all units, each followed by `gap` that stand for the fixed cost of a piece,
+//    form one stream; CTA c takes its c-th equal range, so it may meet several units.
+// Pieces are taken where the largest costs no more than a range with a second piece's fixed cost.
+// Every planning block sums the lengths itself and writes the pieces of its 256 CTAs.
+constexpr int kPrepThreads = kPrepWarps * 32;
+
+__device__ __forceinline__ int seen_blocks(const Kv4Params& p, int L, int n, int& first) {
+    first = p.window > 0 ? max(0, L - p.window + 1) / kKv4Block : 0;
+    return n > 0 ? (L + n - 1) / kKv4Block + 1 - first : 0;
+}
+__device__ __forceinline__ int cuts_of(int blocks, float inv) { return max(1, (int)ceilf((float)blocks * inv - 1e-3f)); }
+
+struct PlanShared {
+    int prefix[kKv4MaxBatch + 1];  // per unit: pieces, or stream length, of the sequences before
+    int ctx[kKv4MaxBatch], fresh[kKv4MaxBatch];
+    int sums[10][kPrepWarps];
+};
+
+__device__ __noinline__ void plan_attention(const Kv4Params& p, PlanShared& sh, int block) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int n_cta = p.split.n_cta, per_seq = p.split.per_seq, gap = p.split.gap;
+    auto all_warps = [&](int row) {
+        int v = 0;
+#pragma unroll
+        for (int w = 0; w < kPrepWarps; ++w) v += sh.sums[row][w];
+        return v;
+    };
+    int blocks = 0, seqs = 0, first;
+    for (int b = tid; b < p.B; b += kPrepThreads) {
+        int L, n;
+        if (!kv4_lens(p, b, L, n)) n = 0;
+        sh.ctx[b] = L;
+        sh.fresh[b] = n;
+        const int nb = seen_blocks(p, L, n, first);
+        blocks += nb;
+        seqs += nb > 0;
+    }
+    blocks = __reduce_add_sync(0xffffffffu, blocks);
+    seqs = __reduce_add_sync(0xffffffffu, seqs);
+    if (lane == 0) {
+        sh.sums[8][warp] = blocks;
+        sh.sums[9][warp] = seqs;
+    }
+    __syncthreads();
+    const float total_f = (float)all_warps(8) * (float)per_seq, units_f = (float)all_warps(9) * (float)per_seq;
+    bool pieces = false;
+    float inv_p = 0.f;
+    if (units_f <= 0.875f * (float)n_cta) {
+        const float most = total_f / ((float)n_cta - units_f) + 1.f;
+        auto size = [&](int k) { return fmaxf((float)p.split.min_blocks, most * (1.f - (float)k / 16.f)); };
+        int count[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        for (int b = tid; b < p.B; b += kPrepThreads) {
+            const int nb = seen_blocks(p, sh.ctx[b], sh.fresh[b], first);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) count[k] += nb ? cuts_of(nb, 1.f / size(k)) : 0;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            count[k] = __reduce_add_sync(0xffffffffu, count[k]);
+            if (lane == 0) sh.sums[k][warp] = count[k];
+        }
+        __syncthreads();
+        float best = 0.f;
+        for (int k = 0; k < 8; ++k)
+            if ((long long)all_warps(k) * per_seq <= n_cta) best = size(k);
+        pieces = best > 0.f && best <= total_f / (float)n_cta + (float)gap;
+        if (pieces) inv_p = 1.f / best;
+    }
+    // prefix sums, kPrepThreads sequences at a time
+    auto weight = [&](int b) {
+        const int nb = seen_blocks(p, sh.ctx[b], sh.fresh[b], first);
+        return nb == 0 ? 0 : (pieces ? cuts_of(nb, inv_p) : nb + gap);
+    };
+    int before = 0;
+    for (int b0 = 0; b0 < p.B; b0 += kPrepThreads) {
+        const int b = b0 + tid, w = b < p.B ? weight(b) : 0;
+        int incl = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        __syncthreads();
+        if (lane == 31) sh.sums[0][warp] = incl;
+        __syncthreads();
+        int at = before;
+        for (int k = 0; k < warp; ++k) at += sh.sums[0][k];
+        if (b < p.B) sh.prefix[b] = at + incl - w;
+        before += all_warps(0);
+    }
+    if (tid == 0) sh.prefix[p.B] = before;
+    __syncthreads();
+
+    const int c = block * kPrepThreads + tid;
+    if (c >= n_cta) return;
+    const long long total = (long long)before * per_seq;
+    const long long R = pieces ? 1 : max((long long)p.split.min_blocks, (total + n_cta - 1) / n_cta);
+    long long pos = c * R;
+    const long long end = min(total, pos + R);
+    int made = 0, at = c;
+    while (pos < end) {
+        int lo = 0, hi = p.B - 1;
+        while (lo < hi) {  // the last sequence that starts at or before pos
+            const int mid = (lo + hi + 1) >> 1;
+            if ((long long)sh.prefix[mid] * per_seq <= pos) lo = mid;
+            else hi = mid - 1;
+        }
+        const int b = lo, w = sh.prefix[b + 1] - sh.prefix[b];
+        const long long seq_base = (long long)sh.prefix[b] * per_seq;
+        int r = (int)((pos - seq_base) / w);
+        const int nb = seen_blocks(p, sh.ctx[b], sh.fresh[b], first);
+        // the pieces of CTA c come after those of the CTAs before it: at most one per CTA and unit
+        if (made == 0 && !pieces) at = c + b * per_seq + r;
+        for (; r < per_seq && pos < end; ++r) {
+            const long long u_start = seq_base + (long long)r * w;
+            Kv4Piece piece{};
+            piece.b = b;
+            piece.r = r;
+            piece.L = sh.ctx[b];
+            piece.n = sh.fresh[b];
+            if (pieces) {
+                const int k = (int)(pos - u_start);
+                piece.blk0 = first + (int)((long long)nb * k / w);
+                piece.blk1 = first + (int)((long long)nb * (k + 1) / w);
+                piece.n_split = w;
+                piece.my_part = c;
+                piece.part0 = c - k;
+                piece.part_step = 1;
+                pos = end;
+            } else {
+                const long long u_end = u_start + nb;
+                if (pos >= u_end) {  // in the unit's gap
+                    pos = u_start + w;
+                    continue;
+                }
+                const long long c0 = u_start / R, c1 = (u_end - 1) / R, stop = min(end, u_end);
+                piece.blk0 = first + (int)(pos - u_start);
+                piece.blk1 = first + (int)(stop - u_start);
+                piece.n_split = (int)(c1 - c0) + 1;
+                // CTA c's slot is 2 c for the piece its range begins with, 2 c + 1 for one that begins later
+                piece.my_part = 2 * c + (pos == c * R ? 0 : 1);
+                piece.part0 = 2 * (int)c0 + (u_start != c0 * R ? 1 : 0);
+                piece.part_step = 2;
+                pos = stop < end ? u_start + w : end;
+            }
+            p.plan[at + made] = piece;
+            ++made;
+        }
+    }
+    p.plan_head[c] = make_int2(at, made);
+}
+
+// Rows of a token: Hq queries (where p.q), Hkv keys and Hkv values (where `append`); after the
+// planning blocks, block (token, chunk) takes rows [chunk * per, (chunk + 1) * per).
 template <int D>
-__global__ void __launch_bounds__(kPrepWarps * 32) kv4_prepare_kernel(const __grid_constant__ Kv4Params p, int append,
-                                                                      int chunks, int per) {
-    __shared__ float vec_all[kPrepWarps * D];
-    __shared__ double2 cs[D / 2];
+__global__ void __launch_bounds__(kPrepThreads) kv4_prepare_kernel(const __grid_constant__ Kv4Params p, int append,
+                                                                   int chunks, int per, int plans) {
+    constexpr int kGroups = D / 32;
+    constexpr size_t kRowBytes = kPrepWarps * D * 4 + D / 2 * sizeof(double2);
+    __shared__ __align__(16) unsigned char smem[kRowBytes > sizeof(PlanShared) ? kRowBytes : sizeof(PlanShared)];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (blockIdx.x < plans) {
+        plan_attention(p, *reinterpret_cast<PlanShared*>(smem), blockIdx.x);
+        return;
+    }
+    double2* const cs = reinterpret_cast<double2*>(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t tok = blockIdx.x / chunks;
-    const int chunk = (int)(blockIdx.x - tok * chunks);
+    float* const vec = reinterpret_cast<float*>(smem + D / 2 * sizeof(double2)) + warp * D;
+    const int block = blockIdx.x - plans;
+    const int64_t tok = block / chunks;
+    const int chunk = block - (int)tok * chunks;
     const int b = (int)(tok / p.T), t = (int)(tok - (int64_t)b * p.T);
+    const int nq = p.q ? p.Hq : 0, rows = nq + (append ? 2 * p.Hkv : 0);
+    const int end = min(rows, (chunk + 1) * per);
+    int r = chunk * per + warp;
+    // every read of the first row is requested before anything waits for one
+    uint32_t raw[kGroups];
+    float wn[kGroups];
+    auto fetch = [&](int row) {
+        const bool is_q = row < nq;
+        const int i = row - nq;
+        const void* src = is_q ? p.q : (i & 1) ? p.v_new : p.k_new;
+        const int64_t at = is_q ? tok * p.q_stride + (int64_t)row * D : tok * p.kv_stride + (int64_t)(i >> 1) * D;
+        const float* w = is_q ? p.q_norm_w : p.k_norm_w;
+#pragma unroll
+        for (int y = 0; y < kGroups; ++y) {
+            raw[y] = load_raw(src, at + lane + 32 * y, p.act_dtype);
+            wn[y] = w ? __ldg(w + lane + 32 * y) : 0.f;
+        }
+    };
+    if (r < end) fetch(r);
     int L, n;
     const bool ok = kv4_lens(p, b, L, n);
     if (!ok && threadIdx.x == 0) atomicOr(p.status, 1);
-    if (p.rope_mode != 0 && threadIdx.x < D / 2) {
+    const bool there = t < n;
+    // the new rows' block of kv head 0; the other heads' follow at one slab's distance
+    uint8_t* const block0 = there && append ? kv4_block_ptr(p, b, 0, L + t) : nullptr;
+    const int64_t slab = (int64_t)(p.page_size / kKv4Block) * kv4_block_bytes(D);
+    if (there && p.rope_mode != 0 && threadIdx.x < D / 2) {
         double sn, c;
         sincos((double)(L + t) * p.inv_freq[threadIdx.x], &sn, &c);
         cs[threadIdx.x] = make_double2(c, sn);
     }
     __syncthreads();
-    const int nq = p.q ? p.Hq : 0, rows = nq + (append ? 2 * p.Hkv : 0);
-    const int end = min(rows, (chunk + 1) * per);
-    for (int r = chunk * per + warp; r < end; r += kPrepWarps) {
-        if (r < nq) prepare_query<D>(p, tok, r, L, t, n, ok, cs, vec_all + warp * D, lane);
-        else
-            append_row<D>(p, tok, (r - nq) >> 1, (r - nq) & 1, L, t, n, ok, cs, vec_all + warp * D, lane);
+    for (; r < end; r += kPrepWarps) {
+        float x[kGroups], w[kGroups];
+#pragma unroll
+        for (int y = 0; y < kGroups; ++y) {
+            x[y] = raw_to_float(raw[y], p.act_dtype);
+            w[y] = wn[y];
+        }
+        if (r + kPrepWarps < end) fetch(r + kPrepWarps);
+        const int i = r - nq;
+        if (!there) {  // no such token: outputs are zero, or NaN where the lengths do not fit
+            const float v = ok ? 0.f : __int_as_float(0x7fc00000);
+            void* dst = i < 0 ? p.o : (i & 1) ? p.v_held : p.k_held;
+            const int64_t at = i < 0 ? (tok * p.Hq + r) * D : (tok * p.Hkv + (i >> 1)) * D;
+            if (dst)
+                for (int d = lane; d < D; d += 32) store_from_float(dst, at + d, v, p.act_dtype);
+        } else if (i < 0) {
+            prepare_query<D>(p, x, w, tok, r, t, cs, vec, lane);
+        } else {
+            append_row<D>(p, x, w, tok, i >> 1, i & 1, L + t, block0 ? block0 + (i >> 1) * slab : nullptr, cs, vec,
+                          lane);
+        }
     }
 }
 
@@ -361,11 +555,12 @@ cudaError_t launch_prepare(const Kv4Params& p, int sm_count, cudaStream_t stream
     }
     // a row per warp while that leaves the GPU room, else longer runs of rows that share their sines
     const int64_t tokens = (int64_t)p.B * p.T;
+    const int plans = p.q ? (p.split.n_cta + kPrepThreads - 1) / kPrepThreads : 0;
     const int rows = (p.q ? p.Hq : 0) + (append ? 2 * p.Hkv : 0);
     const int most = (rows + kPrepWarps - 1) / kPrepWarps;
     const int want = (int)std::max<int64_t>(1, std::min<int64_t>(most, 8 * sm_count / tokens));
     const int per = (rows + want - 1) / want, chunks = (rows + per - 1) / per;
-    kv4_prepare_kernel<D><<<(unsigned)(tokens * chunks), kPrepWarps * 32, 0, stream>>>(p, append, chunks, per);
+    kv4_prepare_kernel<D><<<(unsigned)(plans + tokens * chunks), kPrepThreads, 0, stream>>>(p, append, chunks, per, plans);
     return cudaGetLastError();
 }
 

@@ -25,8 +25,8 @@
 // sums over minima, scales and P are added to their totals in fp32 outside the MMA.
 //
 // Work split.  A unit is (sequence, kv head, tile of query rows); a query row is (token, head of the
-// group), so one cache byte serves every head of its group and every token of a draft.  The blocks
-// of 16 keys of all units form one stream and every CTA takes an equal range of it (stream-K); the
+// group), so one cache byte serves every head of its group and every token of a draft.  The
+// preparation kernel spreads the units' blocks of 16 keys over the CTAs (kv4_append.cu: plan); the
 // pieces of a cut unit meet through partial slots (m, l, O) that the last one to finish joins.
 // Inside a piece each warp walks its own blocks with its own ring of bulk copies: one copy of 20 D
 // bytes is a block, its address comes from page-table entries fetched 32 blocks at a time, and the
@@ -65,8 +65,8 @@ struct Cfg {
     // CTAs per SM, the registers' bound
     static constexpr int kCtas = D <= 64 ? (kTiles == 1 ? 4 : 3) : (D <= 128 ? (kTiles == 1 ? 3 : 2) : (kTiles == 1 ? 3 : 2));
     // fixed cost of a piece in blocks of streaming time, charged to every unit by the split
-    static constexpr int kGapBlocks = D <= 64 ? 16 : (D <= 128 ? 8 : 4);
-    static constexpr int kMinBlocks = 8;  // smallest range of a CTA
+    static constexpr int kGapBlocks = D <= 64 ? 26 : (D <= 96 ? 22 : (D <= 128 ? 18 : 12));
+    static constexpr int kMinBlocks = 8;  // smallest piece
     // q's operand words in shared memory where the accumulators leave no registers for them
     static constexpr bool kQShared = D * kTiles >= 256;
     // head dim 256: the value params are regrouped in shared memory (their rows lie 128 bytes
@@ -79,18 +79,12 @@ struct Cfg {
     static constexpr size_t oMl = oBars + kWarps * kStages * 8;
     static constexpr size_t oMisc = a128(oMl + size_t(kWarps) * kCols * 2 * 4);
     static constexpr size_t kQWords = size_t(kTiles) * kGroups * 32 * 16;
-    static constexpr size_t oQ = oMisc + 128;
+    static constexpr size_t oQ = oMisc + 256;
     static constexpr size_t oPairs = oQ + (kQShared ? kQWords : 0);
-    static constexpr size_t oPrefix = oPairs + (kRegroup ? kWarps * 512 : 0);
-    static size_t total(int B) { return oPrefix + size_t(3 * B + 1) * 4; }
+    static constexpr size_t kSmem = oPairs + (kRegroup ? kWarps * 512 : 0);
     static_assert(kGapBlocks <= kKv4GapBlocksMax, "host launch split assumes this bound");
+    static_assert(kSmem <= 227 * 1024, "shared memory budget");
 };
-
-// The blocks of 16 positions that some new token of a sequence sees: how many, and the first.
-__device__ __forceinline__ int seq_blocks(const Kv4Params& p, int L, int n, int& lo) {
-    lo = p.window > 0 ? max(0, L - p.window + 1) / kKv4Block : 0;
-    return n > 0 ? (L + n - 1) / kKv4Block + 1 - lo : 0;
-}
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
@@ -106,15 +100,41 @@ __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity) {
         if ((i & 255u) == 0 && global_ns() - t0 > kWaitNs) return false;
     }
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-    uint32_t x;
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(a));
-    return x;
+__device__ __forceinline__ uint32_t ld32(const unsigned char* a) { return *reinterpret_cast<const uint32_t*>(a); }
+__device__ __forceinline__ uint2 ld64(const unsigned char* a) { return *reinterpret_cast<const uint2*>(a); }
+// n consecutive params (4 bytes each), 8- or 16-byte aligned as the layout gives them
+template <int N>
+__device__ __forceinline__ void ld_params(const unsigned char* a, uint32_t (&x)[N]) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const uint4 w = *reinterpret_cast<const uint4*>(a + i * 4);
+            x[i] = w.x, x[i + 1] = w.y, x[i + 2] = w.z, x[i + 3] = w.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const uint2 w = ld64(a + i * 4);
+            x[i] = w.x, x[i + 1] = w.y;
+        }
+    }
 }
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-    uint2 x;
-    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x.x), "=r"(x.y) : "r"(a));
-    return x;
+// The warp MMA (16 x 8 x 16, f16 operands, fp32 accumulators) without ordering against other code:
+// d += a b, and d = a b.
+__device__ __forceinline__ void mma_add(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_set(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {  // movmatrix
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+    return y;
 }
 // The A operand of one 16 x 16 tile of codes, or of 15 - codes (flip all ones).
 __device__ __forceinline__ void code_frag(uint32_t (&a)[4], uint32_t w, uint32_t flip = 0) {
@@ -123,27 +143,6 @@ __device__ __forceinline__ void code_frag(uint32_t (&a)[4], uint32_t w, uint32_t
     a[1] = (h ^ flip) & 0x000F000Fu;
     a[2] = (w ^ flip) & 0x00F000F0u;
     a[3] = (h ^ flip) & 0x00F000F0u;
-}
-__device__ __forceinline__ void lds128(uint32_t a, uint32_t* x) {
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(a));
-}
-__device__ __forceinline__ void sts32(uint32_t a, uint32_t x) {
-    asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(x) : "memory");
-}
-// n consecutive params (4 bytes each), 8- or 16-byte aligned as the layout gives them
-template <int N>
-__device__ __forceinline__ void lds_params(uint32_t a, uint32_t (&x)[N]) {
-    if constexpr (N % 4 == 0) {
-#pragma unroll
-        for (int i = 0; i < N; i += 4) lds128(a + i * 4, x + i);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            const uint2 w = lds64(a + i * 4);
-            x[i] = w.x;
-            x[i + 1] = w.y;
-        }
-    }
 }
 __device__ __forceinline__ __half2 h2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
 __device__ __forceinline__ uint32_t u32(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
@@ -166,14 +165,11 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
     float* merge_s = reinterpret_cast<float*>(smem);
     float* ml_s = reinterpret_cast<float*>(smem + C::oMl);
     int* misc = reinterpret_cast<int*>(smem + C::oMisc);
-    int* prefix = reinterpret_cast<int*>(smem + C::oPrefix);
-    int* ctx_s = prefix + p.B + 1;  // cached and new tokens per sequence, 0 and 0 where they do not fit
-    int* new_s = ctx_s + p.B;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, t4 = lane & 3;
-    const uint32_t ring = smem_u32(smem) + warp * kStages * C::kStageBytes;
-    const uint32_t bars = smem_u32(smem + C::oBars) + warp * kStages * 8;
-    const uint32_t pairs = smem_u32(smem + C::oPairs) + warp * 512;
+    unsigned char* const ring = smem + warp * kStages * C::kStageBytes;
+    const uint32_t ring_at = smem_u32(ring), bars = smem_u32(smem + C::oBars) + warp * kStages * 8;
+    unsigned char* const pairs = smem + C::oPairs + warp * 512;
 
     if (lane == 0) {
 #pragma unroll
@@ -181,88 +177,37 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
 
-    // ---------------------------------------------------------------- plan
-    // prefix[b]: stream length (visible blocks and the gap) of the sequences before b, per unit
-    {
-        const int per = (p.B + kThreads - 1) / kThreads;
-        const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
-        int run = 0;
-        for (int b = b0; b < b1; ++b) {
-            int L, n, lo;
-            if (!kv4_lens(p, b, L, n)) n = 0;
-            ctx_s[b] = L;
-            new_s[b] = n;
-            const int nb = seq_blocks(p, L, n, lo);
-            run += nb ? nb + C::kGapBlocks : 0;
-        }
-        int incl = run;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += y;
-        }
-        if (lane == 31) misc[warp] = incl;
-        __syncthreads();
-        int acc = incl - run;
-        for (int w = 0; w < warp; ++w) acc += misc[w];
-        for (int b = b0; b < b1; ++b) {
-            prefix[b] = acc;
-            int lo;
-            const int nb = seq_blocks(p, ctx_s[b], new_s[b], lo);
-            acc += nb ? nb + C::kGapBlocks : 0;
-        }
-        if (tid == kThreads - 1) prefix[p.B] = acc;
-        __syncthreads();
-    }
     const int all_rows = p.T * p.G;
     const int row_tiles = (all_rows + kRows - 1) / kRows;
-    const int per_seq = p.Hkv * row_tiles;
-    const long long total = (long long)prefix[p.B] * per_seq;
-    const long long R = max((long long)C::kMinBlocks, (total + gridDim.x - 1) / gridDim.x);
     const int q_tiles = (all_rows + 7) / 8;  // tiles of 8 rows that the preparation laid out
-    bool dep_done = false, dead = false;     // dead: a copy of this warp did not arrive in time
-    uint32_t it = 0;  // stages this warp has consumed since the launch began: ring slot and parity
+    bool dead = false;  // a copy of this warp did not arrive in time
+    int slot = 0;       // this warp's next stage: its place in the ring and its barrier's parity
+    uint32_t phase = 0;
 
-    for (long long pos = (long long)blockIdx.x * R, end = min(total, pos + R); pos < end;) {
-        int lo_b = 0, hi_b = p.B - 1;
-        while (lo_b < hi_b) {  // the last sequence that starts at or before pos
-            const int mid = (lo_b + hi_b + 1) >> 1;
-            if ((long long)prefix[mid] * per_seq <= pos) lo_b = mid;
-            else hi_b = mid - 1;
-        }
-        const int b = lo_b;
-        const int L = ctx_s[b], n = new_s[b];
-        int first_blk;
-        const int n_blk = seq_blocks(p, L, n, first_blk);
-        const int n_v = n_blk + C::kGapBlocks;
-        const long long seq_base = (long long)prefix[b] * per_seq;
-        const int r = (int)((pos - seq_base) / n_v);
-        const long long u_start = seq_base + (long long)r * n_v, u_end = u_start + n_blk;
-        if (pos >= u_end) {
-            pos = u_start + n_v;
-            continue;
-        }
-        const long long piece_end = min(end, u_end);
+    // the preparation kernel made the plan, the q operands and the new rows' blocks
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int2 mine = p.plan_head[blockIdx.x];
+    const Kv4Piece* piece = p.plan + mine.x;
+    for (int k_piece = 0; k_piece < mine.y; ++k_piece, ++piece) {
+        const int4 w0 = reinterpret_cast<const int4*>(piece)[0], w1 = reinterpret_cast<const int4*>(piece)[1],
+                   w2 = reinterpret_cast<const int4*>(piece)[2];
+        const int b = w0.x, r = w0.y, L = w0.z, n = w0.w;
+        const int n_split = w1.z, my_part = w1.w, part0 = w2.x, part_step = w2.y;
         const int kvh = r / row_tiles, rt = r - kvh * row_tiles;
         // tokens of this tile's rows, and the blocks of the piece that they see
         const int t_lo = rt * kRows / p.G, t_hi = min(n - 1, (rt * kRows + kRows - 1) / p.G);
         const int key_lo = p.window > 0 ? max(0, L + t_lo - p.window + 1) : 0;
-        const int blk0 = max(first_blk + (int)(pos - u_start), key_lo / kKv4Block);
-        const int blk1 =
-            t_lo <= t_hi ? min(first_blk + (int)(piece_end - u_start), (L + t_hi) / kKv4Block + 1) : blk0;
+        const int blk0 = max(w1.x, key_lo / kKv4Block);
+        const int blk1 = t_lo <= t_hi ? min(w1.y, (L + t_hi) / kKv4Block + 1) : blk0;
         const int key_hi = min(L + t_hi, blk1 * kKv4Block - 1);  // last key that some row takes from this piece
-        const long long c0 = u_start / R, c1 = (u_end - 1) / R;
-        const int n_split = (int)(c1 - c0) + 1;
-        const int my_slot = 2 * blockIdx.x + (pos == (long long)blockIdx.x * R ? 0 : 1);
-        const int unit = b * per_seq + r;
-        pos = piece_end;
+        const int unit = b * p.Hkv * row_tiles + r;
 
         // ------------------------------------------------------------ this warp's stages
         // stage i holds blocks blk0 + (warp + 4 i) kSub + 0 .. kSub - 1 (those below blk1)
         const int bpp = p.page_size / kKv4Block;
         const int my_n = max(0, ((blk1 - blk0 + kSub - 1) / kSub - warp + kWarps - 1) / kWarps);
         bool bad = false;
-        auto entry = [&](int x) -> int64_t {  // byte offset of the warp's x-th block, per lane; -1: none
+        auto entry = [&](int x) {  // place in the pool, in blocks, of the warp's x-th block, per lane; -1: none
             const int blk = blk0 + (warp + kWarps * (x / kSub)) * kSub + x % kSub;
             if (x / kSub >= my_n || blk >= blk1) return -1;
             const int slot = blk / bpp, in = blk - slot * bpp;
@@ -271,45 +216,35 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                 bad = true;
                 return 0;
             }
-            return (((int64_t)page * p.Hkv + kvh) * bpp + in) * C::kBlockBytes;
+            return (page * p.Hkv + kvh) * bpp + in;
         };
-        int64_t cur = entry(lane), nxt = entry(32 + lane);
-        auto issue = [&](int i) {  // request the warp's i-th stage
+        int cur = entry(lane), nxt = entry(32 + lane);
+        auto issue = [&](int i, int to) {  // request the warp's i-th stage into ring slot `to`
             const int x = i * kSub;
             if (x > 0 && (x & 31) == 0) {
                 cur = nxt;
                 nxt = entry(x + 32 + lane);
             }
-            int64_t off[kSub];
+            int off[kSub];
 #pragma unroll
             for (int u = 0; u < kSub; ++u) off[u] = __shfl_sync(0xffffffffu, cur, (x & 31) + u);
             if (lane == 0) {
-                const uint32_t s = (it + i) % kStages;
                 uint32_t bytes = 0;
 #pragma unroll
                 for (int u = 0; u < kSub; ++u) bytes += off[u] >= 0 ? C::kBlockBytes : 0;
-                mbar_expect_tx(bars + s * 8, bytes);
+                mbar_expect_tx(bars + to * 8, bytes);
 #pragma unroll
                 for (int u = 0; u < kSub; ++u)
                     if (off[u] >= 0)
-                        bulk_load(ring + s * C::kStageBytes + u * C::kBlockBytes, p.pages + off[u], C::kBlockBytes,
-                                  bars + s * 8);
+                        bulk_load(ring_at + to * C::kStageBytes + u * C::kBlockBytes,
+                                  p.pages + (int64_t)off[u] * C::kBlockBytes, C::kBlockBytes, bars + to * 8);
             }
         };
         int issued = 0;
-        auto fill = [&](int upto) {
-            while (!dead && issued < min(upto, my_n)) issue(issued++);
+        auto fill = [&](int upto) {  // the first stages, into the slots from `slot` on
+            for (; !dead && issued < min(upto, my_n); ++issued)
+                issue(issued, slot + issued < kStages ? slot + issued : slot + issued - kStages);
         };
-        if (!dep_done) {
-            // Blocks below the first new token's are as the kernel before the preparation left them,
-            // so the first ones are requested while the preparation kernel still runs.
-            const int old_blk = L / kKv4Block;
-            int ready = 0;
-            while (ready < min(kStages, my_n) && blk0 + (warp + kWarps * ready + 1) * kSub <= old_blk) ++ready;
-            fill(ready);
-            asm volatile("griddepcontrol.wait;" ::: "memory");
-            dep_done = true;
-        }
         fill(kStages);
 
         // ------------------------------------------------------------ q operands
@@ -379,16 +314,17 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
         __half2 s_bound = __float2half2_rn(1.f);
 
         for (int i = 0; i < my_n && !dead; ++i) {
-            const uint32_t slot = (it + i) % kStages;
-            if (!wait_bounded(bars + slot * 8, ((it + i) / kStages) & 1)) {
+            if (!wait_bounded(bars + slot * 8, phase)) {
                 // report, wait for the others in flight and ask for no more; the outputs are NaN
                 if (lane == 0) atomicOr(p.status, 8);
                 dead = true;
-                for (int k = i + 1; k < issued; ++k)
-                    if (!wait_bounded(bars + (it + k) % kStages * 8, ((it + k) / kStages) & 1)) break;
+                for (int k = 1; k < kStages && i + k < my_n; ++k) {
+                    const bool wrap = slot + k >= kStages;
+                    if (!wait_bounded(bars + (wrap ? slot + k - kStages : slot + k) * 8, phase ^ (wrap ? 1u : 0u))) break;
+                }
                 break;
             }
-            const uint32_t stage = ring + slot * C::kStageBytes;
+            const unsigned char* const stage = ring + slot * C::kStageBytes;
             const int key0 = (blk0 + (warp + kWarps * i) * kSub) * kKv4Block;
             const bool whole = key0 + kSub * kKv4Block - 1 <= all_hi && key0 >= all_lo;
 
@@ -396,24 +332,23 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
             float x[kSub][kSTiles][4];
 #pragma unroll
             for (int u = 0; u < kSub; ++u) {
-                const uint32_t base = stage + u * C::kBlockBytes;
-                const uint32_t kp = base + kv4_off_kparam(D) + g * (2 * kGroups * 4);
+                const unsigned char* const base = stage + u * C::kBlockBytes;
+                const unsigned char* const kp = base + kv4_off_kparam(D) + g * (2 * kGroups * 4);
                 uint32_t kw[2 * kGroups];  // params of keys g and g + 8
-                lds_params(kp, kw);
+                ld_params(kp, kw);
                 // minima of the groups whose sums this lane's k columns hold
                 constexpr int kPairs = (kGroups + 1) / 2;
                 const int y0 = 2 * (t4 % kPairs), y1 = min(y0 + 1, kGroups - 1);
-                const uint32_t za = high_halves(lds32(kp + y0 * 4), lds32(kp + y1 * 4));
-                const uint32_t zb = high_halves(lds32(kp + (kGroups + y0) * 4), lds32(kp + (kGroups + y1) * 4));
+                const uint32_t za = high_halves(ld32(kp + y0 * 4), ld32(kp + y1 * 4));
+                const uint32_t zb = high_halves(ld32(kp + (kGroups + y0) * 4), ld32(kp + (kGroups + y1) * 4));
                 const uint32_t zf[4] = {za, zb, za, zb};
 #pragma unroll
                 for (int j = 0; j < kSTiles; ++j) {
-                    x[u][j][0] = x[u][j][1] = x[u][j][2] = x[u][j][3] = 0.f;
-                    Mma<__half>::run(x[u][j], zf, qz[j][0], qz[j][1]);
+                    mma_set(x[u][j], zf, qz[j][0], qz[j][1]);
                 }
 #pragma unroll
                 for (int y = 0; y < kGroups; ++y) {
-                    const uint2 w = lds64(base + y * 256 + lane * 8);
+                    const uint2 w = ld64(base + y * 256 + lane * 8);
                     uint32_t a[4], c[4];
                     code_frag(a, w.x);
                     code_frag(c, w.y);
@@ -421,16 +356,13 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                     float d[kSTiles][4];
 #pragma unroll
                     for (int j = 0; j < kTiles; ++j) {
-                        float* dj = d[kSplit == 2 ? 0 : j];
-                        if (kSplit != 2 || j == 0) dj[0] = dj[1] = dj[2] = dj[3] = 0.f;
-                        if constexpr (C::kQShared) {
-                            const uint4 q = q_s[(j * kGroups + y) * 32];
-                            Mma<__half>::run(dj, a, q.x, q.y);
-                            Mma<__half>::run(dj, c, q.z, q.w);
-                        } else {
-                            Mma<__half>::run(dj, a, qf[j][y][0], qf[j][y][1]);
-                            Mma<__half>::run(dj, c, qf[j][y][2], qf[j][y][3]);
-                        }
+                        uint4 q;
+                        if constexpr (C::kQShared) q = q_s[(j * kGroups + y) * 32];
+                        else q = make_uint4(qf[j][y][0], qf[j][y][1], qf[j][y][2], qf[j][y][3]);
+                        float(&dj)[4] = d[kSplit == 2 ? 0 : j];
+                        if (kSplit != 2 || j == 0) mma_set(dj, a, q.x, q.y);
+                        else mma_add(dj, a, q.x, q.y);
+                        mma_add(dj, c, q.z, q.w);
                     }
 #pragma unroll
                     for (int j = 0; j < kSTiles; ++j) {
@@ -475,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
             __half2 s_top = __float2half2_rn(0.f);
             auto regroup = [&](int u, bool clean) {  // head dim 256: pairs of keys side by side, in shared memory
                 uint32_t w[4];  // key (lane >> 2) + 8 ((lane >> 1) & 1), groups 4 (lane & 1) + 0 .. 3
-                lds128(stage + u * C::kBlockBytes + kv4_off_vparam(D) + lane * 16, w);
+                ld_params(stage + u * C::kBlockBytes + kv4_off_vparam(D) + lane * 16, w);
                 if (!whole) {
                     const int key = key0 + u * kKv4Block + g + 8 * ((lane >> 1) & 1);
                     if (key < key_lo || key > key_hi) w[0] = w[1] = w[2] = w[3] = 0;
@@ -492,16 +424,17 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                 const uint32_t s0 = low_halves(e0, o0), s1 = low_halves(e1, o1);
                 s_top = __hmax2_nan(s_top, __hmax2_nan(h2(s0), h2(s1)));
                 __syncwarp();  // every lane has read what was there
-                const uint32_t at = pairs + ((4 * (lane & 1) + 2 * odd) * 8 + (g >> 1) * 2 + ((lane >> 1) & 1)) * 4;
-                sts32(at, s0);
-                sts32(at + 32, s1);
-                sts32(at + 256, high_halves(e0, o0));
-                sts32(at + 288, high_halves(e1, o1));
+                uint32_t* const at = reinterpret_cast<uint32_t*>(pairs) + (4 * (lane & 1) + 2 * odd) * 8 + (g >> 1) * 2 +
+                                     ((lane >> 1) & 1);
+                at[0] = s0;
+                at[8] = s1;
+                at[64] = high_halves(e0, o0);
+                at[72] = high_halves(e1, o1);
                 __syncwarp();
-                const uint2 z = lds64(pairs + 256 + (g * 4 + t4) * 8);
+                const uint2 z = ld64(pairs + 256 + (g * 4 + t4) * 8);
                 zv[u][0] = z.x;
                 zv[u][1] = z.y;
-                const uint2 sg = lds64(pairs + (g * 4 + t4) * 8);
+                const uint2 sg = ld64(pairs + (g * 4 + t4) * 8);
                 gv[u][0] = sg.x;
                 gv[u][1] = sg.y;
             };
@@ -510,13 +443,13 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                 if constexpr (C::kRegroup) {
                     regroup(u, false);
                 } else {
-                    const uint32_t vp = stage + u * C::kBlockBytes + kv4_off_vparam(D);
+                    const unsigned char* const vp = stage + u * C::kBlockBytes + kv4_off_vparam(D);
                     uint32_t wa[2 * kGroups], wb[2 * kGroups];  // keys 2t, 2t + 1 (and + 8)
-                    lds_params(vp + 2 * t4 * (2 * kGroups * 4), wa);
-                    lds_params(vp + (2 * t4 + 1) * (2 * kGroups * 4), wb);
-                    const uint32_t gz = vp + (2 * t4 * 2 * kGroups + min(g, kGroups - 1)) * 4;
-                    const uint32_t w0 = lds32(gz), w1 = lds32(gz + 2 * kGroups * 4);
-                    const uint32_t w2 = lds32(gz + kGroups * 4), w3 = lds32(gz + 3 * kGroups * 4);
+                    ld_params(vp + 2 * t4 * (2 * kGroups * 4), wa);
+                    ld_params(vp + (2 * t4 + 1) * (2 * kGroups * 4), wb);
+                    const unsigned char* const gz = vp + (2 * t4 * 2 * kGroups + min(g, kGroups - 1)) * 4;
+                    const uint32_t w0 = ld32(gz), w1 = ld32(gz + 2 * kGroups * 4);
+                    const uint32_t w2 = ld32(gz + kGroups * 4), w3 = ld32(gz + 3 * kGroups * 4);
                     uint32_t z0 = high_halves(w0, w1), z1 = high_halves(w2, w3);
                     uint32_t g0 = low_halves(w0, w1), g1 = low_halves(w2, w3);
                     uint32_t m0 = 0xffffffffu, m1 = 0xffffffffu;
@@ -556,11 +489,11 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                     // that see the key, and counts as zero in the products, whose columns share it.
 #pragma unroll
                     for (int u = 0; u < kSub; ++u) {
-                        const uint32_t vp = stage + u * C::kBlockBytes + kv4_off_vparam(D) + g * (2 * kGroups * 4);
+                        const unsigned char* const vp = stage + u * C::kBlockBytes + kv4_off_vparam(D) + g * (2 * kGroups * 4);
 #pragma unroll
                         for (int y = 0; y < kGroups; ++y) {
-                            const bool na = (lds32(vp + y * 4) & 0x7fffu) > 0x7c00u;
-                            const bool nb = (lds32(vp + (kGroups + y) * 4) & 0x7fffu) > 0x7c00u;
+                            const bool na = (ld32(vp + y * 4) & 0x7fffu) > 0x7c00u;
+                            const bool nb = (ld32(vp + (kGroups + y) * 4) & 0x7fffu) > 0x7c00u;
 #pragma unroll
                             for (int j = 0; j < kSTiles; ++j) {
                                 unsigned hit = 0;  // bit per column
@@ -656,9 +589,9 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                     for (int h = 0; h < 2; ++h) {
                         const float p0 = fast_exp2(x[u][j][2 * h]), p1 = fast_exp2(x[u][j][2 * h + 1]);
                         const __half2 hi = __floats2half2_rn(p0, p1);
-                        ph[j][h] = movmatrix_trans(u32(hi));
+                        ph[j][h] = transpose8(u32(hi));
                         if constexpr (kSplit != 0)
-                            pl[j][h] = movmatrix_trans(pack_half2(p0 - __low2float(hi), p1 - __high2float(hi)));
+                            pl[j][h] = transpose8(pack_half2(p0 - __low2float(hi), p1 - __high2float(hi)));
                     }
                 }
                 const bool flip = kSub == 2 ? u == 1 : (i & 1) != 0;
@@ -675,20 +608,20 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
 #pragma unroll
                 for (int j = 0; j < kTiles; ++j) {
                     const uint32_t zf[4] = {zv[u][0], kOnes, zv[u][1], kOnes};
-                    float d[4] = {0.f, 0.f, 0.f, 0.f};
-                    Mma<__half>::run(d, zf, pz[j][0], pz[j][1]);
+                    float d[4];
+                    mma_set(d, zf, pz[j][0], pz[j][1]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) zl[j][e] += d[e];
                     if (flip) {
                         const uint32_t gf[4] = {gv[u][0], 0u, gv[u][1], 0u};
-                        float c[4] = {0.f, 0.f, 0.f, 0.f};
-                        Mma<__half>::run(c, gf, pz[j][0], pz[j][1]);
+                        float c[4];
+                        mma_set(c, gf, pz[j][0], pz[j][1]);
                         ps[j][0] += c[0];
                         ps[j][1] += c[1];
                     }
                 }
                 const uint32_t flip_codes = flip ? 0xffffffffu : 0u, flip_sign = flip ? 0x80008000u : 0u;
-                uint32_t pa[2], pb[2];  // kSplit 1: the words of the lo columns, zero in the others
+                uint32_t pa[2], pb[2];  // kSplit 1: the lo columns' words (the first negated), zero in the others
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -697,13 +630,13 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                         if constexpr (kSplit != 0) pl[j][h] ^= flip_sign;
                     }
                     if constexpr (kSplit == 1) {
-                        pa[h] = g >= 4 ? ph[0][h] : 0u;
+                        pa[h] = g >= 4 ? ph[0][h] ^ 0x80008000u : 0u;
                         pb[h] = g >= 4 ? pl[0][h] : 0u;
                     }
                 }
 #pragma unroll
                 for (int y = 0; y < kGroups; ++y) {
-                    const uint2 w = lds64(stage + u * C::kBlockBytes + kv4_off_v(D) + y * 256 + lane * 8);
+                    const uint2 w = ld64(stage + u * C::kBlockBytes + kv4_off_v(D) + y * 256 + lane * 8);
                     uint32_t a[4], c[4];
                     code_frag(a, w.x, flip_codes);
                     code_frag(c, w.y, flip_codes);
@@ -712,7 +645,7 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                     const uint32_t av[4] = {a[0], a[2], a[1], a[3]}, cv[4] = {c[0], c[2], c[1], c[3]};
                     uint32_t s[2];
                     if constexpr (C::kRegroup) {
-                        const uint2 sp = lds64(pairs + (y * 4 + t4) * 8);
+                        const uint2 sp = ld64(pairs + (y * 4 + t4) * 8);
                         s[0] = sp.x;
                         s[1] = sp.y;
                     } else {
@@ -727,8 +660,8 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
 #pragma unroll
                             for (int j = 0; j < kTiles; ++j) bf[j][h] = u32(__hmul2(h2(ph[j][h]), sc));
                         } else if constexpr (kSplit == 1) {
-                            const __half2 hi = __hmul2(h2(pa[h]), sc);  // lo columns: what the hi column holds
-                            bf[0][h] = u32(__hfma2(h2(pb[h]), sc, __hfma2(h2(ph[0][h]), sc, __hneg2(hi))));
+                            const __half2 hi = __hmul2(h2(pa[h]), sc);  // lo columns: minus what the hi column holds
+                            bf[0][h] = u32(__hfma2(h2(pb[h]), sc, __hfma2(h2(ph[0][h]), sc, hi)));
                         } else {
                             const __half2 hi = __hmul2(h2(ph[0][h]), sc);
                             bf[0][h] = u32(hi);
@@ -737,15 +670,18 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                     }
 #pragma unroll
                     for (int j = 0; j < kTiles; ++j) {
-                        Mma<__half>::run(acc[j][2 * y], av, bf[j][0], bf[j][1]);
-                        Mma<__half>::run(acc[j][2 * y + 1], cv, bf[j][0], bf[j][1]);
+                        mma_add(acc[j][2 * y], av, bf[j][0], bf[j][1]);
+                        mma_add(acc[j][2 * y + 1], cv, bf[j][0], bf[j][1]);
                     }
                 }
             }
             __syncwarp();  // every lane has read the stage
-            fill(issued + 1);
+            if (i + kStages < my_n) issue(i + kStages, slot);
+            if (++slot == kStages) {
+                slot = 0;
+                phase ^= 1;
+            }
         }
-        it += my_n;
         bad = __any_sync(0xffffffffu, bad);
         if (bad && lane == 0) atomicOr(p.status, 16);
         __syncthreads();  // all rings idle: merge_s may alias them
@@ -791,7 +727,7 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
             }
         }
         __syncthreads();
-        float* slot = p.partials + (int64_t)my_slot * kRows * (D + 2);
+        float* slot = p.partials + (int64_t)my_part * kRows * (D + 2);
         if (tid < kRows) {
             float M = kLowest, l = 0.f;
 #pragma unroll
@@ -837,10 +773,10 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                 __threadfence();
                 const int last = atomicAdd(counter, 1) == n_split - 1;
                 if (last) __threadfence();
-                misc[8] = last;
+                misc[0] = last;
             }
             __syncthreads();
-            if (misc[8]) {
+            if (misc[0]) {
                 // the last piece of the unit joins the slots, in the order of the pieces
                 for (int e = tid; e < kRows * D / 4; e += kThreads) {
                     const int row = e * 4 / D, d = e * 4 - row * D;
@@ -853,9 +789,9 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
 #pragma unroll
                         for (int k = 0; k < kBatch; ++k) {
                             if (c + k >= n_split) break;
-                            const long long cc = c0 + c + k;
-                            const int sub = (c + k == 0 && u_start != c0 * R) ? 1 : 0;
-                            const float* sl = p.partials + (2 * cc + sub) * kRows * (D + 2);
+                            // the pieces after the first begin their CTAs' ranges
+                            const int part = c + k == 0 ? part0 : (part_step == 1 ? part0 : part0 & ~1) + part_step * (c + k);
+                            const float* sl = p.partials + (int64_t)part * kRows * (D + 2);
                             ov[k] = __ldcg(reinterpret_cast<const float4*>(sl + row * D + d));
                             mv[k] = __ldcg(sl + kRows * D + row);
                             lv[k] = __ldcg(sl + kRows * D + kRows + row);
@@ -884,7 +820,6 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
     }
-    if (!dep_done) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 struct LaunchInfo {
@@ -901,10 +836,10 @@ LaunchInfo launch_info(int device) {
     std::call_once(once[device], [device] {
         auto kern = kv4_attn_kernel<C>;
         int occ = 0, sms = 0;
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::total(kKv4MaxBatch)) !=
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem) !=
             cudaSuccess)
             return;
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, kThreads, C::total(256)) != cudaSuccess) return;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, kThreads, C::kSmem) != cudaSuccess) return;
         if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return;
         info[device].grid = occ * sms;
     });
@@ -944,14 +879,18 @@ size_t kv4_frag_bytes(const Kv4Params& p) {
 }
 size_t kv4_sums_bytes(const Kv4Params& p) { return (size_t)q_tiles_of(p) * p.Hkv * (p.D / 32 + 1) * 8 * 4; }
 
-void kv4_attn_workspace(const Kv4Params& p, int device, size_t* partial_bytes, size_t* units_per_seq) {
-    *partial_bytes = 0;
+Kv4Split kv4_attn_split(const Kv4Params& p, int device) {
+    Kv4Split split{};
     dispatch(p, [&](auto cfg) {
         using C = decltype(cfg);
-        *partial_bytes = (size_t)2 * launch_info<C>(device).grid * C::kRows * (C::D + 2) * sizeof(float);
-        *units_per_seq = (size_t)p.Hkv * ((p.T * p.G + C::kRows - 1) / C::kRows);
+        split.n_cta = launch_info<C>(device).grid;
+        split.per_seq = p.Hkv * ((p.T * p.G + C::kRows - 1) / C::kRows);
+        split.gap = C::kGapBlocks;
+        split.min_blocks = C::kMinBlocks;
+        split.partial_bytes = (size_t)2 * split.n_cta * C::kRows * (C::D + 2) * sizeof(float);
         return cudaSuccess;
     });
+    return split;
 }
 
 cudaError_t launch_kv4_attn(const Kv4Params& p, int device, cudaStream_t stream) {
@@ -963,7 +902,7 @@ cudaError_t launch_kv4_attn(const Kv4Params& p, int device, cudaStream_t stream)
         cudaLaunchConfig_t launch = {};
         launch.gridDim = dim3((unsigned)li.grid);
         launch.blockDim = dim3(kThreads);
-        launch.dynamicSmemBytes = C::total(p.B);
+        launch.dynamicSmemBytes = C::kSmem;
         launch.stream = stream;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
