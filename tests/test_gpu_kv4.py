@@ -178,6 +178,12 @@ CASES = {
     "chunk_ragged": dict(ctx=[33, 0, 411], T=150, new=[150, 17, 97], Hq=8, Hkv=1, D=64, dtype=oracle.BF16),
     "chunk_window": dict(ctx=[200], T=140, Hq=4, Hkv=1, D=256, window=50, rope="gemma", norm=True, page=48),
     "chunk_mha_96": dict(ctx=[65, 130], T=200, Hq=2, Hkv=2, D=96, page=16),
+    "chunk_bf16_128": dict(ctx=[100, 0, 1000], T=64, Hq=4, Hkv=2, D=128, page=64, dtype=oracle.BF16),
+    "chunk_bf16_window": dict(ctx=[200, 10], T=140, Hq=4, Hkv=1, D=256, window=50, rope="gemma", norm=True, page=48,
+                              dtype=oracle.BF16),
+    "chunk_bf16_96": dict(ctx=[65, 130, 0], T=300, new=[300, 0, 129], Hq=2, Hkv=2, D=96, page=16, dtype=oracle.BF16),
+    "chunk_bf16_wide_window": dict(ctx=[700, 0, 300], T=257, new=[257, 256, 1], Hq=3, Hkv=1, D=64, window=300, page=80,
+                                   rope=None, dtype=oracle.BF16),
     "chunk_prompt": dict(ctx=[0], T=300, Hq=4, Hkv=2, D=64, rope=None),
 }
 
@@ -302,10 +308,11 @@ def test_large_scores_and_values(ctx):
     c.run_decode(ctx)
 
 
-def test_bad_lengths_and_pages_are_reported_and_contained(ctx):
+@pytest.mark.parametrize("T", [2, 70])
+def test_bad_lengths_and_pages_are_reported_and_contained(ctx, T):
     import torch
     import b200attn
-    c = Case(ctx=[20, 40, 50], T=2, Hq=4, Hkv=2, D=64, seed=5, extra_slots=0)
+    c = Case(ctx=[20, 40, 50], T=T, Hq=4, Hkv=2, D=64, seed=5, extra_slots=0, dtype=oracle.BF16)
     t = c.device()
     t["ctx"][1] = 10 ** 6
     before = t["pages"].clone()
@@ -365,15 +372,16 @@ def test_refusals(ctx):
     ctx.check_device_status()
 
 
+@pytest.mark.parametrize("T", [30, 66])
 @pytest.mark.parametrize("D,Hq,dtype", [(64, 4, oracle.F16), (64, 7, oracle.F16), (96, 5, oracle.BF16), (128, 12, oracle.BF16),
                                         (256, 4, oracle.F16), (256, 6, oracle.F16), (256, 3, oracle.BF16)])
-def test_a_key_held_as_nan_reaches_only_the_rows_that_see_it(ctx, D, Hq, dtype):
+def test_a_key_held_as_nan_reaches_only_the_rows_that_see_it(ctx, D, Hq, dtype, T):
     """A value group or a key group that is held as NaN: the rows before it are untouched; the rows that see it
     are NaN, in that group alone (value) or whole (key); with a window it leaves sight again."""
     import torch
     import b200attn
     for which, window in (("v", 0), ("k", 0), ("v", 20), ("k", 20)):
-        c = Case(ctx=[45, 8], T=30, Hq=Hq, Hkv=1, D=D, rope=None, dtype=dtype, window=window, seed=D + Hq)
+        c = Case(ctx=[45, 8], T=T, Hq=Hq, Hkv=1, D=D, rope=None, dtype=dtype, window=window, seed=D + Hq)
         x = c.k if which == "k" else c.v
         x[0, 4, 0, 33] = np.nan
         t = c.device()
@@ -385,8 +393,8 @@ def test_a_key_held_as_nan_reaches_only_the_rows_that_see_it(ctx, D, Hq, dtype):
         x[0, 4, 0, 33] = 0.0
         o, tol, _, _ = c.expect()
         got = to_np(t["o"])
-        sees = np.zeros((2, 30), bool)
-        sees[0, 4:(24 if window else 30)] = True
+        sees = np.zeros((2, T), bool)
+        sees[0, 4:(24 if window else T)] = True
         bad = np.zeros(got.shape, bool)
         bad[sees] = True
         if which == "v":

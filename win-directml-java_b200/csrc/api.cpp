@@ -1227,10 +1227,106 @@ int check_kv4_query(b2a_context* ctx, const void* q, int64_t q_stride, int Hq, f
     return B2A_OK;
 }
 
+// Sequences [b0, b0 + count) of a call.
+Kv4Params kv4_slice(const Kv4Params& p, int b0, int count) {
+    Kv4Params s = p;
+    const int64_t rows = (int64_t)b0 * p.T;
+    auto advance = [](const void* x, int64_t elems) {
+        return x ? static_cast<char*>(const_cast<void*>(x)) + elems * 2 : nullptr;
+    };
+    s.B = count;
+    s.page_table += (int64_t)b0 * p.max_pages;
+    s.ctx_lens += b0;
+    if (s.new_lens) s.new_lens += b0;
+    s.q = advance(p.q, rows * p.q_stride);
+    s.k_new = advance(p.k_new, rows * p.kv_stride);
+    s.v_new = advance(p.v_new, rows * p.kv_stride);
+    s.k_held = advance(p.k_held, rows * p.Hkv * p.D);
+    s.v_held = advance(p.v_held, rows * p.Hkv * p.D);
+    s.o = advance(p.o, rows * p.Hq * p.D);
+    return s;
+}
+
+// Chunks of prompts with bf16 results go to the tcgen05 kernel from this many tokens a sequence on;
+// shorter ones, whose 128-row query tiles would stand mostly empty, and fp16 results, which carry q
+// and P as two words, take the kernel that reads the codes.
+constexpr int kKv4ChunkTokens = 64;
+constexpr size_t kKv4StageBytes = size_t(1) << 30;  // staged cache rows of one launch (one sequence at least)
+
+bool kv4_chunked(const Kv4Params& p) { return p.act_dtype == B2A_BFLOAT16 && p.T >= kKv4ChunkTokens; }
+
+// A chunk: the append, the operands as fp16 rows (kv4_stage.cu), the tcgen05 kernel, and the rows that
+// see a value held as NaN.  kNoRoom: the staged rows did not fit, nothing was launched.
+constexpr int kNoRoom = -1;
+int run_kv4_chunk(b2a_context* ctx, const Kv4Params& p, cudaStream_t stream) {
+    auto r256 = [](size_t x) { return (x + 255) / 256 * 256; };
+    const int64_t Sk64 = ((int64_t)p.max_pages * p.page_size + 127) / 128 * 128;
+    if (Sk64 > INT32_MAX - 128) return kNoRoom;
+    const int Sk = (int)Sk64;
+    const size_t kv_seq = (size_t)Sk * p.Hkv * p.D * 2, q_seq = (size_t)p.T * p.Hq * p.D * 2;
+    const int per = (int)std::max<size_t>(1, std::min<size_t>(p.B, kKv4StageBytes / (2 * kv_seq + q_seq)));
+    const size_t kv_bytes = r256(kv_seq * per), q_bytes = r256(q_seq * per);
+    if (ensure_buffer(ctx, &ctx->pf_ws, &ctx->pf_ws_bytes, 256 + 2 * kv_bytes + q_bytes, "4-bit cache chunk") != B2A_OK) {
+        ctx->last_error.clear();  // the refused workspace is not an error of this call
+        return kNoRoom;
+    }
+    char* base = static_cast<char*>(ctx->pf_ws);
+    int* nan_flag = reinterpret_cast<int*>(base);
+    AttnParams a{};
+    a.in_dtype = B2A_FLOAT16;
+    a.out_dtype = p.act_dtype;
+    a.S = p.T;
+    a.Sk = Sk;
+    a.Hq = p.Hq;
+    a.Hkv = p.Hkv;
+    a.D = p.D;
+    a.q_sb = (int64_t)p.T * p.Hq * p.D;
+    a.q_ss = (int64_t)p.Hq * p.D;
+    a.q_sh = p.D;
+    a.k_sb = (int64_t)Sk * p.Hkv * p.D;
+    a.k_ss = (int64_t)p.Hkv * p.D;
+    a.k_sh = p.D;
+    a.causal = 1;
+    a.window = p.window;
+    a.scale = p.scale;
+    a.q = base + 256;
+    a.k = base + 256 + q_bytes;
+    a.v = base + 256 + q_bytes + kv_bytes;
+    a.B = per;
+    a.q_pos = p.ctx_lens;
+    a.o = p.o;
+    if (!attn_tcgen05_supported(a)) return kNoRoom;
+    cudaError_t e = cudaSuccess;
+    if (p.k_new) {
+        Kv4Params s = p;
+        s.q = nullptr;
+        e = launch_kv4_prepare(s, ctx->sm_count, stream);
+    }
+    for (int b0 = 0; e == cudaSuccess && b0 < p.B; b0 += per) {
+        Kv4Params s = kv4_slice(p, b0, std::min(per, p.B - b0));
+        a.B = s.B;
+        a.q_pos = s.ctx_lens;
+        a.q_len = s.new_lens;
+        a.o = s.o;
+        e = cudaMemsetAsync(nan_flag, 0, sizeof(int), stream);
+        if (e == cudaSuccess)
+            e = launch_kv4_stage(s, base + 256, const_cast<void*>(a.k), const_cast<void*>(a.v), Sk, nan_flag, ctx->sm_count,
+                                 stream);
+        if (e == cudaSuccess) e = launch_attn_tcgen05(a, ctx->status, stream);
+        if (e == cudaSuccess) e = launch_kv4_nan_rows(s, nan_flag, ctx->sm_count, stream);
+    }
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "4-bit cache chunk launch");
+    return B2A_OK;
+}
+
 // The preparation (q's operands, the plan, and the append where p has new rows), then the attention,
 // at most kKv4MaxBatch sequences and 2^31 blocks of the split's stream at a time.
 int run_kv4_attention(b2a_context* ctx, Kv4Params& p, cudaStream_t stream) {
     DeviceGuard guard(ctx->device);
+    if (kv4_chunked(p)) {
+        const int rc = run_kv4_chunk(ctx, p, stream);
+        if (rc != kNoRoom) return rc;
+    }
     auto r256 = [](size_t x) { return (x + 255) / 256 * 256; };
     const int64_t seq_blocks = (int64_t)p.max_pages * p.page_size / 16 + 1 + kKv4GapBlocksMax;
     const int per_launch = (int)std::max<int64_t>(1, std::min<int64_t>(kKv4MaxBatch, INT32_MAX / seq_blocks));
@@ -1260,21 +1356,7 @@ int run_kv4_attention(b2a_context* ctx, Kv4Params& p, cudaStream_t stream) {
     p.q_sums = reinterpret_cast<float*>(take(sums));
     cudaError_t e = cudaSuccess;
     for (int b0 = 0; e == cudaSuccess && b0 < B; b0 += per_launch) {
-        Kv4Params s = p;
-        const int64_t rows = (int64_t)b0 * p.T;
-        auto advance = [&](const void* x, int64_t elems) {
-            return x ? static_cast<char*>(const_cast<void*>(x)) + elems * 2 : nullptr;
-        };
-        s.B = std::min(per_launch, B - b0);
-        s.page_table += (int64_t)b0 * p.max_pages;
-        s.ctx_lens += b0;
-        if (s.new_lens) s.new_lens += b0;
-        s.q = advance(p.q, rows * p.q_stride);
-        s.k_new = advance(p.k_new, rows * p.kv_stride);
-        s.v_new = advance(p.v_new, rows * p.kv_stride);
-        s.k_held = advance(p.k_held, rows * p.Hkv * p.D);
-        s.v_held = advance(p.v_held, rows * p.Hkv * p.D);
-        s.o = advance(p.o, rows * p.Hq * p.D);
+        Kv4Params s = kv4_slice(p, b0, std::min(per_launch, B - b0));
         e = launch_kv4_prepare(s, ctx->sm_count, stream);
         if (e == cudaSuccess) e = launch_kv4_attn(s, ctx->device, stream);
     }

@@ -44,7 +44,9 @@
 // zero half of the panel is never read.
 // Same semantics as attn_simt.cu / attn_mma.cu (the reference citations are
 // there); operands are fp16 (bf16 callers are converted by the host layer).
-// The additive [B][S] key mask has its own instantiation (kAdditive).
+// The additive [B][S] key mask has its own instantiation (kAdditive), and so has a chunk of a
+// sequence (kChunk): query row q of batch b sits at position q_pos[b] + q among Sk keys that begin at
+// position 0, rows at or past q_len[b] do not exist.
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -104,6 +106,10 @@ struct TcParams {
     // in-kernel operand conversion by warps 10 and 11 (kXformQ / K / V): the staged bf16 tile
     // becomes the fp16 operand in place
     int xform;
+    // kChunk: position of query row 0 and number of rows per batch (q_len NULL: S)
+    const int32_t* q_pos;
+    const int32_t* q_len;
+    int Sk;
 };
 constexpr int kXformQ = 1, kXformK = 2, kXformV = 4;
 
@@ -253,11 +259,43 @@ struct ItemGeo {
     int n_max;
     bool uniform;     // tile A has no valid key (key_len <= 0): every key weighs the same
     bool uniform1;    // the same for tile B
+    int shift;        // position of query row 0
+    int rows;         // query rows that exist
 };
+
+// A chunk's item (kChunk): causal at positions shift + row; empty (n_max 0) past the rows that exist.
+__device__ __forceinline__ ItemGeo chunk_geo(int w, int n_pairs, int tiles, int Hq, int S, int Sk, int window,
+                                             const int32_t* q_pos, const int32_t* q_len) {
+    ItemGeo g;
+    const int x = w % n_pairs, rest = w / n_pairs;
+    g.h = g.h1 = rest % Hq;
+    g.b = g.b1 = rest / Hq;
+    g.shift = q_pos[g.b];
+    g.rows = q_len != nullptr ? q_len[g.b] : S;
+    if (g.shift < 0 || g.rows < 0 || g.rows > S || (long long)g.shift + g.rows > Sk) g.shift = g.rows = 0;
+    g.q0a = (n_pairs - 1 - x) * tiles * kBM;
+    g.q0b = tiles == 2 ? g.q0a + kBM : S;
+    const int end = g.shift + g.rows;
+    g.kb0 = g.kb1 = 0;
+    g.ke0 = min(end, g.shift + g.q0a + kBM);
+    g.ke1 = min(end, g.shift + g.q0b + kBM);
+    if (window > 0) {
+        g.kb0 = max(0, g.shift + g.q0a - window + 1);
+        g.kb1 = max(0, g.shift + g.q0b - window + 1);
+    }
+    g.uniform = g.uniform1 = false;
+    g.t_begin = g.kb0 / kBN;
+    g.nt0 = g.q0a < g.rows ? (g.ke0 + kBN - 1) / kBN - g.t_begin : 0;
+    g.nt1 = tiles == 2 && g.q0b < g.rows ? (g.ke1 + kBN - 1) / kBN - g.t_begin : 0;
+    g.n_max = max(g.nt0, g.nt1);
+    return g;
+}
 
 __device__ __forceinline__ ItemGeo item_geo(int w, int n_pairs, int tiles, int Hq, int S, int causal, int window,
                                             const int32_t* key_len, int packed, int n_heads_total) {
     ItemGeo g;
+    g.shift = 0;
+    g.rows = S;
     if (packed) {
         // two (batch, head) pairs of one 128-row tile each, the whole (<= 128-key) sequence visible
         const int bh0 = 2 * w, bh1 = 2 * w + 1;
@@ -325,6 +363,7 @@ constexpr int kSlotTBegin = 9, kSlotNt0 = 10, kSlotNt1 = 11, kSlotUniform = 12;
 constexpr int kSlotIntLo0 = 13, kSlotIntHi0 = 14, kSlotIntLo1 = 15, kSlotIntHi1 = 16;
 // tile B's batch, head and uniform flag (differ from tile A's for packed items)
 constexpr int kSlotB1 = 17, kSlotH1 = 18, kSlotUniform1 = 19;
+constexpr int kSlotShift = 20, kSlotRows = 21;  // kChunk
 constexpr int kSlotInts = 24;
 
 __device__ __forceinline__ void publish_item(volatile int* ms, bool valid, const ItemGeo& g, int causal, int window) {
@@ -345,11 +384,13 @@ __device__ __forceinline__ void publish_item(volatile int* ms, bool valid, const
     ms[kSlotB1] = g.b1;
     ms[kSlotH1] = g.h1;
     ms[kSlotUniform1] = g.uniform1 ? 1 : 0;
+    ms[kSlotShift] = g.shift;
+    ms[kSlotRows] = g.rows;
     // a key tile [n0, n0 + 128) needs no per-element mask when it lies inside the key range,
     // wholly at or below the diagonal of the tile's first row and wholly inside the window of
     // its last row
     for (int t = 0; t < 2; ++t) {
-        const int q_first = t ? g.q0b : g.q0a, q_last = q_first + kBM - 1;
+        const int q_first = (t ? g.q0b : g.q0a) + g.shift, q_last = q_first + kBM - 1;
         int lo = t ? g.kb1 : g.kb0, hi = (t ? g.ke1 : g.ke0) - kBN;
         if (causal) {
             hi = min(hi, q_first - kBN + 1);
@@ -364,7 +405,7 @@ __device__ __forceinline__ void publish_item(volatile int* ms, bool valid, const
     }
 }
 
-template <int D, bool kAdditive>
+template <int D, bool kAdditive, bool kChunk>
 __global__ void __launch_bounds__(kThreadsTc, 1)
     attn_tcgen05_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                         const __grid_constant__ CUtensorMap tmV, const __grid_constant__ TcParams p) {
@@ -484,8 +525,17 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                 } else {
                     if (k >= 2 && !mbar_wait(bItemEmpty(slot), ((k >> 1) - 1) & 1, abort_flag, status)) break;
                     w = atomicAdd(sched, 1);
-                    it = item_geo(w < n_items ? w : 0, n_pairs, Gm::kTiles, Hq, S, causal, window, key_len, packed,
-                                  n_heads_total);
+                    if constexpr (kChunk) {
+                        it = chunk_geo(w < n_items ? w : 0, n_pairs, Gm::kTiles, Hq, S, p.Sk, window, p.q_pos, p.q_len);
+                        while (w < n_items && it.n_max == 0) {  // rows that do not exist
+                            w = atomicAdd(sched, 1);
+                            it = chunk_geo(w < n_items ? w : 0, n_pairs, Gm::kTiles, Hq, S, p.Sk, window, p.q_pos,
+                                           p.q_len);
+                        }
+                    } else {
+                        it = item_geo(w < n_items ? w : 0, n_pairs, Gm::kTiles, Hq, S, causal, window, key_len, packed,
+                                      n_heads_total);
+                    }
                 }
                 if (p.stall && w == 0) skip_g = g + 1;
                 publish_item(slots + kSlotInts * slot, w < n_items, it, causal, window);
@@ -778,9 +828,10 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
             const int n_base = ms[kSlotTBegin] * kBN;
             // keys this row sees: [row_lo, row_hi); a uniform row (no valid key) weights all keys equally
             int row_lo = ms[t ? kSlotKb1 : kSlotKb0], row_hi = ms[t ? kSlotKe1 : kSlotKe0];
-            if (causal) {
-                row_hi = min(row_hi, q + 1);
-                if (window > 0) row_lo = max(row_lo, q - window + 1);
+            if (kChunk || causal) {
+                const int at = kChunk ? q + ms[kSlotShift] : q;
+                row_hi = min(row_hi, at + 1);
+                if (window > 0) row_lo = max(row_lo, at - window + 1);
             }
             // key tiles starting in [int_lo, int_hi] need no per-element mask
             const int int_lo = ms[t ? kSlotIntLo1 : kSlotIntLo0], int_hi = ms[t ? kSlotIntHi1 : kSlotIntHi0];
@@ -911,7 +962,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     uint32_t r[32];
                     tmem_ld32(o_addr + 32 * c, r);
                     tmem_wait_ld();
-                    if (q < S) {
+                    if (q < (kChunk ? ms[kSlotRows] : S)) {
                         const int64_t off = ms[t ? kSlotB1 : kSlotB] * p.o_sb + (int64_t)q * p.o_ss +
                                             ms[t ? kSlotH1 : kSlotH] * p.o_sh + 32 * c;
 #pragma unroll
@@ -977,7 +1028,7 @@ constexpr int smem_request() {
 // count the softmax warpgroups' increase could not be met, so the kernel is
 // reported unsupported and the caller takes another path).
 constexpr int kMaxDevices = 64;
-template <int D, bool kAdditive>
+template <int D, bool kAdditive, bool kChunk>
 cudaError_t kernel_ready() {
     static std::once_flag once[kMaxDevices];
     static cudaError_t err[kMaxDevices];
@@ -985,10 +1036,10 @@ cudaError_t kernel_ready() {
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
     std::call_once(once[dev], [dev] {
         cudaFuncAttributes fa{};
-        cudaError_t e = cudaFuncGetAttributes(&fa, attn_tcgen05_kernel<D, kAdditive>);
+        cudaError_t e = cudaFuncGetAttributes(&fa, attn_tcgen05_kernel<D, kAdditive, kChunk>);
         if (e == cudaSuccess && fa.numRegs != kRegsLaunch) e = cudaErrorInvalidDeviceFunction;
         if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(attn_tcgen05_kernel<D, kAdditive>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+            e = cudaFuncSetAttribute(attn_tcgen05_kernel<D, kAdditive, kChunk>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      smem_request<D>());
         err[dev] = e;
     });
@@ -996,7 +1047,8 @@ cudaError_t kernel_ready() {
 }
 template <int D>
 cudaError_t kernel_ready_for(const AttnParams& p) {
-    return p.mask != nullptr ? kernel_ready<D, true>() : kernel_ready<D, false>();
+    if (p.q_pos != nullptr) return kernel_ready<D, false, true>();
+    return p.mask != nullptr ? kernel_ready<D, true, false>() : kernel_ready<D, false, false>();
 }
 
 // Bidirectional sequences of at most one tile with two query tiles per item (head dim <= 128)
@@ -1017,9 +1069,10 @@ cudaError_t launch_impl(const AttnParams& a, int* status, cudaStream_t stream, b
     if (ready != cudaSuccess) return ready;
     const int fmt = 0;  // fp16 operands (attn_tcgen05_supported)
     CUtensorMap mq, mk, mv;
+    const int Sk = a.q_pos != nullptr ? a.Sk : a.S;
     if (!make_map(&mq, a.q, fmt, a.B, a.S, a.Hq, a.D, a.q_sb, a.q_ss, a.q_sh) ||
-        !make_map(&mk, a.k, fmt, a.B, a.S, a.Hkv, a.D, a.k_sb, a.k_ss, a.k_sh) ||
-        !make_map(&mv, a.v, fmt, a.B, a.S, a.Hkv, a.D, a.k_sb, a.k_ss, a.k_sh))
+        !make_map(&mk, a.k, fmt, a.B, Sk, a.Hkv, a.D, a.k_sb, a.k_ss, a.k_sh) ||
+        !make_map(&mv, a.v, fmt, a.B, Sk, a.Hkv, a.D, a.k_sb, a.k_ss, a.k_sh))
         return cudaErrorInvalidValue;
     TcParams p{};
     p.B = a.B;
@@ -1047,6 +1100,9 @@ cudaError_t launch_impl(const AttnParams& a, int* status, cudaStream_t stream, b
     p.stall = stall ? 1 : 0;
     p.packed = packed_items(a) ? 1 : 0;
     p.xform = a.xform;
+    p.q_pos = a.q_pos;
+    p.q_len = a.q_len;
+    p.Sk = Sk;
     int dev = 0, sms = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) !=
                                                   cudaSuccess || sms <= 0)
@@ -1064,8 +1120,9 @@ cudaError_t launch_impl(const AttnParams& a, int* status, cudaStream_t stream, b
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (additive) return cudaLaunchKernelEx(&cfg, attn_tcgen05_kernel<D, true>, mq, mk, mv, p);
-    return cudaLaunchKernelEx(&cfg, attn_tcgen05_kernel<D, false>, mq, mk, mv, p);
+    if (a.q_pos != nullptr) return cudaLaunchKernelEx(&cfg, attn_tcgen05_kernel<D, false, true>, mq, mk, mv, p);
+    if (additive) return cudaLaunchKernelEx(&cfg, attn_tcgen05_kernel<D, true, false>, mq, mk, mv, p);
+    return cudaLaunchKernelEx(&cfg, attn_tcgen05_kernel<D, false, false>, mq, mk, mv, p);
 }
 
 }  // namespace

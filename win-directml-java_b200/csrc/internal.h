@@ -105,6 +105,11 @@ struct AttnParams {
     // tcgen05 kernel only: 7 = q, k and v are bf16 (in_dtype) and the kernel converts each staged
     // tile to fp16 in shared memory; 0 = fp16 operands as given.
     int xform;
+    // tcgen05 kernel only, a chunk of a sequence: device [B] position of query row 0 among Sk keys
+    // that begin at position 0, and number of query rows (NULL: S); causal.  NULL q_pos: none of this.
+    const int32_t* q_pos;
+    const int32_t* q_len;
+    int Sk;
 };
 
 // Key split of the generic kernel: partial slots and per-query-block counters (zero
@@ -274,6 +279,14 @@ size_t kv4_sums_bytes(const Kv4Params& p);  // per sequence
 Kv4Split kv4_attn_split(const Kv4Params& p, int device);
 // Directly behind launch_kv4_prepare on the stream: it starts before that kernel has ended.
 cudaError_t launch_kv4_attn(const Kv4Params& p, int device, cudaStream_t stream);
+
+// Chunks of prompts over the cache on the tcgen05 kernel (kv4_stage.cu): q rotated to fp16 at q_out
+// [B][T][Hq][D], positions [0, round128(ctx + new)) of the cache as fp16 rows at k_out / v_out
+// [B][Sk][Hkv][D] (what no query sees is zero); nan_flag is set to 1 where a visible value group is
+// held as NaN (it becomes zero; launch_kv4_nan_rows then marks the rows that see it).
+cudaError_t launch_kv4_stage(const Kv4Params& p, void* q_out, void* k_out, void* v_out, int Sk, int* nan_flag,
+                             int sm_count, cudaStream_t stream);
+cudaError_t launch_kv4_nan_rows(const Kv4Params& p, const int* nan_flag, int sm_count, cudaStream_t stream);
 
 // The page table, reference counts and pages of a paged cache (pages.cu).
 struct PagePoolParams {
