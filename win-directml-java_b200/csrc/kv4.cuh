@@ -118,6 +118,26 @@ __device__ __forceinline__ void kv4_norm_rope(float (&x)[D / 32], bool norm, con
     __syncwarp();
 }
 
+// (cos, sin) of positions pos0 .. pos0 + 15 at cs[row * D / 2 + i], as doubles (Gemma) or floats (NeoX),
+// by the block's first D / 2 threads: two double sincos each -- the first position and one step -- and
+// a complex product per further position (an error of some 2^-50, far below the rounding to float; a
+// sincos is about a hundred double instructions).
+template <int D>
+__device__ __forceinline__ void kv4_block_angles(const Kv4Params& p, int pos0, void* cs, int tid) {
+    if (tid >= D / 2) return;
+    double s, c, s1, c1;
+    sincos((double)pos0 * p.inv_freq[tid], &s, &c);
+    sincos(p.inv_freq[tid], &s1, &c1);
+#pragma unroll
+    for (int row = 0; row < 16; ++row) {
+        if (p.rope_mode == 2) static_cast<double2*>(cs)[row * (D / 2) + tid] = make_double2(c, s);
+        else static_cast<float2*>(cs)[row * (D / 2) + tid] = make_float2((float)c, (float)s);
+        const double next = c * c1 - s * s1;
+        s = s * c1 + c * s1;
+        c = next;
+    }
+}
+
 // Quantises the warp's row: lane + 32 j is element lane of group j.  code[j] in 0..15, sz[j] the
 // group's (s, z); true where every group is finite.
 template <int N>

@@ -341,8 +341,8 @@ __device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
 // One block of 16 positions of a sequence, all kv heads of a chunk.  Thread: key row tid / (D / 8),
 // channels 8 (tid % (D / 8)) .. + 7; the four threads of a group share its minimum and maximum.  A key
 // chunk is rotated with its partner chunk D / 2 away, which the thread loads too (it comes from L1).
-template <int D, typename T>
-__global__ void __launch_bounds__(2 * D) kv4_store_kernel(const __grid_constant__ Kv4Params p, int blocks, int chunks,
+template <int D, typename T, bool kNorm>
+__global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 768 / (2 * D)) kv4_store_kernel(const __grid_constant__ Kv4Params p, int blocks, int chunks,
                                                           int per) {
     constexpr int kChunks = D / 8, kGroups = D / 32, kThreads = 2 * D;
     extern __shared__ __align__(16) unsigned char smem[];
@@ -373,23 +373,7 @@ __global__ void __launch_bounds__(2 * D) kv4_store_kernel(const __grid_constant_
         }
     }
     if (t_first >= n) return;  // nothing to store (the whole CTA)
-    if (p.rope_mode != 0) {
-        for (int i = tid; i < 16 * (D / 2); i += kThreads) {
-            const int pos = blk * kKv4Block + i / (D / 2);
-            double sn, c;
-            sincos((double)pos * p.inv_freq[i % (D / 2)], &sn, &c);
-            if (p.rope_mode == 2) static_cast<double2*>(cs)[i] = make_double2(c, sn);
-            else static_cast<float2*>(cs)[i] = make_float2((float)c, (float)sn);
-        }
-    }
-    const bool full = t_first >= 0 && t_first + kKv4Block <= n;
     const int half = k < kChunks / 2 ? 0 : 1, k2 = half ? k - kChunks / 2 : k + kChunks / 2;
-    float wn[8], wn2[8];  // key norm weights of both chunks
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        wn[i] = p.k_norm_w ? p.k_norm_w[8 * k + i] : 0.f;
-        wn2[i] = p.k_norm_w ? p.k_norm_w[8 * k2 + i] : 0.f;
-    }
     uint4 nk = make_uint4(0, 0, 0, 0), nk2 = nk, nv = nk;  // the next head's loads
     auto fetch = [&](int h) {
         if (!there || h >= h1) return;
@@ -398,6 +382,17 @@ __global__ void __launch_bounds__(2 * D) kv4_store_kernel(const __grid_constant_
         nk2 = *reinterpret_cast<const uint4*>(kr + 8 * k2);
         nv = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.v_new) + tok * p.kv_stride + (int64_t)h * D + 8 * k);
     };
+    fetch(h0);
+    if (p.rope_mode != 0) kv4_block_angles<D>(p, blk * kKv4Block, cs, tid);
+    const bool full = t_first >= 0 && t_first + kKv4Block <= n;
+    float wn[kNorm ? 8 : 1], wn2[kNorm ? 8 : 1];  // key norm weights of both chunks
+    if constexpr (kNorm) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            wn[i] = p.k_norm_w[8 * k + i];
+            wn2[i] = p.k_norm_w[8 * k2 + i];
+        }
+    }
     // one row chunk into the block at `dst`; its bytes of the codes and the group's params
     auto quantise = [&](const float (&x)[8], bool is_v, uint8_t* dst, void* held, int h) {
         float lo = x[0], hi = x[0], odd = 0.f;
@@ -454,7 +449,6 @@ __global__ void __launch_bounds__(2 * D) kv4_store_kernel(const __grid_constant_
         if ((k & 3) == 0)
             reinterpret_cast<__half2*>(dst + kv4_off_kparam(D))[kv4_param(row, y, kGroups)] = __halves2half2(s, z);
     };
-    fetch(h0);
     __syncthreads();
     for (int h = h0; h < h1; ++h) {
         uint8_t* dst = stage + ((h - h0) & 1) * 20 * D;
@@ -463,7 +457,7 @@ __global__ void __launch_bounds__(2 * D) kv4_store_kernel(const __grid_constant_
         unpack8<T>(nk2, y);
         unpack8<T>(nv, v);
         fetch(h + 1);
-        if (p.k_norm_w) {
+        if constexpr (kNorm) {
             double ss = 0.0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) ss += (double)x[i] * (double)x[i];
@@ -535,7 +529,7 @@ cudaError_t launch_store(const Kv4Params& p, int sm_count, cudaStream_t stream) 
     const int want = (int)std::min<int64_t>(p.Hkv, std::max<int64_t>(1, 4 * sm_count / ctas));
     const int per = (p.Hkv + want - 1) / want, chunks = (p.Hkv + per - 1) / per;
     const size_t smem = 2 * 20 * D + 16 * (D / 8) * 8 + 16 * (D / 2) * (p.rope_mode == 2 ? sizeof(double2) : sizeof(float2));
-    auto kern = kv4_store_kernel<D, T>;
+    auto kern = p.k_norm_w ? kv4_store_kernel<D, T, true> : kv4_store_kernel<D, T, false>;
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;

@@ -21,14 +21,19 @@ __device__ __forceinline__ int first_seen(const Kv4Params& p, int L) {
 }
 
 // ---------------------------------------------------------------- q
-// A block takes 16 tokens of a sequence and walks the heads two at a time; a thread holds channels
-// 8 k .. + 7 and their partners D / 2 further.
+// A block takes 16 tokens of a sequence and kStageHeads heads, two at a time; a thread holds channels
+// 8 k .. + 7 and their partners D / 2 further.  Few heads to a block: its time is the latency of its
+// loads one after another, not the sines that it computes again.
+constexpr int kStageHeads = 4;
 template <int D, typename T>
 __device__ __forceinline__ void stage_query(const Kv4Params& p, __half* out, int block, int blocks, unsigned char* smem) {
     constexpr int kHalf = D / 16, kThreads = 2 * D;  // chunk pairs of a row; 2 heads x 16 tokens x kHalf threads
-    double2* const cs = reinterpret_cast<double2*>(smem);           // [16][D / 2]
+    void* const cs = smem;  // [16][D / 2] (cos, sin)
     double* const part = reinterpret_cast<double*>(smem + 16 * (D / 2) * sizeof(double2));
     const int tid = threadIdx.x;
+    const int head_blocks = (p.Hq + kStageHeads - 1) / kStageHeads;
+    const int head0 = block % head_blocks * kStageHeads, head1 = min(p.Hq, head0 + kStageHeads);
+    block /= head_blocks;
     const int b = block / blocks, t0 = (block - b * blocks) * 16;
     int L, n;
     const bool ok = kv4_lens(p, b, L, n);
@@ -40,23 +45,18 @@ __device__ __forceinline__ void stage_query(const Kv4Params& p, __half* out, int
     const bool there = t < n;
     if (!there && t < p.T) {  // no such token: its outputs are zero, or NaN where the lengths do not fit
         const uint32_t v = ok ? 0u : 0x7fff7fffu;
-        for (int h = sub; h < p.Hq; h += 2) {
+        for (int h = head0 + sub; h < head1; h += 2) {
             uint4* o = reinterpret_cast<uint4*>(static_cast<T*>(p.o) + (tok * p.Hq + h) * D + 8 * k);
             o[0] = o[kHalf] = make_uint4(v, v, v, v);
         }
     }
     if (t0 >= n) return;
-    if (p.rope_mode != 0)
-        for (int i = tid; i < 16 * (D / 2); i += kThreads) {
-            double sn, c;
-            sincos((double)(L + t0 + i / (D / 2)) * p.inv_freq[i % (D / 2)], &sn, &c);
-            cs[i] = make_double2(c, sn);
-        }
+    if (p.rope_mode != 0) kv4_block_angles<D>(p, L + t0, cs, tid);
     __syncthreads();
     float top = 0.f;
-    for (int h0 = 0; h0 < p.Hq; h0 += 2) {
+    for (int h0 = head0; h0 < head1; h0 += 2) {
         const int h = h0 + sub;
-        const bool live = there && h < p.Hq;
+        const bool live = there && h < head1;
         float x[8], y[8];
         uint4 wx = make_uint4(0, 0, 0, 0), wy = wx;
         if (live) {
@@ -88,14 +88,16 @@ __device__ __forceinline__ void stage_query(const Kv4Params& p, __half* out, int
         if (p.rope_mode != 0) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const double2 c = cs[row * (D / 2) + 8 * k + i];
+                const int at = row * (D / 2) + 8 * k + i;
                 const float a = x[i], e = y[i];
                 if (p.rope_mode == 2) {
+                    const double2 c = static_cast<const double2*>(cs)[at];
                     x[i] = (float)((double)a * c.x - (double)e * c.y);
                     y[i] = (float)((double)e * c.x + (double)a * c.y);
                 } else {
-                    x[i] = a * (float)c.x - e * (float)c.y;
-                    y[i] = a * (float)c.y + e * (float)c.x;
+                    const float2 c = static_cast<const float2*>(cs)[at];
+                    x[i] = a * c.x - e * c.y;
+                    y[i] = a * c.y + e * c.x;
                 }
             }
         }
@@ -111,48 +113,74 @@ __device__ __forceinline__ void stage_query(const Kv4Params& p, __half* out, int
 }
 
 // ---------------------------------------------------------------- cache rows
-// One block of 16 positions of one kv head at a time, through shared memory: thread (row, chunk of 8
-// channels) gathers its 8 codes' bytes.
+// One warp turns one group (32 channels) of a block of 16 positions into fp16 rows.  A lane's two code
+// words hold, as the MMA wants them, channel pairs of keys g and g + 8 (K) or key pairs of channels
+// (V^T); the latter are transposed 8 x 8 at a time.  s c + z is one f16 FMA on the exact code: rounded
+// once.
 template <int D>
-__device__ __forceinline__ void stage_block(const Kv4Params& p, const uint8_t* src, int pos, int first, int end, __half* k_row0,
-                                            __half* v_row0, int64_t row_stride, int* nan_flag, uint8_t* blk) {
-    constexpr int kChunks = D / 8, kThreads = 2 * D, kGroups = D / 32;
-    const int tid = threadIdx.x, row = tid / kChunks, k = tid - row * kChunks;
-    if (src != nullptr)
-        for (int i = tid; i < 20 * D / 16; i += kThreads)
-            reinterpret_cast<uint4*>(blk)[i] = reinterpret_cast<const uint4*>(src)[i];
-    __syncthreads();
-    const bool there = src != nullptr && pos + row >= first && pos + row < end;
-    const int y = k >> 2, x16 = (k >> 1) & 1, j = k & 1, g = row & 7, r = row >> 3;
+__device__ __forceinline__ void stage_group(const Kv4Params& p, const uint8_t* src, int y, int pos, int first, int end,
+                                            __half* k_row0, __half* v_row0, int64_t row_stride, int* nan_flag,
+                                            int lane) {
+    constexpr int kGroups = D / 32;
+    const int g = lane >> 2, t = lane & 3;
+    auto seen = [&](int key) { return src != nullptr && pos + key >= first && pos + key < end; };
+    uint32_t code[2][2] = {{0, 0}, {0, 0}}, sz[2][3][2] = {};  // [K or V][..]: key g / 2 t / 2 t + 1, + 8
+    if (src != nullptr) {
 #pragma unroll
-    for (int is_v = 0; is_v < 2; ++is_v) {
-        uint4 out = make_uint4(0, 0, 0, 0);
-        if (there) {
-            const uint8_t* code = blk + is_v * kv4_off_v(D);
-            const float2 sz = __half22float2(
-                reinterpret_cast<const __half2*>(code + kv4_off_kparam(D))[kv4_param(row, y, kGroups)]);
-            float v[8];
-            float top = 0.f;
+        for (int is_v = 0; is_v < 2; ++is_v) {
+            const uint8_t* at = src + is_v * kv4_off_v(D);
+            const uint2 w = __ldg(reinterpret_cast<const uint2*>(at + y * 256 + lane * 8));
+            code[is_v][0] = w.x;
+            code[is_v][1] = w.y;
+            const uint32_t* par = reinterpret_cast<const uint32_t*>(at + kv4_off_kparam(D)) + y;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int at = is_v ? ((y * 8 + i) * 4 + (g >> 1)) * 8 + x16 * 4 + 2 * (g & 1) + r
-                                    : ((y * 8 + g) * 4 + (i >> 1)) * 8 + x16 * 4 + 2 * (i & 1) + r;
-                v[i] = fmaf((float)(code[at] >> (4 * j) & 15), sz.x, sz.y);
-                top = fmaxf(top, fabsf(v[i]));
+            for (int r = 0; r < 2; ++r) {
+                if (!is_v) {
+                    sz[0][0][r] = __ldg(par + (g * 2 + r) * kGroups);
+                } else {
+                    sz[1][1][r] = __ldg(par + (2 * t * 2 + r) * kGroups);
+                    sz[1][2][r] = __ldg(par + ((2 * t + 1) * 2 + r) * kGroups);
+                }
             }
-            if (top >= 65520.f) atomicOr(p.status, 4);
-            if (is_v && !(sz.x == sz.x)) {  // held as NaN: zero here, and the rows that see it are marked later
-                *nan_flag = 1;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = 0.f;
-            }
-            uint32_t* w = &out.x;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = pack_half2(v[2 * i], v[2 * i + 1]);
         }
-        *reinterpret_cast<uint4*>((is_v ? v_row0 : k_row0) + row * row_stride + 8 * k) = out;
     }
-    __syncthreads();  // blk is reused
+    auto value = [](uint32_t w, uint32_t s2, uint32_t z2) {
+        const uint32_t c = (w & 0x000F000Fu) | 0x64006400u;  // f16x2 1024 + code
+        const __half2 x = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&c), __float2half2_rn(1024.f)),
+                                  *reinterpret_cast<const __half2*>(&s2), *reinterpret_cast<const __half2*>(&z2));
+        return *reinterpret_cast<const uint32_t*>(&x);
+    };
+    bool big = false, nan = false;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const bool row_seen = seen(g + 8 * r);
+        const uint32_t ks = __byte_perm(sz[0][0][r], 0, 0x1010), kz = __byte_perm(sz[0][0][r], 0, 0x3232);
+        uint32_t vs = __byte_perm(sz[1][1][r], sz[1][2][r], 0x5410), vz = __byte_perm(sz[1][1][r], sz[1][2][r], 0x7632);
+        // a value held as NaN counts as zero here; the rows that see it are marked later
+        if ((vs & 0x7fffu) > 0x7c00u) {
+            nan |= seen(2 * t + 8 * r);
+            vs &= 0xffff0000u, vz &= 0xffff0000u;
+        }
+        if ((vs >> 16 & 0x7fffu) > 0x7c00u) {
+            nan |= seen(2 * t + 1 + 8 * r);
+            vs &= 0xffffu, vz &= 0xffffu;
+        }
+        const int64_t at = (int64_t)(g + 8 * r) * row_stride + 32 * y + 2 * t;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                uint32_t k = value(code[0][x] >> (8 * r + 4 * j), ks, kz);
+                uint32_t v = movmatrix_trans(value(code[1][x] >> (8 * r + 4 * j), vs, vz));
+                if (!row_seen) k = v = 0;
+                big |= (k & 0x7fffu) == 0x7c00u || (k >> 16 & 0x7fffu) == 0x7c00u || (v & 0x7fffu) == 0x7c00u ||
+                       (v >> 16 & 0x7fffu) == 0x7c00u;
+                *reinterpret_cast<uint32_t*>(k_row0 + at + 16 * x + 8 * j) = k;
+                *reinterpret_cast<uint32_t*>(v_row0 + at + 16 * x + 8 * j) = v;
+            }
+    }
+    if (__any_sync(0xffffffffu, big) && lane == 0) atomicOr(p.status, 4);
+    if (__any_sync(0xffffffffu, nan) && lane == 0) *nan_flag = 1;
 }
 
 template <int D, typename T>
@@ -166,21 +194,25 @@ __global__ void __launch_bounds__(2 * D) kv4_stage_kernel(const __grid_constant_
         return;
     }
     const int64_t row_stride = (int64_t)p.Hkv * D;
-    int64_t i = blockIdx.x - q_total;
-    const int64_t step = gridDim.x - q_total;
+    constexpr int kGroups = D / 32, kWarps = 2 * D / 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int64_t i = (int64_t)(blockIdx.x - q_total) * kWarps + warp;
+    const int64_t step = (int64_t)(gridDim.x - q_total) * kWarps;
     for (int b = 0; b < p.B; ++b) {
         int L, n;
         if (!kv4_lens(p, b, L, n) || n == 0) continue;
         const int first = first_seen(p, L), end = L + n;
         const int blk0 = first / 128 * 8, blk1 = min((end + 127) / 128 * 8, Sk / kKv4Block);
-        const int64_t count = (int64_t)(blk1 - blk0) * p.Hkv;
+        const int per_blk = p.Hkv * kGroups;
+        const int64_t count = (int64_t)(blk1 - blk0) * per_blk;
         for (; i < count; i += step) {
-            const int blk = blk0 + (int)(i / p.Hkv), h = (int)(i % p.Hkv), pos = blk * kKv4Block;
+            const int blk = blk0 + (int)(i / per_blk), in = (int)(i % per_blk), h = in / kGroups, y = in % kGroups;
+            const int pos = blk * kKv4Block;
             const bool seen = pos + kKv4Block > first && pos < end;
             const uint8_t* src = seen ? kv4_block_ptr(p, b, h, pos) : nullptr;
-            if (seen && src == nullptr && threadIdx.x == 0) atomicOr(p.status, 16);
+            if (seen && src == nullptr && lane == 0) atomicOr(p.status, 16);
             const int64_t at = ((int64_t)b * Sk + pos) * row_stride + (int64_t)h * D;
-            stage_block<D>(p, src, pos, first, end, k_out + at, v_out + at, row_stride, nan_flag, smem);
+            stage_group<D>(p, src, y, pos, first, end, k_out + at, v_out + at, row_stride, nan_flag, lane);
         }
         i -= count;
     }
@@ -224,14 +256,13 @@ __global__ void __launch_bounds__(256) kv4_nan_rows_kernel(const __grid_constant
 template <int D, typename T>
 cudaError_t launch_stage(const Kv4Params& p, __half* q_out, __half* k_out, __half* v_out, int Sk, int* nan_flag,
                          int sm_count, cudaStream_t stream) {
-    const size_t q_smem = 16 * (D / 2) * sizeof(double2) + 2 * D * sizeof(double);
-    const size_t smem = q_smem > 20 * D ? q_smem : 20 * D;
+    const size_t smem = 16 * (D / 2) * sizeof(double2) + 2 * D * sizeof(double);
     auto kern = kv4_stage_kernel<D, T>;
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
     }
-    const int q_blocks = (p.T + 15) / 16, q_total = p.B * q_blocks;
+    const int q_blocks = (p.T + 15) / 16, q_total = p.B * q_blocks * ((p.Hq + kStageHeads - 1) / kStageHeads);
     kern<<<q_total + sm_count * 8, 2 * D, smem, stream>>>(p, q_out, k_out, v_out, Sk, nan_flag, q_blocks, q_total);
     return cudaGetLastError();
 }
