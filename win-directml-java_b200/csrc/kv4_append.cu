@@ -9,7 +9,7 @@
 // steps -- so every read is requested before the first one is waited for, and the attention kernel
 // is launched behind it early, to be resident when it ends.
 // kv4_store_kernel: prompts. A CTA takes one block of 16 positions and walks kv heads; a thread holds
-// 8 channels of a row (16-byte loads), the block is assembled in shared memory and stored whole.
+// 8 channels of four rows (16-byte loads), the block is assembled in shared memory and stored whole.
 #include <algorithm>
 
 #include "kv4.cuh"
@@ -331,26 +331,77 @@ __global__ void __launch_bounds__(kPrepThreads) kv4_prepare_kernel(const __grid_
 }
 
 // ------------------------------------------------------------------ prompts
-template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
-    const T* e = reinterpret_cast<const T*>(&w);
+__device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8], __half) {
+    const uint32_t* e = &w.x;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = Elem<T>::to_float(e[i]);
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(e + i));
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+    }
+}
+__device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8], __nv_bfloat16) {
+    const uint32_t* e = &w.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __uint_as_float(e[i] << 16);
+        x[2 * i + 1] = __uint_as_float(e[i] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN where either is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+    float d;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// The low 16 bits' nibbles into the low nibbles of four bytes.
+__device__ __forceinline__ uint32_t spread_nibbles(uint32_t x) {
+    x = (x | x << 8) & 0x00FF00FFu;
+    return (x | x << 4) & 0x0F0F0F0Fu;
 }
 
-// One block of 16 positions of a sequence, all kv heads of a chunk.  Thread: key row tid / (D / 8),
-// channels 8 (tid % (D / 8)) .. + 7; the four threads of a group share its minimum and maximum.  A key
-// chunk is rotated with its partner chunk D / 2 away, which the thread loads too (it comes from L1).
+// Threads of one (block of 16 positions, kv head): thread (q, k) holds channels 8 k .. + 7 of rows
+// 2 q, 2 q + 1, 2 q + 8, 2 q + 9 -- the four keys whose codes share the V words -- so that whole 32-bit
+// words are put together in registers.
+template <int D>
+struct StoreGeo {
+    static constexpr int kChunks = D / 8;
+    static constexpr int kPerHead = 4 * kChunks;              // threads: 32, 48, 64, 128
+    static constexpr int kHeads = D <= 64 ? 8 : (D <= 128 ? 4 : 2);  // heads of a CTA side by side, at most
+    static constexpr int kMinHeads = D == 96 ? 2 : 1;         // whole warps
+    static constexpr int kMaxThreads = kHeads * kPerHead;
+    static constexpr int kCtas = D == 96 ? 4 : (D == 256 ? 2 : 3);  // per SM, about 80 registers a thread
+    static size_t smem(int heads, int rope_mode) {
+        return (size_t)heads * (20 * D + 16 * kChunks * 8) +
+               16 * (D / 2) * (rope_mode == 2 ? sizeof(double2) : sizeof(float2));
+    }
+};
+
+// A CTA takes one block of a sequence and heads h0 + group, + groups, ...  A key chunk is rotated with
+// its partner chunk D / 2 away, which the thread loads too (it comes from L1); the four threads of a
+// group share its minimum and maximum.  Bound by its instructions, about 17 per value (measured 2.8
+// per cycle and SM with 291 per 8 values before the words were put together in registers).
 template <int D, typename T, bool kNorm>
-__global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 768 / (2 * D)) kv4_store_kernel(const __grid_constant__ Kv4Params p, int blocks, int chunks,
-                                                          int per) {
-    constexpr int kChunks = D / 8, kGroups = D / 32, kThreads = 2 * D;
+__global__ void __launch_bounds__(StoreGeo<D>::kMaxThreads, StoreGeo<D>::kCtas)
+    kv4_store_kernel(const __grid_constant__ Kv4Params p, int blocks, int chunks, int per) {
+    using Gm = StoreGeo<D>;
+    constexpr int kChunks = Gm::kChunks, kGroups = D / 32;
     extern __shared__ __align__(16) unsigned char smem[];
-    uint8_t* const stage = smem;                                          // two blocks
-    double* const part = reinterpret_cast<double*>(smem + 2 * 20 * D);    // [16][kChunks] sums of squares
-    void* const cs = smem + 2 * 20 * D + 16 * kChunks * 8;                // [16][D / 2] (cos, sin)
-    const int tid = threadIdx.x;
-    const int row = tid / kChunks, k = tid - row * kChunks;
+    const int tid = threadIdx.x, groups = blockDim.x / Gm::kPerHead;
+    const int group = tid / Gm::kPerHead, in_group = tid - group * Gm::kPerHead;
+    const int q = in_group / kChunks, k = in_group - q * kChunks;
+    uint8_t* const stage = smem + group * 20 * D;
+    double* const part = reinterpret_cast<double*>(smem + groups * 20 * D) + group * 16 * kChunks;
+    void* const cs = smem + groups * (20 * D + 16 * kChunks * 8);  // [16][D / 2] (cos, sin)
     const int chunk = blockIdx.x % chunks;
     const int64_t bb = blockIdx.x / chunks;
     const int b = (int)(bb / blocks);
@@ -358,163 +409,215 @@ __global__ void __launch_bounds__(2 * D, D == 256 ? 1 : 768 / (2 * D)) kv4_store
     const bool ok = kv4_lens(p, b, L, n);
     if (!ok && tid == 0) atomicOr(p.status, 1);
     const int blk = L / kKv4Block + (int)(bb - (int64_t)b * blocks);
-    const int t = blk * kKv4Block + row - L;  // this row's token
-    const int t_first = blk * kKv4Block - L;
+    const int t_first = blk * kKv4Block - L;  // token of the block's first position
     if (t_first >= p.T) return;
-    const bool there = t >= 0 && t < n;
-    const int h0 = chunk * per, h1 = min(p.Hkv, h0 + per);
-    const int64_t tok = (int64_t)b * p.T + t;
-    if (t >= n && t < p.T) {  // rows that do not exist
+    const int h_begin = chunk * per, h_end = min(p.Hkv, h_begin + per);
+    auto row_of = [&](int i) { return 2 * q + (i & 1) + 8 * (i >> 1); };  // i = e + 2 r
+    const int64_t seq_tok = (int64_t)b * p.T;
+    for (int i = 0; i < 4; ++i) {  // rows that do not exist
+        const int t = t_first + row_of(i);
+        if (t < n || t >= p.T) continue;
         const uint32_t v = ok ? 0u : 0x7fff7fffu;
-        for (int h = h0; h < h1; ++h) {
-            const int64_t at = (tok * p.Hkv + h) * D + 8 * k;
+        for (int h = h_begin + group; h < h_end; h += groups) {
+            const int64_t at = ((seq_tok + t) * p.Hkv + h) * D + 8 * k;
             if (p.k_held) *reinterpret_cast<uint4*>(static_cast<T*>(p.k_held) + at) = make_uint4(v, v, v, v);
             if (p.v_held) *reinterpret_cast<uint4*>(static_cast<T*>(p.v_held) + at) = make_uint4(v, v, v, v);
         }
     }
     if (t_first >= n) return;  // nothing to store (the whole CTA)
-    const int half = k < kChunks / 2 ? 0 : 1, k2 = half ? k - kChunks / 2 : k + kChunks / 2;
-    uint4 nk = make_uint4(0, 0, 0, 0), nk2 = nk, nv = nk;  // the next head's loads
-    auto fetch = [&](int h) {
-        if (!there || h >= h1) return;
-        const T* kr = static_cast<const T*>(p.k_new) + tok * p.kv_stride + (int64_t)h * D;
-        nk = *reinterpret_cast<const uint4*>(kr + 8 * k);
-        nk2 = *reinterpret_cast<const uint4*>(kr + 8 * k2);
-        nv = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.v_new) + tok * p.kv_stride + (int64_t)h * D + 8 * k);
-    };
-    fetch(h0);
     if (p.rope_mode != 0) kv4_block_angles<D>(p, blk * kKv4Block, cs, tid);
     const bool full = t_first >= 0 && t_first + kKv4Block <= n;
-    float wn[kNorm ? 8 : 1], wn2[kNorm ? 8 : 1];  // key norm weights of both chunks
-    if constexpr (kNorm) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            wn[i] = p.k_norm_w[8 * k + i];
-            wn2[i] = p.k_norm_w[8 * k2 + i];
-        }
-    }
-    // one row chunk into the block at `dst`; its bytes of the codes and the group's params
-    auto quantise = [&](const float (&x)[8], bool is_v, uint8_t* dst, void* held, int h) {
-        float lo = x[0], hi = x[0], odd = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            lo = fminf(lo, x[i]);
-            hi = fmaxf(hi, x[i]);
-            odd = fmaf(x[i], 0.f, odd);  // NaN where some value is not finite
-        }
-#pragma unroll
-        for (int o = 1; o <= 2; o <<= 1) {
-            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-            odd += __shfl_xor_sync(0xffffffffu, odd, o);
-        }
-        __half s = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f)), z = __float2half_rn(lo);
-        const float sf = __half2float(s), zf = __half2float(z);
-        const bool fine = odd == 0.f && isfinite(sf) && isfinite(zf);
-        const float inv = sf > 0.f && fine ? __fdiv_rn(1.0f, sf) : 0.f;
-        uint32_t codes = 0;
-        uint4 out;
-        uint32_t* ow = &out.x;
-        float v[8];
-        const float ns = fine ? sf : __int_as_float(0x7fc00000), nz = fine ? zf : ns;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            // 0 .. 15 first, then to the nearest whole number (ties to even) by 1.5 * 2^23
-            float c = fminf(fmaxf(__fmul_rn(__fsub_rn(x[i], zf), inv), 0.f), 15.f);
-            c = __fadd_rn(c, 12582912.f);
-            codes |= (__float_as_uint(c) & 15u) << (4 * i);
-            v[i] = fmaf(__fsub_rn(c, 12582912.f), ns, nz);
-        }
-        if (!fine) {
-            codes = 0;
-            s = z = __ushort_as_half(0x7fff);
-            if (there) atomicOr(p.status, 32);
-        }
-        if (held && there) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) ow[i] = Elem<T>::pack(v[2 * i], v[2 * i + 1]);
-            *reinterpret_cast<uint4*>(static_cast<T*>(held) + (tok * p.Hkv + h) * D + 8 * k) = out;
-        }
-        const uint32_t other = __shfl_xor_sync(0xffffffffu, codes, 1);
-        const int j = k & 1, x16 = (k >> 1) & 1, y = k >> 2, g = row & 7, r = row >> 3;
-        const uint32_t low = j ? other : codes, high = j ? codes : other;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int i = 4 * j + e;  // channels 8 .. + i and 8 further
-            const uint8_t byte = (uint8_t)((low >> (4 * i) & 15u) | (high >> (4 * i) & 15u) << 4);
-            const int at = is_v ? ((y * 8 + i) * 4 + (g >> 1)) * 8 + x16 * 4 + 2 * (g & 1) + r
-                                : ((y * 8 + g) * 4 + (i >> 1)) * 8 + x16 * 4 + 2 * (i & 1) + r;
-            dst[at] = byte;
-        }
-        if ((k & 3) == 0)
-            reinterpret_cast<__half2*>(dst + kv4_off_kparam(D))[kv4_param(row, y, kGroups)] = __halves2half2(s, z);
-    };
+    const bool upper = k >= kChunks / 2;
+    const int k2 = upper ? k - kChunks / 2 : k + kChunks / 2, k_low = upper ? k2 : k;
+    const int j = k & 1, x16 = (k >> 1) & 1, y = k >> 2;
     __syncthreads();
-    for (int h = h0; h < h1; ++h) {
-        uint8_t* dst = stage + ((h - h0) & 1) * 20 * D;
-        float x[8], y[8], v[8];
-        unpack8<T>(nk, x);
-        unpack8<T>(nk2, y);
-        unpack8<T>(nv, v);
-        fetch(h + 1);
+
+    for (int h0 = h_begin; h0 < h_end; h0 += groups) {
+        const int h = h0 + group;
+        const bool live = h < h_end;
         if constexpr (kNorm) {
-            double ss = 0.0;
+            for (int i = 0; i < 4; ++i) {
+                const int t = t_first + row_of(i);
+                double ss = 0.0;
+                if (live && t >= 0 && t < n) {
+                    float x[8];
+                    unpack8(*reinterpret_cast<const uint4*>(static_cast<const T*>(p.k_new) + (seq_tok + t) * p.kv_stride +
+                                                            (int64_t)h * D + 8 * k), x, T{});
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ss += (double)x[i] * (double)x[i];
-            part[tid] = ss;
+                    for (int c = 0; c < 8; ++c) ss += (double)x[c] * (double)x[c];
+                }
+                part[row_of(i) * kChunks + k] = ss;
+            }
             __syncthreads();
-            ss = 0.0;
-            for (int i = 0; i < kChunks; ++i) ss += part[row * kChunks + i];
-            __syncthreads();
-            const float rms = (float)(1.0 / sqrt(__dadd_rn(ss / (double)D, (double)p.norm_eps)));
+        }
+        // every row is requested before the first one is used: a row after another would pay the
+        // memory's latency eight times
+        uint4 raw[3][4];  // K chunk, its partner, V chunk
+        const int64_t first_row = (seq_tok + t_first + 2 * q) * p.kv_stride + (int64_t)h * D + 8 * k;
+        const T *const k_at = static_cast<const T*>(p.k_new) + first_row, *const v_at = static_cast<const T*>(p.v_new) + first_row;
+        const uint32_t flip = upper ? 0u : 0x80008000u;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[i] = (float)__dmul_rn((double)__fmul_rn(x[i], rms), __dadd_rn(1.0, (double)wn[i]));
-                y[i] = (float)__dmul_rn((double)__fmul_rn(y[i], rms), __dadd_rn(1.0, (double)wn2[i]));
+        for (int i = 0; i < 4; ++i) {
+            const int t = t_first + row_of(i);
+            const int64_t at = ((i & 1) + 8 * (i >> 1)) * p.kv_stride;
+            raw[0][i] = raw[1][i] = raw[2][i] = make_uint4(0, 0, 0, 0);
+            if (!(live && t >= 0 && t < n)) continue;
+            raw[0][i] = __ldg(reinterpret_cast<const uint4*>(k_at + at));
+            if (p.rope_mode != 0) raw[1][i] = __ldg(reinterpret_cast<const uint4*>(k_at + at + 8 * (k2 - k)));
+            raw[2][i] = __ldg(reinterpret_cast<const uint4*>(v_at + at));
+        }
+        const int64_t held_at = ((seq_tok + t_first + 2 * q) * p.Hkv + h) * D + 8 * k;
+        uint32_t bytes[2][4];  // [K, V][row]: the bytes of channels 4 j .. + 3 of the chunk pair (k, k ^ 1)
+#pragma unroll
+        for (int is_v = 0; is_v < 2; ++is_v) {
+            void* held = is_v ? p.v_held : p.k_held;
+            uint8_t* const dst = stage + (is_v ? kv4_off_v(D) : 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = row_of(i), t = t_first + row;
+                const bool there = live && t >= 0 && t < n;
+                float x[8];
+                unpack8(raw[2 * is_v][i], x, T{});
+                if (!is_v) {
+                    float rms = 0.f;
+                    if constexpr (kNorm) {
+                        double ss = 0.0;
+                        for (int c = 0; c < kChunks; ++c) ss += part[row * kChunks + c];
+                        rms = (float)(1.0 / sqrt(__dadd_rn(ss / (double)D, (double)p.norm_eps)));
+#pragma unroll
+                        for (int c = 0; c < 8; ++c)
+                            x[c] = (float)__dmul_rn((double)__fmul_rn(x[c], rms), __dadd_rn(1.0, (double)__ldg(p.k_norm_w + 8 * k + c)));
+                    }
+                    if (p.rope_mode != 0) {
+                        float z[8];
+                        uint4 w = raw[1][i];
+                        w.x ^= flip, w.y ^= flip, w.z ^= flip, w.w ^= flip;
+                        unpack8(w, z, T{});
+                        if constexpr (kNorm) {
+#pragma unroll
+                            for (int c = 0; c < 8; ++c)
+                                z[c] = (float)__dmul_rn((double)__fmul_rn(z[c], rms), __dadd_rn(1.0, (double)__ldg(p.k_norm_w + 8 * k2 + c)));
+                        }
+                        if (p.rope_mode == 2) {
+                            const double2* a = static_cast<const double2*>(cs) + row * (D / 2) + 8 * k_low;
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) {
+                                const double u = __dmul_rn((double)x[c], a[c].x), v = __dmul_rn((double)z[c], a[c].y);
+                                x[c] = (float)__dadd_rn(u, v);
+                            }
+                        } else {
+                            const float4* a = reinterpret_cast<const float4*>(static_cast<const float2*>(cs) + row * (D / 2) + 8 * k_low);
+#pragma unroll
+                            for (int c = 0; c < 8; c += 2) {  // the lower chunk's partner comes negated
+                                const float4 ang = a[c / 2];
+                                x[c] = __fadd_rn(__fmul_rn(x[c], ang.x), __fmul_rn(z[c], ang.y));
+                                x[c + 1] = __fadd_rn(__fmul_rn(x[c + 1], ang.z), __fmul_rn(z[c + 1], ang.w));
+                            }
+                        }
+                    }
+                }
+                // the group's minimum and maximum: NaN reaches `hi`, infinities both
+                float lo = min3(min3(x[0], x[1], x[2]), min3(x[3], x[4], x[5]), fminf(x[6], x[7]));
+                float hi = max_nan(max_nan(x[0], x[1], x[2]), max_nan(x[3], x[4], x[5]), max_nan(x[6], x[7]));
+#pragma unroll
+                for (int o = 1; o <= 2; o <<= 1) {
+                    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+                    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+                }
+                __half s = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f)), z = __float2half_rn(lo);
+                const float sf = __half2float(s), zf = __half2float(z);
+                const bool fine = isfinite(sf) && isfinite(zf);
+                const float inv = sf > 0.f && fine ? __fdiv_rn(1.0f, sf) : 0.f;
+                const float ns = fine ? sf : __int_as_float(0x7fc00000), nz = fine ? zf : ns;
+                float code[8];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) code[c] = __fmul_rn(__fsub_rn(x[c], zf), inv);
+                // into 0 .. 15 where the group's ends leave it (z and s are rounded: rarely)
+                const float u_lo = __fmul_rn(__fsub_rn(lo, zf), inv), u_hi = __fmul_rn(__fsub_rn(hi, zf), inv);
+                if (!(u_lo >= -0.5f && u_hi <= 15.5f)) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) code[c] = fminf(fmaxf(code[c], 0.f), 15.f);
+                }
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    // to the nearest whole number (ties to even) by 1.5 * 2^23
+                    code[c] = __fsub_rn(__fadd_rn(code[c], 12582912.f), 12582912.f);
+                    x[c] = fmaf(code[c], ns, nz);
+                }
+                if (held && there) {
+                    uint4 out;
+                    uint32_t* ow = &out.x;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) ow[c] = Elem<T>::pack(x[2 * c], x[2 * c + 1]);
+                    *reinterpret_cast<uint4*>(static_cast<T*>(held) + held_at + ((i & 1) + 8 * (i >> 1)) * p.Hkv * D) = out;
+                }
+                // four codes to 16 bits, exactly, as c0 + 16 c1 + 256 c2 + 4096 c3
+                uint32_t half[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const float f = fmaf(code[4 * c + 3], 4096.f, fmaf(code[4 * c + 2], 256.f, fmaf(code[4 * c + 1], 16.f, code[4 * c])));
+                    half[c] = fine ? __float_as_uint(__fadd_rn(f, 8388608.f)) & 0xffffu : 0u;
+                }
+                // thread j keeps channels 4 j .. + 3 of both chunks of the pair
+                const uint32_t other = __shfl_xor_sync(0xffffffffu, j ? half[0] : half[1], 1);
+                const uint32_t own = j ? half[1] : half[0];
+                bytes[is_v][i] = spread_nibbles(j ? other : own) | spread_nibbles(j ? own : other) << 4;
+                if (!fine) {
+                    s = z = __ushort_as_half(0x7fff);
+                    if (there) atomicOr(p.status, 32);
+                }
+                if ((k & 3) == 0)
+                    reinterpret_cast<__half2*>(dst + kv4_off_kparam(D))[kv4_param(row, y, kGroups)] = __halves2half2(s, z);
             }
         }
-        if (p.rope_mode == 2) {
-            const double2* c = static_cast<const double2*>(cs) + row * (D / 2) + 8 * (half ? k2 : k);
+        {
+            // K words (lane 4 g + t, x16): bytes (e, r) = channels 2 t + e of keys g + 8 r
+            uint32_t* const kw = reinterpret_cast<uint32_t*>(stage) + y * 64 + x16;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                x[i] = half ? (float)__dadd_rn(__dmul_rn((double)x[i], c[i].x), __dmul_rn((double)y[i], c[i].y))
-                            : (float)__dsub_rn(__dmul_rn((double)x[i], c[i].x), __dmul_rn((double)y[i], c[i].y));
-        } else if (p.rope_mode == 1) {
-            const float2* c = static_cast<const float2*>(cs) + row * (D / 2) + 8 * (half ? k2 : k);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float u = __fmul_rn(x[i], c[i].x), w = __fmul_rn(y[i], c[i].y);
-                x[i] = half ? __fadd_rn(w, u) : __fsub_rn(u, w);
+            for (int e = 0; e < 2; ++e) {
+                const int g = 2 * q + e;
+                const uint32_t a = bytes[0][e], c = bytes[0][e + 2];  // keys g, g + 8
+                kw[(4 * g + 2 * j) * 2] = __byte_perm(a, c, 0x5140);
+                kw[(4 * g + 2 * j + 1) * 2] = __byte_perm(a, c, 0x7362);
             }
+            // V words (lane 4 g + t, x16): bytes (e, r) = channel g of keys 2 t + e + 8 r
+            uint32_t* const vw = reinterpret_cast<uint32_t*>(stage + kv4_off_v(D)) + y * 64 + x16;
+            const uint32_t a = __byte_perm(bytes[1][0], bytes[1][2], 0x5140), c = __byte_perm(bytes[1][1], bytes[1][3], 0x5140);
+            const uint32_t u = __byte_perm(bytes[1][0], bytes[1][2], 0x7362), v = __byte_perm(bytes[1][1], bytes[1][3], 0x7362);
+            vw[(4 * (4 * j + 0) + q) * 2] = __byte_perm(a, c, 0x5410);
+            vw[(4 * (4 * j + 1) + q) * 2] = __byte_perm(a, c, 0x7632);
+            vw[(4 * (4 * j + 2) + q) * 2] = __byte_perm(u, v, 0x5410);
+            vw[(4 * (4 * j + 3) + q) * 2] = __byte_perm(u, v, 0x7632);
         }
-        quantise(x, false, dst, p.k_held, h);
-        quantise(v, true, dst + kv4_off_v(D), p.v_held, h);
         __syncthreads();
-        uint8_t* block = kv4_block_ptr(p, b, h, blk * kKv4Block);
-        if (block == nullptr) {
-            if (tid == 0) atomicOr(p.status, 16);
-        } else if (full) {
-            for (int i = tid; i < 20 * D / 16; i += kThreads)
-                reinterpret_cast<uint4*>(block)[i] = reinterpret_cast<const uint4*>(dst)[i];
-        } else {
-            // the rows that exist: their bytes of the codes, their params
-            auto mine = [&](int key) {
-                const int tk = t_first + key;
-                return tk >= 0 && tk < n;
-            };
-            for (int i = tid; i < 16 * D; i += kThreads) {
-                const bool is_v = i >= 8 * D;
-                const int a = is_v ? i - 8 * D : i;
-                const int r = a & 1, e = (a >> 1) & 1, q = (a >> 3) & 3, g = (a >> 5) & 7;
-                const int at = is_v ? kv4_off_v(D) + a : a;
-                if (mine(is_v ? 2 * q + e + 8 * r : g + 8 * r)) block[at] = dst[at];
-            }
-            for (int i = tid; i < 2 * 16 * kGroups; i += kThreads) {
-                const int w = i % (16 * kGroups), key = (w / kGroups >> 1) + 8 * (w / kGroups & 1);
-                const int at = (i < 16 * kGroups ? kv4_off_kparam(D) : kv4_off_vparam(D)) + 4 * w;
-                if (mine(key)) *reinterpret_cast<uint32_t*>(block + at) = *reinterpret_cast<const uint32_t*>(dst + at);
+        if (live) {
+            uint8_t* const block = kv4_block_ptr(p, b, h, blk * kKv4Block);
+            if (block == nullptr) {
+                if (in_group == 0) atomicOr(p.status, 16);
+            } else if (full) {
+                for (int i = in_group; i < 20 * D / 16; i += Gm::kPerHead)
+                    reinterpret_cast<uint4*>(block)[i] = reinterpret_cast<const uint4*>(stage)[i];
+            } else {
+                // the rows that exist: their bytes of the codes, their params
+                auto mine = [&](int key) {
+                    const int tk = t_first + key;
+                    return tk >= 0 && tk < n;
+                };
+                for (int i = in_group; i < 16 * D; i += Gm::kPerHead) {
+                    const bool is_v = i >= 8 * D;
+                    const int a = is_v ? i - 8 * D : i;
+                    const int r = a & 1, e = (a >> 1) & 1, t = (a >> 3) & 3, g = (a >> 5) & 7;
+                    const int at = is_v ? kv4_off_v(D) + a : a;
+                    if (mine(is_v ? 2 * t + e + 8 * r : g + 8 * r)) block[at] = stage[at];
+                }
+                for (int i = in_group; i < 2 * 16 * kGroups; i += Gm::kPerHead) {
+                    const int w = i % (16 * kGroups), key = (w / kGroups >> 1) + 8 * (w / kGroups & 1);
+                    const int at = (i < 16 * kGroups ? kv4_off_kparam(D) : kv4_off_vparam(D)) + 4 * w;
+                    if (mine(key)) *reinterpret_cast<uint32_t*>(block + at) = *reinterpret_cast<const uint32_t*>(stage + at);
+                }
             }
         }
+        __syncthreads();  // the stage is used again
     }
 }
 
@@ -523,18 +626,21 @@ constexpr int kStoreMinTokens = 16;
 
 template <int D, typename T>
 cudaError_t launch_store(const Kv4Params& p, int sm_count, cudaStream_t stream) {
+    using Gm = StoreGeo<D>;
     const int blocks = (p.T + 2 * kKv4Block - 2) / kKv4Block;  // blocks that T tokens can touch
     const int64_t ctas = (int64_t)p.B * blocks;
+    const int groups = std::max(Gm::kMinHeads, std::min(Gm::kHeads, p.Hkv));
     // a CTA computes its block's sines once for all its heads: heads are cut only where CTAs are few
-    const int want = (int)std::min<int64_t>(p.Hkv, std::max<int64_t>(1, 4 * sm_count / ctas));
-    const int per = (p.Hkv + want - 1) / want, chunks = (p.Hkv + per - 1) / per;
-    const size_t smem = 2 * 20 * D + 16 * (D / 8) * 8 + 16 * (D / 2) * (p.rope_mode == 2 ? sizeof(double2) : sizeof(float2));
+    const int rounds = (p.Hkv + groups - 1) / groups;
+    const int want = (int)std::min<int64_t>(rounds, std::max<int64_t>(1, 4 * sm_count / ctas));
+    const int per = (rounds + want - 1) / want * groups, chunks = (p.Hkv + per - 1) / per;
+    const size_t smem = Gm::smem(groups, p.rope_mode);
     auto kern = p.k_norm_w ? kv4_store_kernel<D, T, true> : kv4_store_kernel<D, T, false>;
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
     }
-    kern<<<(unsigned)(ctas * chunks), 2 * D, smem, stream>>>(p, blocks, chunks, per);
+    kern<<<(unsigned)(ctas * chunks), groups * Gm::kPerHead, smem, stream>>>(p, blocks, chunks, per);
     return cudaGetLastError();
 }
 
