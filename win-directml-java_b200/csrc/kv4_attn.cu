@@ -126,23 +126,33 @@ __device__ __forceinline__ void mma_add(float (&d)[4], const uint32_t (&a)[4], u
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_set(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+// (zero: four registers that hold 0; a constant would be copied into d's registers each time)
+struct Zero {
+    float r[4];
+    __device__ __forceinline__ Zero() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) asm volatile("mov.f32 %0, 0f00000000;" : "=f"(r[i]));
+    }
+};
+__device__ __forceinline__ void mma_set(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const Zero& z) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(z.r[0]), "f"(z.r[1]), "f"(z.r[2]),
+          "f"(z.r[3]));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {  // movmatrix
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
     return y;
 }
-// The A operand of one 16 x 16 tile of codes, or of 15 - codes (flip all ones).
-__device__ __forceinline__ void code_frag(uint32_t (&a)[4], uint32_t w, uint32_t flip = 0) {
+// The A operand of one 16 x 16 tile of codes, or of 15 - codes (kFlip).
+template <bool kFlip = false>
+__device__ __forceinline__ void code_frag(uint32_t (&a)[4], uint32_t w) {
     const uint32_t h = w >> 8;
-    a[0] = (w ^ flip) & 0x000F000Fu;
-    a[1] = (h ^ flip) & 0x000F000Fu;
-    a[2] = (w ^ flip) & 0x00F000F0u;
-    a[3] = (h ^ flip) & 0x00F000F0u;
+    a[0] = (kFlip ? ~w : w) & 0x000F000Fu;
+    a[1] = (kFlip ? ~h : h) & 0x000F000Fu;
+    a[2] = (kFlip ? ~w : w) & 0x00F000F0u;
+    a[3] = (kFlip ? ~h : h) & 0x00F000F0u;
 }
 __device__ __forceinline__ __half2 h2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
 __device__ __forceinline__ uint32_t u32(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
@@ -313,7 +323,9 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
         float s_log = 0.f;                                 // log2 of the bound on the value scales
         __half2 s_bound = __float2half2_rn(1.f);
 
-        for (int i = 0; i < my_n && !dead; ++i) {
+        const Zero zero;
+        // one stage; `odd`: its blocks are the complemented ones (with two blocks a stage, the second is)
+        auto step = [&](int i, auto odd) {
             if (!wait_bounded(bars + slot * 8, phase)) {
                 // report, wait for the others in flight and ask for no more; the outputs are NaN
                 if (lane == 0) atomicOr(p.status, 8);
@@ -322,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                     const bool wrap = slot + k >= kStages;
                     if (!wait_bounded(bars + (wrap ? slot + k - kStages : slot + k) * 8, phase ^ (wrap ? 1u : 0u))) break;
                 }
-                break;
+                return;
             }
             const unsigned char* const stage = ring + slot * C::kStageBytes;
             const int key0 = (blk0 + (warp + kWarps * i) * kSub) * kKv4Block;
@@ -344,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                 const uint32_t zf[4] = {za, zb, za, zb};
 #pragma unroll
                 for (int j = 0; j < kSTiles; ++j) {
-                    mma_set(x[u][j], zf, qz[j][0], qz[j][1]);
+                    mma_set(x[u][j], zf, qz[j][0], qz[j][1], zero);
                 }
 #pragma unroll
                 for (int y = 0; y < kGroups; ++y) {
@@ -360,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                         if constexpr (C::kQShared) q = q_s[(j * kGroups + y) * 32];
                         else q = make_uint4(qf[j][y][0], qf[j][y][1], qf[j][y][2], qf[j][y][3]);
                         float(&dj)[4] = d[kSplit == 2 ? 0 : j];
-                        if (kSplit != 2 || j == 0) mma_set(dj, a, q.x, q.y);
+                        if (kSplit != 2 || j == 0) mma_set(dj, a, q.x, q.y, zero);
                         else mma_add(dj, a, q.x, q.y);
                         mma_add(dj, c, q.z, q.w);
                     }
@@ -579,8 +591,9 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
             }
 
             // ---------------------------------------------------- P, and the second product
-#pragma unroll
-            for (int u = 0; u < kSub; ++u) {
+            auto second_product = [&](auto block, auto complemented) {
+                constexpr int u = decltype(block)::value;
+                constexpr bool flip = decltype(complemented)::value;
                 // B operands: P of keys 0..7 and 8..15 of the block (hi words; lo words where kept)
                 uint32_t ph[kSTiles][2], pl[kSplit ? kSTiles : 1][2];
 #pragma unroll
@@ -594,7 +607,6 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                             pl[j][h] = transpose8(pack_half2(p0 - __low2float(hi), p1 - __high2float(hi)));
                     }
                 }
-                const bool flip = kSub == 2 ? u == 1 : (i & 1) != 0;
                 // zl += [z^T; 1] P, and for a complemented block ps += s^T P
                 uint32_t pz[kTiles][2];
 #pragma unroll
@@ -609,18 +621,18 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                 for (int j = 0; j < kTiles; ++j) {
                     const uint32_t zf[4] = {zv[u][0], kOnes, zv[u][1], kOnes};
                     float d[4];
-                    mma_set(d, zf, pz[j][0], pz[j][1]);
+                    mma_set(d, zf, pz[j][0], pz[j][1], zero);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) zl[j][e] += d[e];
-                    if (flip) {
+                    if constexpr (flip) {
                         const uint32_t gf[4] = {gv[u][0], 0u, gv[u][1], 0u};
                         float c[4];
-                        mma_set(c, gf, pz[j][0], pz[j][1]);
+                        mma_set(c, gf, pz[j][0], pz[j][1], zero);
                         ps[j][0] += c[0];
                         ps[j][1] += c[1];
                     }
                 }
-                const uint32_t flip_codes = flip ? 0xffffffffu : 0u, flip_sign = flip ? 0x80008000u : 0u;
+                constexpr uint32_t flip_sign = flip ? 0x80008000u : 0u;
                 uint32_t pa[2], pb[2];  // kSplit 1: the lo columns' words (the first negated), zero in the others
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -638,8 +650,8 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                 for (int y = 0; y < kGroups; ++y) {
                     const uint2 w = ld64(stage + u * C::kBlockBytes + kv4_off_v(D) + y * 256 + lane * 8);
                     uint32_t a[4], c[4];
-                    code_frag(a, w.x, flip_codes);
-                    code_frag(c, w.y, flip_codes);
+                    code_frag<flip>(a, w.x);
+                    code_frag<flip>(c, w.y);
                     // V^T's tile has the channel as its row: registers in the order (channel g, keys 2t),
                     // (g + 8, 2t), (g, 2t + 8), (g + 8, 2t + 8)
                     const uint32_t av[4] = {a[0], a[2], a[1], a[3]}, cv[4] = {c[0], c[2], c[1], c[3]};
@@ -674,12 +686,26 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                         mma_add(acc[j][2 * y + 1], cv, bf[j][0], bf[j][1]);
                     }
                 }
+            };
+            if constexpr (kSub == 2) {
+                second_product(std::integral_constant<int, 0>{}, std::false_type{});
+                second_product(std::integral_constant<int, 1>{}, std::true_type{});
+            } else {
+                second_product(std::integral_constant<int, 0>{}, odd);
             }
             __syncwarp();  // every lane has read the stage
             if (i + kStages < my_n) issue(i + kStages, slot);
             if (++slot == kStages) {
                 slot = 0;
                 phase ^= 1;
+            }
+        };
+        if constexpr (kSub == 2) {
+            for (int i = 0; i < my_n && !dead; ++i) step(i, std::false_type{});
+        } else {
+            for (int i = 0; i < my_n && !dead; i += 2) {
+                step(i, std::false_type{});
+                if (i + 1 < my_n && !dead) step(i + 1, std::true_type{});
             }
         }
         bad = __any_sync(0xffffffffu, bad);
