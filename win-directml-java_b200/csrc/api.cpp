@@ -1334,12 +1334,11 @@ int run_kv4_attention(b2a_context* ctx, Kv4Params& p, cudaStream_t stream) {
     if (p.split.n_cta <= 0) return fail(ctx, B2A_ECUDA, "no attention kernel for this device");
     const int B = p.B, most = std::min(B, per_launch);
     const size_t units = (size_t)most * p.split.per_seq;
-    const size_t part = r256(p.split.partial_bytes), head = r256(p.split.n_cta * sizeof(int2)),
-                 plan = r256((p.split.n_cta + units) * sizeof(Kv4Piece)), frag = r256(kv4_frag_bytes(p) * most),
+    const size_t part = r256(p.split.partial_bytes), plan = r256((p.split.n_cta + units) * sizeof(Kv4Piece)), frag = r256(kv4_frag_bytes(p) * most),
                  sums = r256(kv4_sums_bytes(p) * most);
     size_t counter_bytes = 0;
     const int rc = ensure_counted_buffer(ctx, &ctx->kv4_ws, &ctx->kv4_ws_bytes, &ctx->kv4_counter_bytes, units,
-                                         part + head + plan + frag + sums, "4-bit cache attention", stream, false,
+                                         part + plan + frag + sums, "4-bit cache attention", stream, false,
                                          &counter_bytes);
     if (rc) return rc;
     char* at = static_cast<char*>(ctx->kv4_ws);
@@ -1350,7 +1349,6 @@ int run_kv4_attention(b2a_context* ctx, Kv4Params& p, cudaStream_t stream) {
     };
     p.counters = reinterpret_cast<int*>(take(counter_bytes));
     p.partials = reinterpret_cast<float*>(take(part));
-    p.plan_head = reinterpret_cast<int2*>(take(head));
     p.plan = reinterpret_cast<Kv4Piece*>(take(plan));
     p.q_frag = reinterpret_cast<uint4*>(take(frag));
     p.q_sums = reinterpret_cast<float*>(take(sums));

@@ -224,7 +224,9 @@ cudaError_t launch_linear_tc(const LinearArgs& a, int* status, cudaStream_t stre
 struct Kv4Piece {
     int b, r, L, n;
     int blk0, blk1, n_split, my_part;
-    int part0, part_step, pad0, pad1;
+    int part0, part_step;
+    int count, more;  // of a CTA's first piece: its pieces, and where the second one lies (the others follow
+                      // at the places of their units)
 };
 // How the attention kernel wants its work spread (kv4_attn.cu).
 struct Kv4Split {
@@ -264,8 +266,7 @@ struct Kv4Params {
     float* q_sums;
     int* counters;
     float* partials;
-    int2* plan_head;  // [n_cta]: first piece and number of pieces of each attention CTA
-    Kv4Piece* plan;   // [n_cta + units]
+    Kv4Piece* plan;   // [n_cta] each attention CTA's first piece, then by unit the others
     Kv4Split split;
     double inv_freq[kMaxHeadDim / 2];
 };

@@ -198,10 +198,13 @@ __device__ __noinline__ void plan_attention(const Kv4Params& p, PlanShared& sh, 
     const int c = block * kPrepThreads + tid;
     if (c >= n_cta) return;
     const long long total = (long long)before * per_seq;
-    const long long R = pieces ? 1 : max((long long)p.split.min_blocks, (total + n_cta - 1) / n_cta);
+    const bool small = total + n_cta <= (long long)INT32_MAX;  // 32-bit divisions
+    auto quotient = [&](long long a, long long d) { return small ? (long long)((int)a / (int)d) : a / d; };
+    const long long R = pieces ? 1 : max((long long)p.split.min_blocks, quotient(total + n_cta - 1, n_cta));
     long long pos = c * R;
     const long long end = min(total, pos + R);
-    int made = 0, at = c;
+    int made = 0, more = 0;
+    Kv4Piece first_piece{};
     while (pos < end) {
         int lo = 0, hi = p.B - 1;
         while (lo < hi) {  // the last sequence that starts at or before pos
@@ -211,10 +214,10 @@ __device__ __noinline__ void plan_attention(const Kv4Params& p, PlanShared& sh, 
         }
         const int b = lo, w = sh.prefix[b + 1] - sh.prefix[b];
         const long long seq_base = (long long)sh.prefix[b] * per_seq;
-        int r = (int)((pos - seq_base) / w);
+        int r = (int)quotient(pos - seq_base, w);
         const int nb = seen_blocks(p, sh.ctx[b], sh.fresh[b], first);
-        // the pieces of CTA c come after those of the CTAs before it: at most one per CTA and unit
-        if (made == 0 && !pieces) at = c + b * per_seq + r;
+        // pieces after the first lie from n_cta + their unit's number on: a unit that is not a CTA's
+        // first begins inside that CTA's range, so no other CTA's range begins it
         for (; r < per_seq && pos < end; ++r) {
             const long long u_start = seq_base + (long long)r * w;
             Kv4Piece piece{};
@@ -223,9 +226,9 @@ __device__ __noinline__ void plan_attention(const Kv4Params& p, PlanShared& sh, 
             piece.L = sh.ctx[b];
             piece.n = sh.fresh[b];
             if (pieces) {
-                const int k = (int)(pos - u_start);
-                piece.blk0 = first + (int)((long long)nb * k / w);
-                piece.blk1 = first + (int)((long long)nb * (k + 1) / w);
+                const int k = (int)(pos - u_start), each = nb / w, rest = nb - each * w;
+                piece.blk0 = first + k * each + k * rest / w;
+                piece.blk1 = first + (k + 1) * each + (k + 1) * rest / w;
                 piece.n_split = w;
                 piece.my_part = c;
                 piece.part0 = c - k;
@@ -237,7 +240,7 @@ __device__ __noinline__ void plan_attention(const Kv4Params& p, PlanShared& sh, 
                     pos = u_start + w;
                     continue;
                 }
-                const long long c0 = u_start / R, c1 = (u_end - 1) / R, stop = min(end, u_end);
+                const long long c0 = quotient(u_start, R), c1 = quotient(u_end - 1, R), stop = min(end, u_end);
                 piece.blk0 = first + (int)(pos - u_start);
                 piece.blk1 = first + (int)(stop - u_start);
                 piece.n_split = (int)(c1 - c0) + 1;
@@ -247,11 +250,18 @@ __device__ __noinline__ void plan_attention(const Kv4Params& p, PlanShared& sh, 
                 piece.part_step = 2;
                 pos = stop < end ? u_start + w : end;
             }
-            p.plan[at + made] = piece;
+            if (made == 0) {
+                first_piece = piece;
+            } else {
+                if (made == 1) more = n_cta + b * per_seq + r;
+                p.plan[n_cta + b * per_seq + r] = piece;
+            }
             ++made;
         }
     }
-    p.plan_head[c] = make_int2(at, made);
+    first_piece.count = made;
+    first_piece.more = more;
+    p.plan[c] = first_piece;
 }
 
 // Rows of a token: Hq queries (where p.q), Hkv keys and Hkv values (where `append`); after the

@@ -196,11 +196,16 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
 
     // the preparation kernel made the plan, the q operands and the new rows' blocks
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int2 mine = p.plan_head[blockIdx.x];
-    const Kv4Piece* piece = p.plan + mine.x;
-    for (int k_piece = 0; k_piece < mine.y; ++k_piece, ++piece) {
+    const Kv4Piece* piece = p.plan + blockIdx.x;
+    int pieces_left = 1, next = 0;
+    for (bool begin = true; pieces_left > 0; --pieces_left, begin = false, piece = p.plan + next++) {
         const int4 w0 = reinterpret_cast<const int4*>(piece)[0], w1 = reinterpret_cast<const int4*>(piece)[1],
                    w2 = reinterpret_cast<const int4*>(piece)[2];
+        if (begin) {
+            pieces_left = w2.z;
+            next = w2.w;
+            if (pieces_left == 0) break;
+        }
         const int b = w0.x, r = w0.y, L = w0.z, n = w0.w;
         const int n_split = w1.z, my_part = w1.w, part0 = w2.x, part_step = w2.y;
         const int kvh = r / row_tiles, rt = r - kvh * row_tiles;
@@ -255,8 +260,6 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
             for (; !dead && issued < min(upto, my_n); ++issued)
                 issue(issued, slot + issued < kStages ? slot + issued : slot + issued - kStages);
         };
-        fill(kStages);
-
         // ------------------------------------------------------------ q operands
         // B operand words per column tile and group: four a lane (two 16-channel steps), column g
         uint32_t qf[kTiles][kGroups][4], qz[kSTiles][2];
@@ -298,6 +301,8 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                 }
             }
         }
+        // requested after q's operands: the page-table entries arrive meanwhile
+        fill(kStages);
         if (C::kQShared) __syncthreads();
         // keys [all_lo, all_hi] are seen by every present row of the tile (what an absent row
         // computes is not used, and its q operand is zero)
