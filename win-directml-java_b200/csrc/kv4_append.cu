@@ -100,12 +100,13 @@ __device__ __forceinline__ void append_row(const Kv4Params& p, float (&x)[D / 32
 
 // Spreads the attention's work over its CTAs, in one of two ways:
 //  * pieces: every unit is cut into k near-equal pieces of at most P blocks, one piece per CTA.  P is
-//    the smallest of eight sizes, from the guaranteed one, blocks / (CTAs - units), down, that needs
-//    no more pieces than there are CTAs.
+//    the smallest of three sizes, the guaranteed one, blocks / (CTAs - units), 7/8 and 13/16 of it,
+//    that needs no more pieces than there are CTAs.
 //  * ranges: the blocks of all units, each followed by `gap` that stand for the fixed cost of a piece,
 //    form one stream; CTA c takes its c-th equal range, so it may meet several units.
 // Pieces are taken where the largest costs no more than a range with a second piece's fixed cost.
-// Every planning block sums the lengths itself and writes the pieces of its 256 CTAs.
+// Every planning block sums the lengths itself and writes the pieces of its 256 CTAs.  The attention
+// waits for the plan, so it is written for few steps: 32-bit arithmetic wherever the stream allows.
 constexpr int kPrepThreads = kPrepWarps * 32;
 
 __device__ __forceinline__ int seen_blocks(const Kv4Params& p, int L, int n, int& first) {
@@ -117,8 +118,64 @@ __device__ __forceinline__ int cuts_of(int blocks, float inv) { return max(1, (i
 struct PlanShared {
     int prefix[kKv4MaxBatch + 1];  // per unit: pieces, or stream length, of the sequences before
     int ctx[kKv4MaxBatch], fresh[kKv4MaxBatch];
-    int sums[10][kPrepWarps];
+    int sums[6][kPrepWarps];
 };
+
+// One piece, with what its CTA's first one tells about the others.
+__device__ __forceinline__ void put_piece(Kv4Piece* to, int b, int r, int L, int n, int blk0, int blk1, int n_split,
+                                          int my_part, int part0, int part_step) {
+    int4* w = reinterpret_cast<int4*>(to);
+    w[0] = make_int4(b, r, L, n);
+    w[1] = make_int4(blk0, blk1, n_split, my_part);
+    *reinterpret_cast<int2*>(&to->part0) = make_int2(part0, part_step);
+}
+
+// The pieces of CTA c where the units' stream (prefix sums of weights w per unit, `total` in all) fits Int.
+template <typename Int>
+__device__ __forceinline__ void emit_pieces(const Kv4Params& p, const PlanShared& sh, int c, Int total, bool pieces) {
+    const int n_cta = p.split.n_cta, per_seq = p.split.per_seq;
+    const Int R = pieces ? 1 : max((Int)p.split.min_blocks, (total + n_cta - 1) / n_cta);
+    Int pos = c * R;
+    const Int end = min(total, pos + R);
+    int made = 0, more = 0;
+    while (pos < end) {
+        int lo = 0, hi = p.B - 1;
+        while (lo < hi) {  // the last sequence that starts at or before pos
+            const int mid = (lo + hi + 1) >> 1;
+            if ((Int)sh.prefix[mid] * per_seq <= pos) lo = mid;
+            else hi = mid - 1;
+        }
+        const int b = lo, w = sh.prefix[b + 1] - sh.prefix[b], L = sh.ctx[b], n = sh.fresh[b];
+        const Int seq_base = (Int)sh.prefix[b] * per_seq;
+        int r = (int)((pos - seq_base) / w), first;
+        const int nb = seen_blocks(p, L, n, first);
+        if (pieces) {
+            const int k = (int)(pos - seq_base) - r * w, each = nb / w, rest = nb - each * w;
+            put_piece(p.plan + c, b, r, L, n, first + k * each + k * rest / w, first + (k + 1) * each + (k + 1) * rest / w,
+                      w, c, c - k, 1);
+            made = 1;
+            break;
+        }
+        // pieces after the first lie from n_cta + their unit's number on: a unit that is not a CTA's
+        // first begins inside that CTA's range, so no other CTA's range begins it
+        for (; r < per_seq && pos < end; ++r) {
+            const Int u_start = seq_base + (Int)r * w, u_end = u_start + nb;
+            if (pos >= u_end) {  // in the unit's gap
+                pos = u_start + w;
+                continue;
+            }
+            const Int c0 = u_start / R, c1 = (u_end - 1) / R, stop = min(end, u_end);
+            const int place = made == 0 ? c : n_cta + b * per_seq + r;
+            if (made == 1) more = place;
+            // CTA c's slot is 2 c for the piece its range begins with, 2 c + 1 for one that begins later
+            put_piece(p.plan + place, b, r, L, n, first + (int)(pos - u_start), first + (int)(stop - u_start),
+                      (int)(c1 - c0) + 1, 2 * c + (pos == c * R ? 0 : 1), 2 * (int)c0 + (u_start != c0 * R ? 1 : 0), 2);
+            ++made;
+            pos = stop < end ? u_start + w : end;
+        }
+    }
+    *reinterpret_cast<int2*>(&p.plan[c].count) = make_int2(made, more);
+}
 
 __device__ __noinline__ void plan_attention(const Kv4Params& p, PlanShared& sh, int block) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -129,7 +186,7 @@ __device__ __noinline__ void plan_attention(const Kv4Params& p, PlanShared& sh, 
         for (int w = 0; w < kPrepWarps; ++w) v += sh.sums[row][w];
         return v;
     };
-    int blocks = 0, seqs = 0, first;
+    int blocks = 0, seqs = 0, longest = 0, first;
     for (int b = tid; b < p.B; b += kPrepThreads) {
         int L, n;
         if (!kv4_lens(p, b, L, n)) n = 0;
@@ -138,37 +195,47 @@ __device__ __noinline__ void plan_attention(const Kv4Params& p, PlanShared& sh, 
         const int nb = seen_blocks(p, L, n, first);
         blocks += nb;
         seqs += nb > 0;
+        longest = max(longest, nb);
     }
+    longest = __reduce_max_sync(0xffffffffu, longest);
     blocks = __reduce_add_sync(0xffffffffu, blocks);
     seqs = __reduce_add_sync(0xffffffffu, seqs);
     if (lane == 0) {
-        sh.sums[8][warp] = blocks;
-        sh.sums[9][warp] = seqs;
+        sh.sums[3][warp] = blocks;
+        sh.sums[4][warp] = seqs;
+        sh.sums[5][warp] = longest;
     }
     __syncthreads();
-    const float total_f = (float)all_warps(8) * (float)per_seq, units_f = (float)all_warps(9) * (float)per_seq;
+    const float total_f = (float)all_warps(3) * (float)per_seq, units_f = (float)all_warps(4) * (float)per_seq;
     bool pieces = false;
     float inv_p = 0.f;
     if (units_f <= 0.875f * (float)n_cta) {
-        const float most = total_f / ((float)n_cta - units_f) + 1.f;
-        auto size = [&](int k) { return fmaxf((float)p.split.min_blocks, most * (1.f - (float)k / 16.f)); };
-        int count[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        const float most = __fdividef(total_f, (float)n_cta - units_f) + 1.f, least = (float)p.split.min_blocks;
+        const float size[3] = {fmaxf(least, most), fmaxf(least, most * 0.875f), fmaxf(least, most * 0.8125f)};
+        const float inv[3] = {__fdividef(1.f, size[0]), __fdividef(1.f, size[1]), __fdividef(1.f, size[2])};
+        int count[3] = {0, 0, 0};
         for (int b = tid; b < p.B; b += kPrepThreads) {
             const int nb = seen_blocks(p, sh.ctx[b], sh.fresh[b], first);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) count[k] += nb ? cuts_of(nb, 1.f / size(k)) : 0;
+            for (int k = 0; k < 3; ++k) count[k] += nb ? cuts_of(nb, inv[k]) : 0;
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < 3; ++k) {
             count[k] = __reduce_add_sync(0xffffffffu, count[k]);
             if (lane == 0) sh.sums[k][warp] = count[k];
         }
         __syncthreads();
+        longest = 0;
+#pragma unroll
+        for (int w = 0; w < kPrepWarps; ++w) longest = max(longest, sh.sums[5][w]);
         float best = 0.f;
-        for (int k = 0; k < 8; ++k)
-            if ((long long)all_warps(k) * per_seq <= n_cta) best = size(k);
-        pieces = best > 0.f && best <= total_f / (float)n_cta + (float)gap;
-        if (pieces) inv_p = 1.f / best;
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+            if ((float)all_warps(k) * (float)per_seq <= (float)n_cta) {
+                best = fminf(size[k], (float)longest);
+                inv_p = inv[k];
+            }
+        pieces = best > 0.f && best * (float)n_cta <= total_f + (float)(gap * n_cta);
     }
     // prefix sums, kPrepThreads sequences at a time
     auto weight = [&](int b) {
@@ -194,74 +261,11 @@ __device__ __noinline__ void plan_attention(const Kv4Params& p, PlanShared& sh, 
     }
     if (tid == 0) sh.prefix[p.B] = before;
     __syncthreads();
-
     const int c = block * kPrepThreads + tid;
     if (c >= n_cta) return;
     const long long total = (long long)before * per_seq;
-    const bool small = total + n_cta <= (long long)INT32_MAX;  // 32-bit divisions
-    auto quotient = [&](long long a, long long d) { return small ? (long long)((int)a / (int)d) : a / d; };
-    const long long R = pieces ? 1 : max((long long)p.split.min_blocks, quotient(total + n_cta - 1, n_cta));
-    long long pos = c * R;
-    const long long end = min(total, pos + R);
-    int made = 0, more = 0;
-    Kv4Piece first_piece{};
-    while (pos < end) {
-        int lo = 0, hi = p.B - 1;
-        while (lo < hi) {  // the last sequence that starts at or before pos
-            const int mid = (lo + hi + 1) >> 1;
-            if ((long long)sh.prefix[mid] * per_seq <= pos) lo = mid;
-            else hi = mid - 1;
-        }
-        const int b = lo, w = sh.prefix[b + 1] - sh.prefix[b];
-        const long long seq_base = (long long)sh.prefix[b] * per_seq;
-        int r = (int)quotient(pos - seq_base, w);
-        const int nb = seen_blocks(p, sh.ctx[b], sh.fresh[b], first);
-        // pieces after the first lie from n_cta + their unit's number on: a unit that is not a CTA's
-        // first begins inside that CTA's range, so no other CTA's range begins it
-        for (; r < per_seq && pos < end; ++r) {
-            const long long u_start = seq_base + (long long)r * w;
-            Kv4Piece piece{};
-            piece.b = b;
-            piece.r = r;
-            piece.L = sh.ctx[b];
-            piece.n = sh.fresh[b];
-            if (pieces) {
-                const int k = (int)(pos - u_start), each = nb / w, rest = nb - each * w;
-                piece.blk0 = first + k * each + k * rest / w;
-                piece.blk1 = first + (k + 1) * each + (k + 1) * rest / w;
-                piece.n_split = w;
-                piece.my_part = c;
-                piece.part0 = c - k;
-                piece.part_step = 1;
-                pos = end;
-            } else {
-                const long long u_end = u_start + nb;
-                if (pos >= u_end) {  // in the unit's gap
-                    pos = u_start + w;
-                    continue;
-                }
-                const long long c0 = quotient(u_start, R), c1 = quotient(u_end - 1, R), stop = min(end, u_end);
-                piece.blk0 = first + (int)(pos - u_start);
-                piece.blk1 = first + (int)(stop - u_start);
-                piece.n_split = (int)(c1 - c0) + 1;
-                // CTA c's slot is 2 c for the piece its range begins with, 2 c + 1 for one that begins later
-                piece.my_part = 2 * c + (pos == c * R ? 0 : 1);
-                piece.part0 = 2 * (int)c0 + (u_start != c0 * R ? 1 : 0);
-                piece.part_step = 2;
-                pos = stop < end ? u_start + w : end;
-            }
-            if (made == 0) {
-                first_piece = piece;
-            } else {
-                if (made == 1) more = n_cta + b * per_seq + r;
-                p.plan[n_cta + b * per_seq + r] = piece;
-            }
-            ++made;
-        }
-    }
-    first_piece.count = made;
-    first_piece.more = more;
-    p.plan[c] = first_piece;
+    if (total + n_cta <= (long long)INT32_MAX) emit_pieces<int>(p, sh, c, (int)total, pieces);
+    else emit_pieces<long long>(p, sh, c, total, pieces);
 }
 
 // Rows of a token: Hq queries (where p.q), Hkv keys and Hkv values (where `append`); after the

@@ -65,7 +65,7 @@ struct Cfg {
     // CTAs per SM, the registers' bound
     static constexpr int kCtas = D <= 64 ? (kTiles == 1 ? 4 : 3) : (D <= 128 ? (kTiles == 1 ? 3 : 2) : (kTiles == 1 ? 3 : 2));
     // fixed cost of a piece in blocks of streaming time, charged to every unit by the split
-    static constexpr int kGapBlocks = D <= 64 ? 26 : (D <= 96 ? 22 : (D <= 128 ? 18 : 12));
+    static constexpr int kGapBlocks = D <= 64 ? 26 : (D <= 96 ? 22 : (D <= 128 ? 20 : 16));
     static constexpr int kMinBlocks = 8;  // smallest piece
     // q's operand words in shared memory where the accumulators leave no registers for them
     static constexpr bool kQShared = D * kTiles >= 256;
