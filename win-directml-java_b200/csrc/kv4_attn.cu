@@ -62,13 +62,19 @@ struct Cfg {
     static constexpr int kSub = D <= 96 ? 2 : 1;  // blocks per ring stage
     static constexpr int kStages = D <= 96 ? 3 : (D <= 128 ? 4 : 3);
     static constexpr int kStageBytes = kSub * kBlockBytes;
+    // Side by side in the loop: the scores of one stage and the second product of the one before.  It
+    // takes the registers of a third CTA per SM.  Where a launch is short, one warp's own speed counts:
+    // head dim 256 decode over a 512-key window 30.9 -> 26.8 us, 5-token drafts 20.6 -> 19.3 us; long
+    // contexts lose what the third CTA hid (head dim 256, 17 k keys: 275 -> 299 us), and at head dim
+    // 64 with two-word operands the third CTA is worth more throughout (31 against 34 us).
+    static constexpr bool kPipelined = D == 256 || (kSplit == 0 && kTiles == 2);
     // CTAs per SM, the registers' bound
-    static constexpr int kCtas = D <= 64 ? (kTiles == 1 ? 4 : 3) : (D <= 128 ? (kTiles == 1 ? 3 : 2) : (kTiles == 1 ? 3 : 2));
+    static constexpr int kCtas = kPipelined ? 2 : (D <= 64 ? (kTiles == 1 ? 4 : 3) : (kTiles == 1 ? 3 : 2));
     // fixed cost of a piece in blocks of streaming time, charged to every unit by the split
     static constexpr int kGapBlocks = D <= 64 ? 26 : (D <= 96 ? 22 : (D <= 128 ? 20 : 16));
     static constexpr int kMinBlocks = 8;  // smallest piece
     // q's operand words in shared memory where the accumulators leave no registers for them
-    static constexpr bool kQShared = D * kTiles >= 256;
+    static constexpr bool kQShared = D * kTiles > 256;
     // head dim 256: the value params are regrouped in shared memory (their rows lie 128 bytes
     // apart, so that reading pairs of keys directly would meet in the same banks)
     static constexpr bool kRegroup = D >= 256;
@@ -329,24 +335,16 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
         __half2 s_bound = __float2half2_rn(1.f);
 
         const Zero zero;
-        // one stage; `odd`: its blocks are the complemented ones (with two blocks a stage, the second is)
-        auto step = [&](int i, auto odd) {
-            if (!wait_bounded(bars + slot * 8, phase)) {
-                // report, wait for the others in flight and ask for no more; the outputs are NaN
-                if (lane == 0) atomicOr(p.status, 8);
-                dead = true;
-                for (int k = 1; k < kStages && i + k < my_n; ++k) {
-                    const bool wrap = slot + k >= kStages;
-                    if (!wait_bounded(bars + (wrap ? slot + k - kStages : slot + k) * 8, phase ^ (wrap ? 1u : 0u))) break;
-                }
-                return;
-            }
-            const unsigned char* const stage = ring + slot * C::kStageBytes;
-            const int key0 = (blk0 + (warp + kWarps * i) * kSub) * kKv4Block;
-            const bool whole = key0 + kSub * kKv4Block - 1 <= all_hi && key0 >= all_lo;
+        // What a stage carries from its softmax to its second product.
+        // sv[u][h][y]: scales of keys 2t + 8h and 2t + 8h + 1, group y
+        // zv, gv: minima and scales of these keys in group g, the A operands of their sums
+        // ph, pl: P of keys 0..7 and 8..15 of the block as B operands (lo words where kept)
+        [[maybe_unused]] uint32_t sv[kSub][2][C::kRegroup ? 1 : kGroups];
+        uint32_t zv[kSub][2], gv[kSub][2], ph[kSub][kSTiles][2];
+        [[maybe_unused]] uint32_t pl[kSub][kSplit ? kSTiles : 1][2];
+        float x[kSub][kSTiles][4];  // scores, then their distance from the reference
 
-            // ---------------------------------------------------- scores against the reference
-            float x[kSub][kSTiles][4];
+        auto scores = [&](const unsigned char* stage) {
 #pragma unroll
             for (int u = 0; u < kSub; ++u) {
                 const unsigned char* const base = stage + u * C::kBlockBytes;
@@ -390,6 +388,11 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                     }
                 }
             }
+        };
+
+        auto softmax = [&](const unsigned char* stage, int i) {
+            const int key0 = (blk0 + (warp + kWarps * i) * kSub) * kKv4Block;
+            const bool whole = key0 + kSub * kKv4Block - 1 <= all_hi && key0 >= all_lo;
             float over = -INFINITY;
 #pragma unroll
             for (int u = 0; u < kSub; ++u) {
@@ -418,9 +421,6 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
             }
 
             // ---------------------------------------------------- value params
-            // sv[u][h][y]: scales of keys 2t + 8h and 2t + 8h + 1, group y
-            // zv, gv: minima and scales of these keys in group g, the A operands of their sums
-            uint32_t sv[kSub][2][C::kRegroup ? 1 : kGroups], zv[kSub][2], gv[kSub][2];
             __half2 s_top = __float2half2_rn(0.f);
             auto regroup = [&](int u, bool clean) {  // head dim 256: pairs of keys side by side, in shared memory
                 uint32_t w[4];  // key (lane >> 2) + 8 ((lane >> 1) & 1), groups 4 (lane & 1) + 0 .. 3
@@ -595,32 +595,36 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                 fresh = __any_sync(0xffffffffu, unset);
             }
 
-            // ---------------------------------------------------- P, and the second product
-            auto second_product = [&](auto block, auto complemented) {
-                constexpr int u = decltype(block)::value;
-                constexpr bool flip = decltype(complemented)::value;
-                // B operands: P of keys 0..7 and 8..15 of the block (hi words; lo words where kept)
-                uint32_t ph[kSTiles][2], pl[kSplit ? kSTiles : 1][2];
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) {
 #pragma unroll
                 for (int j = 0; j < kSTiles; ++j) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const float p0 = fast_exp2(x[u][j][2 * h]), p1 = fast_exp2(x[u][j][2 * h + 1]);
                         const __half2 hi = __floats2half2_rn(p0, p1);
-                        ph[j][h] = transpose8(u32(hi));
+                        ph[u][j][h] = transpose8(u32(hi));
                         if constexpr (kSplit != 0)
-                            pl[j][h] = transpose8(pack_half2(p0 - __low2float(hi), p1 - __high2float(hi)));
+                            pl[u][j][h] = transpose8(pack_half2(p0 - __low2float(hi), p1 - __high2float(hi)));
                     }
                 }
+            }
+        };
+
+        // acc += [codes] [P s], zl, ps: block u of the stage, complemented or not
+        auto second_product = [&](const unsigned char* stage, auto block, auto complemented) {
+            constexpr int u = decltype(block)::value;
+            constexpr bool flip = decltype(complemented)::value;
+            constexpr uint32_t flip_sign = flip ? 0x80008000u : 0u;
                 // zl += [z^T; 1] P, and for a complemented block ps += s^T P
                 uint32_t pz[kTiles][2];
 #pragma unroll
                 for (int j = 0; j < kTiles; ++j)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        if constexpr (kSplit == 0) pz[j][h] = ph[j][h];
-                        else if constexpr (kSplit == 1) pz[j][h] = g >= 4 ? pl[0][h] : ph[0][h];
-                        else pz[j][h] = j ? pl[0][h] : ph[0][h];
+                        if constexpr (kSplit == 0) pz[j][h] = ph[u][j][h];
+                        else if constexpr (kSplit == 1) pz[j][h] = g >= 4 ? pl[u][0][h] : ph[u][0][h];
+                        else pz[j][h] = j ? pl[u][0][h] : ph[u][0][h];
                     }
 #pragma unroll
                 for (int j = 0; j < kTiles; ++j) {
@@ -637,18 +641,17 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                         ps[j][1] += c[1];
                     }
                 }
-                constexpr uint32_t flip_sign = flip ? 0x80008000u : 0u;
-                uint32_t pa[2], pb[2];  // kSplit 1: the lo columns' words (the first negated), zero in the others
+                [[maybe_unused]] uint32_t pa[2], pb[2];  // kSplit 1: the lo columns' words (the first negated), zero in the others
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
 #pragma unroll
                     for (int j = 0; j < kSTiles; ++j) {
-                        ph[j][h] ^= flip_sign;
-                        if constexpr (kSplit != 0) pl[j][h] ^= flip_sign;
+                        ph[u][j][h] ^= flip_sign;
+                        if constexpr (kSplit != 0) pl[u][j][h] ^= flip_sign;
                     }
                     if constexpr (kSplit == 1) {
-                        pa[h] = g >= 4 ? ph[0][h] ^ 0x80008000u : 0u;
-                        pb[h] = g >= 4 ? pl[0][h] : 0u;
+                        pa[h] = g >= 4 ? ph[u][0][h] ^ 0x80008000u : 0u;
+                        pb[h] = g >= 4 ? pl[u][0][h] : 0u;
                     }
                 }
 #pragma unroll
@@ -675,14 +678,14 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                         const __half2 sc = h2(s[h]);
                         if constexpr (kSplit == 0) {
 #pragma unroll
-                            for (int j = 0; j < kTiles; ++j) bf[j][h] = u32(__hmul2(h2(ph[j][h]), sc));
+                            for (int j = 0; j < kTiles; ++j) bf[j][h] = u32(__hmul2(h2(ph[u][j][h]), sc));
                         } else if constexpr (kSplit == 1) {
                             const __half2 hi = __hmul2(h2(pa[h]), sc);  // lo columns: minus what the hi column holds
-                            bf[0][h] = u32(__hfma2(h2(pb[h]), sc, __hfma2(h2(ph[0][h]), sc, hi)));
+                            bf[0][h] = u32(__hfma2(h2(pb[h]), sc, __hfma2(h2(ph[u][0][h]), sc, hi)));
                         } else {
-                            const __half2 hi = __hmul2(h2(ph[0][h]), sc);
+                            const __half2 hi = __hmul2(h2(ph[u][0][h]), sc);
                             bf[0][h] = u32(hi);
-                            bf[1][h] = u32(__hfma2(h2(pl[0][h]), sc, __hfma2(h2(ph[0][h]), sc, __hneg2(hi))));
+                            bf[1][h] = u32(__hfma2(h2(pl[u][0][h]), sc, __hfma2(h2(ph[u][0][h]), sc, __hneg2(hi))));
                         }
                     }
 #pragma unroll
@@ -691,20 +694,62 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                         mma_add(acc[j][2 * y + 1], cv, bf[j][0], bf[j][1]);
                     }
                 }
-            };
+        };
+        auto second_products = [&](const unsigned char* stage, auto odd) {
             if constexpr (kSub == 2) {
-                second_product(std::integral_constant<int, 0>{}, std::false_type{});
-                second_product(std::integral_constant<int, 1>{}, std::true_type{});
+                second_product(stage, std::integral_constant<int, 0>{}, std::false_type{});
+                second_product(stage, std::integral_constant<int, 1>{}, std::true_type{});
             } else {
-                second_product(std::integral_constant<int, 0>{}, odd);
-            }
-            __syncwarp();  // every lane has read the stage
-            if (i + kStages < my_n) issue(i + kStages, slot);
-            if (++slot == kStages) {
-                slot = 0;
-                phase ^= 1;
+                second_product(stage, std::integral_constant<int, 0>{}, odd);
             }
         };
+
+        auto arrived = [&](int at, uint32_t parity, int i) {  // stage i, in ring slot `at`
+            if (wait_bounded(bars + at * 8, parity)) return true;
+            // report, wait for the others in flight and ask for no more; the outputs are NaN
+            if (lane == 0) atomicOr(p.status, 8);
+            dead = true;
+            for (int k = 1; k < kStages && i + k < my_n; ++k) {
+                const bool wrap = at + k >= kStages;
+                if (!wait_bounded(bars + (wrap ? at + k - kStages : at + k) * 8, parity ^ (wrap ? 1u : 0u))) break;
+            }
+            return false;
+        };
+        auto release = [&](int i, int at, uint32_t parity) {  // stage i is used; go on to ring slot `at`
+            __syncwarp();  // every lane has read the stage
+            if (!dead && i + kStages < my_n) issue(i + kStages, slot);
+            slot = at;
+            phase = parity;
+        };
+        auto step = [&](int i, auto odd) {
+            const unsigned char* const stage = ring + slot * C::kStageBytes;
+            const int at = slot + 1 == kStages ? 0 : slot + 1;
+            const uint32_t parity = at ? phase : phase ^ 1u;
+            if constexpr (C::kPipelined) {  // stage i, whose P is known, with the scores of stage i + 1
+                const unsigned char* const after = ring + at * C::kStageBytes;
+                const bool more = i + 1 < my_n;
+                if (more && arrived(at, parity, i + 1)) {
+                    scores(after);
+                    second_products(stage, odd);
+                } else {
+                    second_products(stage, odd);
+                }
+                release(i, at, parity);
+                if (more && !dead) softmax(after, i + 1);
+            } else {
+                if (!arrived(slot, phase, i)) return;
+                scores(stage);
+                softmax(stage, i);
+                second_products(stage, odd);
+                release(i, at, parity);
+            }
+        };
+        if constexpr (C::kPipelined) {
+            if (my_n > 0 && !dead && arrived(slot, phase, 0)) {
+                scores(ring + slot * C::kStageBytes);
+                softmax(ring + slot * C::kStageBytes, 0);
+            }
+        }
         if constexpr (kSub == 2) {
             for (int i = 0; i < my_n && !dead; ++i) step(i, std::false_type{});
         } else {
