@@ -65,9 +65,11 @@ struct b2a_context {
     void* kv4_ws = nullptr;
     size_t kv4_ws_bytes = 0;
     size_t kv4_counter_bytes = 0;
-    // paged cache: the page operations' lists
+    int kv4_epoch = 0;  // 4-bit cache chunks so far
+    // paged cache: [words between blocks][the page operations' lists]
     void* pg_ws = nullptr;
     size_t pg_ws_bytes = 0;
+    size_t pg_sync_bytes = 0;
     // b2a_set_decode_early_start: tensor-core decodes launched with programmatic serialisation
     bool decode_early_start = false;
     // test hook (b2a_test_last_attention_kernel): the kernel the last whole-sequence
@@ -1266,12 +1268,12 @@ int run_kv4_chunk(b2a_context* ctx, const Kv4Params& p, cudaStream_t stream) {
     const size_t kv_seq = (size_t)Sk * p.Hkv * p.D * 2, q_seq = (size_t)p.T * p.Hq * p.D * 2;
     const int per = (int)std::max<size_t>(1, std::min<size_t>(p.B, kKv4StageBytes / (2 * kv_seq + q_seq)));
     const size_t kv_bytes = r256(kv_seq * per), q_bytes = r256(q_seq * per);
-    if (ensure_buffer(ctx, &ctx->pf_ws, &ctx->pf_ws_bytes, 256 + 2 * kv_bytes + q_bytes, "4-bit cache chunk") != B2A_OK) {
+    if (ensure_buffer(ctx, &ctx->pf_ws, &ctx->pf_ws_bytes, 2 * kv_bytes + q_bytes, "4-bit cache chunk") != B2A_OK) {
         ctx->last_error.clear();  // the refused workspace is not an error of this call
         return kNoRoom;
     }
     char* base = static_cast<char*>(ctx->pf_ws);
-    int* nan_flag = reinterpret_cast<int*>(base);
+    int* nan_flag = ctx->status + kStatusNanWord;
     AttnParams a{};
     a.in_dtype = B2A_FLOAT16;
     a.out_dtype = p.act_dtype;
@@ -1289,9 +1291,9 @@ int run_kv4_chunk(b2a_context* ctx, const Kv4Params& p, cudaStream_t stream) {
     a.causal = 1;
     a.window = p.window;
     a.scale = p.scale;
-    a.q = base + 256;
-    a.k = base + 256 + q_bytes;
-    a.v = base + 256 + q_bytes + kv_bytes;
+    a.q = base;
+    a.k = base + q_bytes;
+    a.v = base + q_bytes + kv_bytes;
     a.B = per;
     a.q_pos = p.ctx_lens;
     a.o = p.o;
@@ -1308,10 +1310,14 @@ int run_kv4_chunk(b2a_context* ctx, const Kv4Params& p, cudaStream_t stream) {
         a.q_pos = s.ctx_lens;
         a.q_len = s.new_lens;
         a.o = s.o;
-        e = cudaMemsetAsync(nan_flag, 0, sizeof(int), stream);
+        if (ctx->kv4_epoch == INT32_MAX) {  // start over
+            ctx->kv4_epoch = 0;
+            e = cudaMemsetAsync(nan_flag, 0, sizeof(int), stream);
+        }
+        s.epoch = ++ctx->kv4_epoch;
         if (e == cudaSuccess)
-            e = launch_kv4_stage(s, base + 256, const_cast<void*>(a.k), const_cast<void*>(a.v), Sk, nan_flag, ctx->sm_count,
-                                 stream);
+            e = launch_kv4_stage(s, base, const_cast<void*>(a.k), const_cast<void*>(a.v), Sk, nan_flag,
+                                 p.k_new != nullptr && b0 == 0, ctx->sm_count, stream);
         if (e == cudaSuccess) e = launch_attn_tcgen05(a, ctx->status, stream);
         if (e == cudaSuccess) e = launch_kv4_nan_rows(s, nan_flag, ctx->sm_count, stream);
     }
@@ -1390,10 +1396,13 @@ int check_pool(b2a_context* ctx, const b2a_page_pool* pool, bool with_pages, Pag
     return B2A_OK;
 }
 
-int pages_workspace(b2a_context* ctx, int num_pages, int** out) {
-    const int rc = ensure_buffer(ctx, &ctx->pg_ws, &ctx->pg_ws_bytes, pages_workspace_ints(num_pages) * sizeof(int),
-                                 "page operations");
-    *out = static_cast<int*>(ctx->pg_ws);
+int pages_workspace(b2a_context* ctx, int num_pages, cudaStream_t stream, int** sync, int** ws) {
+    size_t sync_bytes = 0;
+    const int rc = ensure_counted_buffer(ctx, &ctx->pg_ws, &ctx->pg_ws_bytes, &ctx->pg_sync_bytes, kPageSyncInts,
+                                         pages_workspace_ints(num_pages) * sizeof(int), "page operations", stream,
+                                         false, &sync_bytes);
+    *sync = static_cast<int*>(ctx->pg_ws);
+    *ws = reinterpret_cast<int*>(static_cast<char*>(ctx->pg_ws) + sync_bytes);
     return rc;
 }
 
@@ -1487,9 +1496,9 @@ B2A_API int b2a_pages_reserve(b2a_context* ctx, const b2a_page_pool* pool, const
     if (!ctx_lens || !new_lens || !counts) return fail(ctx, B2A_EINVAL, "ctx_lens, new_lens and counts must not be null");
     if (page_size <= 0) return fail(ctx, B2A_EINVAL, "page_size must be > 0");
     DeviceGuard guard(ctx->device);
-    int* ws = nullptr;
-    if ((rc = pages_workspace(ctx, p.num_pages, &ws))) return rc;
-    const cudaError_t e = launch_pages_reserve(p, ctx_lens, new_lens, page_size, counts, ws, ctx->sm_count,
+    int *sync = nullptr, *ws = nullptr;
+    if ((rc = pages_workspace(ctx, p.num_pages, static_cast<cudaStream_t>(stream), &sync, &ws))) return rc;
+    const cudaError_t e = launch_pages_reserve(p, ctx_lens, new_lens, page_size, counts, sync, ws, ctx->sm_count,
                                                static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_fail(ctx, e, "page reserve launch");
     return B2A_OK;
@@ -1502,9 +1511,9 @@ B2A_API int b2a_pages_compact(b2a_context* ctx, const b2a_page_pool* pool, int32
     if (rc) return rc;
     if (!counts) return fail(ctx, B2A_EINVAL, "counts must not be null");
     DeviceGuard guard(ctx->device);
-    int* ws = nullptr;
-    if ((rc = pages_workspace(ctx, p.num_pages, &ws))) return rc;
-    const cudaError_t e = launch_pages_compact(p, counts, ws, ctx->sm_count, static_cast<cudaStream_t>(stream));
+    int *sync = nullptr, *ws = nullptr;
+    if ((rc = pages_workspace(ctx, p.num_pages, static_cast<cudaStream_t>(stream), &sync, &ws))) return rc;
+    const cudaError_t e = launch_pages_compact(p, counts, sync, ws, ctx->sm_count, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_fail(ctx, e, "page compact launch");
     return B2A_OK;
 }

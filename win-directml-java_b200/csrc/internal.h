@@ -133,10 +133,12 @@ cudaError_t launch_attn_f32(const AttnParams& p, cudaStream_t stream);
 // per-launch abort word (a CTA whose bounded wait ran out sets it so that the launch's other
 // CTAs stop too).  All three are zero between launches: the last CTA of each launch resets
 // them, so one timed-out launch does not abort the next ones (the sticky report stays in
-// the error flags until they are read).
+// the error flags until they are read).  Word kStatusNanWord holds the number of the last 4-bit cache
+// chunk whose keys included a value held as NaN.
 constexpr int kStatusWords = 4;
 constexpr int kStatusSchedWord = 4;
 constexpr int kStatusAbortWord = 6;
+constexpr int kStatusNanWord = 7;
 constexpr int kStatusBufferInts = 8;
 
 // tcgen05 / TMEM / TMA kernel (fp16 operands, head_dim 64, 96, 128); status bit 3 = bounded wait ran out.
@@ -268,6 +270,7 @@ struct Kv4Params {
     float* partials;
     Kv4Piece* plan;   // [n_cta] each attention CTA's first piece, then by unit the others
     Kv4Split split;
+    int epoch;        // chunks: this call's number
     double inv_freq[kMaxHeadDim / 2];
 };
 constexpr int kMaxPageSize = 1024;
@@ -283,10 +286,12 @@ cudaError_t launch_kv4_attn(const Kv4Params& p, int device, cudaStream_t stream)
 
 // Chunks of prompts over the cache on the tcgen05 kernel (kv4_stage.cu): q rotated to fp16 at q_out
 // [B][T][Hq][D], positions [0, round128(ctx + new)) of the cache as fp16 rows at k_out / v_out
-// [B][Sk][Hkv][D] (what no query sees is zero); nan_flag is set to 1 where a visible value group is
-// held as NaN (it becomes zero; launch_kv4_nan_rows then marks the rows that see it).
+// [B][Sk][Hkv][D] (what no query sees is zero); nan_flag takes the value p.epoch, which grows from call
+// to call, where a visible value group is held as NaN (it becomes zero; launch_kv4_nan_rows then marks
+// the rows that see it).  after_append: the kernel just before on the stream is this call's append,
+// which needs none of what this one writes; the queries' part then runs beside it.
 cudaError_t launch_kv4_stage(const Kv4Params& p, void* q_out, void* k_out, void* v_out, int Sk, int* nan_flag,
-                             int sm_count, cudaStream_t stream);
+                             bool after_append, int sm_count, cudaStream_t stream);
 cudaError_t launch_kv4_nan_rows(const Kv4Params& p, const int* nan_flag, int sm_count, cudaStream_t stream);
 
 // The page table, reference counts and pages of a paged cache (pages.cu).
@@ -301,13 +306,16 @@ struct PagePoolParams {
     int* status;      // bits 0 (lengths), 4 (page table entry), 6 (parents entry)
 };
 constexpr int kMaxForkRows = 56 * 1024;  // rows of one table column in shared memory
+// sync: kPageSyncInts ints, zero between launches; ws: pages_workspace_ints(num_pages) ints.
+constexpr int kPageSyncInts = 2;
 size_t pages_workspace_ints(int num_pages);
 cudaError_t launch_pages_free(const PagePoolParams& p, const int* keep_from, const int* keep_to, int page_size,
                               cudaStream_t stream);
 cudaError_t launch_pages_fork(const PagePoolParams& p, const int* parents, cudaStream_t stream);
 cudaError_t launch_pages_reserve(const PagePoolParams& p, const int* ctx_lens, const int* new_lens, int page_size,
-                                 int* counts, int* ws, int sm_count, cudaStream_t stream);
-cudaError_t launch_pages_compact(const PagePoolParams& p, int* counts, int* ws, int sm_count, cudaStream_t stream);
+                                 int* counts, int* sync, int* ws, int sm_count, cudaStream_t stream);
+cudaError_t launch_pages_compact(const PagePoolParams& p, int* counts, int* sync, int* ws, int sm_count,
+                                 cudaStream_t stream);
 
 // Sets the message b2a_last_error(NULL, ...) returns on this thread.
 void set_thread_error(const char* msg);

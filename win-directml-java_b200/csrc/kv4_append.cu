@@ -409,6 +409,7 @@ __global__ void __launch_bounds__(StoreGeo<D>::kMaxThreads, StoreGeo<D>::kCtas)
     kv4_store_kernel(const __grid_constant__ Kv4Params p, int blocks, int chunks, int per) {
     using Gm = StoreGeo<D>;
     constexpr int kChunks = Gm::kChunks, kGroups = D / 32;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // a chunk's query staging may run beside this
     extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, groups = blockDim.x / Gm::kPerHead;
     const int group = tid / Gm::kPerHead, in_group = tid - group * Gm::kPerHead;

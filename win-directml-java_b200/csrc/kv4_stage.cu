@@ -150,7 +150,8 @@ __device__ __forceinline__ void stage_group(const Kv4Params& p, const uint8_t* s
                                   *reinterpret_cast<const __half2*>(&s2), *reinterpret_cast<const __half2*>(&z2));
         return *reinterpret_cast<const uint32_t*>(&x);
     };
-    bool big = false, nan = false;
+    bool nan = false;
+    __half2 top = __float2half2_rn(0.f);  // largest |value|: infinite where one left the fp16 range
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         const bool row_seen = seen(g + 8 * r);
@@ -173,14 +174,15 @@ __device__ __forceinline__ void stage_group(const Kv4Params& p, const uint8_t* s
                 uint32_t k = value(code[0][x] >> (8 * r + 4 * j), ks, kz);
                 uint32_t v = movmatrix_trans(value(code[1][x] >> (8 * r + 4 * j), vs, vz));
                 if (!row_seen) k = v = 0;
-                big |= (k & 0x7fffu) == 0x7c00u || (k >> 16 & 0x7fffu) == 0x7c00u || (v & 0x7fffu) == 0x7c00u ||
-                       (v >> 16 & 0x7fffu) == 0x7c00u;
+                top = __hmax2(top, __hmax2(__habs2(*reinterpret_cast<const __half2*>(&k)),
+                                           __habs2(*reinterpret_cast<const __half2*>(&v))));
                 *reinterpret_cast<uint32_t*>(k_row0 + at + 16 * x + 8 * j) = k;
                 *reinterpret_cast<uint32_t*>(v_row0 + at + 16 * x + 8 * j) = v;
             }
     }
+    const bool big = __hisinf(__low2half(top)) || __hisinf(__high2half(top));
     if (__any_sync(0xffffffffu, big) && lane == 0) atomicOr(p.status, 4);
-    if (__any_sync(0xffffffffu, nan) && lane == 0) *nan_flag = 1;
+    if (__any_sync(0xffffffffu, nan) && lane == 0) atomicMax(nan_flag, p.epoch);
 }
 
 template <int D, typename T>
@@ -193,11 +195,13 @@ __global__ void __launch_bounds__(2 * D) kv4_stage_kernel(const __grid_constant_
         stage_query<D, T>(p, q_out, blockIdx.x, q_blocks, smem);
         return;
     }
+    // the append before this launch wrote the new rows' codes; the queries above did not need them
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int64_t row_stride = (int64_t)p.Hkv * D;
     constexpr int kGroups = D / 32, kWarps = 2 * D / 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int64_t i = (int64_t)(blockIdx.x - q_total) * kWarps + warp;
-    const int64_t step = (int64_t)(gridDim.x - q_total) * kWarps;
+    const int step = (gridDim.x - q_total) * kWarps;
     for (int b = 0; b < p.B; ++b) {
         int L, n;
         if (!kv4_lens(p, b, L, n) || n == 0) continue;
@@ -206,7 +210,9 @@ __global__ void __launch_bounds__(2 * D) kv4_stage_kernel(const __grid_constant_
         const int per_blk = p.Hkv * kGroups;
         const int64_t count = (int64_t)(blk1 - blk0) * per_blk;
         for (; i < count; i += step) {
-            const int blk = blk0 + (int)(i / per_blk), in = (int)(i % per_blk), h = in / kGroups, y = in % kGroups;
+            // below 2^31: a group is 2 KB of staged rows
+            const unsigned at_blk = (unsigned)i / (unsigned)per_blk, in = (unsigned)i - at_blk * per_blk;
+            const int blk = blk0 + (int)at_blk, h = in / kGroups, y = in % kGroups;
             const int pos = blk * kKv4Block;
             const bool seen = pos + kKv4Block > first && pos < end;
             const uint8_t* src = seen ? kv4_block_ptr(p, b, h, pos) : nullptr;
@@ -222,7 +228,7 @@ __global__ void __launch_bounds__(2 * D) kv4_stage_kernel(const __grid_constant_
 // (the group's channels; all of the row's).  Runs to its end only where the staging met one.
 __global__ void __launch_bounds__(256) kv4_nan_rows_kernel(const __grid_constant__ Kv4Params p, const int* nan_flag) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (*nan_flag == 0 && (*p.status & 16) == 0) return;
+    if (*nan_flag != p.epoch && (*p.status & 16) == 0) return;
     const int D = p.D, groups = D / 32;
     const int64_t rows = (int64_t)p.B * p.T * p.Hkv;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -255,7 +261,7 @@ __global__ void __launch_bounds__(256) kv4_nan_rows_kernel(const __grid_constant
 
 template <int D, typename T>
 cudaError_t launch_stage(const Kv4Params& p, __half* q_out, __half* k_out, __half* v_out, int Sk, int* nan_flag,
-                         int sm_count, cudaStream_t stream) {
+                         bool after_append, int sm_count, cudaStream_t stream) {
     const size_t smem = 16 * (D / 2) * sizeof(double2) + 2 * D * sizeof(double);
     auto kern = kv4_stage_kernel<D, T>;
     if (smem > 48 * 1024) {
@@ -263,19 +269,29 @@ cudaError_t launch_stage(const Kv4Params& p, __half* q_out, __half* k_out, __hal
         if (e != cudaSuccess) return e;
     }
     const int q_blocks = (p.T + 15) / 16, q_total = p.B * q_blocks * ((p.Hq + kStageHeads - 1) / kStageHeads);
-    kern<<<q_total + sm_count * 8, 2 * D, smem, stream>>>(p, q_out, k_out, v_out, Sk, nan_flag, q_blocks, q_total);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(q_total + sm_count * 8));
+    cfg.blockDim = dim3(2 * D);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    // beside an append that was launched just before: the queries' blocks come first
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = after_append ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kern, p, q_out, k_out, v_out, Sk, nan_flag, q_blocks, q_total);
 }
 
 }  // namespace
 
 cudaError_t launch_kv4_stage(const Kv4Params& p, void* q_out, void* k_out, void* v_out, int Sk, int* nan_flag,
-                             int sm_count, cudaStream_t stream) {
+                             bool after_append, int sm_count, cudaStream_t stream) {
     __half *q = static_cast<__half*>(q_out), *k = static_cast<__half*>(k_out), *v = static_cast<__half*>(v_out);
     auto go = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        return p.act_dtype == kF16 ? launch_stage<D, __half>(p, q, k, v, Sk, nan_flag, sm_count, stream)
-                                   : launch_stage<D, __nv_bfloat16>(p, q, k, v, Sk, nan_flag, sm_count, stream);
+        return p.act_dtype == kF16 ? launch_stage<D, __half>(p, q, k, v, Sk, nan_flag, after_append, sm_count, stream)
+                                   : launch_stage<D, __nv_bfloat16>(p, q, k, v, Sk, nan_flag, after_append, sm_count, stream);
     };
     switch (p.D) {
         case 64: return go(std::integral_constant<int, 64>{});

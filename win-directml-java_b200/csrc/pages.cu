@@ -5,6 +5,10 @@
 // table entries name a page; 0: free).  Every result is a function of the state at the call's start:
 // counts change by integer atomics (their order does not matter), and what depends on order -- which
 // free page goes to which slot, which page moves where -- comes from prefix sums, lowest first.
+//
+// Reserve and compact are one launch each (the host's cost of a launch is about that of their work):
+// block 0 plans, the others wait for it, then all copy pages.  Block 0 waits for nobody and is
+// dispatched first, so the wait ends; it is bounded all the same.
 #include "internal.h"
 
 namespace b2a {
@@ -37,6 +41,68 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums, int* total) {
     *total = warp_sums[(blockDim.x >> 5) - 1];
     __syncthreads();  // warp_sums may be written again
     return off + incl - v;
+}
+
+// Words of the workspace that are zero between launches.
+struct PlanSync {
+    int planned;  // block 0 is done
+    int left;     // blocks that are done
+};
+constexpr unsigned long long kPlanWaitNs = 1000000000ull;
+
+__device__ __forceinline__ unsigned long long now_ns() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+// After block 0's plan: its writes are visible to all threads of the block.  False (status bit 3) where
+// the plan did not come in time.
+__device__ __forceinline__ bool plan_ready(const PagePoolParams& p, PlanSync* sync) {
+    __shared__ int ok_s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int ok = 1;
+        if (blockIdx.x == 0) {
+            __threadfence();
+            atomicExch(&sync->planned, 1);
+        } else {
+            const unsigned long long t0 = now_ns();
+            while (*reinterpret_cast<volatile int*>(&sync->planned) == 0) {
+                if (now_ns() - t0 > kPlanWaitNs) {
+                    atomicOr(p.status, 8);
+                    ok = 0;
+                    break;
+                }
+                __nanosleep(100);
+            }
+            __threadfence();
+        }
+        ok_s = ok;
+    }
+    __syncthreads();
+    return ok_s != 0;
+}
+// The last block to leave restores the words for the next launch.
+__device__ __forceinline__ void leave(PlanSync* sync) {
+    __syncthreads();
+    if (threadIdx.x == 0 && atomicAdd(&sync->left, 1) == (int)gridDim.x - 1) {
+        atomicExch(&sync->left, 0);
+        atomicExch(&sync->planned, 0);
+    }
+}
+
+// Copies page src[i] to page dst[i] in every layer, i < n, where src[i] >= 0; all blocks, all threads.
+__device__ __forceinline__ void copy_pages(const PagePoolParams& p, const int* src, const int* dst, int n) {
+    const int64_t words = p.page_bytes / 16;
+    for (int64_t w = blockIdx.x; w < (int64_t)n * p.n_layers; w += gridDim.x) {
+        const int i = (int)(w / p.n_layers);
+        const int from = __ldcg(src + i);
+        if (from < 0) continue;
+        uint8_t* layer = p.pages + (w - (int64_t)i * p.n_layers) * p.layer_stride;
+        const uint4* a = reinterpret_cast<const uint4*>(layer + (int64_t)from * p.page_bytes);
+        uint4* b = reinterpret_cast<uint4*>(layer + (int64_t)__ldcg(dst + i) * p.page_bytes);
+        for (int64_t k = threadIdx.x; k < words; k += blockDim.x) b[k] = a[k];
+    }
 }
 
 __device__ __forceinline__ bool page_ok(const PagePoolParams& p, int page) {
@@ -96,13 +162,14 @@ struct Span {
 };
 __device__ __forceinline__ Span written_slots(const PagePoolParams& p, const int* ctx_lens, const int* new_lens,
                                               int row, int page_size) {
-    const int64_t ctx = ctx_lens[row], n = new_lens[row];
+    const int ctx = ctx_lens[row], n = new_lens[row];
     if (n <= 0) return Span{0, 0};
-    if (ctx < 0 || ctx + n > (int64_t)p.max_pages * page_size) {
+    if (ctx < 0 || (int64_t)ctx + n > (int64_t)p.max_pages * page_size) {
         atomicOr(p.status, 1);
         return Span{0, 0};
     }
-    return Span{(int)(ctx / page_size), (int)((ctx + n - 1) / page_size) + 1};
+    const unsigned size = page_size, last = (unsigned)ctx + (unsigned)n - 1;
+    return Span{(int)((unsigned)ctx / size), (int)(last / size) + 1};
 }
 // Whether a written slot needs a page: it has none, or one that other rows hold too.
 __device__ __forceinline__ bool wants_page(const PagePoolParams& p, int page) {
@@ -111,27 +178,50 @@ __device__ __forceinline__ bool wants_page(const PagePoolParams& p, int page) {
 
 // One block: who wants a page, the lowest free pages, who gets which.
 // list[i], src[i]: the i-th page given out and the page to copy into it (-1: none); job[0]: how many.
-__global__ void __launch_bounds__(kPlanThreads) pages_reserve_plan(const PagePoolParams p, const int* ctx_lens,
-                                                                   const int* new_lens, int page_size, int* list,
-                                                                   int* src, int* job, int* counts) {
+__device__ __forceinline__ void plan_reserve(const PagePoolParams& p, const int* ctx_lens, const int* new_lens,
+                                             int page_size, int* list, int* src, int* job, int* counts) {
     __shared__ int sums[32];
     const int tid = threadIdx.x;
     const int per = (p.n_seq + kPlanThreads - 1) / kPlanThreads;
     const int r0 = min(p.n_seq, tid * per), r1 = min(p.n_seq, r0 + per);
+    // four consecutive counts a thread; the first ones are requested before the rows are looked at
+    int refs[4];
+    auto fetch = [&](int base) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int page = base + 4 * tid + k;
+            refs[k] = page < p.num_pages ? p.ref_counts[page] : 1;
+        }
+    };
+    fetch(0);
+    // a thread's only row (the usual case) is kept for the assignment below: its span and which of its
+    // first 32 slots want a page
+    Span kept{0, 0};
+    unsigned kept_wants = 0;
     int mine = 0, need = 0;
     for (int row = r0; row < r1; ++row) {
         const Span s = written_slots(p, ctx_lens, new_lens, row, page_size);
-        for (int slot = s.s0; slot < s.s1; ++slot)
-            mine += wants_page(p, p.page_table[(int64_t)row * p.max_pages + slot]);
+        kept = s;
+        for (int slot = s.s0; slot < s.s1; ++slot) {
+            const bool wants = wants_page(p, p.page_table[(int64_t)row * p.max_pages + slot]);
+            mine += wants;
+            if (slot - s.s0 < 32) kept_wants |= (unsigned)wants << (slot - s.s0);
+        }
     }
     int at = block_scan(mine, sums, &need);
     int found = 0;
-    for (int base = 0; base < p.num_pages && found < need; base += kPlanThreads) {
-        const int page = base + tid;
-        const int is_free = page < p.num_pages && p.ref_counts[page] == 0;
-        int total;
-        const int rank = found + block_scan(is_free, sums, &total);
-        if (is_free && rank < need) list[rank] = page;
+    for (int base = 0; base < p.num_pages && found < need; base += 4 * kPlanThreads) {
+        if (base > 0) fetch(base);
+        int n_free = 0, total;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) n_free += refs[k] == 0;
+        int rank = found + block_scan(n_free, sums, &total);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (refs[k] == 0) {
+                if (rank < need) list[rank] = base + 4 * tid + k;
+                ++rank;
+            }
         found += total;
     }
     __syncthreads();
@@ -143,9 +233,10 @@ __global__ void __launch_bounds__(kPlanThreads) pages_reserve_plan(const PagePoo
         }
         return;
     }
-    for (int row = r0; row < r1; ++row) {
-        const Span s = written_slots(p, ctx_lens, new_lens, row, page_size);
+    for (int row = r0; row < r1 && mine > 0; ++row) {
+        const Span s = per == 1 ? kept : written_slots(p, ctx_lens, new_lens, row, page_size);
         for (int slot = s.s0; slot < s.s1; ++slot) {
+            if (per == 1 && slot - s.s0 < 32 && !(kept_wants >> (slot - s.s0) & 1)) continue;
             int* entry = p.page_table + (int64_t)row * p.max_pages + slot;
             const int old = *entry;
             if (!wants_page(p, old)) continue;
@@ -166,26 +257,18 @@ __global__ void __launch_bounds__(kPlanThreads) pages_reserve_plan(const PagePoo
     }
 }
 
-// Copies page src[i] to page dst[i] in every layer, i < job[0], where src[i] >= 0.
-__global__ void pages_copy_kernel(const PagePoolParams p, const int* src, const int* dst, const int* job) {
-    const int n = job[0];
-    const int64_t words = p.page_bytes / 16;
-    for (int64_t w = blockIdx.x; w < (int64_t)n * p.n_layers; w += gridDim.x) {
-        const int i = (int)(w / p.n_layers);
-        const int from = src[i];
-        if (from < 0) continue;
-        uint8_t* layer = p.pages + (w - (int64_t)i * p.n_layers) * p.layer_stride;
-        const uint4* a = reinterpret_cast<const uint4*>(layer + (int64_t)from * p.page_bytes);
-        uint4* b = reinterpret_cast<uint4*>(layer + (int64_t)dst[i] * p.page_bytes);
-        for (int64_t k = threadIdx.x; k < words; k += blockDim.x) b[k] = a[k];
-    }
+__global__ void __launch_bounds__(kPlanThreads) pages_reserve_kernel(const PagePoolParams p, const int* ctx_lens,
+                                                                     const int* new_lens, int page_size, int* list,
+                                                                     int* src, int* job, PlanSync* sync, int* counts) {
+    if (blockIdx.x == 0) plan_reserve(p, ctx_lens, new_lens, page_size, list, src, job, counts);
+    if (plan_ready(p, sync)) copy_pages(p, src, list, __ldcg(job));
+    leave(sync);
 }
 
 // -------------------------------------------------------------------- compact
 // One block: n live pages; live ones at n or above (src) go into the free places below n (dst), both
 // in order; to[page - n] is where a moved page went.
-__global__ void __launch_bounds__(kPlanThreads) pages_compact_plan(const PagePoolParams p, int* src, int* dst, int* to,
-                                                                   int* job, int* counts) {
+__device__ __forceinline__ void plan_compact(const PagePoolParams& p, int* src, int* dst, int* to, int* job, int* counts) {
     __shared__ int sums[32];
     const int tid = threadIdx.x;
     int mine = 0, n = 0;
@@ -218,13 +301,19 @@ __global__ void __launch_bounds__(kPlanThreads) pages_compact_plan(const PagePoo
     }
 }
 
-__global__ void pages_remap_kernel(const PagePoolParams p, const int* to, const int* job) {
-    const int n = job[1];
-    const int64_t total = (int64_t)p.n_seq * p.max_pages;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-        const int page = p.page_table[i];
-        if (page >= n && page_ok(p, page)) p.page_table[i] = to[page - n];
+__global__ void __launch_bounds__(kPlanThreads) pages_compact_kernel(const PagePoolParams p, int* src, int* dst, int* to,
+                                                                     int* job, PlanSync* sync, int* counts) {
+    if (blockIdx.x == 0) plan_compact(p, src, dst, to, job, counts);
+    if (plan_ready(p, sync)) {
+        copy_pages(p, src, dst, __ldcg(job));
+        const int n = __ldcg(job + 1);
+        const int64_t total = (int64_t)p.n_seq * p.max_pages;
+        for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+            const int page = p.page_table[i];
+            if (page >= n && page_ok(p, page)) p.page_table[i] = __ldcg(to + page - n);
+        }
     }
+    leave(sync);
 }
 
 }  // namespace
@@ -252,18 +341,18 @@ cudaError_t launch_pages_fork(const PagePoolParams& p, const int* parents, cudaS
 }
 
 cudaError_t launch_pages_reserve(const PagePoolParams& p, const int* ctx_lens, const int* new_lens, int page_size,
-                                 int* counts, int* ws, int sm_count, cudaStream_t stream) {
-    int *job = ws, *list = ws + 64, *src = list + p.num_pages;
-    pages_reserve_plan<<<1, kPlanThreads, 0, stream>>>(p, ctx_lens, new_lens, page_size, list, src, job, counts);
-    pages_copy_kernel<<<sm_count * 4, 256, 0, stream>>>(p, src, list, job);
+                                 int* counts, int* sync, int* ws, int sm_count, cudaStream_t stream) {
+    int *list = ws, *src = list + p.num_pages, *job = src + p.num_pages;
+    pages_reserve_kernel<<<sm_count, kPlanThreads, 0, stream>>>(p, ctx_lens, new_lens, page_size, list, src, job,
+                                                                reinterpret_cast<PlanSync*>(sync), counts);
     return cudaGetLastError();
 }
 
-cudaError_t launch_pages_compact(const PagePoolParams& p, int* counts, int* ws, int sm_count, cudaStream_t stream) {
-    int *job = ws, *src = ws + 64, *dst = src + p.num_pages, *to = dst + p.num_pages;
-    pages_compact_plan<<<1, kPlanThreads, 0, stream>>>(p, src, dst, to, job, counts);
-    pages_copy_kernel<<<sm_count * 4, 256, 0, stream>>>(p, src, dst, job);
-    pages_remap_kernel<<<sm_count * 2, 256, 0, stream>>>(p, to, job);
+cudaError_t launch_pages_compact(const PagePoolParams& p, int* counts, int* sync, int* ws, int sm_count,
+                                 cudaStream_t stream) {
+    int *src = ws, *dst = src + p.num_pages, *to = dst + p.num_pages, *job = to + p.num_pages;
+    pages_compact_kernel<<<sm_count, kPlanThreads, 0, stream>>>(p, src, dst, to, job, reinterpret_cast<PlanSync*>(sync),
+                                                                counts);
     return cudaGetLastError();
 }
 
