@@ -64,13 +64,15 @@ class Case:
 
     def _store(self, b, start, codes):
         """Rows from position `start` on, into the pages."""
-        kc, ks, vc, vs = codes
-        for i in range(kc.shape[0]):
-            pos = start + i
-            page, at = self.table[b, pos // self.page], pos % self.page
+        n, P = codes[0].shape[0], self.page
+        for slot in range(start // P, -(-(start + n) // P)):
+            lo, hi = max(start, slot * P), min(start + n, (slot + 1) * P)
+            if lo >= hi:
+                continue
+            page = self.table[b, slot]
             got = kv.unpack(self.pages[page], self.D)
-            for dst, src in zip(got, (kc, ks, vc, vs)):
-                dst[:, at] = src[i]
+            for dst, src in zip(got, codes):  # [Hkv, P, ...] <- [n, Hkv, ...]
+                dst[:, lo - slot * P:hi - slot * P] = np.swapaxes(src[lo - start:hi - start], 0, 1)
             self.pages[page] = kv.pack(*got)
 
     def expect(self):
@@ -268,6 +270,79 @@ def test_fused_rows_strides_and_side_stream(ctx):
     ctx.check_device_status()
     o, tol, _, _ = c.expect()
     c.check_out(to_np(t["o"]), o, tol)
+
+
+def test_more_sequences_than_one_launch_takes(ctx):
+    """2100 short sequences, one and several tokens each: the call runs in two slices."""
+    lens = np.arange(2100) % 37
+    Case(ctx=lens, Hq=2, Hkv=1, D=64, page=16, seed=3, rope=None).run_decode(ctx)
+    Case(ctx=lens, T=2, new=(np.arange(2100) % 3), Hq=1, Hkv=1, D=64, page=16, seed=5, dtype=oracle.BF16).run_decode(ctx)
+
+
+def test_pages_beyond_four_gigabytes(ctx):
+    """The pages in use lie past 2^32 bytes of their pool."""
+    import torch
+    for T, dtype in ((3, oracle.F16), (70, oracle.BF16)):
+        c = Case(ctx=[1500, 40], T=T, Hq=4, Hkv=2, D=64, page=64, seed=6, dtype=dtype)
+        t = c.device()
+        page_bytes = c.pages[0].size
+        first = (1 << 32) // page_bytes + 5
+        big = torch.empty((first + c.pages.shape[0], 2, 64 * 80), dtype=torch.uint8, device="cuda")
+        big[first:] = t["pages"]
+        t["table"] = torch.where(t["table"] >= 0, t["table"] + first, t["table"])
+        import b200attn
+        b200attn.kv4_decode(ctx, t["q"], t["k"], t["v"], big, t["table"], t["ctx"], t["o"], c.scale, **c.more())
+        ctx.check_device_status()
+        o, tol, _, _ = c.expect()
+        c.check_out(to_np(t["o"]), o, tol)
+        c.check_pages(big[first:].cpu().numpy(), exact=False)
+        del big
+
+
+@pytest.mark.parametrize("T", [1, 5, 80])
+def test_graph_replays_recompute_the_step(ctx, T):
+    import torch
+    import b200attn
+    c = Case(ctx=[700, 3, 90], T=T, Hq=4, Hkv=2, D=128, dtype=oracle.BF16, seed=T)
+    t = c.device()
+    run = lambda: b200attn.kv4_decode(ctx, t["q"], t["k"], t["v"], t["pages"], t["table"], t["ctx"], t["o"], c.scale, **c.more())
+    run()  # workspaces reach their final size before capture
+    torch.cuda.synchronize()
+    g, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s), torch.cuda.graph(g, stream=s):
+        run()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    o, tol, _, _ = c.expect()
+    for _ in range(3):
+        t["o"].fill_(float("nan"))
+        g.replay()
+        torch.cuda.synchronize()
+        c.check_out(to_np(t["o"]), o, tol)
+    del g
+    ctx.check_device_status()
+
+
+def test_workspace_limit_and_its_fallback():
+    """A cap below the decode workspace is B2A_EOOM; one that only leaves no room for a chunk's staged
+    rows makes the chunk read the codes instead."""
+    import b200attn
+    c = Case(ctx=[300, 20], T=2, Hq=4, Hkv=2, D=64, seed=2)
+    t = c.device()
+    with b200attn.Context(0) as small:
+        small.set_workspace_limit(4096)
+        with pytest.raises(b200attn.B200RuntimeException) as ei:
+            b200attn.kv4_decode(small, t["q"], t["k"], t["v"], t["pages"], t["table"], t["ctx"], t["o"], c.scale, **c.more())
+        assert ei.value.status == b200attn.B2A_EOOM and "exceeds the context limit" in str(ei.value)
+        assert small.workspace_bytes() <= 4096
+        small.set_workspace_limit(0)
+        c.run_decode(small)
+    c = Case(ctx=[5000, 20], T=70, Hq=2, Hkv=1, D=64, seed=2, dtype=oracle.BF16, extra_slots=20000)
+    with b200attn.Context(0) as small:
+        small.set_workspace_limit(30 << 20)
+        c.run_decode(small)
+        assert small.workspace_bytes() <= 30 << 20
 
 
 def test_attention_alone_and_repeated_calls_agree(ctx):

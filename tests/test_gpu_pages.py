@@ -200,3 +200,44 @@ def test_pages_refusals_and_device_checks(ctx):
         ctx.check_device_status()
     m.counts[:] = 0
     m.check(t)
+
+
+def test_graph_replays_of_a_step(ctx):
+    """A captured step (trim, fork, reserve, compact) replayed: each replay acts on the state it finds."""
+    import torch
+    import b200attn
+    rng = np.random.default_rng(9)
+    m = Model(rng, 12, 10, 200, 16, share=0.2, fill=0.4)
+    m.lens = np.minimum(m.lens, 60).astype(np.int32)
+    t = m.device()
+    new = np.full(12, 9, np.int32)
+    parents = np.asarray([0, 0, 2, 3, 1, 5, 6, 6, -1, 9, 10, 11], np.int32)
+    new_d, parents_d = _dev(new), _dev(parents)
+
+    def step():
+        b200attn.pages_free(ctx, t["table"], t["refs"], None, t["lens"], 16)
+        b200attn.pages_fork(ctx, t["table"], t["refs"], parents_d)
+        b200attn.pages_reserve(ctx, t["table"], t["refs"], t["lens"], new_d, t["pages"], 16, t["counts"])
+        b200attn.pages_compact(ctx, t["table"], t["refs"], t["pages"], t["counts"])
+
+    def model_step():
+        m.free(None, m.lens)
+        m.fork(parents)
+        m.reserve(m.lens, new)
+        m.compact()
+
+    step()
+    model_step()
+    m.check(t)
+    g, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s), torch.cuda.graph(g, stream=s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        model_step()
+        m.check(t)
+    del g
+    ctx.check_device_status()

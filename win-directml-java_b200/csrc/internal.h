@@ -227,8 +227,7 @@ struct Kv4Piece {
     int b, r, L, n;
     int blk0, blk1, n_split, my_part;
     int part0, part_step;
-    int count, more;  // of a CTA's first piece: its pieces, and where the second one lies (the others follow
-                      // at the places of their units)
+    int count, more;  // of a CTA's first piece: its pieces; of each piece: where the CTA's next one lies
 };
 // How the attention kernel wants its work spread (kv4_attn.cu).
 struct Kv4Split {

@@ -137,7 +137,7 @@ __device__ __forceinline__ void emit_pieces(const Kv4Params& p, const PlanShared
     const Int R = pieces ? 1 : max((Int)p.split.min_blocks, (total + n_cta - 1) / n_cta);
     Int pos = c * R;
     const Int end = min(total, pos + R);
-    int made = 0, more = 0;
+    int made = 0, before = c;  // pieces so far, the last one's place
     while (pos < end) {
         int lo = 0, hi = p.B - 1;
         while (lo < hi) {  // the last sequence that starts at or before pos
@@ -166,7 +166,8 @@ __device__ __forceinline__ void emit_pieces(const Kv4Params& p, const PlanShared
             }
             const Int c0 = u_start / R, c1 = (u_end - 1) / R, stop = min(end, u_end);
             const int place = made == 0 ? c : n_cta + b * per_seq + r;
-            if (made == 1) more = place;
+            if (made > 0) p.plan[before].more = place;
+            before = place;
             // CTA c's slot is 2 c for the piece its range begins with, 2 c + 1 for one that begins later
             put_piece(p.plan + place, b, r, L, n, first + (int)(pos - u_start), first + (int)(stop - u_start),
                       (int)(c1 - c0) + 1, 2 * c + (pos == c * R ? 0 : 1), 2 * (int)c0 + (u_start != c0 * R ? 1 : 0), 2);
@@ -174,7 +175,7 @@ __device__ __forceinline__ void emit_pieces(const Kv4Params& p, const PlanShared
             pos = stop < end ? u_start + w : end;
         }
     }
-    *reinterpret_cast<int2*>(&p.plan[c].count) = make_int2(made, more);
+    p.plan[c].count = made;
 }
 
 __device__ __noinline__ void plan_attention(const Kv4Params& p, PlanShared& sh, int block) {

@@ -203,15 +203,12 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
     // the preparation kernel made the plan, the q operands and the new rows' blocks
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const Kv4Piece* piece = p.plan + blockIdx.x;
-    int pieces_left = 1, next = 0;
-    for (bool begin = true; pieces_left > 0; --pieces_left, begin = false, piece = p.plan + next++) {
+    for (int left = -1; left != 0; --left) {
         const int4 w0 = reinterpret_cast<const int4*>(piece)[0], w1 = reinterpret_cast<const int4*>(piece)[1],
                    w2 = reinterpret_cast<const int4*>(piece)[2];
-        if (begin) {
-            pieces_left = w2.z;
-            next = w2.w;
-            if (pieces_left == 0) break;
-        }
+        if (left < 0) left = w2.z;
+        if (left == 0) break;
+        piece = p.plan + w2.w;  // the next one, where there is one
         const int b = w0.x, r = w0.y, L = w0.z, n = w0.w;
         const int n_split = w1.z, my_part = w1.w, part0 = w2.x, part_step = w2.y;
         const int kvh = r / row_tiles, rt = r - kvh * row_tiles;
