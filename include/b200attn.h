@@ -388,7 +388,8 @@ B2A_API size_t b2a_kv4_page_bytes(int num_kv_heads, int head_dim, int page_size)
  *       (b2a_pages_reserve sees to both).  Lengths that do not fit the table raise the device
  *       status, store nothing and give NaN.
  *   k_held, v_held : optional [B,T,Hkv,D] act_dtype, the rows as the cache holds them (zeros where
- *       t >= new_lens[b]): the values every later step sees, for a prompt's own attention.
+ *       t >= new_lens[b]): the values every later step sees, for a prompt's own attention.  Must not
+ *       overlap the inputs.
  * Sequences of one call must not share the pages they write. */
 B2A_API int b2a_kv4_append(b2a_context* ctx, const b2a_kv4_cache* cache, int act_dtype, const void* k_new,
                            const void* v_new, int64_t kv_token_stride, const int32_t* ctx_lens,

@@ -508,22 +508,65 @@ def _kv_rows(k_new, v_new, first, shape):
     return k, v, step
 
 
+def _kv4_call_rows(k_new, v_new, pages, page_table, ctx_lens, new_lens, k_held, v_held, dtype, kv_shape):
+    """The addresses that kv4_append and kv4_decode share, where every tensor is as it usually is (dense, on
+    the device, of the expected types and shapes); None otherwise -- the caller's checks then say what is wrong
+    or accept the less usual (strided rows)."""
+    i32, u8 = (_rt or _runtime())[:2]
+    B, T, Hkv, D = kv_shape
+    if not (k_new.dtype is dtype and v_new.dtype is dtype and v_new.shape == kv_shape and pages.dtype is u8
+            and page_table.dtype is i32 and ctx_lens.dtype is i32 and ctx_lens.shape == (B,)):
+        return None
+    if new_lens is not None and not (new_lens.dtype is i32 and new_lens.shape == (B,) and new_lens.is_cuda
+                                     and new_lens.is_contiguous()):
+        return None
+    for held in (k_held, v_held):
+        if held is not None and not (held.dtype is dtype and held.shape == kv_shape and held.is_cuda
+                                     and held.is_contiguous()):
+            return None
+    if not (k_new.is_cuda and v_new.is_cuda and pages.is_cuda and page_table.is_cuda and ctx_lens.is_cuda
+            and k_new.is_contiguous() and v_new.is_contiguous() and pages.is_contiguous()
+            and page_table.is_contiguous() and ctx_lens.is_contiguous()):
+        return None
+    pool, table = pages.shape, page_table.shape
+    if not (len(pool) == 3 and len(table) == 2 and table[0] == B and pool[1] == Hkv):
+        return None
+    page_size, rest = divmod(pool[2] * 4, D * 5)
+    if rest or page_size == 0:
+        return None
+    return (_Kv4Cache(pages.data_ptr(), page_table.data_ptr(), pool[0], page_size, table[1], Hkv, D), k_new.data_ptr(),
+            v_new.data_ptr(), ctx_lens.data_ptr(), None if new_lens is None else new_lens.data_ptr(),
+            None if k_held is None else k_held.data_ptr(), None if v_held is None else v_held.data_ptr())
+
+
+def _kv4_check_rows(k_new, v_new, pages, page_table, ctx_lens, new_lens, k_held, v_held, first, kv_shape):
+    """The same with every check by itself, and the rows' token stride."""
+    B, T, Hkv, D = kv_shape
+    cache = _kv4_cache(pages, page_table, B, D, Hkv)
+    k, v, step = _kv_rows(k_new, v_new, first, kv_shape)
+    return (cache, k, v, _int32(ctx_lens, "ctx_lens", (B,)),
+            None if new_lens is None else _int32(new_lens, "new_lens", (B,)),
+            _row_like(k_held, "k_held", first, kv_shape), _row_like(v_held, "v_held", first, kv_shape)), step
+
+
 def kv4_append(ctx: Context, k_new, v_new, pages, page_table, ctx_lens, *, new_lens=None, rope_mode: int = ROPE_NEOX,
                rope_theta: float = 10000.0, k_norm_w=None, norm_eps: float = 1e-6, k_held=None, v_held=None,
                stream=None):
     """Append new K/V rows [B,T,Hkv,D] (fp16 / bf16; slices of fused rows may be passed) to a paged 4-bit
     cache: key norm, RoPE at ctx_lens[b] + t, quantisation, store.  pages: uint8 [num_pages, Hkv,
     page_size * D * 5 // 4]; page_table int32 [B, max_pages]; ctx_lens, new_lens int32 [B] (new_lens: how many
-    of the T tokens exist).  k_held / v_held [B,T,Hkv,D] receive the rows as the cache holds them."""
+    of the T tokens exist).  k_held / v_held [B,T,Hkv,D] receive the rows as the cache holds them (not in the
+    place of the rows themselves)."""
     shape = k_new.shape
     B, T, Hkv, D = shape
-    cache = _kv4_cache(pages, page_table, B, D, Hkv)
-    k, v, step = _kv_rows(k_new, v_new, k_new, shape)
+    dtype, step = k_new.dtype, 0
+    rows = _kv4_call_rows(k_new, v_new, pages, page_table, ctx_lens, new_lens, k_held, v_held, dtype, shape)
+    if rows is None:
+        rows, step = _kv4_check_rows(k_new, v_new, pages, page_table, ctx_lens, new_lens, k_held, v_held, k_new, shape)
+    cache, k, v, lens, new, kh, vh = rows
     rc = (_lib or lib()).b2a_kv4_append(
-        ctx._h, cache, _kv4_dtype(k_new), k, v, step, _int32(ctx_lens, "ctx_lens", (B,)),
-        None if new_lens is None else _int32(new_lens, "new_lens", (B,)), B, T, rope_mode, rope_theta,
-        _norm_w(k_norm_w, "k_norm_w", D), norm_eps, _row_like(k_held, "k_held", k_new, shape),
-        _row_like(v_held, "v_held", k_new, shape), _raw_stream(stream))
+        ctx._h, cache, _kv4_dtype(k_new), k, v, step, lens, new, B, T, rope_mode, rope_theta,
+        _norm_w(k_norm_w, "k_norm_w", D), norm_eps, kh, vh, _raw_stream(stream))
     if rc:
         ctx.check(rc)
 
@@ -553,16 +596,19 @@ def kv4_decode(ctx: Context, q, k_new, v_new, pages, page_table, ctx_lens, o, sc
     verification of a draft, or a chunk of a prompt on a cached prefix."""
     shape = q.shape
     B, T, Hq, D = shape
-    Hkv = k_new.shape[2] if k_new.dim() == 4 else 0
-    kv_shape = (B, T, Hkv, D)
-    cache = _kv4_cache(pages, page_table, B, D, Hkv)
+    dtype, step = q.dtype, 0
+    kv_shape = (B, T, k_new.shape[2] if k_new.dim() == 4 else 0, D)
+    rows = None
+    if k_new.shape == kv_shape:
+        rows = _kv4_call_rows(k_new, v_new, pages, page_table, ctx_lens, new_lens, k_held, v_held, dtype, kv_shape)
+    if rows is None:
+        rows, step = _kv4_check_rows(k_new, v_new, pages, page_table, ctx_lens, new_lens, k_held, v_held, q, kv_shape)
+    cache, k, v, lens, new, kh, vh = rows
     qp, q_step = _token_rows(q, "q", shape)
-    k, v, step = _kv_rows(k_new, v_new, q, kv_shape)
     rc = (_lib or lib()).b2a_kv4_decode(
-        ctx._h, cache, _kv4_dtype(q), qp, q_step, k, v, step, _int32(ctx_lens, "ctx_lens", (B,)),
-        None if new_lens is None else _int32(new_lens, "new_lens", (B,)), B, T, Hq, scale, rope_mode, rope_theta,
-        window, _norm_w(q_norm_w, "q_norm_w", D), _norm_w(k_norm_w, "k_norm_w", D), norm_eps,
-        _row_like(k_held, "k_held", q, kv_shape), _row_like(v_held, "v_held", q, kv_shape),
+        ctx._h, cache, _kv4_dtype(q), qp, q_step, k, v, step, lens, new, B, T, Hq, scale, rope_mode, rope_theta,
+        window, None if q_norm_w is None else _norm_w(q_norm_w, "q_norm_w", D),
+        None if k_norm_w is None else _norm_w(k_norm_w, "k_norm_w", D), norm_eps, kh, vh,
         _row_like(o, "o", q, shape), _raw_stream(stream))
     if rc:
         ctx.check(rc)

@@ -36,6 +36,7 @@
 // s_max (s_max: the largest value scale seen, at least 1), to where the largest is 2^7 / s_max: a
 // block normally costs no reduction across lanes, P and P s stay inside fp16 with at least 2^21 of
 // range below the largest weight before subnormals begin, and sums are in fp32 throughout.
+#include <algorithm>
 #include <mutex>
 #include <type_traits>
 
@@ -49,7 +50,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr float kLowest = -1e37f;  // largest score before any key: finite, so differences are numbers
 
-template <int D_, int kTiles_, int kSplit_>
+template <int D_, int kTiles_, int kSplit_, bool kPipelined_ = false>
 struct Cfg {
     static constexpr int D = D_;
     static constexpr int kTiles = kTiles_;  // column tiles of 8 in the second product
@@ -63,18 +64,15 @@ struct Cfg {
     static constexpr int kStages = D <= 96 ? 3 : (D <= 128 ? 4 : 3);
     static constexpr int kStageBytes = kSub * kBlockBytes;
     // Side by side in the loop: the scores of one stage and the second product of the one before.  It
-    // takes the registers of a third CTA per SM.  Where a launch is short, one warp's own speed counts:
-    // head dim 256 decode over a 512-key window 30.9 -> 26.8 us, 5-token drafts 20.6 -> 19.3 us; long
-    // contexts lose what the third CTA hid (head dim 256, 17 k keys: 275 -> 299 us), and at head dim
-    // 64 with two-word operands the third CTA is worth more throughout (31 against 34 us).
-    static constexpr bool kPipelined = D == 256 || (kSplit == 0 && kTiles == 2);
+    // takes the registers of a third CTA per SM (dispatch says when that pays).
+    static constexpr bool kPipelined = kPipelined_;
     // CTAs per SM, the registers' bound
     static constexpr int kCtas = kPipelined ? 2 : (D <= 64 ? (kTiles == 1 ? 4 : 3) : (kTiles == 1 ? 3 : 2));
     // fixed cost of a piece in blocks of streaming time, charged to every unit by the split
     static constexpr int kGapBlocks = D <= 64 ? 26 : (D <= 96 ? 22 : (D <= 128 ? 20 : 16));
     static constexpr int kMinBlocks = 8;  // smallest piece
     // q's operand words in shared memory where the accumulators leave no registers for them
-    static constexpr bool kQShared = D * kTiles > 256;
+    static constexpr bool kQShared = D * kTiles > (kPipelined ? 256 : 128);
     // head dim 256: the value params are regrouped in shared memory (their rows lie 128 bytes
     // apart, so that reading pairs of keys directly would meet in the same banks)
     static constexpr bool kRegroup = D >= 256;
@@ -919,19 +917,36 @@ LaunchInfo launch_info(int device) {
     return info[device];
 }
 
-// Calls f with the instantiation for (D, query rows per sequence and kv head, element type): fp16
-// results carry q and P as two words; bf16 ones take 16 columns where there are as many rows (a
-// cache byte then serves twice as many), except at head dim 256, whose accumulators fill the
-// registers with 8.
+// Calls f with the instantiation for (D, query rows per sequence and kv head, element type).
+//  * fp16 results carry q and P as two words.
+//  * bf16 ones take 16 columns where there are as many rows (a cache byte then serves twice as many),
+//    except at head dim 256, whose accumulators fill the registers with 8.
+//  * Pipelined at head dim 256 where a CTA has few blocks to walk and one warp's own speed counts (256
+//    sequences over a 512-key window, 33 blocks each: 30.9 -> 26.8 us); long contexts want the third CTA
+//    (the same sequences over 17 k keys: 299 pipelined, 275 us not).  What a CTA has is bounded by the
+//    window, else by the table's capacity.  With 16 columns always: the third CTA does not fit anyway
+//    (5-token drafts at head dim 64: 20.6 -> 19.3 us); at head dim 64 with two-word operands never (64
+//    sequences of 4 k keys: 34 pipelined, 31 us not).
+constexpr int kPipelineBlocks = 128;
+
 template <typename F>
 cudaError_t dispatch(const Kv4Params& p, F&& f) {
     const int rows = p.T * p.G;
     auto by_rows = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        if (p.act_dtype == kF16) return rows <= 4 ? f(Cfg<D, 1, 1>{}) : f(Cfg<D, 2, 2>{});
-        if constexpr (D < 256)
-            if (rows > 8) return f(Cfg<D, 2, 0>{});
-        return f(Cfg<D, 1, 0>{});
+        if constexpr (D == 256) {
+            const int64_t keys = std::min<int64_t>(p.window > 0 ? p.window + p.T : INT32_MAX, (int64_t)p.max_pages * p.page_size);
+            const int64_t units = (int64_t)p.B * p.Hkv * ((rows + 7) / 8);
+            const bool few = units * (keys / kKv4Block) <= (int64_t)kPipelineBlocks * 2 * 148;
+            if (p.act_dtype == kF16) {
+                if (rows > 4) return f(Cfg<D, 2, 2, true>{});
+                return few ? f(Cfg<D, 1, 1, true>{}) : f(Cfg<D, 1, 1, false>{});
+            }
+            return few ? f(Cfg<D, 1, 0, true>{}) : f(Cfg<D, 1, 0, false>{});
+        } else {
+            if (p.act_dtype == kF16) return rows <= 4 ? f(Cfg<D, 1, 1>{}) : f(Cfg<D, 2, 2>{});
+            return rows > 8 ? f(Cfg<D, 2, 0, true>{}) : f(Cfg<D, 1, 0>{});
+        }
     };
     switch (p.D) {
         case 64: return by_rows(std::integral_constant<int, 64>{});
