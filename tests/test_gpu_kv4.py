@@ -279,6 +279,15 @@ def test_more_sequences_than_one_launch_takes(ctx):
     Case(ctx=lens, T=2, new=(np.arange(2100) % 3), Hq=1, Hkv=1, D=64, page=16, seed=5, dtype=oracle.BF16).run_decode(ctx)
 
 
+def test_slices_of_a_call_share_their_variant(ctx):
+    """At head dim 256 the kernel's variant follows the whole call's work, of which the last slice has
+    little."""
+    lens = np.arange(2100) % 29
+    lens[2090] = 330
+    Case(ctx=lens, Hq=2, Hkv=1, D=256, page=16, seed=4, rope=None, dtype=oracle.BF16).run_decode(ctx)
+    Case(ctx=lens, Hq=1, Hkv=1, D=256, page=16, seed=7, rope=None).run_decode(ctx)
+
+
 def test_pages_beyond_four_gigabytes(ctx):
     """The pages in use lie past 2^32 bytes of their pool."""
     import torch

@@ -235,6 +235,7 @@ struct Kv4Split {
     int per_seq;     // units per sequence
     int gap;         // fixed cost of a piece, in blocks
     int min_blocks;  // smallest piece
+    bool few;        // the variant for few blocks per CTA: every launch of a call takes the same one
     size_t partial_bytes;
 };
 

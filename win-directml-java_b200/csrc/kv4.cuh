@@ -118,9 +118,11 @@ __device__ __forceinline__ void kv4_norm_rope(float (&x)[D / 32], bool norm, con
     __syncwarp();
 }
 
-// (cos, sin) of positions pos0 .. pos0 + 15 at cs[row * D / 2 + i], as doubles (Gemma) or floats (NeoX),
-// by the block's first D / 2 threads: two double sincos each -- the first position and one step -- and
-// a complex product per further position (an error of some 2^-50, far below the rounding to float; a
+// Cosines and sines of positions pos0 .. pos0 + 15, in 16-byte units that hold one channel's (cos, sin)
+// as doubles (Gemma) or two channels' (cos, cos', sin, sin') as floats (NeoX): of channels 8 k .. + 7 a
+// row, unit u lies at [row][u][k], so that neighbouring threads read neighbouring units.  By the
+// block's first D / 2 threads: two double sincos each -- the first position and one step -- and a
+// complex product per further position (an error of some 2^-50, far below the rounding to float; a
 // sincos is about a hundred double instructions).
 template <int D>
 __device__ __forceinline__ void kv4_block_angles(const Kv4Params& p, int pos0, void* cs, int tid) {
@@ -130,8 +132,13 @@ __device__ __forceinline__ void kv4_block_angles(const Kv4Params& p, int pos0, v
     sincos(p.inv_freq[tid], &s1, &c1);
 #pragma unroll
     for (int row = 0; row < 16; ++row) {
-        if (p.rope_mode == 2) static_cast<double2*>(cs)[row * (D / 2) + tid] = make_double2(c, s);
-        else static_cast<float2*>(cs)[row * (D / 2) + tid] = make_float2((float)c, (float)s);
+        if (p.rope_mode == 2) {
+            static_cast<double2*>(cs)[row * (D / 2) + (tid & 7) * (D / 16) + (tid >> 3)] = make_double2(c, s);
+        } else {
+            float* at = static_cast<float*>(cs) + (row * (D / 4) + (tid >> 1 & 3) * (D / 16) + (tid >> 3)) * 4 + (tid & 1);
+            at[0] = (float)c;
+            at[2] = (float)s;
+        }
         const double next = c * c1 - s * s1;
         s = s * c1 + c * s1;
         c = next;

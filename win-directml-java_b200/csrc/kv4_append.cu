@@ -13,6 +13,7 @@
 #include <algorithm>
 
 #include "kv4.cuh"
+#include "sm100.cuh"
 
 namespace b2a {
 namespace {
@@ -378,6 +379,24 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
     asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
+// Two floats at once, each rounded by itself: sm_100 issues the pair as one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<uint64_t&>(d))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 // The low 16 bits' nibbles into the low nibbles of four bytes.
 __device__ __forceinline__ uint32_t spread_nibbles(uint32_t x) {
     x = (x | x << 8) & 0x00FF00FFu;
@@ -394,17 +413,28 @@ struct StoreGeo {
     static constexpr int kHeads = D <= 64 ? 8 : (D <= 128 ? 4 : 2);  // heads of a CTA side by side, at most
     static constexpr int kMinHeads = D == 96 ? 2 : 1;         // whole warps
     static constexpr int kMaxThreads = kHeads * kPerHead;
-    static constexpr int kCtas = D == 96 ? 4 : (D == 256 ? 2 : 3);  // per SM, about 80 registers a thread
-    static size_t smem(int heads, int rope_mode) {
-        return (size_t)heads * (20 * D + 16 * kChunks * 8) +
-               16 * (D / 2) * (rope_mode == 2 ? sizeof(double2) : sizeof(float2));
+    static constexpr int kCtas = D == 96 ? 5 : 3;  // per SM: 64 registers a thread at head dim 96, else 80
+    // an operand's 16 rows of the CTA's heads; the pad keeps rows two apart on other banks
+    __host__ __device__ static constexpr int pitch(int heads) { return heads * D * 2 + (D == 96 ? 32 : 0); }
+    __host__ __device__ static size_t stage_at(int heads) { return 2 * 16 * (size_t)pitch(heads); }
+    __host__ __device__ static size_t cs_at(int heads) { return stage_at(heads) + heads * 20 * D; }
+    __host__ __device__ static size_t part_at(int heads, int rope_mode) {
+        return cs_at(heads) + (rope_mode == 0 ? 0 : 16 * (D / 2) * (rope_mode == 2 ? sizeof(double2) : sizeof(float2)));
+    }
+    static size_t smem(int heads, int rope_mode, bool norm) {
+        return part_at(heads, rope_mode) + (norm ? heads * 16 * kChunks * 8 : 0);
     }
 };
 
-// A CTA takes one block of a sequence and heads h0 + group, + groups, ...  A key chunk is rotated with
-// its partner chunk D / 2 away, which the thread loads too (it comes from L1); the four threads of a
-// group share its minimum and maximum.  Bound by its instructions, about 17 per value (measured 2.8
-// per cycle and SM with 291 per 8 values before the words were put together in registers).
+// A CTA takes one block of a sequence and heads h0 + group, + groups, ...  Its rows of K, then of V, come
+// by bulk copies into a place each, asked for again as soon as the last ones are in registers, so that
+// a round's rows travel while the round before is worked on.  A key chunk is rotated with its partner
+// chunk D / 2 away, which the thread reads too.  The four threads of a group exchange minima and
+// maxima so that each ends with one of the four rows, and computes that row's scale for all.
+// Bound by issue and latency rather than by HBM: 8 x 4096 tokens of 32 heads of 96 with held rows (932
+// MB) take 193 us, 4.8 TB/s.  What it took: packed float pairs (201 -> 159 million warp instructions),
+// the rows' scales shared out (148 million, 261 -> 213 us), conflict-free angles (193 us).  Rows loaded
+// into registers ahead instead of by bulk copies: 209 us; 4 and 6 CTAs per SM: 220 and 245 us.
 template <int D, typename T, bool kNorm>
 __global__ void __launch_bounds__(StoreGeo<D>::kMaxThreads, StoreGeo<D>::kCtas)
     kv4_store_kernel(const __grid_constant__ Kv4Params p, int blocks, int chunks, int per) {
@@ -412,12 +442,15 @@ __global__ void __launch_bounds__(StoreGeo<D>::kMaxThreads, StoreGeo<D>::kCtas)
     constexpr int kChunks = Gm::kChunks, kGroups = D / 32;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // a chunk's query staging may run beside this
     extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ __align__(8) uint64_t full[2];  // K's place, V's place
     const int tid = threadIdx.x, groups = blockDim.x / Gm::kPerHead;
     const int group = tid / Gm::kPerHead, in_group = tid - group * Gm::kPerHead;
     const int q = in_group / kChunks, k = in_group - q * kChunks;
-    uint8_t* const stage = smem + group * 20 * D;
-    double* const part = reinterpret_cast<double*>(smem + groups * 20 * D) + group * 16 * kChunks;
-    void* const cs = smem + groups * (20 * D + 16 * kChunks * 8);  // [16][D / 2] (cos, sin)
+    const int pitch = Gm::pitch(groups);
+    uint8_t* const stage = smem + Gm::stage_at(groups) + group * 20 * D;
+    void* const cs = smem + Gm::cs_at(groups);  // [16][D / 2] (cos, sin)
+    double* const part = reinterpret_cast<double*>(smem + Gm::part_at(groups, p.rope_mode)) + group * 16 * kChunks;
+    const uint32_t bar = smem_u32(full);
     const int chunk = blockIdx.x % chunks;
     const int64_t bb = blockIdx.x / chunks;
     const int b = (int)(bb / blocks);
@@ -441,59 +474,67 @@ __global__ void __launch_bounds__(StoreGeo<D>::kMaxThreads, StoreGeo<D>::kCtas)
         }
     }
     if (t_first >= n) return;  // nothing to store (the whole CTA)
+    const int row_first = max(0, -t_first), row_end = min(kKv4Block, n - t_first);  // rows that exist
+    const bool full_block = row_end - row_first == kKv4Block;
+    auto request = [&](int is_v, int h0) {  // warp 0: a round's rows into their place
+        const uint32_t bytes = min(groups, h_end - h0) * D * 2;
+        if (tid == 0) mbar_expect_tx(bar + is_v * 8, (row_end - row_first) * bytes);
+        __syncwarp();
+        if (tid < row_first || tid >= row_end) return;
+        const T* src = static_cast<const T*>(is_v ? p.v_new : p.k_new) + (seq_tok + t_first + tid) * p.kv_stride + (int64_t)h0 * D;
+        bulk_load(smem_u32(smem) + (is_v * 16 + tid) * pitch, src, bytes, bar + is_v * 8);
+    };
+    if (tid < 32) {
+        if (tid == 0) {
+            mbar_init(bar, 1);
+            mbar_init(bar + 8, 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncwarp();
+        request(0, h_begin);
+        request(1, h_begin);
+    }
     if (p.rope_mode != 0) kv4_block_angles<D>(p, blk * kKv4Block, cs, tid);
-    const bool full = t_first >= 0 && t_first + kKv4Block <= n;
     const bool upper = k >= kChunks / 2;
     const int k2 = upper ? k - kChunks / 2 : k + kChunks / 2, k_low = upper ? k2 : k;
     const int j = k & 1, x16 = (k >> 1) & 1, y = k >> 2;
     __syncthreads();
 
-    for (int h0 = h_begin; h0 < h_end; h0 += groups) {
+    uint32_t parity = 0;
+    const unsigned char* const mine = smem + 2 * q * pitch + group * D * 2 + k * 16;
+    for (int h0 = h_begin; h0 < h_end; h0 += groups, parity ^= 1) {
         const int h = h0 + group;
         const bool live = h < h_end;
-        if constexpr (kNorm) {
-            for (int i = 0; i < 4; ++i) {
-                const int t = t_first + row_of(i);
-                double ss = 0.0;
-                if (live && t >= 0 && t < n) {
-                    float x[8];
-                    unpack8(*reinterpret_cast<const uint4*>(static_cast<const T*>(p.k_new) + (seq_tok + t) * p.kv_stride +
-                                                            (int64_t)h * D + 8 * k), x, T{});
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) ss += (double)x[c] * (double)x[c];
-                }
-                part[row_of(i) * kChunks + k] = ss;
-            }
-            __syncthreads();
-        }
-        // every row is requested before the first one is used: a row after another would pay the
-        // memory's latency eight times
-        uint4 raw[3][4];  // K chunk, its partner, V chunk
-        const int64_t first_row = (seq_tok + t_first + 2 * q) * p.kv_stride + (int64_t)h * D + 8 * k;
-        const T *const k_at = static_cast<const T*>(p.k_new) + first_row, *const v_at = static_cast<const T*>(p.v_new) + first_row;
-        const uint32_t flip = upper ? 0u : 0x80008000u;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int t = t_first + row_of(i);
-            const int64_t at = ((i & 1) + 8 * (i >> 1)) * p.kv_stride;
-            raw[0][i] = raw[1][i] = raw[2][i] = make_uint4(0, 0, 0, 0);
-            if (!(live && t >= 0 && t < n)) continue;
-            raw[0][i] = __ldg(reinterpret_cast<const uint4*>(k_at + at));
-            if (p.rope_mode != 0) raw[1][i] = __ldg(reinterpret_cast<const uint4*>(k_at + at + 8 * (k2 - k)));
-            raw[2][i] = __ldg(reinterpret_cast<const uint4*>(v_at + at));
-        }
+        const float2 side = both(upper ? 1.f : -1.f);  // x cos -+ partner sin
         const int64_t held_at = ((seq_tok + t_first + 2 * q) * p.Hkv + h) * D + 8 * k;
-        uint32_t bytes[2][4];  // [K, V][row]: the bytes of channels 4 j .. + 3 of the chunk pair (k, k ^ 1)
+        auto exists = [&](int i) { return live && row_of(i) >= row_first && row_of(i) < row_end; };
 #pragma unroll
         for (int is_v = 0; is_v < 2; ++is_v) {
-            void* held = is_v ? p.v_held : p.k_held;
             uint8_t* const dst = stage + (is_v ? kv4_off_v(D) : 0);
+            const unsigned char* const from = mine + is_v * 16 * pitch;
+            auto row_at = [&](int i) { return from + ((i & 1) + 8 * (i >> 1)) * pitch; };
+            const bool came = wait_bounded(bar + is_v * 8, parity);
+            if (kNorm && !is_v) {
+                for (int i = 0; i < 4; ++i) {
+                    double ss = 0.0;
+                    if (exists(i)) {
+                        float x[8];
+                        unpack8(*reinterpret_cast<const uint4*>(row_at(i)), x, T{});
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) ss += (double)x[c] * (double)x[c];
+                    }
+                    part[row_of(i) * kChunks + k] = ss;
+                }
+                __syncthreads();
+            }
+            // ---- the rows' values, each thread's minima and maxima: NaN reaches `hi`, infinities both
+            float2 x[4][4];
+            float lo[4], hi[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int row = row_of(i), t = t_first + row;
-                const bool there = live && t >= 0 && t < n;
-                float x[8];
-                unpack8(raw[2 * is_v][i], x, T{});
+                const int row = row_of(i);
+                float v[8];
+                unpack8(exists(i) ? *reinterpret_cast<const uint4*>(row_at(i)) : make_uint4(0, 0, 0, 0), v, T{});
                 if (!is_v) {
                     float rms = 0.f;
                     if constexpr (kNorm) {
@@ -502,138 +543,174 @@ __global__ void __launch_bounds__(StoreGeo<D>::kMaxThreads, StoreGeo<D>::kCtas)
                         rms = (float)(1.0 / sqrt(__dadd_rn(ss / (double)D, (double)p.norm_eps)));
 #pragma unroll
                         for (int c = 0; c < 8; ++c)
-                            x[c] = (float)__dmul_rn((double)__fmul_rn(x[c], rms), __dadd_rn(1.0, (double)__ldg(p.k_norm_w + 8 * k + c)));
+                            v[c] = (float)__dmul_rn((double)__fmul_rn(v[c], rms), __dadd_rn(1.0, (double)__ldg(p.k_norm_w + 8 * k + c)));
                     }
                     if (p.rope_mode != 0) {
                         float z[8];
-                        uint4 w = raw[1][i];
-                        w.x ^= flip, w.y ^= flip, w.z ^= flip, w.w ^= flip;
-                        unpack8(w, z, T{});
+                        unpack8(exists(i) ? *reinterpret_cast<const uint4*>(row_at(i) + 16 * (k2 - k)) : make_uint4(0, 0, 0, 0), z, T{});
                         if constexpr (kNorm) {
 #pragma unroll
                             for (int c = 0; c < 8; ++c)
                                 z[c] = (float)__dmul_rn((double)__fmul_rn(z[c], rms), __dadd_rn(1.0, (double)__ldg(p.k_norm_w + 8 * k2 + c)));
                         }
                         if (p.rope_mode == 2) {
-                            const double2* a = static_cast<const double2*>(cs) + row * (D / 2) + 8 * k_low;
+                            const double2* a = static_cast<const double2*>(cs) + row * (D / 2) + k_low;
 #pragma unroll
                             for (int c = 0; c < 8; ++c) {
-                                const double u = __dmul_rn((double)x[c], a[c].x), v = __dmul_rn((double)z[c], a[c].y);
-                                x[c] = (float)__dadd_rn(u, v);
+                                const double e = __dmul_rn((double)v[c], a[c * (D / 16)].x), f = __dmul_rn((double)z[c], a[c * (D / 16)].y);
+                                v[c] = (float)(upper ? __dadd_rn(e, f) : __dsub_rn(e, f));
                             }
                         } else {
-                            const float4* a = reinterpret_cast<const float4*>(static_cast<const float2*>(cs) + row * (D / 2) + 8 * k_low);
+                            const float4* a = static_cast<const float4*>(cs) + row * (D / 4) + k_low;
 #pragma unroll
-                            for (int c = 0; c < 8; c += 2) {  // the lower chunk's partner comes negated
-                                const float4 ang = a[c / 2];
-                                x[c] = __fadd_rn(__fmul_rn(x[c], ang.x), __fmul_rn(z[c], ang.y));
-                                x[c + 1] = __fadd_rn(__fmul_rn(x[c + 1], ang.z), __fmul_rn(z[c + 1], ang.w));
+                            for (int c = 0; c < 8; c += 2) {  // times +-1 is exact: the FMA adds or subtracts
+                                const float4 ang = a[c / 2 * (D / 16)];
+                                const float2 e = mul2(make_float2(v[c], v[c + 1]), make_float2(ang.x, ang.y));
+                                const float2 f = mul2(make_float2(z[c], z[c + 1]), make_float2(ang.z, ang.w));
+                                const float2 turned = fma2(f, side, e);
+                                v[c] = turned.x;
+                                v[c + 1] = turned.y;
                             }
                         }
                     }
                 }
-                // the group's minimum and maximum: NaN reaches `hi`, infinities both
-                float lo = min3(min3(x[0], x[1], x[2]), min3(x[3], x[4], x[5]), fminf(x[6], x[7]));
-                float hi = max_nan(max_nan(x[0], x[1], x[2]), max_nan(x[3], x[4], x[5]), max_nan(x[6], x[7]));
+                lo[i] = min3(min3(v[0], v[1], v[2]), min3(v[3], v[4], v[5]), fminf(v[6], v[7]));
+                hi[i] = max_nan(max_nan(v[0], v[1], v[2]), max_nan(v[3], v[4], v[5]), max_nan(v[6], v[7]));
 #pragma unroll
-                for (int o = 1; o <= 2; o <<= 1) {
-                    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-                    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-                }
-                __half s = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f)), z = __float2half_rn(lo);
+                for (int c = 0; c < 4; ++c) x[i][c] = make_float2(v[2 * c], v[2 * c + 1]);
+            }
+            if (__syncthreads_or(!came)) {  // the wait ran out: nothing more is stored or asked for
+                if (tid == 0) atomicOr(p.status, 8);
+                mbar_drain(bar, parity);
+                mbar_drain(bar + 8, parity);
+                return;
+            }
+            if (tid < 32 && h0 + groups < h_end) request(is_v, h0 + groups);
+            // ---- the groups' scales, one row of the four to each of a group's four threads
+            uint32_t sz;
+            float inv;
+            bool outside;
+            {
+                const bool b1 = k & 2, b0 = k & 1;
+                auto other = [&](float v, int o) { return __shfl_xor_sync(0xffffffffu, v, o); };
+                const float lo0 = fminf(b1 ? lo[2] : lo[0], other(b1 ? lo[0] : lo[2], 2));
+                const float lo1 = fminf(b1 ? lo[3] : lo[1], other(b1 ? lo[1] : lo[3], 2));
+                const float hi0 = max_nan(b1 ? hi[2] : hi[0], other(b1 ? hi[0] : hi[2], 2));
+                const float hi1 = max_nan(b1 ? hi[3] : hi[1], other(b1 ? hi[1] : hi[3], 2));
+                const float low = fminf(b0 ? lo1 : lo0, other(b0 ? lo0 : lo1, 1));
+                const float high = max_nan(b0 ? hi1 : hi0, other(b0 ? hi0 : hi1, 1));
+                __half s = __float2half_rn(__fmul_rn(__fsub_rn(high, low), 1.0f / 15.0f)), z = __float2half_rn(low);
                 const float sf = __half2float(s), zf = __half2float(z);
                 const bool fine = isfinite(sf) && isfinite(zf);
-                const float inv = sf > 0.f && fine ? __fdiv_rn(1.0f, sf) : 0.f;
-                const float ns = fine ? sf : __int_as_float(0x7fc00000), nz = fine ? zf : ns;
-                float code[8];
-#pragma unroll
-                for (int c = 0; c < 8; ++c) code[c] = __fmul_rn(__fsub_rn(x[c], zf), inv);
-                // into 0 .. 15 where the group's ends leave it (z and s are rounded: rarely)
-                const float u_lo = __fmul_rn(__fsub_rn(lo, zf), inv), u_hi = __fmul_rn(__fsub_rn(hi, zf), inv);
-                if (!(u_lo >= -0.5f && u_hi <= 15.5f)) {
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) code[c] = fminf(fmaxf(code[c], 0.f), 15.f);
+                inv = sf > 0.f && fine ? __fdiv_rn(1.0f, sf) : 0.f;
+                // codes leave 0 .. 15 only where the group's ends do (z and s are rounded: rarely); a group
+                // that is not finite counts as such, and its codes become 0 with the others'
+                outside = !(__fmul_rn(__fsub_rn(low, zf), inv) >= -0.5f && __fmul_rn(__fsub_rn(high, zf), inv) <= 15.5f);
+                if (!fine) {
+                    s = z = __ushort_as_half(0x7fff);
+                    if (exists(k & 3)) atomicOr(p.status, 32);
                 }
+                const __half2 both_sz = __halves2half2(s, z);
+                sz = *reinterpret_cast<const uint32_t*>(&both_sz);
+                reinterpret_cast<uint32_t*>(dst + kv4_off_kparam(D))[kv4_param(row_of(k & 3), y, kGroups)] = sz;
+            }
+            const bool clamp = __any_sync(0xffffffffu, outside);
+            // ---- codes
+            uint32_t bytes[4];  // by row, channels 4 j .. + 3 of the chunk pair (k, k ^ 1)
+            float invs[4];
+            float2 szs[4];
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    // to the nearest whole number (ties to even) by 1.5 * 2^23
-                    code[c] = __fsub_rn(__fadd_rn(code[c], 12582912.f), 12582912.f);
-                    x[c] = fmaf(code[c], ns, nz);
-                }
-                if (held && there) {
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t w = __shfl_sync(0xffffffffu, sz, i, 4);
+                szs[i] = __half22float2(*reinterpret_cast<const __half2*>(&w));
+                invs[i] = __shfl_sync(0xffffffffu, inv, i, 4);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) x[i][c] = mul2(add2(x[i][c], both(-szs[i].y)), both(invs[i]));
+            }
+            if (clamp) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        x[i][c].x = fminf(fmaxf(x[i][c].x, 0.f), 15.f);
+                        x[i][c].y = fminf(fmaxf(x[i][c].y, 0.f), 15.f);
+                    }
+            }
+            T* const held = static_cast<T*>(is_v ? p.v_held : p.k_held);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                // to the nearest whole number (ties to even) by 1.5 * 2^23
+                float2 code[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) code[c] = add2(add2(x[i][c], both(12582912.f)), both(-12582912.f));
+                if (held && exists(i)) {
                     uint4 out;
                     uint32_t* ow = &out.x;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) ow[c] = Elem<T>::pack(x[2 * c], x[2 * c + 1]);
-                    *reinterpret_cast<uint4*>(static_cast<T*>(held) + held_at + ((i & 1) + 8 * (i >> 1)) * p.Hkv * D) = out;
+                    for (int c = 0; c < 4; ++c) {
+                        const float2 v = fma2(code[c], both(szs[i].x), both(szs[i].y));
+                        ow[c] = Elem<T>::pack(v.x, v.y);
+                    }
+                    *reinterpret_cast<uint4*>(held + held_at + ((i & 1) + 8 * (i >> 1)) * p.Hkv * D) = out;
                 }
-                // four codes to 16 bits, exactly, as c0 + 16 c1 + 256 c2 + 4096 c3
+                // four codes to 16 bits, exactly, as c0 + 16 c1 + 256 c2 + 4096 c3 (sums of whole numbers
+                // below 2^24), beside 2^23, whose bits they then are
                 uint32_t half[2];
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    const float f = fmaf(code[4 * c + 3], 4096.f, fmaf(code[4 * c + 2], 256.f, fmaf(code[4 * c + 1], 16.f, code[4 * c])));
-                    half[c] = fine ? __float_as_uint(__fadd_rn(f, 8388608.f)) & 0xffffu : 0u;
+                    const float2 f = fma2(code[2 * c + 1], both(256.f), code[2 * c]);
+                    half[c] = __float_as_uint(fmaf(f.y, 16.f, __fadd_rn(f.x, 8388608.f))) & 0xffffu;
                 }
                 // thread j keeps channels 4 j .. + 3 of both chunks of the pair
-                const uint32_t other = __shfl_xor_sync(0xffffffffu, j ? half[0] : half[1], 1);
+                const uint32_t swap = __shfl_xor_sync(0xffffffffu, j ? half[0] : half[1], 1);
                 const uint32_t own = j ? half[1] : half[0];
-                bytes[is_v][i] = spread_nibbles(j ? other : own) | spread_nibbles(j ? own : other) << 4;
-                if (!fine) {
-                    s = z = __ushort_as_half(0x7fff);
-                    if (there) atomicOr(p.status, 32);
-                }
-                if ((k & 3) == 0)
-                    reinterpret_cast<__half2*>(dst + kv4_off_kparam(D))[kv4_param(row, y, kGroups)] = __halves2half2(s, z);
+                bytes[i] = spread_nibbles(j ? swap : own) | spread_nibbles(j ? own : swap) << 4;
             }
-        }
-        {
-            // K words (lane 4 g + t, x16): bytes (e, r) = channels 2 t + e of keys g + 8 r
-            uint32_t* const kw = reinterpret_cast<uint32_t*>(stage) + y * 64 + x16;
+            uint32_t* const words = reinterpret_cast<uint32_t*>(dst) + y * 64 + x16;
+            if (!is_v) {
+                // K words (lane 4 g + t, x16): bytes (e, r) = channels 2 t + e of keys g + 8 r
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int g = 2 * q + e;
-                const uint32_t a = bytes[0][e], c = bytes[0][e + 2];  // keys g, g + 8
-                kw[(4 * g + 2 * j) * 2] = __byte_perm(a, c, 0x5140);
-                kw[(4 * g + 2 * j + 1) * 2] = __byte_perm(a, c, 0x7362);
+                for (int e = 0; e < 2; ++e) {
+                    const int g = 2 * q + e;
+                    words[(4 * g + 2 * j) * 2] = __byte_perm(bytes[e], bytes[e + 2], 0x5140);
+                    words[(4 * g + 2 * j + 1) * 2] = __byte_perm(bytes[e], bytes[e + 2], 0x7362);
+                }
+            } else {
+                // V words (lane 4 g + t, x16): bytes (e, r) = channel g of keys 2 t + e + 8 r
+                const uint32_t a = __byte_perm(bytes[0], bytes[2], 0x5140), c = __byte_perm(bytes[1], bytes[3], 0x5140);
+                const uint32_t u = __byte_perm(bytes[0], bytes[2], 0x7362), v = __byte_perm(bytes[1], bytes[3], 0x7362);
+                words[(4 * (4 * j + 0) + q) * 2] = __byte_perm(a, c, 0x5410);
+                words[(4 * (4 * j + 1) + q) * 2] = __byte_perm(a, c, 0x7632);
+                words[(4 * (4 * j + 2) + q) * 2] = __byte_perm(u, v, 0x5410);
+                words[(4 * (4 * j + 3) + q) * 2] = __byte_perm(u, v, 0x7632);
             }
-            // V words (lane 4 g + t, x16): bytes (e, r) = channel g of keys 2 t + e + 8 r
-            uint32_t* const vw = reinterpret_cast<uint32_t*>(stage + kv4_off_v(D)) + y * 64 + x16;
-            const uint32_t a = __byte_perm(bytes[1][0], bytes[1][2], 0x5140), c = __byte_perm(bytes[1][1], bytes[1][3], 0x5140);
-            const uint32_t u = __byte_perm(bytes[1][0], bytes[1][2], 0x7362), v = __byte_perm(bytes[1][1], bytes[1][3], 0x7362);
-            vw[(4 * (4 * j + 0) + q) * 2] = __byte_perm(a, c, 0x5410);
-            vw[(4 * (4 * j + 1) + q) * 2] = __byte_perm(a, c, 0x7632);
-            vw[(4 * (4 * j + 2) + q) * 2] = __byte_perm(u, v, 0x5410);
-            vw[(4 * (4 * j + 3) + q) * 2] = __byte_perm(u, v, 0x7632);
         }
         __syncthreads();
         if (live) {
             uint8_t* const block = kv4_block_ptr(p, b, h, blk * kKv4Block);
             if (block == nullptr) {
                 if (in_group == 0) atomicOr(p.status, 16);
-            } else if (full) {
+            } else if (full_block) {
                 for (int i = in_group; i < 20 * D / 16; i += Gm::kPerHead)
                     reinterpret_cast<uint4*>(block)[i] = reinterpret_cast<const uint4*>(stage)[i];
             } else {
                 // the rows that exist: their bytes of the codes, their params
-                auto mine = [&](int key) {
-                    const int tk = t_first + key;
-                    return tk >= 0 && tk < n;
-                };
+                auto stored = [&](int key) { return key >= row_first && key < row_end; };
                 for (int i = in_group; i < 16 * D; i += Gm::kPerHead) {
                     const bool is_v = i >= 8 * D;
                     const int a = is_v ? i - 8 * D : i;
                     const int r = a & 1, e = (a >> 1) & 1, t = (a >> 3) & 3, g = (a >> 5) & 7;
                     const int at = is_v ? kv4_off_v(D) + a : a;
-                    if (mine(is_v ? 2 * t + e + 8 * r : g + 8 * r)) block[at] = stage[at];
+                    if (stored(is_v ? 2 * t + e + 8 * r : g + 8 * r)) block[at] = stage[at];
                 }
                 for (int i = in_group; i < 2 * 16 * kGroups; i += Gm::kPerHead) {
                     const int w = i % (16 * kGroups), key = (w / kGroups >> 1) + 8 * (w / kGroups & 1);
                     const int at = (i < 16 * kGroups ? kv4_off_kparam(D) : kv4_off_vparam(D)) + 4 * w;
-                    if (mine(key)) *reinterpret_cast<uint32_t*>(block + at) = *reinterpret_cast<const uint32_t*>(stage + at);
+                    if (stored(key)) *reinterpret_cast<uint32_t*>(block + at) = *reinterpret_cast<const uint32_t*>(stage + at);
                 }
             }
         }
-        __syncthreads();  // the stage is used again
+        // (the next round writes to the stage behind its first barrier)
     }
 }
 
@@ -645,12 +722,12 @@ cudaError_t launch_store(const Kv4Params& p, int sm_count, cudaStream_t stream) 
     using Gm = StoreGeo<D>;
     const int blocks = (p.T + 2 * kKv4Block - 2) / kKv4Block;  // blocks that T tokens can touch
     const int64_t ctas = (int64_t)p.B * blocks;
-    const int groups = std::max(Gm::kMinHeads, std::min(Gm::kHeads, p.Hkv));
+    const int heads = std::min(Gm::kHeads, p.Hkv), groups = (heads + Gm::kMinHeads - 1) / Gm::kMinHeads * Gm::kMinHeads;
     // a CTA computes its block's sines once for all its heads: heads are cut only where CTAs are few
     const int rounds = (p.Hkv + groups - 1) / groups;
     const int want = (int)std::min<int64_t>(rounds, std::max<int64_t>(1, 4 * sm_count / ctas));
     const int per = (rounds + want - 1) / want * groups, chunks = (p.Hkv + per - 1) / per;
-    const size_t smem = Gm::smem(groups, p.rope_mode);
+    const size_t smem = Gm::smem(groups, p.rope_mode, p.k_norm_w != nullptr);
     auto kern = p.k_norm_w ? kv4_store_kernel<D, T, true> : kv4_store_kernel<D, T, false>;
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);

@@ -90,20 +90,6 @@ struct Cfg {
     static_assert(kSmem <= 227 * 1024, "shared memory budget");
 };
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-                 "l"(src), "r"(bytes), "r"(bar)
-                 : "memory");
-}
-// Bounded wait; false after kWaitNs.
-__device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity) {
-    if (mbar_test(bar, parity)) return true;
-    const uint64_t t0 = global_ns();
-    for (uint32_t i = 1;; ++i) {
-        if (mbar_test(bar, parity)) return true;
-        if ((i & 255u) == 0 && global_ns() - t0 > kWaitNs) return false;
-    }
-}
 __device__ __forceinline__ uint32_t ld32(const unsigned char* a) { return *reinterpret_cast<const uint32_t*>(a); }
 __device__ __forceinline__ uint2 ld64(const unsigned char* a) { return *reinterpret_cast<const uint2*>(a); }
 // n consecutive params (4 bytes each), 8- or 16-byte aligned as the layout gives them
@@ -929,15 +915,19 @@ LaunchInfo launch_info(int device) {
 //    sequences of 4 k keys: 34 pipelined, 31 us not).
 constexpr int kPipelineBlocks = 128;
 
+bool few_blocks(const Kv4Params& p) {
+    const int64_t keys = std::min<int64_t>(p.window > 0 ? p.window + p.T : INT32_MAX, (int64_t)p.max_pages * p.page_size);
+    const int64_t units = (int64_t)p.B * p.Hkv * ((p.T * p.G + 7) / 8);
+    return units * (keys / kKv4Block) <= (int64_t)kPipelineBlocks * 2 * 148;
+}
+
+// few: few_blocks of the whole call, of which p may be a part.
 template <typename F>
-cudaError_t dispatch(const Kv4Params& p, F&& f) {
+cudaError_t dispatch(const Kv4Params& p, bool few, F&& f) {
     const int rows = p.T * p.G;
     auto by_rows = [&](auto d) {
         constexpr int D = decltype(d)::value;
         if constexpr (D == 256) {
-            const int64_t keys = std::min<int64_t>(p.window > 0 ? p.window + p.T : INT32_MAX, (int64_t)p.max_pages * p.page_size);
-            const int64_t units = (int64_t)p.B * p.Hkv * ((rows + 7) / 8);
-            const bool few = units * (keys / kKv4Block) <= (int64_t)kPipelineBlocks * 2 * 148;
             if (p.act_dtype == kF16) {
                 if (rows > 4) return f(Cfg<D, 2, 2, true>{});
                 return few ? f(Cfg<D, 1, 1, true>{}) : f(Cfg<D, 1, 1, false>{});
@@ -969,7 +959,8 @@ size_t kv4_sums_bytes(const Kv4Params& p) { return (size_t)q_tiles_of(p) * p.Hkv
 
 Kv4Split kv4_attn_split(const Kv4Params& p, int device) {
     Kv4Split split{};
-    dispatch(p, [&](auto cfg) {
+    split.few = few_blocks(p);
+    dispatch(p, split.few, [&](auto cfg) {
         using C = decltype(cfg);
         split.n_cta = launch_info<C>(device).grid;
         split.per_seq = p.Hkv * ((p.T * p.G + C::kRows - 1) / C::kRows);
@@ -982,7 +973,7 @@ Kv4Split kv4_attn_split(const Kv4Params& p, int device) {
 }
 
 cudaError_t launch_kv4_attn(const Kv4Params& p, int device, cudaStream_t stream) {
-    return dispatch(p, [&](auto cfg) {
+    return dispatch(p, p.split.few, [&](auto cfg) {
         using C = decltype(cfg);
         const LaunchInfo li = launch_info<C>(device);
         if (li.grid <= 0) return cudaErrorInvalidConfiguration;

@@ -85,20 +85,25 @@ __device__ __forceinline__ void stage_query(const Kv4Params& p, __half* out, int
                 y[i] = (float)((double)__fmul_rn(y[i], rms) * (1.0 + (double)p.q_norm_w[D / 2 + 8 * k + i]));
             }
         }
-        if (p.rope_mode != 0) {
+        if (p.rope_mode == 2) {
+            const double2* at = static_cast<const double2*>(cs) + row * (D / 2) + k;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int at = row * (D / 2) + 8 * k + i;
                 const float a = x[i], e = y[i];
-                if (p.rope_mode == 2) {
-                    const double2 c = static_cast<const double2*>(cs)[at];
-                    x[i] = (float)((double)a * c.x - (double)e * c.y);
-                    y[i] = (float)((double)e * c.x + (double)a * c.y);
-                } else {
-                    const float2 c = static_cast<const float2*>(cs)[at];
-                    x[i] = a * c.x - e * c.y;
-                    y[i] = a * c.y + e * c.x;
-                }
+                const double2 c = at[i * kHalf];
+                x[i] = (float)((double)a * c.x - (double)e * c.y);
+                y[i] = (float)((double)e * c.x + (double)a * c.y);
+            }
+        } else if (p.rope_mode != 0) {
+            const float4* at = static_cast<const float4*>(cs) + row * (D / 4) + k;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                const float4 c = at[i / 2 * kHalf];
+                const float a0 = x[i], e0 = y[i], a1 = x[i + 1], e1 = y[i + 1];
+                x[i] = a0 * c.x - e0 * c.z;
+                y[i] = a0 * c.z + e0 * c.x;
+                x[i + 1] = a1 * c.y - e1 * c.w;
+                y[i + 1] = a1 * c.w + e1 * c.y;
             }
         }
         if (live) {

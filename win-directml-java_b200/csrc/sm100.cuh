@@ -69,11 +69,27 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
         }
     }
 }
+// Bounded wait without an abort flag; false after kWaitNs.
+__device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity) {
+    if (mbar_test(bar, parity)) return true;
+    const uint64_t t0 = global_ns();
+    for (uint32_t i = 1;; ++i) {
+        if (mbar_test(bar, parity)) return true;
+        if ((i & 255u) == 0 && global_ns() - t0 > kWaitNs) return false;
+    }
+}
 // Bounded wait on the exit path (no abort short-cut).
 __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
     const uint64_t t0 = global_ns();
     while (!mbar_test(bar, parity))
         if (global_ns() - t0 > kWaitNs) return;
+}
+
+// bytes (a multiple of 16) between 16-byte boundaries
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
 }
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2,
