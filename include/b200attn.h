@@ -147,7 +147,9 @@ B2A_API int b2a_reserve_decode(b2a_context* ctx, int max_batch, int num_q_heads,
  *   B2A_ETIMEOUT  a bounded device-side wait ran out and the launch aborted
  *                 (its outputs are undefined); takes precedence over the others;
  *   B2A_EDEVICE   a device-side argument check failed (a ctx_lens entry outside
- *                 [0, max_seq), a bf16 input beyond the fp16 operand range);
+ *                 [0, max_seq), a bf16 input beyond the fp16 operand range; of the
+ *                 paged cache: lengths that do not fit the page table, an entry that
+ *                 names no page, a value group that is held as NaN);
  *   B2A_OK        nothing was flagged.
  * The compute calls are asynchronous, as CUDA launches are; a binding that
  * mirrors the reference's synchronous dispatch (DirectMlAttentionKernel.dispatch
@@ -401,8 +403,13 @@ B2A_API int b2a_kv4_append(b2a_context* ctx, const b2a_kv4_cache* cache, int act
  * those before it must have been appended.
  *   q : [B][T] token rows of [Hq][D], q_token_stride elements apart (0: Hq * D); optional norm
  *       (q_norm_w) and RoPE at p, as b2a_decode.   o : [B,T,Hq,D], act_dtype.
- * Rows t >= new_lens[b] give zeros.  Softmax and sums are held in fp32; q and the probabilities
- * are rounded once to 11 significant bits for the tensor cores. */
+ * Rows t >= new_lens[b] give zeros.  A row that sees a position whose key is held as NaN is NaN; where
+ * a value group is, its 32 channels are; positions that a row does not see never reach it.
+ * Softmax statistics and sums are held in fp32.  fp16 calls carry q and the probabilities as two fp16
+ * words; bf16 calls round both once to fp16's 11 significant bits (what bf16 results keep is 8).
+ * bf16 calls of 64 and more tokens turn the cache's rows into fp16 (s * c + z rounded once to 11 bits;
+ * workspace: the rows of as many sequences as fit 1 GiB, one at least): a rotated q beyond the fp16
+ * range raises the device status there.  B * T is at most 2^24. */
 B2A_API int b2a_kv4_attention(b2a_context* ctx, const b2a_kv4_cache* cache, int act_dtype, const void* q,
                               int64_t q_token_stride, const int32_t* ctx_lens, const int32_t* new_lens, int B, int T,
                               int Hq, float scale, int rope_mode, double rope_theta, int window,
@@ -438,7 +445,8 @@ typedef struct b2a_page_pool {
 
 /* Row i of the table becomes what row parents[i] (DEVICE int32 [n_seq]) was; -1 empties it.  A beam
  * step, n samples of one prompt, moving rows and retiring sequences are all this.  Pages are shared,
- * not copied; counts follow. */
+ * not copied; counts follow.  A parent outside [-1, n_seq) raises the device status and leaves its
+ * row.  n_seq is at most 56 * 1024. */
 B2A_API int b2a_pages_fork(b2a_context* ctx, const b2a_page_pool* pool, const int32_t* parents, void* stream);
 
 /* Slots that hold no position of [keep_from[row], keep_to[row]) give their page back (DEVICE int32

@@ -7,7 +7,8 @@
 // (query heads, key heads, value heads), a warp one row at a time, and computes the token's sines and
 // cosines once. It is all latency -- lengths, rows, page table, then a chain of double-precision
 // steps -- so every read is requested before the first one is waited for, and the attention kernel
-// is launched behind it early, to be resident when it ends.
+// is launched behind it early, to be resident when it ends.  Measured: 3.8 us for one sequence of a
+// small model, 5.1 us for 64, 8.7 us for 256 sequences of head dim 256 with norms and double rotation.
 // kv4_store_kernel: prompts. A CTA takes one block of 16 positions and walks kv heads; a thread holds
 // 8 channels of four rows (16-byte loads), the block is assembled in shared memory and stored whole.
 #include <algorithm>

@@ -12,6 +12,10 @@
 // provided the instructions per key stay few.  Per 16 keys and 32 channels a warp spends twenty
 // integer instructions on 2 x 512 codes (two masks and a shift per word pair; the block layout is
 // the MMA's own operand order) and four MMAs of 16 keys (K) or 16 channels (V^T) x 8 columns.
+// Measured at head dim 256, 256 sequences of 16.9 k keys (1.38 GB of codes): 272 us, 5.1 TB/s, where
+// copying the rings alone takes 215 us; some 620 warp instructions a block keep 60% of the issue slots
+// and 54% of the integer pipe busy, and registers allow three warps a scheduler.  Short work is
+// latency: 64 sequences of 4.4 k keys, head dim 64 (45 MB), take 31 us, of them 13 in the loop.
 //
 // Precision.  q and P are f16 operands.  One rounding of each is far below a bf16 result's own; for
 // fp16 results each is carried as two words (hi + lo): with at most four query rows the lo words take

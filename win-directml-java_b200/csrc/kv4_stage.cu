@@ -2,10 +2,14 @@
 // cache (kv4.cuh): q rotated and converted to fp16, the visible cache rows as fp16.
 //
 // A chunk reads every key of its sequence once per 256 of its tokens and head, so the codes are turned
-// into fp16 rows once, by one launch that is bound by HBM (0.625 D bytes in, 2 D out per row), and the
+// into fp16 rows once, by one launch (0.625 D bytes in, 2 D out per row), and the
 // tensor-core kernel streams those through TMA; per key and head that is far less than the chunk's
-// own multiplications.  A value beyond fp16 becomes infinite and raises status bit 2, as bf16 inputs
-// of the other entry points do.
+// own multiplications.  Measured for 2 x 1000 tokens of 32 heads of 128 on 2 x 3000 cached ones (8 kv
+// heads, 87 MB moved): 24 us alone, 18 us of it behind the append beside which the queries are staged,
+// before an attention of 102 us; half of its issue slots are busy, its warps wait for loads.  Turning
+// the blocks before the appended ones while the append runs gained nothing (the GPU is full).
+// A value beyond fp16 becomes infinite and raises status bit 2, as bf16 inputs of the other entry
+// points do.
 #include <type_traits>
 
 #include "kv4.cuh"
