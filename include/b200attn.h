@@ -406,7 +406,8 @@ B2A_API int b2a_kv4_append(b2a_context* ctx, const b2a_kv4_cache* cache, int act
  * Rows t >= new_lens[b] give zeros.  A row that sees a position whose key is held as NaN is NaN; where
  * a value group is, its 32 channels are; positions that a row does not see never reach it.
  * Softmax statistics and sums are held in fp32.  fp16 calls carry q and the probabilities as two fp16
- * words; bf16 calls round both once to fp16's 11 significant bits (what bf16 results keep is 8).
+ * words; bf16 calls round both once to fp16's 11 significant bits (what bf16 results keep is 8), the
+ * probabilities times s, so that an output's error is 2^-12 of its group's range rather than its own.
  * bf16 calls of 64 and more tokens turn the cache's rows into fp16 (s * c + z rounded once to 11 bits;
  * workspace: the rows of as many sequences as fit 1 GiB, one at least): a rotated q beyond the fp16
  * range raises the device status there.  B * T is at most 2^24. */

@@ -20,7 +20,9 @@
 // Precision.  q and P are f16 operands.  One rounding of each is far below a bf16 result's own; for
 // fp16 results each is carried as two words (hi + lo): with at most four query rows the lo words take
 // the columns 4..7 of the same MMAs (kSplit 1, nothing extra to multiply), else a second column tile
-// (kSplit 2).  The rounding of P s is corrected exactly: lo = fma(P, s, -hi) + P_lo s.
+// (kSplit 2).  The rounding of P s is corrected exactly: lo = fma(P, s, -hi) + P_lo s.  With one word an
+// output errs by up to 2^-12 of what it is made of, s c and z, not of their sum: a value far below
+// its group's range has the absolute error of the group's large ones.
 //
 // The tensor cores add to their fp32 accumulators by truncation, a loss towards zero that grows with
 // the number of blocks, and the codes are all positive.  Every second block therefore enters as
