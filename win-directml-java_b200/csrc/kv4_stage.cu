@@ -5,8 +5,8 @@
 // into fp16 rows once, by one launch (0.625 D bytes in, 2 D out per row), and the
 // tensor-core kernel streams those through TMA; per key and head that is far less than the chunk's
 // own multiplications.  Measured for 2 x 1000 tokens of 32 heads of 128 on 2 x 3000 cached ones (8 kv
-// heads, 87 MB moved): 24 us alone, 18 us of it behind the append beside which the queries are staged,
-// before an attention of 102 us; half of its issue slots are busy, its warps wait for loads.  Turning
+// heads, 87 MB moved): 27 us, of them 16 behind the append beside which the queries are staged,
+// before an attention of 102 us; its warps wait for loads, half of the issue slots are idle.  Turning
 // the blocks before the appended ones while the append runs gained nothing (the GPU is full).
 // A value beyond fp16 becomes infinite and raises status bit 2, as bf16 inputs of the other entry
 // points do.
@@ -26,9 +26,9 @@ __device__ __forceinline__ int first_seen(const Kv4Params& p, int L) {
 
 // ---------------------------------------------------------------- q
 // A block takes 16 tokens of a sequence and kStageHeads heads, two at a time; a thread holds channels
-// 8 k .. + 7 and their partners D / 2 further.  Few heads to a block: its time is the latency of its
-// loads one after another, not the sines that it computes again.
-constexpr int kStageHeads = 4;
+// 8 k .. + 7 and their partners D / 2 further.  Its sines serve eight heads (32 heads of 128, 2 x
+// 1000 tokens: with 2, 4, 8 and 16 the launch takes 31.6, 28.8, 27.5 and 27.7 us).
+constexpr int kStageHeads = 8;
 template <int D, typename T>
 __device__ __forceinline__ void stage_query(const Kv4Params& p, __half* out, int block, int blocks, unsigned char* smem) {
     constexpr int kHalf = D / 16, kThreads = 2 * D;  // chunk pairs of a row; 2 heads x 16 tokens x kHalf threads
@@ -122,10 +122,21 @@ __device__ __forceinline__ void stage_query(const Kv4Params& p, __half* out, int
 }
 
 // ---------------------------------------------------------------- cache rows
+__device__ __forceinline__ void quad_transpose(uint32_t (&w)[4], int t) {  // lane t of four: w[c] of lane c's w[t]
+#pragma unroll
+    for (int bit = 1; bit <= 2; bit <<= 1)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int lo = bit == 1 ? 2 * i : i;
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, t & bit ? w[lo] : w[lo + bit], bit);
+            if (t & bit) w[lo] = got;
+            else w[lo + bit] = got;
+        }
+}
 // One warp turns one group (32 channels) of a block of 16 positions into fp16 rows.  A lane's two code
 // words hold, as the MMA wants them, channel pairs of keys g and g + 8 (K) or key pairs of channels
 // (V^T); the latter are transposed 8 x 8 at a time.  s c + z is one f16 FMA on the exact code: rounded
-// once.
+// once.  (Rows written 4 bytes a lane, without the exchange below: 2 us more of 29.)
 template <int D>
 __device__ __forceinline__ void stage_group(const Kv4Params& p, const uint8_t* src, int y, int pos, int first, int end,
                                             __half* k_row0, __half* v_row0, int64_t row_stride, int* nan_flag,
@@ -175,19 +186,21 @@ __device__ __forceinline__ void stage_group(const Kv4Params& p, const uint8_t* s
             nan |= seen(2 * t + 1 + 8 * r);
             vs &= 0xffffu, vz &= 0xffffu;
         }
-        const int64_t at = (int64_t)(g + 8 * r) * row_stride + 32 * y + 2 * t;
+        uint32_t k[4], v[4];  // channels 8 c + 2 t, + 1
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                uint32_t k = value(code[0][x] >> (8 * r + 4 * j), ks, kz);
-                uint32_t v = movmatrix_trans(value(code[1][x] >> (8 * r + 4 * j), vs, vz));
-                if (!row_seen) k = v = 0;
-                top = __hmax2(top, __hmax2(__habs2(*reinterpret_cast<const __half2*>(&k)),
-                                           __habs2(*reinterpret_cast<const __half2*>(&v))));
-                *reinterpret_cast<uint32_t*>(k_row0 + at + 16 * x + 8 * j) = k;
-                *reinterpret_cast<uint32_t*>(v_row0 + at + 16 * x + 8 * j) = v;
-            }
+        for (int c = 0; c < 4; ++c) {
+            k[c] = value(code[0][c >> 1] >> (8 * r + 4 * (c & 1)), ks, kz);
+            v[c] = movmatrix_trans(value(code[1][c >> 1] >> (8 * r + 4 * (c & 1)), vs, vz));
+            if (!row_seen) k[c] = v[c] = 0;
+            top = __hmax2(top, __hmax2(__habs2(*reinterpret_cast<const __half2*>(&k[c])),
+                                       __habs2(*reinterpret_cast<const __half2*>(&v[c]))));
+        }
+        // the row's four lanes exchange, so that each writes 16 bytes: channels 8 t .. + 7
+        quad_transpose(k, t);
+        quad_transpose(v, t);
+        const int64_t at = (int64_t)(g + 8 * r) * row_stride + 32 * y + 8 * t;
+        *reinterpret_cast<uint4*>(k_row0 + at) = make_uint4(k[0], k[1], k[2], k[3]);
+        *reinterpret_cast<uint4*>(v_row0 + at) = make_uint4(v[0], v[1], v[2], v[3]);
     }
     const bool big = __hisinf(__low2half(top)) || __hisinf(__high2half(top));
     if (__any_sync(0xffffffffu, big) && lane == 0) atomicOr(p.status, 4);
