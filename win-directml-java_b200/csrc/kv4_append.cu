@@ -422,8 +422,9 @@ struct StoreGeo {
     __host__ __device__ static size_t part_at(int heads, int rope_mode) {
         return cs_at(heads) + (rope_mode == 0 ? 0 : 16 * (D / 2) * (rope_mode == 2 ? sizeof(double2) : sizeof(float2)));
     }
+    // norms: 1 + weight as doubles, sums of squares [head][row][chunk], the rows' factors
     static size_t smem(int heads, int rope_mode, bool norm) {
-        return part_at(heads, rope_mode) + (norm ? heads * 16 * kChunks * 8 : 0);
+        return part_at(heads, rope_mode) + (norm ? D * 8 + heads * 16 * (kChunks * 8 + 4) : 0);
     }
 };
 
@@ -450,7 +451,9 @@ __global__ void __launch_bounds__(StoreGeo<D>::kMaxThreads, StoreGeo<D>::kCtas)
     const int pitch = Gm::pitch(groups);
     uint8_t* const stage = smem + Gm::stage_at(groups) + group * 20 * D;
     void* const cs = smem + Gm::cs_at(groups);  // [16][D / 2] (cos, sin)
-    double* const part = reinterpret_cast<double*>(smem + Gm::part_at(groups, p.rope_mode)) + group * 16 * kChunks;
+    double* const weight = reinterpret_cast<double*>(smem + Gm::part_at(groups, p.rope_mode));
+    double* const part = weight + D + group * 16 * kChunks;
+    float* const factor = reinterpret_cast<float*>(weight + D + groups * 16 * kChunks) + group * 16;
     const uint32_t bar = smem_u32(full);
     const int chunk = blockIdx.x % chunks;
     const int64_t bb = blockIdx.x / chunks;
@@ -496,6 +499,8 @@ __global__ void __launch_bounds__(StoreGeo<D>::kMaxThreads, StoreGeo<D>::kCtas)
         request(1, h_begin);
     }
     if (p.rope_mode != 0) kv4_block_angles<D>(p, blk * kKv4Block, cs, tid);
+    if constexpr (kNorm)
+        for (int i = tid; i < D; i += blockDim.x) weight[i] = __dadd_rn(1.0, (double)__ldg(p.k_norm_w + i));
     const bool upper = k >= kChunks / 2;
     const int k2 = upper ? k - kChunks / 2 : k + kChunks / 2, k_low = upper ? k2 : k;
     const int j = k & 1, x16 = (k >> 1) & 1, y = k >> 2;
@@ -527,6 +532,12 @@ __global__ void __launch_bounds__(StoreGeo<D>::kMaxThreads, StoreGeo<D>::kCtas)
                     part[row_of(i) * kChunks + k] = ss;
                 }
                 __syncthreads();
+                if (in_group < 16) {  // a row's factor, once
+                    double ss = 0.0;
+                    for (int c = 0; c < kChunks; ++c) ss += part[in_group * kChunks + c];
+                    factor[in_group] = (float)(1.0 / sqrt(__dadd_rn(ss / (double)D, (double)p.norm_eps)));
+                }
+                __syncthreads();
             }
             // ---- the rows' values, each thread's minima and maxima: NaN reaches `hi`, infinities both
             float2 x[4][4];
@@ -537,22 +548,23 @@ __global__ void __launch_bounds__(StoreGeo<D>::kMaxThreads, StoreGeo<D>::kCtas)
                 float v[8];
                 unpack8(exists(i) ? *reinterpret_cast<const uint4*>(row_at(i)) : make_uint4(0, 0, 0, 0), v, T{});
                 if (!is_v) {
-                    float rms = 0.f;
+                    [[maybe_unused]] const float rms = kNorm ? factor[row] : 0.f;
                     if constexpr (kNorm) {
-                        double ss = 0.0;
-                        for (int c = 0; c < kChunks; ++c) ss += part[row * kChunks + c];
-                        rms = (float)(1.0 / sqrt(__dadd_rn(ss / (double)D, (double)p.norm_eps)));
 #pragma unroll
-                        for (int c = 0; c < 8; ++c)
-                            v[c] = (float)__dmul_rn((double)__fmul_rn(v[c], rms), __dadd_rn(1.0, (double)__ldg(p.k_norm_w + 8 * k + c)));
+                        for (int c = 0; c < 8; ++c) v[c] = (float)__dmul_rn((double)__fmul_rn(v[c], rms), weight[8 * k + c]);
                     }
                     if (p.rope_mode != 0) {
                         float z[8];
-                        unpack8(exists(i) ? *reinterpret_cast<const uint4*>(row_at(i) + 16 * (k2 - k)) : make_uint4(0, 0, 0, 0), z, T{});
-                        if constexpr (kNorm) {
+                        if constexpr (kNorm && D != 96) {  // the partner is a lane of this warp
 #pragma unroll
-                            for (int c = 0; c < 8; ++c)
-                                z[c] = (float)__dmul_rn((double)__fmul_rn(z[c], rms), __dadd_rn(1.0, (double)__ldg(p.k_norm_w + 8 * k2 + c)));
+                            for (int c = 0; c < 8; ++c) z[c] = __shfl_xor_sync(0xffffffffu, v[c], kChunks / 2);
+                        } else {
+                            unpack8(exists(i) ? *reinterpret_cast<const uint4*>(row_at(i) + 16 * (k2 - k)) : make_uint4(0, 0, 0, 0), z, T{});
+                            if constexpr (kNorm) {
+#pragma unroll
+                                for (int c = 0; c < 8; ++c)
+                                    z[c] = (float)__dmul_rn((double)__fmul_rn(z[c], rms), weight[8 * k2 + c]);
+                            }
                         }
                         if (p.rope_mode == 2) {
                             const double2* a = static_cast<const double2*>(cs) + row * (D / 2) + k_low;
