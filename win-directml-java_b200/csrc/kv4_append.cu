@@ -414,7 +414,9 @@ struct StoreGeo {
     static constexpr int kHeads = D <= 64 ? 8 : (D <= 128 ? 4 : 2);  // heads of a CTA side by side, at most
     static constexpr int kMinHeads = D == 96 ? 2 : 1;         // whole warps
     static constexpr int kMaxThreads = kHeads * kPerHead;
-    static constexpr int kCtas = D == 96 ? 5 : 3;  // per SM: 64 registers a thread at head dim 96, else 80
+    // per SM: 64 (with norms 80) registers a thread at head dim 96, where 4 CTAs take 220 us instead of 193
+    // (with norms 303 instead of 347); else 80
+    static constexpr int ctas(bool norm) { return D == 96 ? (norm ? 4 : 5) : 3; }
     // an operand's 16 rows of the CTA's heads; the pad keeps rows two apart on other banks
     __host__ __device__ static constexpr int pitch(int heads) { return heads * D * 2 + (D == 96 ? 32 : 0); }
     __host__ __device__ static size_t stage_at(int heads) { return 2 * 16 * (size_t)pitch(heads); }
@@ -441,7 +443,7 @@ struct StoreGeo {
 // tokens of 16 heads of 128, fp16 (bf16 without norms: 128 us, with held rows), take 170 us, and 201 us with
 // the double-precision rotation; the rows' factors computed by every thread: 214 and 252 us.
 template <int D, typename T, bool kNorm>
-__global__ void __launch_bounds__(StoreGeo<D>::kMaxThreads, StoreGeo<D>::kCtas)
+__global__ void __launch_bounds__(StoreGeo<D>::kMaxThreads, StoreGeo<D>::ctas(kNorm))
     kv4_store_kernel(const __grid_constant__ Kv4Params p, int blocks, int chunks, int per) {
     using Gm = StoreGeo<D>;
     constexpr int kChunks = Gm::kChunks, kGroups = D / 32;
