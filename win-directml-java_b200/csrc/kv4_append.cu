@@ -621,9 +621,10 @@ __global__ void __launch_bounds__(StoreGeo<D>::kMaxThreads, StoreGeo<D>::ctas(kN
                 const float sf = __half2float(s), zf = __half2float(z);
                 const bool fine = isfinite(sf) && isfinite(zf);
                 inv = sf > 0.f && fine ? __fdiv_rn(1.0f, sf) : 0.f;
-                // codes leave 0 .. 15 only where the group's ends do (z and s are rounded: rarely); a group
-                // that is not finite counts as such, and its codes become 0 with the others'
-                outside = !(__fmul_rn(__fsub_rn(low, zf), inv) >= -0.5f && __fmul_rn(__fsub_rn(high, zf), inv) <= 15.5f);
+                // codes leave 0 .. 15 only where the group's ends do (z and s are rounded: rarely; -0.5 goes to
+                // the even 0, but 15.5 to the even 16); a group that is not finite counts as such, and its codes
+                // become 0 with the others'
+                outside = !(__fmul_rn(__fsub_rn(low, zf), inv) >= -0.5f && __fmul_rn(__fsub_rn(high, zf), inv) < 15.5f);
                 if (!fine) {
                     s = z = __ushort_as_half(0x7fff);
                     if (exists(k & 3)) atomicOr(p.status, 32);
