@@ -452,6 +452,8 @@ def _token_rows(t, name, shape):
     if sd != 1 or (H > 1 and sh != D) or (T > 1 and B > 1 and sb != T * st):
         raise ValueError(f"{name} must hold its tokens at one distance and its heads side by side, "
                          f"got strides {t.stride()}")
+    if step < H * D:  # broadcast or overlapping rows; the library takes a distance of 0 as H * D
+        raise ValueError(f"{name} must hold its tokens at least {H * D} elements apart, got strides {t.stride()}")
     return t.data_ptr(), step
 
 
