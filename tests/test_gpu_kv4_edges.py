@@ -29,3 +29,35 @@ def test_prompt_store_clamps_a_tie_at_the_top(ctx, D, dtype):
     c.check_pages(t["pages"].cpu().numpy(), exact=True)
     np.testing.assert_array_equal(to_np(t["k_held"]), kh)
     np.testing.assert_array_equal(to_np(t["v_held"]), vh)
+
+
+@pytest.mark.parametrize("page,slots,L", [(48, 3, 100), (16, 10, 97), (16, 9, 144)])
+def test_lengths_past_the_table_but_inside_its_last_tile(ctx, page, slots, L):
+    """A chunk's rows are staged for whole tiles of 128 keys; lengths between the table's room and the tile's end
+    do not fit all the same: NaN, nothing stored, the other sequences as ever."""
+    import torch
+    import b200attn
+    c = Case(ctx=[20, 60, 50], T=70, Hq=4, Hkv=2, D=64, page=page, dtype=oracle.BF16, seed=page)
+    c.table = np.pad(c.table, ((0, 0), (0, max(0, slots - c.table.shape[1]))), constant_values=-1)[:, :slots]
+    room = slots * page
+    assert room < L + c.T <= -(-room // 128) * 128
+    t = c.device()
+    b200attn.kv4_decode(ctx, t["q"], t["k"], t["v"], t["pages"], t["table"], t["ctx"], t["o"], c.scale, **c.more())
+    ctx.check_device_status()
+    o, tol, _, _ = c.expect()
+    c.check_out(to_np(t["o"]), o, tol)
+    t["ctx"][1] = L
+    before = t["pages"].clone()
+
+    def check():
+        with pytest.raises(b200attn.B200RuntimeException, match="ctx_lens"):
+            ctx.check_device_status()
+        assert bool(torch.isnan(t["o"][1]).all())
+        c.check_out(to_np(t["o"])[[0, 2]], o[[0, 2]], tol[[0, 2]])
+        assert torch.equal(t["pages"], before)
+
+    b200attn.kv4_decode(ctx, t["q"], t["k"], t["v"], t["pages"], t["table"], t["ctx"], t["o"], c.scale, **c.more())
+    check()
+    t["o"].zero_()
+    b200attn.kv4_attention(ctx, t["q"], t["pages"], t["table"], t["ctx"], t["o"], c.scale, **c.more())
+    check()

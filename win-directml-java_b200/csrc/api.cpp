@@ -1279,6 +1279,7 @@ int run_kv4_chunk(b2a_context* ctx, const Kv4Params& p, cudaStream_t stream) {
     a.out_dtype = p.act_dtype;
     a.S = p.T;
     a.Sk = Sk;
+    a.room = p.max_pages * p.page_size;  // Sk is whole tiles
     a.Hq = p.Hq;
     a.Hkv = p.Hkv;
     a.D = p.D;

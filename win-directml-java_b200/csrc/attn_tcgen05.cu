@@ -106,10 +106,10 @@ struct TcParams {
     // in-kernel operand conversion by warps 10 and 11 (kXformQ / K / V): the staged bf16 tile
     // becomes the fp16 operand in place
     int xform;
-    // kChunk: position of query row 0 and number of rows per batch (q_len NULL: S)
+    // kChunk: position of query row 0 and number of rows per batch (q_len NULL: S); positions end at room
     const int32_t* q_pos;
     const int32_t* q_len;
-    int Sk;
+    int room;
 };
 constexpr int kXformQ = 1, kXformK = 2, kXformV = 4;
 
@@ -263,8 +263,9 @@ struct ItemGeo {
     int rows;         // query rows that exist
 };
 
-// A chunk's item (kChunk): causal at positions shift + row; empty (n_max 0) past the rows that exist.
-__device__ __forceinline__ ItemGeo chunk_geo(int w, int n_pairs, int tiles, int Hq, int S, int Sk, int window,
+// A chunk's item (kChunk): causal at positions shift + row; empty (n_max 0) past the rows that exist, and
+// where the lengths leave [0, room): such a sequence has no staged rows.
+__device__ __forceinline__ ItemGeo chunk_geo(int w, int n_pairs, int tiles, int Hq, int S, int room, int window,
                                              const int32_t* q_pos, const int32_t* q_len) {
     ItemGeo g;
     const int x = w % n_pairs, rest = w / n_pairs;
@@ -272,7 +273,7 @@ __device__ __forceinline__ ItemGeo chunk_geo(int w, int n_pairs, int tiles, int 
     g.b = g.b1 = rest / Hq;
     g.shift = q_pos[g.b];
     g.rows = q_len != nullptr ? q_len[g.b] : S;
-    if (g.shift < 0 || g.rows < 0 || g.rows > S || (long long)g.shift + g.rows > Sk) g.shift = g.rows = 0;
+    if (g.shift < 0 || g.rows < 0 || g.rows > S || (long long)g.shift + g.rows > room) g.shift = g.rows = 0;
     g.q0a = (n_pairs - 1 - x) * tiles * kBM;
     g.q0b = tiles == 2 ? g.q0a + kBM : S;
     const int end = g.shift + g.rows;
@@ -526,10 +527,10 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     if (k >= 2 && !mbar_wait(bItemEmpty(slot), ((k >> 1) - 1) & 1, abort_flag, status)) break;
                     w = atomicAdd(sched, 1);
                     if constexpr (kChunk) {
-                        it = chunk_geo(w < n_items ? w : 0, n_pairs, Gm::kTiles, Hq, S, p.Sk, window, p.q_pos, p.q_len);
+                        it = chunk_geo(w < n_items ? w : 0, n_pairs, Gm::kTiles, Hq, S, p.room, window, p.q_pos, p.q_len);
                         while (w < n_items && it.n_max == 0) {  // rows that do not exist
                             w = atomicAdd(sched, 1);
-                            it = chunk_geo(w < n_items ? w : 0, n_pairs, Gm::kTiles, Hq, S, p.Sk, window, p.q_pos,
+                            it = chunk_geo(w < n_items ? w : 0, n_pairs, Gm::kTiles, Hq, S, p.room, window, p.q_pos,
                                            p.q_len);
                         }
                     } else {
@@ -1102,7 +1103,7 @@ cudaError_t launch_impl(const AttnParams& a, int* status, cudaStream_t stream, b
     p.xform = a.xform;
     p.q_pos = a.q_pos;
     p.q_len = a.q_len;
-    p.Sk = Sk;
+    p.room = a.room;
     int dev = 0, sms = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) !=
                                                   cudaSuccess || sms <= 0)

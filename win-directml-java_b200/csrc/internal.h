@@ -106,10 +106,11 @@ struct AttnParams {
     // tile to fp16 in shared memory; 0 = fp16 operands as given.
     int xform;
     // tcgen05 kernel only, a chunk of a sequence: device [B] position of query row 0 among Sk keys
-    // that begin at position 0, and number of query rows (NULL: S); causal.  NULL q_pos: none of this.
+    // that begin at position 0, and number of query rows (NULL: S); causal.  Sequences whose rows do not
+    // end by position room (at most Sk) get no outputs.  NULL q_pos: none of this.
     const int32_t* q_pos;
     const int32_t* q_len;
-    int Sk;
+    int Sk, room;
 };
 
 // Key split of the generic kernel: partial slots and per-query-block counters (zero
