@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 
+import kv4_helpers as kv
 import oracle
 from helpers import to_np
 from test_gpu_kv4 import Case
@@ -61,3 +62,90 @@ def test_lengths_past_the_table_but_inside_its_last_tile(ctx, page, slots, L):
     t["o"].zero_()
     b200attn.kv4_attention(ctx, t["q"], t["pages"], t["table"], t["ctx"], t["o"], c.scale, **c.more())
     check()
+
+
+def _hold_nan(c, b, pos, which, head=0, group=1):
+    """Position pos of sequence b holds NaN in one key ("k") or value group."""
+    page, at = c.table[b, pos // c.page], pos % c.page
+    parts = kv.unpack(c.pages[page], c.D)
+    parts[1 if which == "k" else 3][head, at, group] = np.nan
+    c.pages[page] = kv.pack(*parts)
+
+
+def _capture(run):
+    """A CUDA graph of run(), which has been called before with these sizes."""
+    import torch
+    torch.cuda.synchronize()
+    g, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s), torch.cuda.graph(g, stream=s):
+        run()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    return g
+
+
+def test_replayed_chunks_mark_the_rows_that_see_nan(ctx):
+    """Two chunk calls in one graph (two layers).  A value group held as NaN in the second one's cache, then in the
+    first one's, then in none: each replay marks what this replay reads."""
+    import torch
+    import b200attn
+    layers = [Case(ctx=[40, 90], T=64, Hq=4, Hkv=2, D=128, dtype=oracle.BF16, rope=None, seed=s) for s in (31, 37)]
+    dev = [c.device() for c in layers]
+
+    def run():
+        for c, t in zip(layers, dev):
+            b200attn.kv4_decode(ctx, t["q"], t["k"], t["v"], t["pages"], t["table"], t["ctx"], t["o"], c.scale, **c.more())
+
+    run()
+    clean = [t["pages"].clone() for t in dev]
+    g = _capture(run)
+    want = [t["o"].clone() for t in dev]
+    for bad in (1, 0, None, 0, 1, None):
+        for i, (c, t) in enumerate(zip(layers, dev)):
+            t["o"].zero_()
+            t["pages"].copy_(clean[i])
+            if i == bad:
+                raw = c.pages.copy()
+                _hold_nan(c, 0, 17, "v")
+                page = int(c.table[0, 17 // c.page])
+                t["pages"][page] = torch.from_numpy(c.pages[page]).cuda()
+                c.pages = raw
+        g.replay()
+        torch.cuda.synchronize()
+        for i, t in enumerate(dev):
+            nan = torch.zeros_like(t["o"], dtype=torch.bool)
+            if i == bad:
+                nan[0, :, :2, 32:64] = True  # kv head 0's queries, group 1
+            assert torch.equal(torch.isnan(t["o"]), nan), (bad, i)
+            assert torch.equal(t["o"][~nan], want[i][~nan]), (bad, i)
+    del g
+    ctx.check_device_status()
+
+
+def test_chunks_whose_staged_rows_come_in_slices(ctx):
+    """A table so wide that one sequence's staged rows fill a slice: three slices, NaN in the second alone."""
+    import torch
+    import b200attn
+    c = Case(ctx=[40, 90, 7], T=66, Hq=4, Hkv=2, D=64, page=64, dtype=oracle.BF16, rope=None, seed=29,
+             extra_slots=40000)
+    t = c.device()
+    more = dict(c.more(), new_lens=t["new"])
+    b200attn.kv4_decode(ctx, t["q"], t["k"], t["v"], t["pages"], t["table"], t["ctx"], t["o"], c.scale, **more)
+    ctx.check_device_status()
+    o, tol, _, _ = c.expect()
+    c.check_out(to_np(t["o"]), o, tol)
+    clean = t["o"].clone()
+    _hold_nan(c, 1, 50, "v")
+    page = int(c.table[1, 50 // c.page])
+    t["pages"][page] = torch.from_numpy(c.pages[page]).cuda()
+    nan = torch.zeros_like(clean, dtype=torch.bool)
+    nan[1, :, :2, 32:64] = True  # kv head 0's queries, group 1
+    for run in (lambda: b200attn.kv4_attention(ctx, t["q"], t["pages"], t["table"], t["ctx"], t["o"], c.scale, **more),
+                lambda: b200attn.kv4_decode(ctx, t["q"], t["k"], t["v"], t["pages"], t["table"], t["ctx"], t["o"],
+                                            c.scale, **more)):
+        t["o"].zero_()
+        run()
+        ctx.check_device_status()
+        assert torch.equal(torch.isnan(t["o"]), nan)
+        assert torch.equal(t["o"][~nan], clean[~nan])

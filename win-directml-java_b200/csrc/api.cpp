@@ -65,7 +65,6 @@ struct b2a_context {
     void* kv4_ws = nullptr;
     size_t kv4_ws_bytes = 0;
     size_t kv4_counter_bytes = 0;
-    int kv4_epoch = 0;  // 4-bit cache chunks so far
     // paged cache: [words between blocks][the page operations' lists]
     void* pg_ws = nullptr;
     size_t pg_ws_bytes = 0;
@@ -1253,6 +1252,7 @@ Kv4Params kv4_slice(const Kv4Params& p, int b0, int count) {
 // shorter ones, whose 128-row query tiles would stand mostly empty, and fp16 results, which carry q
 // and P as two words, take the kernel that reads the codes.
 constexpr int kKv4ChunkTokens = 64;
+static_assert(kKv4ChunkTokens >= kKv4StoreTokens, "a chunk's append clears its flag");
 constexpr size_t kKv4StageBytes = size_t(1) << 30;  // staged cache rows of one launch (one sequence at least)
 
 bool kv4_chunked(const Kv4Params& p) { return p.act_dtype == B2A_BFLOAT16 && p.T >= kKv4ChunkTokens; }
@@ -1273,7 +1273,6 @@ int run_kv4_chunk(b2a_context* ctx, const Kv4Params& p, cudaStream_t stream) {
         return kNoRoom;
     }
     char* base = static_cast<char*>(ctx->pf_ws);
-    int* nan_flag = ctx->status + kStatusNanWord;
     AttnParams a{};
     a.in_dtype = B2A_FLOAT16;
     a.out_dtype = p.act_dtype;
@@ -1303,6 +1302,7 @@ int run_kv4_chunk(b2a_context* ctx, const Kv4Params& p, cudaStream_t stream) {
     if (p.k_new) {
         Kv4Params s = p;
         s.q = nullptr;
+        s.nan_flag = ctx->status + kStatusNanWord;
         e = launch_kv4_prepare(s, ctx->sm_count, stream);
     }
     for (int b0 = 0; e == cudaSuccess && b0 < p.B; b0 += per) {
@@ -1311,16 +1311,14 @@ int run_kv4_chunk(b2a_context* ctx, const Kv4Params& p, cudaStream_t stream) {
         a.q_pos = s.ctx_lens;
         a.q_len = s.new_lens;
         a.o = s.o;
-        if (ctx->kv4_epoch == INT32_MAX) {  // start over
-            ctx->kv4_epoch = 0;
-            e = cudaMemsetAsync(nan_flag, 0, sizeof(int), stream);
-        }
-        s.epoch = ++ctx->kv4_epoch;
+        s.nan_flag = ctx->status + kStatusNanWord;
+        const bool after_append = p.k_new != nullptr && b0 == 0;  // which has cleared the flag
+        if (!after_append) e = cudaMemsetAsync(s.nan_flag, 0, sizeof(int), stream);
         if (e == cudaSuccess)
-            e = launch_kv4_stage(s, base, const_cast<void*>(a.k), const_cast<void*>(a.v), Sk, nan_flag,
-                                 p.k_new != nullptr && b0 == 0, ctx->sm_count, stream);
+            e = launch_kv4_stage(s, base, const_cast<void*>(a.k), const_cast<void*>(a.v), Sk, after_append,
+                                 ctx->sm_count, stream);
         if (e == cudaSuccess) e = launch_attn_tcgen05(a, ctx->status, stream);
-        if (e == cudaSuccess) e = launch_kv4_nan_rows(s, nan_flag, ctx->sm_count, stream);
+        if (e == cudaSuccess) e = launch_kv4_nan_rows(s, ctx->sm_count, stream);
     }
     if (e != cudaSuccess) return cuda_fail(ctx, e, "4-bit cache chunk launch");
     return B2A_OK;

@@ -134,8 +134,8 @@ cudaError_t launch_attn_f32(const AttnParams& p, cudaStream_t stream);
 // per-launch abort word (a CTA whose bounded wait ran out sets it so that the launch's other
 // CTAs stop too).  All three are zero between launches: the last CTA of each launch resets
 // them, so one timed-out launch does not abort the next ones (the sticky report stays in
-// the error flags until they are read).  Word kStatusNanWord holds the number of the last 4-bit cache
-// chunk whose keys included a value held as NaN.
+// the error flags until they are read).  Word kStatusNanWord belongs to one 4-bit cache chunk at a
+// time, which clears it first: whether a visible key or value is held as NaN.
 constexpr int kStatusWords = 4;
 constexpr int kStatusSchedWord = 4;
 constexpr int kStatusAbortWord = 6;
@@ -271,13 +271,15 @@ struct Kv4Params {
     float* partials;
     Kv4Piece* plan;   // [n_cta] each attention CTA's first piece, then by unit the others
     Kv4Split split;
-    int epoch;        // chunks: this call's number
+    int* nan_flag;    // chunks: a word for "some row sees NaN", cleared by the append (below)
     double inv_freq[kMaxHeadDim / 2];
 };
 constexpr int kMaxPageSize = 1024;
 constexpr int kKv4MaxBatch = 2048;      // sequences of one plan and attention launch
 constexpr int kKv4GapBlocksMax = 26;    // largest per-unit allowance of the attention's split, in blocks
-// Appends k_new / v_new where given; lays out q and plans the attention where q is given.
+constexpr int kKv4StoreTokens = 16;     // tokens per sequence from which the append stores whole blocks
+// Appends k_new / v_new where given; lays out q and plans the attention where q is given.  From
+// kKv4StoreTokens tokens on the append clears *nan_flag, where p has one.
 cudaError_t launch_kv4_prepare(const Kv4Params& p, int sm_count, cudaStream_t stream);
 size_t kv4_frag_bytes(const Kv4Params& p);  // per sequence
 size_t kv4_sums_bytes(const Kv4Params& p);  // per sequence
@@ -287,13 +289,13 @@ cudaError_t launch_kv4_attn(const Kv4Params& p, int device, cudaStream_t stream)
 
 // Chunks of prompts over the cache on the tcgen05 kernel (kv4_stage.cu): q rotated to fp16 at q_out
 // [B][T][Hq][D], positions [0, round128(ctx + new)) of the cache as fp16 rows at k_out / v_out
-// [B][Sk][Hkv][D] (what no query sees is zero); nan_flag takes the value p.epoch, which grows from call
-// to call, where a visible value group is held as NaN (it becomes zero; launch_kv4_nan_rows then marks
-// the rows that see it).  after_append: the kernel just before on the stream is this call's append,
+// [B][Sk][Hkv][D] (what no query sees is zero); *p.nan_flag, clear before, is raised where a visible
+// value group is held as NaN (it becomes zero) or a visible page is missing; launch_kv4_nan_rows then
+// marks the rows that see it.  after_append: the kernel just before on the stream is this call's append,
 // which needs none of what this one writes; the queries' part then runs beside it.
-cudaError_t launch_kv4_stage(const Kv4Params& p, void* q_out, void* k_out, void* v_out, int Sk, int* nan_flag,
-                             bool after_append, int sm_count, cudaStream_t stream);
-cudaError_t launch_kv4_nan_rows(const Kv4Params& p, const int* nan_flag, int sm_count, cudaStream_t stream);
+cudaError_t launch_kv4_stage(const Kv4Params& p, void* q_out, void* k_out, void* v_out, int Sk, bool after_append,
+                             int sm_count, cudaStream_t stream);
+cudaError_t launch_kv4_nan_rows(const Kv4Params& p, int sm_count, cudaStream_t stream);
 
 // The page table, reference counts and pages of a paged cache (pages.cu).
 struct PagePoolParams {

@@ -460,6 +460,7 @@ __global__ void __launch_bounds__(StoreGeo<D>::kMaxThreads, StoreGeo<D>::ctas(kN
     double* const part = weight + D + group * 16 * kChunks;
     float* const factor = reinterpret_cast<float*>(weight + D + groups * 16 * kChunks) + group * 16;
     const uint32_t bar = smem_u32(full);
+    if (p.nan_flag != nullptr && blockIdx.x == 0 && tid == 0) *p.nan_flag = 0;
     const int chunk = blockIdx.x % chunks;
     const int64_t bb = blockIdx.x / chunks;
     const int b = (int)(bb / blocks);
@@ -733,9 +734,6 @@ __global__ void __launch_bounds__(StoreGeo<D>::kMaxThreads, StoreGeo<D>::ctas(kN
     }
 }
 
-// Tokens per sequence from which whole blocks are stored: below it a block would be mostly absent rows.
-constexpr int kStoreMinTokens = 16;
-
 template <int D, typename T>
 cudaError_t launch_store(const Kv4Params& p, int sm_count, cudaStream_t stream) {
     using Gm = StoreGeo<D>;
@@ -759,7 +757,7 @@ cudaError_t launch_store(const Kv4Params& p, int sm_count, cudaStream_t stream) 
 template <int D>
 cudaError_t launch_prepare(const Kv4Params& p, int sm_count, cudaStream_t stream) {
     int append = p.k_new ? 1 : 0;
-    if (append && p.T >= kStoreMinTokens) {
+    if (append && p.T >= kKv4StoreTokens) {  // below it a block would be mostly absent rows
         const cudaError_t e = p.act_dtype == kF16 ? launch_store<D, __half>(p, sm_count, stream)
                                                   : launch_store<D, __nv_bfloat16>(p, sm_count, stream);
         if (e != cudaSuccess || !p.q) return e;

@@ -139,8 +139,7 @@ __device__ __forceinline__ void quad_transpose(uint32_t (&w)[4], int t) {  // la
 // once.  (Rows written 4 bytes a lane, without the exchange below: 2 us more of 29.)
 template <int D>
 __device__ __forceinline__ void stage_group(const Kv4Params& p, const uint8_t* src, int y, int pos, int first, int end,
-                                            __half* k_row0, __half* v_row0, int64_t row_stride, int* nan_flag,
-                                            int lane) {
+                                            __half* k_row0, __half* v_row0, int64_t row_stride, int lane) {
     constexpr int kGroups = D / 32;
     const int g = lane >> 2, t = lane & 3;
     auto seen = [&](int key) { return src != nullptr && pos + key >= first && pos + key < end; };
@@ -204,13 +203,12 @@ __device__ __forceinline__ void stage_group(const Kv4Params& p, const uint8_t* s
     }
     const bool big = __hisinf(__low2half(top)) || __hisinf(__high2half(top));
     if (__any_sync(0xffffffffu, big) && lane == 0) atomicOr(p.status, 4);
-    if (__any_sync(0xffffffffu, nan) && lane == 0) atomicMax(nan_flag, p.epoch);
+    if (__any_sync(0xffffffffu, nan) && lane == 0) atomicExch(p.nan_flag, 1);
 }
 
 template <int D, typename T>
 __global__ void __launch_bounds__(2 * D) kv4_stage_kernel(const __grid_constant__ Kv4Params p, __half* q_out, __half* k_out,
-                                                          __half* v_out, int Sk, int* nan_flag, int q_blocks,
-                                                          int q_total) {
+                                                          __half* v_out, int Sk, int q_blocks, int q_total) {
     extern __shared__ __align__(16) unsigned char smem[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if ((int)blockIdx.x < q_total) {
@@ -238,9 +236,12 @@ __global__ void __launch_bounds__(2 * D) kv4_stage_kernel(const __grid_constant_
             const int pos = blk * kKv4Block;
             const bool seen = pos + kKv4Block > first && pos < end;
             const uint8_t* src = seen ? kv4_block_ptr(p, b, h, pos) : nullptr;
-            if (seen && src == nullptr && lane == 0) atomicOr(p.status, 16);
+            if (seen && src == nullptr && lane == 0) {
+                atomicOr(p.status, 16);
+                atomicExch(p.nan_flag, 1);
+            }
             const int64_t at = ((int64_t)b * Sk + pos) * row_stride + (int64_t)h * D;
-            stage_group<D>(p, src, y, pos, first, end, k_out + at, v_out + at, row_stride, nan_flag, lane);
+            stage_group<D>(p, src, y, pos, first, end, k_out + at, v_out + at, row_stride, lane);
         }
         i -= count;
     }
@@ -248,9 +249,9 @@ __global__ void __launch_bounds__(2 * D) kv4_stage_kernel(const __grid_constant_
 
 // Rows that see a value group held as NaN, or a page that does not exist: their outputs become NaN
 // (the group's channels; all of the row's).  Runs to its end only where the staging met one.
-__global__ void __launch_bounds__(256) kv4_nan_rows_kernel(const __grid_constant__ Kv4Params p, const int* nan_flag) {
+__global__ void __launch_bounds__(256) kv4_nan_rows_kernel(const __grid_constant__ Kv4Params p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (*nan_flag != p.epoch && (*p.status & 16) == 0) return;
+    if (__ldcg(p.nan_flag) == 0) return;
     const int D = p.D, groups = D / 32;
     const int64_t rows = (int64_t)p.B * p.T * p.Hkv;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -282,8 +283,8 @@ __global__ void __launch_bounds__(256) kv4_nan_rows_kernel(const __grid_constant
 }
 
 template <int D, typename T>
-cudaError_t launch_stage(const Kv4Params& p, __half* q_out, __half* k_out, __half* v_out, int Sk, int* nan_flag,
-                         bool after_append, int sm_count, cudaStream_t stream) {
+cudaError_t launch_stage(const Kv4Params& p, __half* q_out, __half* k_out, __half* v_out, int Sk, bool after_append,
+                         int sm_count, cudaStream_t stream) {
     const size_t smem = 16 * (D / 2) * sizeof(double2) + 2 * D * sizeof(double);
     auto kern = kv4_stage_kernel<D, T>;
     if (smem > 48 * 1024) {
@@ -302,18 +303,18 @@ cudaError_t launch_stage(const Kv4Params& p, __half* q_out, __half* k_out, __hal
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = after_append ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kern, p, q_out, k_out, v_out, Sk, nan_flag, q_blocks, q_total);
+    return cudaLaunchKernelEx(&cfg, kern, p, q_out, k_out, v_out, Sk, q_blocks, q_total);
 }
 
 }  // namespace
 
-cudaError_t launch_kv4_stage(const Kv4Params& p, void* q_out, void* k_out, void* v_out, int Sk, int* nan_flag,
-                             bool after_append, int sm_count, cudaStream_t stream) {
+cudaError_t launch_kv4_stage(const Kv4Params& p, void* q_out, void* k_out, void* v_out, int Sk, bool after_append,
+                             int sm_count, cudaStream_t stream) {
     __half *q = static_cast<__half*>(q_out), *k = static_cast<__half*>(k_out), *v = static_cast<__half*>(v_out);
     auto go = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        return p.act_dtype == kF16 ? launch_stage<D, __half>(p, q, k, v, Sk, nan_flag, after_append, sm_count, stream)
-                                   : launch_stage<D, __nv_bfloat16>(p, q, k, v, Sk, nan_flag, after_append, sm_count, stream);
+        return p.act_dtype == kF16 ? launch_stage<D, __half>(p, q, k, v, Sk, after_append, sm_count, stream)
+                                   : launch_stage<D, __nv_bfloat16>(p, q, k, v, Sk, after_append, sm_count, stream);
     };
     switch (p.D) {
         case 64: return go(std::integral_constant<int, 64>{});
@@ -324,7 +325,7 @@ cudaError_t launch_kv4_stage(const Kv4Params& p, void* q_out, void* k_out, void*
     }
 }
 
-cudaError_t launch_kv4_nan_rows(const Kv4Params& p, const int* nan_flag, int sm_count, cudaStream_t stream) {
+cudaError_t launch_kv4_nan_rows(const Kv4Params& p, int sm_count, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)sm_count * 2);
     cfg.blockDim = dim3(256);
@@ -334,7 +335,7 @@ cudaError_t launch_kv4_nan_rows(const Kv4Params& p, const int* nan_flag, int sm_
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kv4_nan_rows_kernel, p, nan_flag);
+    return cudaLaunchKernelEx(&cfg, kv4_nan_rows_kernel, p);
 }
 
 }  // namespace b2a
