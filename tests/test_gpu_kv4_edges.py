@@ -149,3 +149,36 @@ def test_chunks_whose_staged_rows_come_in_slices(ctx):
         ctx.check_device_status()
         assert torch.equal(torch.isnan(t["o"]), nan)
         assert torch.equal(t["o"][~nan], clean[~nan])
+
+
+@pytest.mark.parametrize("D,window", [(64, 0), (64, 24), (96, 24), (128, 24), (256, 24), (128, 0)])
+@pytest.mark.parametrize("cached", [True, False])
+def test_a_chunk_sees_a_key_held_as_nan_at_every_place_of_a_block(ctx, D, window, cached):
+    """Sixteen sequences with the key at one place of the block each, and a clean one: the rows that see it are NaN,
+    the others as if it were not there."""
+    import b200attn
+    B, L, T = 17, 60, 64
+    c = Case(ctx=[L] * B, T=T, Hq=2, Hkv=1, D=D, page=32, dtype=oracle.BF16, rope=None, window=window, seed=D + window)
+    at = (40 if cached else L + 4) + np.arange(16)
+    for b in range(16):
+        if cached:
+            _hold_nan(c, b, at[b], "k")
+        else:
+            c.k[b, at[b] - L, 0, 33] = np.nan
+    t = c.device()
+    b200attn.kv4_decode(ctx, t["q"], t["k"], t["v"], t["pages"], t["table"], t["ctx"], t["o"], c.scale, window=window,
+                        **c.more())
+    if cached:
+        ctx.check_device_status()  # it was reported when it was stored
+    else:
+        with pytest.raises(b200attn.B200RuntimeException, match="4-bit cache's range"):
+            ctx.check_device_status()
+        for b in range(16):
+            c.k[b, at[b] - L, 0, 32:64] = 0.0
+    o, tol, _, _ = c.expect()
+    pos = L + np.arange(T)
+    sees = np.zeros((B, T), bool)
+    sees[:16] = (at[:, None] <= pos) & (at[:, None] > pos - (window or 1 << 30))
+    got = to_np(t["o"])
+    np.testing.assert_array_equal(np.isnan(got), np.broadcast_to(sees[..., None, None], got.shape))
+    assert np.all((np.abs(got - o) <= tol)[~sees])

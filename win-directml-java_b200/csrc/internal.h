@@ -290,8 +290,8 @@ cudaError_t launch_kv4_attn(const Kv4Params& p, int device, cudaStream_t stream)
 // Chunks of prompts over the cache on the tcgen05 kernel (kv4_stage.cu): q rotated to fp16 at q_out
 // [B][T][Hq][D], positions [0, round128(ctx + new)) of the cache as fp16 rows at k_out / v_out
 // [B][Sk][Hkv][D] (what no query sees is zero); *p.nan_flag, clear before, is raised where a visible
-// value group is held as NaN (it becomes zero) or a visible page is missing; launch_kv4_nan_rows then
-// marks the rows that see it.  after_append: the kernel just before on the stream is this call's append,
+// value group is held as NaN (it becomes zero), a visible key is, or a visible page is missing;
+// launch_kv4_nan_rows then marks the rows that see it.  after_append: the kernel just before on the stream is this call's append,
 // which needs none of what this one writes; the queries' part then runs beside it.
 cudaError_t launch_kv4_stage(const Kv4Params& p, void* q_out, void* k_out, void* v_out, int Sk, bool after_append,
                              int sm_count, cudaStream_t stream);

@@ -174,6 +174,9 @@ __device__ __forceinline__ void stage_group(const Kv4Params& p, const uint8_t* s
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         const bool row_seen = seen(g + 8 * r);
+        // a key held as NaN scores NaN, which a part of the softmax's exponentials would take for a small
+        // number: its rows are marked later too
+        nan |= row_seen && (sz[0][0][r] & 0x7fffu) > 0x7c00u;
         const uint32_t ks = __byte_perm(sz[0][0][r], 0, 0x1010), kz = __byte_perm(sz[0][0][r], 0, 0x3232);
         uint32_t vs = __byte_perm(sz[1][1][r], sz[1][2][r], 0x5410), vz = __byte_perm(sz[1][1][r], sz[1][2][r], 0x7632);
         // a value held as NaN counts as zero here; the rows that see it are marked later
@@ -247,8 +250,9 @@ __global__ void __launch_bounds__(2 * D) kv4_stage_kernel(const __grid_constant_
     }
 }
 
-// Rows that see a value group held as NaN, or a page that does not exist: their outputs become NaN
-// (the group's channels; all of the row's).  Runs to its end only where the staging met one.
+// Rows that see a value group held as NaN, a key held as NaN, or a page that does not exist: their
+// outputs become NaN (the group's channels; all of the row's).  Runs to its end only where the staging
+// met one.
 __global__ void __launch_bounds__(256) kv4_nan_rows_kernel(const __grid_constant__ Kv4Params p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (__ldcg(p.nan_flag) == 0) return;
@@ -261,16 +265,20 @@ __global__ void __launch_bounds__(256) kv4_nan_rows_kernel(const __grid_constant
         int L, n;
         if (!kv4_lens(p, b, L, n) || t >= n) continue;
         const int first = p.window > 0 ? max(0, L + t - p.window + 1) : 0;
-        unsigned hit = 0;  // bit per group, bit 31: a page is missing
+        unsigned hit = 0;  // bit per value group, bit 31: the key, or a page that is missing
         for (int key = first + lane; key <= L + t; key += 32) {
             const uint8_t* block = kv4_block_ptr(p, b, kvh, key);
             if (block == nullptr) {
                 hit |= 1u << 31;
                 continue;
             }
-            const __half2* sz = reinterpret_cast<const __half2*>(block + kv4_off_vparam(D));
-            for (int y = 0; y < groups; ++y)
-                if (__hisnan(__low2half(sz[kv4_param(key % kKv4Block, y, groups)]))) hit |= 1u << y;
+            const __half2* ks = reinterpret_cast<const __half2*>(block + kv4_off_kparam(D));
+            const __half2* vs = reinterpret_cast<const __half2*>(block + kv4_off_vparam(D));
+            for (int y = 0; y < groups; ++y) {
+                const int at = kv4_param(key % kKv4Block, y, groups);
+                if (__hisnan(__low2half(ks[at]))) hit |= 1u << 31;
+                if (__hisnan(__low2half(vs[at]))) hit |= 1u << y;
+            }
         }
         hit = __reduce_or_sync(0xffffffffu, hit);
         if (hit == 0) continue;
