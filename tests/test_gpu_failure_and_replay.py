@@ -206,3 +206,47 @@ def test_decode_graph_replays_recompute_the_step(ctx):
         assert_close(to_np(out), want, what=f"decode graph replay {rep}")
     del g
     ctx.check_device_status()
+
+
+def test_decode_counters_are_untouched_by_a_captured_decode_of_other_sizes():
+    """A captured decode with few units and large partial slots, then one with many units and small slots in the same
+    workspace: replaying the first must leave the counters of the second at zero."""
+    import torch
+    import b200attn
+
+    def inputs(B, Hq, Hkv, D, S, length, seed):
+        g = torch.Generator("cuda").manual_seed(seed)
+        r = lambda *s: torch.randn(*s, generator=g, device="cuda").half()
+        lens = length - torch.arange(B, dtype=torch.int32, device="cuda") % 90  # uneven: units are cut
+        return (r(B, Hq, D), r(B, Hkv, D), r(B, Hkv, D), r(B, Hkv, S, D), r(B, Hkv, S, D), lens,
+                torch.empty(B, Hq, D, device="cuda"), 1 / math.sqrt(D))
+
+    few = inputs(2, 4, 1, 256, 4096, 4000, 1)
+    many = inputs(800, 8, 4, 64, 1000, 997, 2)
+    with b200attn.Context(0) as one:
+        def run(x):
+            x[6].fill_(float("nan"))
+            b200attn.decode(one, *x)
+
+        run(few)
+        torch.cuda.synchronize()
+        g, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s), torch.cuda.graph(g, stream=s):
+            run(few)
+        torch.cuda.current_stream().wait_stream(s)
+        size = one.workspace_bytes()
+        run(many)
+        torch.cuda.synchronize()
+        first = [x[6].clone() for x in (few, many)]
+        assert bool(torch.isfinite(first[1]).all())
+        assert one.workspace_bytes() <= size + (1 << 16)  # more counters at most: the graph's slots stayed in place
+        for _ in range(2):
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(few[6], first[0])
+            run(many)
+            torch.cuda.synchronize()
+            assert torch.equal(many[6], first[1])
+        del g
+        one.check_device_status()

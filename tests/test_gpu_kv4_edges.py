@@ -182,3 +182,35 @@ def test_a_chunk_sees_a_key_held_as_nan_at_every_place_of_a_block(ctx, D, window
     got = to_np(t["o"])
     np.testing.assert_array_equal(np.isnan(got), np.broadcast_to(sees[..., None, None], got.shape))
     assert np.all((np.abs(got - o) <= tol)[~sees])
+
+
+def test_a_captured_call_and_a_later_one_with_more_units():
+    """The merge counters of a call must stay zero between launches whatever an earlier captured call does: few units
+    with large slots (captured), then many units with small ones, in the same workspace."""
+    import torch
+    import b200attn
+    few = Case(ctx=[5000, 4100], T=2, Hq=4, Hkv=1, D=256, page=64, rope=None, seed=41)
+    many = Case(ctx=60 + np.arange(1200) % 90, Hq=2, Hkv=1, D=64, page=32, rope=None, seed=43)
+    a, b = few.device(), many.device()
+    with b200attn.Context(0) as one:
+        def run(c, t):
+            t["o"].fill_(float("nan"))
+            b200attn.kv4_decode(one, t["q"], t["k"], t["v"], t["pages"], t["table"], t["ctx"], t["o"], c.scale, **c.more())
+
+        run(few, a)
+        g = _capture(lambda: run(few, a))
+        size = one.workspace_bytes()
+        run(many, b)
+        torch.cuda.synchronize()
+        first_a, first_b = a["o"].clone(), b["o"].clone()
+        assert bool(torch.isfinite(first_b.float()).all())
+        assert one.workspace_bytes() <= size + (1 << 16)  # more counters at most: the graph's slots stayed in place
+        for _ in range(2):
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(a["o"], first_a)
+            run(many, b)
+            torch.cuda.synchronize()
+            assert torch.equal(b["o"], first_b)
+        del g
+        one.check_device_status()

@@ -19,6 +19,17 @@
 
 using namespace b2a;
 
+// Counters that are zero between launches.  They grow into a new allocation and the old one stays until
+// the context ends, since a captured launch goes on counting there; and they share no allocation with
+// anything that is written otherwise, so what such a launch writes never lands on a later call's counters.
+struct Counters {
+    static constexpr int kMost = 48;  // each at least twice the one before
+    int* at[kMost] = {};
+    int n = 0;
+    size_t bytes = 0;  // of the last one
+    size_t total = 0;
+};
+
 struct b2a_context {
     int device = 0;
     int sm_count = 0;
@@ -29,10 +40,7 @@ struct b2a_context {
     // decode workspace: [counters][partials]
     void* dec_ws = nullptr;
     size_t dec_ws_bytes = 0;
-    // counter region at the start of dec_ws, partial slots after it; the region never
-    // shrinks (a later, smaller batch's slots would otherwise land on counters a larger
-    // batch relies on being zero) and is zeroed whenever it grows or the buffer is new
-    size_t dec_counter_bytes = 0;
+    Counters dec_counters;
     // prefill workspace: rope table + rotated q/k staging
     void* pf_ws = nullptr;
     size_t pf_ws_bytes = 0;
@@ -49,11 +57,10 @@ struct b2a_context {
     // split-K projections: [tile counters][fp32 accumulator], all zero between launches
     void* lin_ws = nullptr;
     size_t lin_ws_bytes = 0;
-    size_t lin_region = 0;
-    // generic-kernel key split: [counters][partial slots], the same layout rules as dec_ws
+    // generic-kernel key split: partial slots
     void* split_ws = nullptr;
     size_t split_ws_bytes = 0;
-    size_t split_counter_bytes = 0;
+    Counters split_counters;
     // test hook (b2a_test_inject_wait_timeout): the next tcgen05 attention launch
     // leaves one K/V copy unissued
     bool inject_wait_timeout = false;
@@ -61,14 +68,14 @@ struct b2a_context {
     double kv4_inv_freq[kMaxHeadDim / 2] = {};
     double kv4_theta = 0.0;
     int kv4_inv_dim = 0;
-    // paged 4-bit cache: [merge counters][partial slots][plan][q operands][q sums]
+    // paged 4-bit cache: [partial slots][plan][q operands][q sums]
     void* kv4_ws = nullptr;
     size_t kv4_ws_bytes = 0;
-    size_t kv4_counter_bytes = 0;
-    // paged cache: [words between blocks][the page operations' lists]
+    Counters kv4_counters;
+    // paged cache: the page operations' lists and the words between their blocks
     void* pg_ws = nullptr;
     size_t pg_ws_bytes = 0;
-    size_t pg_sync_bytes = 0;
+    Counters pg_sync;
     // b2a_set_decode_early_start: tensor-core decodes launched with programmatic serialisation
     bool decode_early_start = false;
     // test hook (b2a_test_last_attention_kernel): the kernel the last whole-sequence
@@ -113,14 +120,24 @@ struct DeviceGuard {
 bool valid_dtype(int d) { return d == B2A_FLOAT32 || d == B2A_FLOAT16 || d == B2A_BFLOAT16; }
 size_t dtype_size(int d) { return d == B2A_FLOAT32 ? 4 : 2; }
 
+size_t workspace_total(const b2a_context* ctx) {
+    return ctx->dec_ws_bytes + ctx->pf_ws_bytes + ctx->split_ws_bytes + ctx->blk_ws_bytes + ctx->rope_tab_bytes +
+           ctx->lin_ws_bytes + ctx->pg_ws_bytes + ctx->kv4_ws_bytes + ctx->dec_counters.total +
+           ctx->split_counters.total + ctx->kv4_counters.total + ctx->pg_sync.total;
+}
+
+// Whether `more` bytes beside `others` stay within the context's limit.
+int check_limit(b2a_context* ctx, size_t more, size_t others, const char* what) {
+    if (ctx->ws_limit != 0 && more + others > ctx->ws_limit)
+        return fail(ctx, B2A_EOOM, "%s workspace of %zu bytes exceeds the context limit of %zu bytes", what,
+                    more + others, ctx->ws_limit);
+    return B2A_OK;
+}
+
 int ensure_buffer(b2a_context* ctx, void** buf, size_t* have, size_t need, const char* what) {
     if (*have >= need) return B2A_OK;
-    const size_t other =
-        ctx->dec_ws_bytes + ctx->pf_ws_bytes + ctx->split_ws_bytes + ctx->blk_ws_bytes + ctx->rope_tab_bytes +
-        ctx->lin_ws_bytes + ctx->pg_ws_bytes + ctx->kv4_ws_bytes - *have;
-    if (ctx->ws_limit != 0 && need + other > ctx->ws_limit)
-        return fail(ctx, B2A_EOOM, "%s workspace of %zu bytes exceeds the context limit of %zu bytes", what,
-                    need + other, ctx->ws_limit);
+    const int rc = check_limit(ctx, need, workspace_total(ctx) - *have, what);
+    if (rc) return rc;
     if (*buf) {
         cudaFree(*buf);  // implicitly waits for work that may still use it
         *buf = nullptr;
@@ -135,25 +152,43 @@ int ensure_buffer(b2a_context* ctx, void** buf, size_t* have, size_t need, const
     return B2A_OK;
 }
 
-// Sizes a [counters][partial slots] workspace: the counter region keeps the largest size
-// any call needed, the partial slots start after it, and the counters are zeroed (on
-// `stream`, or synchronously when it is null and `sync`) when the buffer is new or the
-// region grows.  Returns the counter region's size in *counter_bytes.
-int ensure_counted_buffer(b2a_context* ctx, void** buf, size_t* have, size_t* region, size_t counter_ints,
-                          size_t partial_bytes, const char* what, cudaStream_t stream, bool sync,
-                          size_t* counter_bytes) {
-    const size_t need_counters = (counter_ints * sizeof(int) + 255) / 256 * 256;
-    const size_t cb = std::max(need_counters, *region);
-    const bool grow = cb + partial_bytes > *have;
-    const int rc = ensure_buffer(ctx, buf, have, cb + partial_bytes, what);
-    if (rc != B2A_OK) return rc;
-    if (grow || cb > *region) {
-        const cudaError_t e = sync ? cudaMemset(*buf, 0, cb) : cudaMemsetAsync(*buf, 0, cb, stream);
-        if (e != cudaSuccess) return cuda_fail(ctx, e, what);
-        *region = cb;
+// At least `ints` counters at *at, zeroed (on `stream`, or synchronously with `sync`) when they are new.
+int ensure_counters(b2a_context* ctx, Counters& c, size_t ints, const char* what, cudaStream_t stream, bool sync,
+                    int** at) {
+    const size_t need = (ints * sizeof(int) + 255) / 256 * 256;
+    if (c.n == 0 || c.bytes < need) {
+        const size_t bytes = std::max(need, 2 * c.bytes);
+        const int rc = check_limit(ctx, bytes, workspace_total(ctx), what);
+        if (rc) return rc;
+        if (c.n == Counters::kMost) return fail(ctx, B2A_EOOM, "%s: the counters grew too often", what);
+        void* fresh = nullptr;
+        cudaError_t e = cudaMalloc(&fresh, bytes);
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            return cuda_fail(ctx, e, what);
+        }
+        e = sync ? cudaMemset(fresh, 0, bytes) : cudaMemsetAsync(fresh, 0, bytes, stream);
+        if (e != cudaSuccess) {
+            cudaFree(fresh);
+            return cuda_fail(ctx, e, what);
+        }
+        c.at[c.n++] = static_cast<int*>(fresh);
+        c.bytes = bytes;
+        c.total += bytes;
     }
-    *counter_bytes = cb;
+    *at = c.at[c.n - 1];
     return B2A_OK;
+}
+
+void free_counters(Counters& c) {
+    for (int i = 0; i < c.n; ++i) cudaFree(c.at[i]);
+}
+
+// Partial slots of at least slot_bytes at *buf and counters at *counters.
+int ensure_counted_buffer(b2a_context* ctx, void** buf, size_t* have, Counters& c, size_t counter_ints,
+                          size_t slot_bytes, const char* what, cudaStream_t stream, bool sync, int** counters) {
+    const int rc = ensure_buffer(ctx, buf, have, slot_bytes, what);
+    return rc ? rc : ensure_counters(ctx, c, counter_ints, what, stream, sync, counters);
 }
 
 void inv_freq_table(double theta, int D, double* out) {
@@ -232,11 +267,10 @@ cudaError_t launch_attention(b2a_context* ctx, const AttnParams& p, cudaStream_t
     size_t part_bytes = 0, counter_ints = 0;
     const int nsplit = attn_simt_split_plan(p, ctx->sm_count, &part_bytes, &counter_ints);
     if (nsplit > 1) {
-        size_t counter_bytes = 0;
-        if (ensure_counted_buffer(ctx, &ctx->split_ws, &ctx->split_ws_bytes, &ctx->split_counter_bytes, counter_ints,
-                                  part_bytes, "attention split workspace", s, false, &counter_bytes) == B2A_OK) {
-            const SimtSplit sp{reinterpret_cast<float*>(static_cast<char*>(ctx->split_ws) + counter_bytes),
-                               static_cast<int*>(ctx->split_ws), nsplit, kSimtSplitKeys};
+        int* counters = nullptr;
+        if (ensure_counted_buffer(ctx, &ctx->split_ws, &ctx->split_ws_bytes, ctx->split_counters, counter_ints,
+                                  part_bytes, "attention split workspace", s, false, &counters) == B2A_OK) {
+            const SimtSplit sp{static_cast<float*>(ctx->split_ws), counters, nsplit, kSimtSplitKeys};
             return launch_attn_simt(p, s, &sp);
         }
         ctx->last_error.clear();  // the refused workspace is not an error of this call
@@ -256,12 +290,10 @@ int run_decode(b2a_context* ctx, DecodeParams& p, cudaStream_t stream, bool allo
         decode_tc_workspace(ctx->device, p.B, p.Hkv, p.n_hg, p.D, p.cache_dtype, &target, &cap, &partial_bytes);
         const int bmax = std::min(p.B, kDecodeMaxBatchPerLaunch);
         const size_t counter_ints = (size_t)bmax * p.Hkv * p.n_hg;
-        size_t counter_bytes = 0;
-        int rc = ensure_counted_buffer(ctx, &ctx->dec_ws, &ctx->dec_ws_bytes, &ctx->dec_counter_bytes, counter_ints,
-                                       partial_bytes, "decode workspace", stream, false, &counter_bytes);
+        int rc = ensure_counted_buffer(ctx, &ctx->dec_ws, &ctx->dec_ws_bytes, ctx->dec_counters, counter_ints,
+                                       partial_bytes, "decode workspace", stream, false, &p.counters);
         if (rc != B2A_OK) return rc;
-        p.counters = static_cast<int*>(ctx->dec_ws);
-        p.partials = reinterpret_cast<float*>(static_cast<char*>(ctx->dec_ws) + counter_bytes);
+        p.partials = static_cast<float*>(ctx->dec_ws);
         p.target_items = target;
         p.item_capacity = cap;
         p.early_start = ctx->decode_early_start ? 1 : 0;
@@ -370,6 +402,10 @@ B2A_API int b2a_destroy(b2a_context* ctx) {
         if (ctx->lin_ws) cudaFree(ctx->lin_ws);
         if (ctx->pg_ws) cudaFree(ctx->pg_ws);
         if (ctx->kv4_ws) cudaFree(ctx->kv4_ws);
+        free_counters(ctx->dec_counters);
+        free_counters(ctx->split_counters);
+        free_counters(ctx->kv4_counters);
+        free_counters(ctx->pg_sync);
     }
     delete ctx;
     return B2A_OK;
@@ -399,8 +435,7 @@ B2A_API int b2a_set_decode_early_start(b2a_context* ctx, int enable) {
 
 B2A_API int b2a_workspace_bytes(const b2a_context* ctx, size_t* bytes) {
     if (!ctx || !bytes) return B2A_EINVAL;
-    *bytes = ctx->dec_ws_bytes + ctx->pf_ws_bytes + ctx->split_ws_bytes + ctx->blk_ws_bytes + ctx->rope_tab_bytes +
-             ctx->lin_ws_bytes + ctx->pg_ws_bytes + ctx->kv4_ws_bytes;
+    *bytes = workspace_total(ctx);
     return B2A_OK;
 }
 
@@ -418,9 +453,9 @@ B2A_API int b2a_reserve_decode(b2a_context* ctx, int max_batch, int num_q_heads,
     decode_tc_workspace(ctx->device, max_batch, num_kv_heads, n_hg, head_dim, B2A_FLOAT16, &target, &cap,
                         &partial_bytes);
     const size_t counter_ints = (size_t)std::min(max_batch, kDecodeMaxBatchPerLaunch) * num_kv_heads * n_hg;
-    size_t counter_bytes = 0;
-    return ensure_counted_buffer(ctx, &ctx->dec_ws, &ctx->dec_ws_bytes, &ctx->dec_counter_bytes, counter_ints,
-                                 partial_bytes, "decode workspace", nullptr, true, &counter_bytes);
+    int* counters = nullptr;
+    return ensure_counted_buffer(ctx, &ctx->dec_ws, &ctx->dec_ws_bytes, ctx->dec_counters, counter_ints,
+                                 partial_bytes, "decode workspace", nullptr, true, &counters);
 }
 
 B2A_API int b2a_test_inject_wait_timeout(b2a_context* ctx) {
@@ -1024,12 +1059,14 @@ int run_linear(b2a_context* ctx, int in_dtype, int out_dtype, const void* x, con
     size_t acc_bytes = 0, counter_ints = 0;
     const int ks = linear_split_plan(M, N, K, ctx->sm_count, &acc_bytes, &counter_ints);
     if (ks > 1) {
-        // the accumulator counts as counter region: zeroed when new or grown, kept zero by the kernel
-        const size_t region_ints = counter_ints + (acc_bytes + sizeof(int) - 1) / sizeof(int) + 64;
-        size_t region_bytes = 0;
-        if (ensure_counted_buffer(ctx, &ctx->lin_ws, &ctx->lin_ws_bytes, &ctx->lin_region, region_ints, 0,
-                                  "projection split workspace", static_cast<cudaStream_t>(stream), false,
-                                  &region_bytes) == B2A_OK) {
+        // counters and accumulator: zeroed when new, kept zero by the kernel
+        const size_t bytes = (counter_ints * sizeof(int) + acc_bytes + 511) / 256 * 256;
+        const bool grow = bytes > ctx->lin_ws_bytes;
+        if (ensure_buffer(ctx, &ctx->lin_ws, &ctx->lin_ws_bytes, bytes, "projection split workspace") == B2A_OK) {
+            if (grow) {
+                const cudaError_t e = cudaMemsetAsync(ctx->lin_ws, 0, bytes, static_cast<cudaStream_t>(stream));
+                if (e != cudaSuccess) return cuda_fail(ctx, e, "projection split workspace");
+            }
             a.ksplit = ks;
             a.counters = static_cast<int*>(ctx->lin_ws);
             a.acc = reinterpret_cast<float*>(static_cast<char*>(ctx->lin_ws) + (counter_ints * sizeof(int) + 255) / 256 * 256);
@@ -1341,10 +1378,9 @@ int run_kv4_attention(b2a_context* ctx, Kv4Params& p, cudaStream_t stream) {
     const size_t units = (size_t)most * p.split.per_seq;
     const size_t part = r256(p.split.partial_bytes), plan = r256((p.split.n_cta + units) * sizeof(Kv4Piece)), frag = r256(kv4_frag_bytes(p) * most),
                  sums = r256(kv4_sums_bytes(p) * most);
-    size_t counter_bytes = 0;
-    const int rc = ensure_counted_buffer(ctx, &ctx->kv4_ws, &ctx->kv4_ws_bytes, &ctx->kv4_counter_bytes, units,
+    const int rc = ensure_counted_buffer(ctx, &ctx->kv4_ws, &ctx->kv4_ws_bytes, ctx->kv4_counters, units,
                                          part + plan + frag + sums, "4-bit cache attention", stream, false,
-                                         &counter_bytes);
+                                         &p.counters);
     if (rc) return rc;
     char* at = static_cast<char*>(ctx->kv4_ws);
     auto take = [&](size_t bytes) {
@@ -1352,7 +1388,6 @@ int run_kv4_attention(b2a_context* ctx, Kv4Params& p, cudaStream_t stream) {
         at += bytes;
         return here;
     };
-    p.counters = reinterpret_cast<int*>(take(counter_bytes));
     p.partials = reinterpret_cast<float*>(take(part));
     p.plan = reinterpret_cast<Kv4Piece*>(take(plan));
     p.q_frag = reinterpret_cast<uint4*>(take(frag));
@@ -1396,12 +1431,10 @@ int check_pool(b2a_context* ctx, const b2a_page_pool* pool, bool with_pages, Pag
 }
 
 int pages_workspace(b2a_context* ctx, int num_pages, cudaStream_t stream, int** sync, int** ws) {
-    size_t sync_bytes = 0;
-    const int rc = ensure_counted_buffer(ctx, &ctx->pg_ws, &ctx->pg_ws_bytes, &ctx->pg_sync_bytes, kPageSyncInts,
+    const int rc = ensure_counted_buffer(ctx, &ctx->pg_ws, &ctx->pg_ws_bytes, ctx->pg_sync, kPageSyncInts,
                                          pages_workspace_ints(num_pages) * sizeof(int), "page operations", stream,
-                                         false, &sync_bytes);
-    *sync = static_cast<int*>(ctx->pg_ws);
-    *ws = reinterpret_cast<int*>(static_cast<char*>(ctx->pg_ws) + sync_bytes);
+                                         false, sync);
+    *ws = static_cast<int*>(ctx->pg_ws);
     return rc;
 }
 
