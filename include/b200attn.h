@@ -431,7 +431,8 @@ B2A_API int b2a_kv4_decode(b2a_context* ctx, const b2a_kv4_cache* cache, int act
  *   pages      : n_layers arrays [num_pages][page_bytes], layer_stride bytes apart (whatever they
  *                hold; page_bytes a multiple of 16).  Only reserve and compact touch them.
  * Results depend on the state at the call's start alone: free pages are given out lowest first, in
- * the order of rows and slots.  Table entries >= num_pages raise the device status and are left. */
+ * the order of rows and slots.  Table entries >= num_pages that a call meets raise the device status and
+ * change no count; reserve, free and compact leave them, fork hands a parent's on like any other. */
 typedef struct b2a_page_pool {
     int32_t* page_table;
     int32_t* ref_counts;

@@ -241,3 +241,53 @@ def test_graph_replays_of_a_step(ctx):
         m.check(t)
     del g
     ctx.check_device_status()
+
+
+def test_entries_beyond_the_pool_are_reported(ctx):
+    """An entry >= num_pages raises the status in every operation that meets it and changes no count.  reserve, free
+    and compact leave it; fork hands it on like any other entry and replaces it in a row that gets a parent."""
+    import b200attn
+    bad = 10 ** 6
+
+    def fresh():
+        m = Model(np.random.default_rng(4), 3, 4, 12, 16, share=0, fill=0)
+        m.table[0, :2], m.table[1, :2], m.table[2, :1] = (0, 1), (4, bad), (9,)
+        m.refs[[0, 1, 4, 9]] = 1
+        return m, m.device()
+
+    def reported():
+        with pytest.raises(b200attn.B200RuntimeException, match="page_table") as ei:
+            ctx.check_device_status()
+        assert ei.value.status == b200attn.B2A_EDEVICE
+        ctx.check_device_status()
+
+    m, t = fresh()  # row 1 writes positions 20..39: slot 1 is the bad one, slot 2 gets the lowest free page
+    b200attn.pages_reserve(ctx, t["table"], t["refs"], _dev([0, 20, 0]), _dev([0, 20, 0]), t["pages"], 16, t["counts"])
+    reported()
+    m.table[1, 2], m.refs[2] = 2, 1
+    m.counts[:] = 1, 0
+    m.check(t)
+    m, t = fresh()  # the bad slot alone is written: nothing to give out
+    b200attn.pages_reserve(ctx, t["table"], t["refs"], _dev([0, 20, 0]), _dev([0, 1, 0]), t["pages"], 16, t["counts"])
+    reported()
+    m.check(t)
+    m, t = fresh()
+    b200attn.pages_free(ctx, t["table"], t["refs"], None, _dev([0, 0, 0]), 16)
+    reported()
+    m.table[:] = -1
+    m.table[1, 1] = bad
+    m.refs[:] = 0
+    m.check(t)
+    m, t = fresh()
+    b200attn.pages_compact(ctx, t["table"], t["refs"], t["pages"], t["counts"])
+    reported()
+    m.compact()
+    m.check(t)
+    for parents in ([0, 0, 2], [0, 1, 1], [0, -1, 2]):
+        m, t = fresh()
+        b200attn.pages_fork(ctx, t["table"], t["refs"], _dev(parents))
+        reported()
+        m.table = np.where(np.asarray(parents)[:, None] >= 0, m.table[np.maximum(parents, 0)], -1).astype(np.int32)
+        m.refs[:] = 0
+        np.add.at(m.refs, m.table[(m.table >= 0) & (m.table < 12)], 1)
+        m.check(t)

@@ -179,7 +179,7 @@ __device__ __forceinline__ Span written_slots(const PagePoolParams& p, const int
 }
 // Whether a written slot needs a page: it has none, or one that other rows hold too.
 __device__ __forceinline__ bool wants_page(const PagePoolParams& p, int page) {
-    return page < 0 || (page < p.num_pages && p.ref_counts[page] > 1);
+    return page < 0 || (page_ok(p, page) && p.ref_counts[page] > 1);
 }
 
 // One block: who wants a page, the lowest free pages, who gets which.
