@@ -430,6 +430,16 @@ struct StoreGeo {
     }
 };
 
+// The wait for a round's rows at place `failed` (0: K's, 1: V's) ran out: the parity of the last copy
+// asked for at `place`.  K's place has been asked for the next round's rows, where there are `more`, by
+// the time V's are waited for.
+__host__ __device__ constexpr uint32_t pending_parity(int place, int failed, bool more, uint32_t parity) {
+    return place < failed && more ? parity ^ 1u : parity;
+}
+static_assert(pending_parity(0, 1, true, 0) == 1 && pending_parity(0, 1, true, 1) == 0, "the next round's keys");
+static_assert(pending_parity(0, 1, false, 1) == 1 && pending_parity(1, 1, true, 0) == 0, "this round's rows");
+static_assert(pending_parity(0, 0, true, 1) == 1 && pending_parity(1, 0, true, 1) == 1, "this round's rows");
+
 // A CTA takes one block of a sequence and heads h0 + group, + groups, ...  Its rows of K, then of V, come
 // by bulk copies into a place each, asked for again as soon as the last ones are in registers, so that
 // a round's rows travel while the round before is worked on.  A key chunk is rotated with its partner
@@ -600,8 +610,8 @@ __global__ void __launch_bounds__(StoreGeo<D>::kMaxThreads, StoreGeo<D>::ctas(kN
             }
             if (__syncthreads_or(!came)) {  // the wait ran out: nothing more is stored or asked for
                 if (tid == 0) atomicOr(p.status, 8);
-                mbar_drain(bar, parity);
-                mbar_drain(bar + 8, parity);
+                for (int place = 0; place < 2; ++place)
+                    mbar_drain(bar + place * 8, pending_parity(place, is_v, h0 + groups < h_end, parity));
                 return;
             }
             if (tid < 32 && h0 + groups < h_end) request(is_v, h0 + groups);
