@@ -4,7 +4,7 @@ import pytest
 
 import kv4_helpers as kv
 import oracle
-from helpers import to_np
+from helpers import normal, to_np
 from test_gpu_kv4 import Case
 
 pytestmark = pytest.mark.gpu
@@ -214,3 +214,45 @@ def test_a_captured_call_and_a_later_one_with_more_units():
             assert torch.equal(b["o"], first_b)
         del g
         one.check_device_status()
+
+
+@pytest.mark.parametrize("D,G,T", [(64, 4, 1), (64, 7, 2), (96, 3, 1), (128, 8, 1), (256, 4, 1), (256, 4, 3)])
+def test_large_key_minima_against_queries_that_cancel(ctx, D, G, T):
+    """Keys whose groups lie thousands from zero, each group elsewhere, and queries whose groups sum to nearly zero
+    (exact in fp16, no rotation), so that a score is made of large minima times small sums.  Two fp16 words hold a
+    sum to 2^-22 of itself (the second word's rounding); products and sums are fp32, with at most 2^-20 lost of what
+    they are made of (16 additions by truncation, of 2^-23 each, and the scaling).  With
+        ds = scale * (2^-21 sum_y |z_y sum q| + 2^-19 sum_y (|z_y sum q| + s_y sum_i |q_i| c_i))
+    an output may differ by 2^-11 of itself and (2 ds + 2^-20 + 1e-5) A, A = sum_j p_j |v_j|."""
+    import b200attn
+    L = 40
+    c = Case(ctx=[L, 25], T=T, Hq=G, Hkv=1, D=D, rope=None, seed=D + G)
+    rng = np.random.default_rng(D + G)
+    q = rng.normal(size=c.q.shape).reshape(*c.q.shape[:-1], -1, 32)
+    q = (q - q.mean(-1, keepdims=True)).reshape(c.q.shape)
+    c.q = q.astype(np.float16).astype(np.float32)
+    ds = np.zeros((2, T, G))
+    for b in range(2):
+        n = int(c.ctx[b])
+        far = 2000.0 * rng.normal(size=(n, 1, D // 32, 1))
+        k = (far + 0.3 * rng.normal(size=(n, 1, D // 32, 32))).reshape(n, 1, D).astype(np.float32)
+        kc, ks = kv.quantise(k)
+        vc, vs = kv.quantise(c.rows[b][1].astype(np.float32))
+        c.rows[b] = [kv.values(kc, ks), kv.values(vc, vs)]
+        c._store(b, 0, (kc, ks, vc, vs))
+        qg = c.q[b].astype(np.float64).reshape(T, G, D // 32, 32)
+        sums = np.abs(qg.sum(-1))[:, :, None]                                     # [T, G, 1, groups]
+        low = np.abs(ks[:, 0, :, 1].astype(np.float64)) * sums                    # [T, G, n, groups]
+        codes = np.einsum("tgyi,nyi->tgny", np.abs(qg), kc.reshape(n, -1, 32).astype(np.float64)) * ks[:, 0, :, 0].astype(np.float64)
+        ds[b] = c.scale * (2.0 ** -21 * low.sum(-1) + 2.0 ** -19 * (low + codes).sum(-1)).max(-1)
+    t = c.device()
+    b200attn.kv4_decode(ctx, t["q"], t["k"], t["v"], t["pages"], t["table"], t["ctx"], t["o"], c.scale, **c.more())
+    ctx.check_device_status()
+    o, _, kh, vh = c.expect()
+    for b in range(2):
+        pos = int(c.ctx[b]) + np.arange(T)
+        K, V = np.concatenate([c.rows[b][0], kh[b]]), np.concatenate([c.rows[b][1], vh[b]])
+        A = kv.attend(c.q[b].astype(np.float64), K, np.abs(V), pos, 0, c.scale)
+        tol = 2.0 ** -11 * np.abs(o[b]) + (2 * ds[b][..., None] + 2.0 ** -20 + 1e-5) * A
+        err = np.abs(to_np(t["o"])[b] - o[b])
+        assert np.all(err <= tol), (float((err / tol).max()), float(err.max()))

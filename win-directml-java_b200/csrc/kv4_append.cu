@@ -25,7 +25,7 @@ constexpr int kPrepWarps = 8;
 // 2 t + e of group y goes to half e of operand word (y, lane 4 (r % 8) + t, 2 x + j) of 8-row tile
 // r / 8, as q 2^-E / 16^j with |q 2^-E| < 2^14 (the codes of channels with j = 1 enter the product
 // 16 times larger); fp16 activations keep a second word with what the first rounding lost.
-// q_sums: sum of the group's operand values 2^-24 per group, then scale log2(e) 2^(E + 24).
+// q_sums: sum of the group's operand values 2^-4 (at most 2^15) per group, then scale log2(e) 2^(E + 24).
 template <int D>
 __device__ __forceinline__ void prepare_query(const Kv4Params& p, float (&x)[D / 32], const float (&wn)[D / 32],
                                               int64_t tok, int h, int t, const double2* cs, float* vec, int lane) {
@@ -63,7 +63,7 @@ __device__ __forceinline__ void prepare_query(const Kv4Params& p, float (&x)[D /
             frag[kGroups * 32 * 4 * 2 + at] = lo;
             used[y] += __half2float(lo);
         }
-        used[y] *= j ? 0x1p-20f : 0x1p-24f;
+        used[y] *= j ? 1.f : 0x1p-4f;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)

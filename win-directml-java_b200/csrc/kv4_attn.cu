@@ -277,7 +277,8 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
                 else qf[j][y][0] = w.x, qf[j][y][1] = w.y, qf[j][y][2] = w.z, qf[j][y][3] = w.w;
             }
             if (j < kSTiles) {
-                // the groups' sums of q, two halves each (k = group and k = 8 + group)
+                // the groups' sums of q, two halves each (k = group and k = 8 + group): 2^20 times as large as
+                // the products with the codes, so that the second half is no subnormal and keeps its bits
                 float s0 = 0.f, s1 = 0.f;
                 const float* sums = p.q_sums + at * (kGroups + 1) * 8;
                 if (there && !lo_word && 2 * t4 < kGroups) s0 = sums[2 * t4 * 8 + (row & 7)];
@@ -347,6 +348,8 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
 #pragma unroll
                 for (int j = 0; j < kSTiles; ++j) {
                     mma_set(x[u][j], zf, qz[j][0], qz[j][1], zero);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[u][j][e] *= 0x1p-20f;
                 }
 #pragma unroll
                 for (int y = 0; y < kGroups; ++y) {
