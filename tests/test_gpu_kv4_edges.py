@@ -256,3 +256,22 @@ def test_large_key_minima_against_queries_that_cancel(ctx, D, G, T):
         tol = 2.0 ** -11 * np.abs(o[b]) + (2 * ds[b][..., None] + 2.0 ** -20 + 1e-5) * A
         err = np.abs(to_np(t["o"])[b] - o[b])
         assert np.all(err <= tol), (float((err / tol).max()), float(err.max()))
+
+
+@pytest.mark.parametrize("T,dtype", [(1, oracle.F16), (1, oracle.BF16), (66, oracle.BF16)])
+def test_the_widest_window_is_no_window(ctx, T, dtype):
+    """Over a wide table at head dim 256, where the variant follows the keys in reach: the same bits."""
+    import torch
+    import b200attn
+    c = Case(ctx=[1500 + 7 * b for b in range(16)], T=T, Hq=4, Hkv=1, D=256, page=64, dtype=dtype, rope=None, seed=T,
+             extra_slots=1000)
+    got = []
+    for window in (0, 2 ** 31 - 1):
+        t = c.device()
+        b200attn.kv4_decode(ctx, t["q"], t["k"], t["v"], t["pages"], t["table"], t["ctx"], t["o"], c.scale,
+                            window=window, **c.more())
+        ctx.check_device_status()
+        got.append(t["o"])
+    o, tol, _, _ = c.expect()
+    c.check_out(to_np(got[0]), o, tol)
+    assert torch.equal(got[0], got[1])

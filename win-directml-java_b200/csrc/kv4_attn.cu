@@ -890,6 +890,7 @@ __global__ void __launch_bounds__(kThreads, C::kCtas) kv4_attn_kernel(const __gr
 
 struct LaunchInfo {
     int grid = 0;
+    int sms = 0;
 };
 
 // Kernel attributes, set up once for each device (the caller has made `device` current).
@@ -908,6 +909,7 @@ LaunchInfo launch_info(int device) {
         if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, kThreads, C::kSmem) != cudaSuccess) return;
         if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return;
         info[device].grid = occ * sms;
+        info[device].sms = sms;
     });
     return info[device];
 }
@@ -924,10 +926,12 @@ LaunchInfo launch_info(int device) {
 //    sequences of 4 k keys: 34 pipelined, 31 us not).
 constexpr int kPipelineBlocks = 128;
 
-bool few_blocks(const Kv4Params& p) {
-    const int64_t keys = std::min<int64_t>(p.window > 0 ? p.window + p.T : INT32_MAX, (int64_t)p.max_pages * p.page_size);
+bool few_blocks(const Kv4Params& p, int device) {
+    const int64_t keys = std::min<int64_t>(p.window > 0 ? (int64_t)p.window + p.T : INT32_MAX,
+                                           (int64_t)p.max_pages * p.page_size);
     const int64_t units = (int64_t)p.B * p.Hkv * ((p.T * p.G + 7) / 8);
-    return units * (keys / kKv4Block) <= (int64_t)kPipelineBlocks * 2 * 148;
+    // (the pipelined variant has two CTAs per SM)
+    return units * (keys / kKv4Block) <= (int64_t)kPipelineBlocks * 2 * launch_info<Cfg<256, 1, 1, true>>(device).sms;
 }
 
 // few: few_blocks of the whole call, of which p may be a part.
@@ -968,7 +972,7 @@ size_t kv4_sums_bytes(const Kv4Params& p) { return (size_t)q_tiles_of(p) * p.Hkv
 
 Kv4Split kv4_attn_split(const Kv4Params& p, int device) {
     Kv4Split split{};
-    split.few = few_blocks(p);
+    split.few = few_blocks(p, device);
     dispatch(p, split.few, [&](auto cfg) {
         using C = decltype(cfg);
         split.n_cta = launch_info<C>(device).grid;
