@@ -49,3 +49,17 @@ def test_heads_apart_and_uneven_tokens_are_refused():
     for t in (torch.zeros(3, 5, 8, 64)[:, :, ::2], torch.zeros(3, 6, 2, 64)[:, :5], torch.zeros(3, 5, 2, 128)[..., ::2]):
         with pytest.raises(ValueError, match="one distance"):
             _token_rows(Rows(t), "q", t.shape)
+
+
+def test_empty_pools_and_rows_are_refused_by_name():
+    """Sizes of zero end in the message of the check, not in a division by them."""
+    from b200attn import _kv4_cache, _kv4_call_rows, _page_pool
+    i32 = lambda *s: Rows(torch.zeros(*s, dtype=torch.int32))
+    u8 = lambda *s: Rows(torch.zeros(*s, dtype=torch.uint8))
+    for pages in (u8(0, 4, 16), u8(2, 0, 16)):
+        with pytest.raises(ValueError, match="at least one layer and one page"):
+            _page_pool(i32(3, 5), i32(pages.shape[1]), pages)
+    with pytest.raises(ValueError, match="no whole rows"):
+        _kv4_cache(u8(4, 2, 640), i32(3, 5), 3, 0, 2)
+    rows = Rows(torch.zeros(3, 1, 2, 0, dtype=torch.float16))
+    assert _kv4_call_rows(rows, rows, u8(4, 2, 640), i32(3, 5), i32(3), None, None, None, torch.float16, rows.shape) is None

@@ -463,7 +463,7 @@ def _kv4_cache(pages, page_table, B, D, num_kv_heads=None):
     num_pages, heads, row = pages.shape
     if num_kv_heads is not None and heads != num_kv_heads:
         raise ValueError(f"pages hold {heads} kv heads, the new rows {num_kv_heads}")
-    page_size, rest = divmod(row * 4, D * 5)
+    page_size, rest = divmod(row * 4, D * 5) if D else (0, 0)
     if rest or page_size == 0:
         raise ValueError(f"a page of {row} bytes per kv head holds no whole rows of head_dim {D}")
     if page_table.dim() != 2:
@@ -531,7 +531,7 @@ def _kv4_call_rows(k_new, v_new, pages, page_table, ctx_lens, new_lens, k_held, 
             and page_table.is_contiguous() and ctx_lens.is_contiguous()):
         return None
     pool, table = pages.shape, page_table.shape
-    if not (len(pool) == 3 and len(table) == 2 and table[0] == B and pool[1] == Hkv):
+    if not (len(pool) == 3 and len(table) == 2 and table[0] == B and pool[1] == Hkv and D):
         return None
     page_size, rest = divmod(pool[2] * 4, D * 5)
     if rest or page_size == 0:
@@ -629,6 +629,8 @@ def _page_pool(page_table, ref_counts, pages=None):
     if pages.dim() < 2 or pages.shape[1] != num_pages:
         raise ValueError(f"pages must be [n_layers, {num_pages}, ...], got {list(pages.shape)}")
     n_layers = pages.shape[0]
+    if n_layers == 0 or num_pages == 0:
+        raise ValueError(f"pages must hold at least one layer and one page, got {list(pages.shape)}")
     layer = pages.numel() // n_layers * pages.element_size()
     return _PagePool(table, refs, _address(pages, "pages"), layer, layer // num_pages, n_seq, max_pages, num_pages,
                      n_layers)
