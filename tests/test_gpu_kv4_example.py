@@ -25,3 +25,11 @@ def test_prompts_samples_drafts_and_compaction():
         assert refs[page] == (table == page).sum()
     for row, n in enumerate(s.lens.tolist()):
         assert (table[row] >= 0).sum() == -(-n // paged_kv4.PAGE)
+
+
+def test_every_output_of_the_example_lies_within_its_own_bound():
+    """Element by element, from the weights and values that make the output (see Server.compare)."""
+    sys.path.insert(0, EXAMPLES)
+    import paged_kv4
+    s = paged_kv4.main()
+    assert 0 < s.worst_of_bound <= 1

@@ -32,7 +32,8 @@ class Server:
         self.counts = torch.zeros(2, dtype=torch.int32, device="cuda")
         self.lens = torch.zeros(rows, dtype=torch.int32, device="cuda")
         self.held = [[torch.zeros(2, 0, HKV, D, device="cuda") for _ in range(rows)] for _ in range(LAYERS)]
-        self.worst = 0.0
+        self.worst = 0.0  # largest difference from dense attention
+        self.worst_of_bound = 0.0  # the same, as a share of what roundings allow that element
 
     def step(self, new):
         """Appends and attends new[row] tokens per row (a chunk, a draft, one token, or none)."""
@@ -85,8 +86,18 @@ class Server:
         q = torch.cat([a * c - b * s, b * c + a * s], -1).view(n, HKV, HQ // HKV, D)
         score = SCALE * torch.einsum("nhgd,khd->nhgk", q, k)
         score.masked_fill_((torch.arange(total, device="cuda") > pos[:, None])[:, None, None], -math.inf)
-        want = torch.einsum("nhgk,khd->nhgd", score.softmax(-1), v).reshape(n, HQ, D)
-        self.worst = max(self.worst, float((out.double() - want).abs().max()))
+        p = score.softmax(-1)
+        want = torch.einsum("nhgk,khd->nhgd", p, v)
+        # bf16 rounds the held keys and values and the output by 2^-9 each, the kernels round q, P, P s and a
+        # chunk's rows by 2^-11 each: `off` of a score, which moves its weight by as much, and of a value
+        off = (2 ** -9 + 2 * 2 ** -11) * SCALE * torch.einsum("nhgd,khd->nhgk", q.abs(), k.abs())
+        bound = 2 ** -8 * want.abs() + (2 ** -9 + 4 * 2 ** -11 + 1e-5) * torch.einsum("nhgk,khd->nhgd", p, v.abs())
+        for h in range(HKV):  # sum_j p_j off_j |v_j - o|
+            far = (v[None, None, :, h] - want[:, h, :, None]).abs()
+            bound[:, h] += torch.einsum("ngk,ngkd->ngd", p[:, h] * off[:, h], far)
+        err = (out.double().view_as(want) - want).abs()
+        self.worst = max(self.worst, float(err.max()))
+        self.worst_of_bound = max(self.worst_of_bound, float((err / bound).max()))
 
 
 def main():
@@ -105,7 +116,7 @@ def main():
     s.step([1, 1, 1, 70, 0, 0])                        # they go on beside a new prompt
     s.step([1, 1, 1, 1, 0, 0])
     print(f"rows of {s.lens.tolist()} tokens on {int((s.refs > 0).sum())} pages ({used} after compaction, which moved "
-          f"{moved}); largest difference from dense attention {s.worst:.2e}")
+          f"{moved}); largest difference from dense attention {s.worst:.2e}, {s.worst_of_bound:.0%} of its bound")
     return s
 
 
