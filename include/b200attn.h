@@ -409,8 +409,9 @@ B2A_API int b2a_kv4_append(b2a_context* ctx, const b2a_kv4_cache* cache, int act
  * words; bf16 calls round both once to fp16's 11 significant bits (what bf16 results keep is 8), the
  * probabilities times s, so that an output's error is 2^-12 of its group's range rather than its own.
  * bf16 calls of 64 and more tokens turn the cache's rows into fp16 (s * c + z rounded once to 11 bits;
- * workspace: the rows of as many sequences as fit 1 GiB, one at least): a rotated q beyond the fp16
- * range raises the device status there.  B * T is at most 2^24. */
+ * workspace: the rows of as many sequences as fit 1 GiB, one at least, by the table's capacity): a
+ * rotated q or a seen row's s * c + z beyond the fp16 range raises the device status there and counts as
+ * infinite.  B * T is at most 2^24. */
 B2A_API int b2a_kv4_attention(b2a_context* ctx, const b2a_kv4_cache* cache, int act_dtype, const void* q,
                               int64_t q_token_stride, const int32_t* ctx_lens, const int32_t* new_lens, int B, int T,
                               int Hq, float scale, int rope_mode, double rope_theta, int window,

@@ -1287,7 +1287,12 @@ Kv4Params kv4_slice(const Kv4Params& p, int b0, int count) {
 
 // Chunks of prompts with bf16 results go to the tcgen05 kernel from this many tokens a sequence on;
 // shorter ones, whose 128-row query tiles would stand mostly empty, and fp16 results, which carry q
-// and P as two words, take the kernel that reads the codes.
+// and P as two words, take the kernel that reads the codes (2 x 1000 tokens on 3000, 32 / 8 heads of
+// 128: 1.6 ms in fp16, 0.16 ms in bf16).  Codes / staged rows, bf16: 4 sequences of 2000 cached, 32 / 8
+// heads of 128, 48 tokens 78 / 57 us, 64 tokens 98 / 59 us; 16 of 1000, 14 / 2 of 64, 48 tokens 60 / 55 us,
+// 64 tokens 73 / 55 us; where few sequences of long contexts let the staging's and the unsplit tiles' cost
+// show, more tokens are needed: 8 of 2000, 4 / 1 of 256, 64 tokens 60 / 74 us, 96 tokens 75 / 74 us; 1 of
+// 8000, 32 / 8 of 128, 64 tokens 82 / 127 us, 128 tokens 141 / 129 us.
 constexpr int kKv4ChunkTokens = 64;
 static_assert(kKv4ChunkTokens >= kKv4StoreTokens, "a chunk's append clears its flag");
 constexpr size_t kKv4StageBytes = size_t(1) << 30;  // staged cache rows of one launch (one sequence at least)

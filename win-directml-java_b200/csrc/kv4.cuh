@@ -82,7 +82,9 @@ __device__ __forceinline__ double kv4_warp_sum(double v) {
 // Optional zero-centred RMS norm, and RoPE with the position's (cos, sin) cs[0 .. D/2), of a row whose
 // element lane + 32 j is x[j]; the whole warp, vec[0..D) is its scratch.  The arithmetic is that of
 // b2a_decode's prologue (double sum of squares and angles; NeoX rotates in float, Gemma in double),
-// each operation rounded by itself, so that the codes decided on the result are reproducible.
+// each operation rounded by itself, so that the codes decided on the result are reproducible: exactly
+// without rotation; with it, as far as the double sine and cosine, which short appends take one by one
+// and prompts from kv4_block_angles, round to the same float.
 template <int D>
 __device__ __forceinline__ void kv4_norm_rope(float (&x)[D / 32], bool norm, const float (&norm_w)[D / 32], float eps,
                                               int rope_mode, const double2* cs, float* vec, int lane) {

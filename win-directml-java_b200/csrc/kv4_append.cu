@@ -415,7 +415,9 @@ struct StoreGeo {
     static constexpr int kMinHeads = D == 96 ? 2 : 1;         // whole warps
     static constexpr int kMaxThreads = kHeads * kPerHead;
     // per SM: 64 (with norms 80) registers a thread at head dim 96, where 4 CTAs take 220 us instead of 193
-    // (with norms 303 instead of 347); else 80
+    // (with norms 303 instead of 347); else 80.  With 2, 3, 4 and 5 CTAs, 8 x 4096 tokens with held rows, bf16
+    // without / fp16 with norms: 16 heads of 64 80, 70, 67, 83 / 106, 95, 95, 112 us; 16 heads of 128 138, 127,
+    // 125, 161 / 195, 181, 195, 224 us; 4 heads of 256 84, 75, 79, 98 / 112, 102, 110, 131 us
     static constexpr int ctas(bool norm) { return D == 96 ? (norm ? 4 : 5) : 3; }
     // an operand's 16 rows of the CTA's heads; the pad keeps rows two apart on other banks
     __host__ __device__ static constexpr int pitch(int heads) { return heads * D * 2 + (D == 96 ? 32 : 0); }
@@ -446,12 +448,13 @@ static_assert(pending_parity(0, 0, true, 1) == 1 && pending_parity(1, 0, true, 1
 // chunk D / 2 away, which the thread reads too.  The four threads of a group exchange minima and
 // maxima so that each ends with one of the four rows, and computes that row's scale for all.
 // Bound by issue and latency rather than by HBM: 8 x 4096 tokens of 32 heads of 96 with held rows (932
-// MB) take 193 us, 4.8 TB/s.  What it took: packed float pairs (201 -> 159 million warp instructions),
+// MB) take 193 us back to back, 4.8 TB/s, and 201 to 209 us as one call behind an L2 flush.  What it took: packed float pairs (201 -> 159 million warp instructions),
 // the rows' scales shared out (148 million, 261 -> 213 us), conflict-free angles (193 us).  Rows loaded
 // into registers ahead instead of by bulk copies: 209 us; 4 and 6 CTAs per SM: 220 and 245 us.
 // With key norms the sums of squares and the products with 1 + w are doubles as in b2a_decode: 8 x 4096
-// tokens of 16 heads of 128, fp16 (bf16 without norms: 128 us, with held rows), take 170 us, and 201 us with
-// the double-precision rotation; the rows' factors computed by every thread: 214 and 252 us.
+// tokens of 16 heads of 128, fp16 with held rows, take 180 us (without norms 123), and 210 us with the
+// double-precision rotation (146); the rows' factors computed by every thread: 44 and 51 us more.  32 heads of
+// 96, bf16: 322 us, where the partner chunk's norm is computed a second time in doubles.
 template <int D, typename T, bool kNorm>
 __global__ void __launch_bounds__(StoreGeo<D>::kMaxThreads, StoreGeo<D>::ctas(kNorm))
     kv4_store_kernel(const __grid_constant__ Kv4Params p, int blocks, int chunks, int per) {
@@ -767,7 +770,7 @@ cudaError_t launch_store(const Kv4Params& p, int sm_count, cudaStream_t stream) 
 template <int D>
 cudaError_t launch_prepare(const Kv4Params& p, int sm_count, cudaStream_t stream) {
     int append = p.k_new ? 1 : 0;
-    if (append && p.T >= kKv4StoreTokens) {  // below it a block would be mostly absent rows
+    if (append && p.T >= kKv4StoreTokens) {
         const cudaError_t e = p.act_dtype == kF16 ? launch_store<D, __half>(p, sm_count, stream)
                                                   : launch_store<D, __nv_bfloat16>(p, sm_count, stream);
         if (e != cudaSuccess || !p.q) return e;

@@ -12,8 +12,8 @@
 // provided the instructions per key stay few.  Per 16 keys and 32 channels a warp spends twenty
 // integer instructions on 2 x 512 codes (two masks and a shift per word pair; the block layout is
 // the MMA's own operand order) and four MMAs of 16 keys (K) or 16 channels (V^T) x 8 columns.
-// Measured at head dim 256, 256 sequences of 16.9 k keys (1.38 GB of codes): 272 us, 5.1 TB/s, where
-// copying the rings alone takes 215 us; some 620 warp instructions a block keep 60% of the issue slots
+// Measured at head dim 256, 256 sequences of 16.9 k keys (1.38 GB of codes): 272 us back to back, 5.1
+// TB/s (290 to 302 us as one call behind an L2 flush), where copying the rings alone takes 215 us; some 620 warp instructions a block keep 60% of the issue slots
 // and 54% of the integer pipe busy, and registers allow three warps a scheduler.  Short work is
 // latency: 64 sequences of 4.4 k keys, head dim 64 (45 MB), take 31 us, of them 13 in the loop.
 //
@@ -921,7 +921,8 @@ LaunchInfo launch_info(int device) {
 //  * Pipelined at head dim 256 where a CTA has few blocks to walk and one warp's own speed counts (256
 //    sequences over a 512-key window, 33 blocks each: 30.9 -> 26.8 us); long contexts want the third CTA
 //    (the same sequences over 17 k keys: 299 pipelined, 275 us not).  What a CTA has is bounded by the
-//    window, else by the table's capacity.  With 16 columns always: the third CTA does not fit anyway
+//    window, else by the table's capacity: the lengths are on the device, so short contexts in a wide table
+//    take the form for long ones.  With 16 columns always: the third CTA does not fit anyway
 //    (5-token drafts at head dim 64: 20.6 -> 19.3 us); at head dim 64 with two-word operands never (64
 //    sequences of 4 k keys: 34 pipelined, 31 us not).
 constexpr int kPipelineBlocks = 128;

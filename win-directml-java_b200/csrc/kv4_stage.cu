@@ -6,7 +6,7 @@
 // tensor-core kernel streams those through TMA; per key and head that is far less than the chunk's
 // own multiplications.  Measured for 2 x 1000 tokens of 32 heads of 128 on 2 x 3000 cached ones (8 kv
 // heads, 87 MB moved): 27 us, of them 16 behind the append beside which the queries are staged,
-// before an attention of 102 us; its warps wait for loads, half of the issue slots are idle.  Turning
+// before an attention of 102 us (the whole call: 152 to 177 us on one GPU, the attention's clock moving); its warps wait for loads, half of the issue slots are idle.  Turning
 // the blocks before the appended ones while the append runs gained nothing (the GPU is full).
 // A value beyond fp16 becomes infinite and raises status bit 2, as bf16 inputs of the other entry
 // points do.

@@ -13,7 +13,10 @@
 // All of it is latency: tables and counts are some 100 KB, and what is copied (a few MB) would take HBM
 // 1 to 2 us.  Measured: 1024 rows of 257 slots freed in 3.0 us and reserved in 12 us (8 rows of 72: 1.8
 // and 8.0 us); compacting 48 rows of some 18 pages after 5 have left 11 us, with 80 pages of 4 layers
-// moved or copied.  A plan is read, scanned and written by one block, two passes over the counts.
+// moved or copied.  A plan is read, scanned and written by one block, two passes over the counts, which
+// is what a large pool costs: reserving a page for each of 1024 rows takes 12 to 14 us where free pages lie
+// among the first 4096, but 32 us behind 89 k live ones packed at the front and 70 us behind 255 k;
+// compacting a pool of 100 k, 300 k and 1 M pages takes 100, 284 and 940 us before anything moves.
 #include "internal.h"
 
 namespace b2a {
