@@ -208,7 +208,8 @@ def test_decode_graph_replays_recompute_the_step(ctx):
     ctx.check_device_status()
 
 
-def test_decode_counters_are_untouched_by_a_captured_decode_of_other_sizes():
+@pytest.mark.parametrize("B,Hkv,length", [(800, 4, 997), (2040, 9, 190)])
+def test_decode_counters_are_untouched_by_a_captured_decode_of_other_sizes(B, Hkv, length):
     """A captured decode with few units and large partial slots, then one with many units and small slots in the same
     workspace: replaying the first must leave the counters of the second at zero."""
     import torch
@@ -222,7 +223,7 @@ def test_decode_counters_are_untouched_by_a_captured_decode_of_other_sizes():
                 torch.empty(B, Hq, D, device="cuda"), 1 / math.sqrt(D))
 
     few = inputs(2, 4, 1, 256, 4096, 4000, 1)
-    many = inputs(800, 8, 4, 64, 1000, 997, 2)
+    many = inputs(B, 2 * Hkv, Hkv, 64, length + 3, length, 2)
     with b200attn.Context(0) as one:
         def run(x):
             x[6].fill_(float("nan"))
@@ -240,7 +241,7 @@ def test_decode_counters_are_untouched_by_a_captured_decode_of_other_sizes():
         torch.cuda.synchronize()
         first = [x[6].clone() for x in (few, many)]
         assert bool(torch.isfinite(first[1]).all())
-        assert one.workspace_bytes() <= size + (1 << 16)  # more counters at most: the graph's slots stayed in place
+        assert one.workspace_bytes() <= size + (1 << 17)  # more counters at most: the graph's slots stayed in place
         for _ in range(2):
             g.replay()
             torch.cuda.synchronize()

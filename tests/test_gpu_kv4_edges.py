@@ -184,13 +184,16 @@ def test_a_chunk_sees_a_key_held_as_nan_at_every_place_of_a_block(ctx, D, window
     assert np.all((np.abs(got - o) <= tol)[~sees])
 
 
-def test_a_captured_call_and_a_later_one_with_more_units():
+@pytest.mark.parametrize("few,many", [
+    (dict(ctx=[5000, 4100], T=2, Hq=4, Hkv=1, D=256, page=64), dict(ctx=60 + np.arange(1200) % 90, Hq=1, Hkv=1, D=64)),
+    (dict(ctx=[1500] * 10, T=60, Hq=72, Hkv=9, D=256, page=64), dict(ctx=20 + np.arange(2040) % 30, Hq=9, Hkv=9, D=64)),
+], ids=["hundreds", "beyond_the_workspace"])
+def test_a_captured_call_and_a_later_one_with_more_units(few, many):
     """The merge counters of a call must stay zero between launches whatever an earlier captured call does: few units
     with large slots (captured), then many units with small ones, in the same workspace."""
     import torch
     import b200attn
-    few = Case(ctx=[5000, 4100], T=2, Hq=4, Hkv=1, D=256, page=64, rope=None, seed=41)
-    many = Case(ctx=60 + np.arange(1200) % 90, Hq=2, Hkv=1, D=64, page=32, rope=None, seed=43)
+    few, many = Case(rope=None, seed=41, **few), Case(rope=None, seed=43, **many)
     a, b = few.device(), many.device()
     with b200attn.Context(0) as one:
         def run(c, t):
@@ -204,7 +207,7 @@ def test_a_captured_call_and_a_later_one_with_more_units():
         torch.cuda.synchronize()
         first_a, first_b = a["o"].clone(), b["o"].clone()
         assert bool(torch.isfinite(first_b.float()).all())
-        assert one.workspace_bytes() <= size + (1 << 16)  # more counters at most: the graph's slots stayed in place
+        assert one.workspace_bytes() <= size + (1 << 17)  # more counters at most: the graph's slots stayed in place
         for _ in range(2):
             g.replay()
             torch.cuda.synchronize()

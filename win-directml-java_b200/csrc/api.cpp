@@ -19,9 +19,9 @@
 
 using namespace b2a;
 
-// Counters that are zero between launches.  They grow into a new allocation and the old one stays until
-// the context ends, since a captured launch goes on counting there; and they share no allocation with
-// anything that is written otherwise, so what such a launch writes never lands on a later call's counters.
+// Counters that are zero between launches, for calls that need more of them than a workspace holds at its
+// start (kInlineCounters).  They grow into a new allocation and the old one stays until the context ends,
+// since a captured launch goes on counting there.
 struct Counters {
     static constexpr int kMost = 48;  // each at least twice the one before
     int* at[kMost] = {};
@@ -38,6 +38,7 @@ struct b2a_context {
     int* status = nullptr;  // device int[kStatusBufferInts]: error flags, prefill work-item counters
     int* status_host = nullptr;  // pinned int[kStatusWords]: where b2a_check_device_status reads the flags
     // decode workspace: [counters][partials]
+    // [counters][slots] (ensure_counted_buffer)
     void* dec_ws = nullptr;
     size_t dec_ws_bytes = 0;
     Counters dec_counters;
@@ -57,10 +58,9 @@ struct b2a_context {
     // split-K projections: [tile counters][fp32 accumulator], all zero between launches
     void* lin_ws = nullptr;
     size_t lin_ws_bytes = 0;
-    // generic-kernel key split: partial slots
+    // generic-kernel key split: [counters][partial slots]
     void* split_ws = nullptr;
     size_t split_ws_bytes = 0;
-    Counters split_counters;
     // test hook (b2a_test_inject_wait_timeout): the next tcgen05 attention launch
     // leaves one K/V copy unissued
     bool inject_wait_timeout = false;
@@ -68,14 +68,13 @@ struct b2a_context {
     double kv4_inv_freq[kMaxHeadDim / 2] = {};
     double kv4_theta = 0.0;
     int kv4_inv_dim = 0;
-    // paged 4-bit cache: [partial slots][plan][q operands][q sums]
+    // paged 4-bit cache: [counters][partial slots][plan][q operands][q sums]
     void* kv4_ws = nullptr;
     size_t kv4_ws_bytes = 0;
     Counters kv4_counters;
-    // paged cache: the page operations' lists and the words between their blocks
+    // paged cache: [words between blocks][the page operations' lists]
     void* pg_ws = nullptr;
     size_t pg_ws_bytes = 0;
-    Counters pg_sync;
     // b2a_set_decode_early_start: tensor-core decodes launched with programmatic serialisation
     bool decode_early_start = false;
     // test hook (b2a_test_last_attention_kernel): the kernel the last whole-sequence
@@ -122,8 +121,7 @@ size_t dtype_size(int d) { return d == B2A_FLOAT32 ? 4 : 2; }
 
 size_t workspace_total(const b2a_context* ctx) {
     return ctx->dec_ws_bytes + ctx->pf_ws_bytes + ctx->split_ws_bytes + ctx->blk_ws_bytes + ctx->rope_tab_bytes +
-           ctx->lin_ws_bytes + ctx->pg_ws_bytes + ctx->kv4_ws_bytes + ctx->dec_counters.total +
-           ctx->split_counters.total + ctx->kv4_counters.total + ctx->pg_sync.total;
+           ctx->lin_ws_bytes + ctx->pg_ws_bytes + ctx->kv4_ws_bytes + ctx->dec_counters.total + ctx->kv4_counters.total;
 }
 
 // Whether `more` bytes beside `others` stay within the context's limit.
@@ -184,11 +182,28 @@ void free_counters(Counters& c) {
     for (int i = 0; i < c.n; ++i) cudaFree(c.at[i]);
 }
 
-// Partial slots of at least slot_bytes at *buf and counters at *counters.
-int ensure_counted_buffer(b2a_context* ctx, void** buf, size_t* have, Counters& c, size_t counter_ints,
-                          size_t slot_bytes, const char* what, cudaStream_t stream, bool sync, int** counters) {
-    const int rc = ensure_buffer(ctx, buf, have, slot_bytes, what);
-    return rc ? rc : ensure_counters(ctx, c, counter_ints, what, stream, sync, counters);
+// Sizes a workspace for slot_bytes at *slots and counters at *counters.  The counters lie before the slots
+// (in an allocation of their own a decode step of 24 layers took 0.662 ms instead of 0.655), in a region of
+// one size whatever the call: no launch's slots, of a graph captured long ago either, lie where a later
+// call of other sizes counts.  Calls that need more counters than that have them in `more` (null: such calls
+// do not occur).
+constexpr size_t kInlineCounters = 64 << 10;  // bytes
+int ensure_counted_buffer(b2a_context* ctx, void** buf, size_t* have, Counters* more, size_t counter_ints,
+                          size_t slot_bytes, const char* what, cudaStream_t stream, bool sync, int** counters,
+                          void** slots) {
+    const bool fresh = kInlineCounters + slot_bytes > *have;
+    const int rc = ensure_buffer(ctx, buf, have, kInlineCounters + slot_bytes, what);
+    if (rc) return rc;
+    if (fresh) {
+        const cudaError_t e =
+            sync ? cudaMemset(*buf, 0, kInlineCounters) : cudaMemsetAsync(*buf, 0, kInlineCounters, stream);
+        if (e != cudaSuccess) return cuda_fail(ctx, e, what);
+    }
+    *slots = static_cast<char*>(*buf) + kInlineCounters;
+    *counters = static_cast<int*>(*buf);
+    if (counter_ints * sizeof(int) <= kInlineCounters) return B2A_OK;
+    if (!more) return fail(ctx, B2A_ENOTSUP, "%s: too many counters", what);
+    return ensure_counters(ctx, *more, counter_ints, what, stream, sync, counters);
 }
 
 void inv_freq_table(double theta, int D, double* out) {
@@ -268,9 +283,10 @@ cudaError_t launch_attention(b2a_context* ctx, const AttnParams& p, cudaStream_t
     const int nsplit = attn_simt_split_plan(p, ctx->sm_count, &part_bytes, &counter_ints);
     if (nsplit > 1) {
         int* counters = nullptr;
-        if (ensure_counted_buffer(ctx, &ctx->split_ws, &ctx->split_ws_bytes, ctx->split_counters, counter_ints,
-                                  part_bytes, "attention split workspace", s, false, &counters) == B2A_OK) {
-            const SimtSplit sp{static_cast<float*>(ctx->split_ws), counters, nsplit, kSimtSplitKeys};
+        void* slots = nullptr;
+        if (ensure_counted_buffer(ctx, &ctx->split_ws, &ctx->split_ws_bytes, nullptr, counter_ints,
+                                  part_bytes, "attention split workspace", s, false, &counters, &slots) == B2A_OK) {
+            const SimtSplit sp{static_cast<float*>(slots), counters, nsplit, kSimtSplitKeys};
             return launch_attn_simt(p, s, &sp);
         }
         ctx->last_error.clear();  // the refused workspace is not an error of this call
@@ -290,10 +306,11 @@ int run_decode(b2a_context* ctx, DecodeParams& p, cudaStream_t stream, bool allo
         decode_tc_workspace(ctx->device, p.B, p.Hkv, p.n_hg, p.D, p.cache_dtype, &target, &cap, &partial_bytes);
         const int bmax = std::min(p.B, kDecodeMaxBatchPerLaunch);
         const size_t counter_ints = (size_t)bmax * p.Hkv * p.n_hg;
-        int rc = ensure_counted_buffer(ctx, &ctx->dec_ws, &ctx->dec_ws_bytes, ctx->dec_counters, counter_ints,
-                                       partial_bytes, "decode workspace", stream, false, &p.counters);
+        void* slots = nullptr;
+        int rc = ensure_counted_buffer(ctx, &ctx->dec_ws, &ctx->dec_ws_bytes, &ctx->dec_counters, counter_ints,
+                                       partial_bytes, "decode workspace", stream, false, &p.counters, &slots);
         if (rc != B2A_OK) return rc;
-        p.partials = static_cast<float*>(ctx->dec_ws);
+        p.partials = static_cast<float*>(slots);
         p.target_items = target;
         p.item_capacity = cap;
         p.early_start = ctx->decode_early_start ? 1 : 0;
@@ -403,9 +420,7 @@ B2A_API int b2a_destroy(b2a_context* ctx) {
         if (ctx->pg_ws) cudaFree(ctx->pg_ws);
         if (ctx->kv4_ws) cudaFree(ctx->kv4_ws);
         free_counters(ctx->dec_counters);
-        free_counters(ctx->split_counters);
         free_counters(ctx->kv4_counters);
-        free_counters(ctx->pg_sync);
     }
     delete ctx;
     return B2A_OK;
@@ -454,8 +469,9 @@ B2A_API int b2a_reserve_decode(b2a_context* ctx, int max_batch, int num_q_heads,
                         &partial_bytes);
     const size_t counter_ints = (size_t)std::min(max_batch, kDecodeMaxBatchPerLaunch) * num_kv_heads * n_hg;
     int* counters = nullptr;
-    return ensure_counted_buffer(ctx, &ctx->dec_ws, &ctx->dec_ws_bytes, ctx->dec_counters, counter_ints,
-                                 partial_bytes, "decode workspace", nullptr, true, &counters);
+    void* slots = nullptr;
+    return ensure_counted_buffer(ctx, &ctx->dec_ws, &ctx->dec_ws_bytes, &ctx->dec_counters, counter_ints,
+                                 partial_bytes, "decode workspace", nullptr, true, &counters, &slots);
 }
 
 B2A_API int b2a_test_inject_wait_timeout(b2a_context* ctx) {
@@ -1383,11 +1399,12 @@ int run_kv4_attention(b2a_context* ctx, Kv4Params& p, cudaStream_t stream) {
     const size_t units = (size_t)most * p.split.per_seq;
     const size_t part = r256(p.split.partial_bytes), plan = r256((p.split.n_cta + units) * sizeof(Kv4Piece)), frag = r256(kv4_frag_bytes(p) * most),
                  sums = r256(kv4_sums_bytes(p) * most);
-    const int rc = ensure_counted_buffer(ctx, &ctx->kv4_ws, &ctx->kv4_ws_bytes, ctx->kv4_counters, units,
+    void* slots = nullptr;
+    const int rc = ensure_counted_buffer(ctx, &ctx->kv4_ws, &ctx->kv4_ws_bytes, &ctx->kv4_counters, units,
                                          part + plan + frag + sums, "4-bit cache attention", stream, false,
-                                         &p.counters);
+                                         &p.counters, &slots);
     if (rc) return rc;
-    char* at = static_cast<char*>(ctx->kv4_ws);
+    char* at = static_cast<char*>(slots);
     auto take = [&](size_t bytes) {
         char* here = at;
         at += bytes;
@@ -1436,10 +1453,11 @@ int check_pool(b2a_context* ctx, const b2a_page_pool* pool, bool with_pages, Pag
 }
 
 int pages_workspace(b2a_context* ctx, int num_pages, cudaStream_t stream, int** sync, int** ws) {
-    const int rc = ensure_counted_buffer(ctx, &ctx->pg_ws, &ctx->pg_ws_bytes, ctx->pg_sync, kPageSyncInts,
+    void* lists = nullptr;
+    const int rc = ensure_counted_buffer(ctx, &ctx->pg_ws, &ctx->pg_ws_bytes, nullptr, kPageSyncInts,
                                          pages_workspace_ints(num_pages) * sizeof(int), "page operations", stream,
-                                         false, sync);
-    *ws = static_cast<int*>(ctx->pg_ws);
+                                         false, sync, &lists);
+    *ws = static_cast<int*>(lists);
     return rc;
 }
 
