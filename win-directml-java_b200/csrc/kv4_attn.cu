@@ -13,7 +13,7 @@
 // integer instructions on 2 x 512 codes (two masks and a shift per word pair; the block layout is
 // the MMA's own operand order) and four MMAs of 16 keys (K) or 16 channels (V^T) x 8 columns.
 // Measured at head dim 256, 256 sequences of 16.9 k keys (1.38 GB of codes): 272 us back to back, 5.1
-// TB/s (290 to 302 us as one call behind an L2 flush), where copying the rings alone takes 215 us; some 620 warp instructions a block keep 60% of the issue slots
+// TB/s (283 to 303 us as one call behind an L2 flush), where copying the rings alone takes 215 us; some 620 warp instructions a block keep 60% of the issue slots
 // and 54% of the integer pipe busy, and registers allow three warps a scheduler.  Short work is
 // latency: 64 sequences of 4.4 k keys, head dim 64 (45 MB), take 31 us, of them 13 in the loop.
 //
